@@ -79,6 +79,9 @@ typedef void *sfb_stream; /* a cudaStream_t */
 /* float element types of sfb_scan / sfb_quantize */
 #define SFB_F32 0
 #define SFB_F64 1
+/* and of the tensor-core linear and the AdamW step */
+#define SFB_BF16 2
+#define SFB_F16 3
 
 /* Statistics of a float tensor and of its quantization (device memory; the
  * caller zeroes it): scan -> nan_count, inf_count, absmax (largest finite |x|);
@@ -361,6 +364,32 @@ SFB_API int sfb_elementwise_signmag(int op, int bits, const uint16_t *a, const u
  * Device buffers. */
 SFB_API int sfb_sweep(int op, int bits, int64_t a_lo, int64_t a_hi, uint32_t *row_digest, sfb_counts *counts,
                       sfb_stream stream);
+
+/* One AdamW step over `count` tensors.  No counterpart in the reference, whose
+ * straight-through training uses torch's optimizers.  `table` is HOST memory,
+ * eight words a tensor: the device addresses of the parameter, its gradient, the
+ * first and the second moment, the scales of the first and of the second moment
+ * (sf8 only), the number of elements, and a seed that sets this tensor's dither
+ * apart from the others'.  Parameters and gradients are dtype (SFB_F32, SFB_BF16
+ * or SFB_F16); the moments float32, or with sf8 != 0 int8 codes and one float32
+ * scale for every 256 elements.  `dither` seeds the rounding of sf8 codes: give
+ * another number each step.  `constants` NULL: the constants come from lr .. step.
+ * Otherwise they are those that sfb_adamw_advance left in that device buffer, and
+ * lr .. dither are not read.  A tensor given twice is refused. */
+#define SFB_ADAMW_CONSTANTS 64 /* bytes of the buffer */
+SFB_API int sfb_adamw(const int64_t *table, int count, int dtype, int sf8, double lr, double beta1, double beta2,
+                      double eps, double weight_decay, int64_t step, unsigned dither, const void *constants,
+                      sfb_stream stream);
+
+/* Adds one to the step counter in device memory and writes the constants of
+ * that step: what a step captured into a graph replays before its sfb_adamw. */
+SFB_API int sfb_adamw_advance(int64_t *step, void *constants, double lr, double beta1, double beta2, double eps,
+                              double weight_decay, unsigned seed, sfb_stream stream);
+
+/* The float32 values that sf8 moments stand for: power 2 for the first moment,
+ * 4 for the second.  `table` as sfb_adamw's: word 0 the output, 1 the codes,
+ * 4 the scales, 6 the number of elements. */
+SFB_API int sfb_sf8_values(const int64_t *table, int count, int power, sfb_stream stream);
 
 #ifdef __cplusplus
 }

@@ -68,6 +68,11 @@ SIGNATURES = {
                                    _i64, _p, _i64, _p, _p]),
     "sfb_wide_finish": (_i32, [_i32, _i32, _p, _i64, _i64, _p, _p, _p, _p, _i32, _i32, _i32, _p, _p, _p, _p, _p,
                                _p, _p]),
+    "sfb_adamw": (_i32, [_p, _i32, _i32, _i32, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
+                         ctypes.c_double, _i64, ctypes.c_uint, _p, _p]),
+    "sfb_adamw_advance": (_i32, [_p, _p, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
+                                 ctypes.c_double, ctypes.c_uint, _p]),
+    "sfb_sf8_values": (_i32, [_p, _i32, _i32, _p]),
 }
 
 _lib = None
@@ -338,3 +343,56 @@ def matmul_wide(bits, mx, A, B, shift_arr, shift, out, flags, counts, batch, M, 
                                 _ptr(flags), batch, M, N, K, lda, ldb, sa, sb, so, ssb, ssm, ssn,
                                 _ptr(workspace), ws_bytes, _ptr(counts), _stream(stream))
     check(rc, "sf matmul (wide)")
+
+
+# --- on the device of the tensors, whichever is current: the AdamW step and the tensor-core linear ---------------
+
+ADAMW_WORDS, ADAMW_CONSTANTS = 8, 64       # words of a table entry, bytes of the constants' buffer
+ELEMENT = {"float32": 0, "bfloat16": 2, "float16": 3}
+
+
+class on_device:
+    """The launches inside go to CUDA device ``index``, on its current stream (the attribute ``stream``)."""
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self):
+        import torch
+        self.before = torch.cuda.current_device()
+        ensure_current(self.index)
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        self.stream = torch.cuda.current_stream(self.index).cuda_stream
+        return self
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            import torch
+            torch.cuda.set_device(self.before)
+
+
+def ensure_current(index: int) -> None:
+    """sfb_device_init once per device, the current device left as it was."""
+    if index in _ready_devices:
+        return
+    import torch
+    before = torch.cuda.current_device()
+    try:
+        ensure_device(index)
+    finally:
+        torch.cuda.set_device(before)
+
+
+def adamw(table, count, dtype, sf8, lr, betas, eps, weight_decay, step, dither, constants, stream) -> None:
+    check(load().sfb_adamw(table, count, dtype, int(sf8), lr, betas[0], betas[1], eps, weight_decay, step, dither,
+                           constants, stream), "sf adamw step")
+
+
+def adamw_advance(step, constants, lr, betas, eps, weight_decay, seed, stream) -> None:
+    check(load().sfb_adamw_advance(step, constants, lr, betas[0], betas[1], eps, weight_decay, seed, stream),
+          "sf adamw step counter")
+
+
+def sf8_values(table, count, power, stream) -> None:
+    check(load().sfb_sf8_values(table, count, power, stream), "sf8 moment values")

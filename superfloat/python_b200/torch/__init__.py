@@ -17,6 +17,7 @@ from ._backend import GraphReport, compile_report, compile_reports, superfloat  
 from ._core import weight_cache  # noqa: F401
 from ._modules import (ConversionReport, SFConfig, SFConv2d, SFHFConv1D, SFLinear, conversion_report, convert,
                        find_lm_heads, is_hf_conv1d)
+from ._optim import AdamW, SF8Moment, adamw_step, moment_values
 from ._status import SFLayerStatus, capture_status, last_status, reset_status
 
 
@@ -61,4 +62,5 @@ def matmul(a, b, dtype="sf16", headroom="bound", name="matmul", *, accumulate="c
 
 __all__ = ["quantize", "linear", "matmul", "SFLinear", "SFConv2d", "SFHFConv1D", "SFConfig", "convert",
            "find_lm_heads", "is_hf_conv1d", "conversion_report", "ConversionReport", "last_status",
-           "reset_status", "capture_status", "SFLayerStatus", "compile_report", "compile_reports", "GraphReport"]
+           "reset_status", "capture_status", "SFLayerStatus", "compile_report", "compile_reports", "GraphReport",
+           "AdamW", "SF8Moment", "adamw_step", "moment_values"]

@@ -1,0 +1,359 @@
+"""AdamW over many tensors at once, with moments in float32 or in sf8.
+
+The straight-through training of converted layers (``sf::linear`` and its
+kin) keeps float parameters; this is the optimizer step that goes with it.
+The reference trains with torch's optimizers and has no counterpart.
+
+    p <- p (1 - lr wd) - lr / bc1 * m / (sqrt(v / bc2) + eps)
+    m <- b1 m + (1 - b1) g,   v <- b2 v + (1 - b2) g^2,   bc_i = 1 - b_i^step
+
+An sf8 moment is int8 codes in [-127, 127] with one float32 scale for every
+256 elements in storage order; a code c stands for ``scale (c / 127)^2`` with
+c's sign in the first moment and ``scale (c / 127)^4`` in the second.  Codes
+are rounded by a dither that keeps the value unbiased.  ``csrc/sfb_adamw.cu``
+has the kernels and the reasons.
+"""
+from __future__ import annotations
+
+import math
+from array import array
+from dataclasses import dataclass
+
+import torch
+
+from .. import _lib
+from .._errors import SFShapeError, SFTypeError, SFUnsupportedError
+
+BLOCK = 256                        # elements that share a scale
+SF8_FROM = 4096                    # AdamW(state="sf8") keeps smaller tensors' moments in float32
+_ELEMENT = {torch.float32: _lib.ELEMENT["float32"], torch.bfloat16: _lib.ELEMENT["bfloat16"],
+            torch.float16: _lib.ELEMENT["float16"]}
+_POWER = {"first": 2, "second": 4}
+_SEED_STEP = 0x9E3779B9            # between the dithers of neighbouring tensors
+
+
+@dataclass
+class SF8Moment:
+    """A moment of ``codes.numel()`` elements: int8 codes in the parameter's
+    storage order, and a float32 scale for every 256 of them."""
+
+    codes: torch.Tensor
+    scale: torch.Tensor
+
+    @classmethod
+    def zeros(cls, n: int, device) -> "SF8Moment":
+        return cls(torch.zeros(n, dtype=torch.int8, device=device),
+                   torch.zeros(-(-n // BLOCK), dtype=torch.float32, device=device))
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether the elements fill one stretch of memory, each place once."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.shape == b.shape and (a.stride() == b.stride() or (a.is_contiguous() and b.is_contiguous()))
+
+
+def _check_sf8(m: SF8Moment, n: int, device, what: str) -> None:
+    c, s = m.codes, m.scale
+    if c.dtype != torch.int8 or s.dtype != torch.float32:
+        raise SFTypeError(f"{what}: an sf8 moment has int8 codes and float32 scales, got {c.dtype} and {s.dtype}")
+    if c.numel() != n or s.numel() != -(-n // BLOCK):
+        raise SFShapeError(f"{what}: {n} elements need {n} codes and {-(-n // BLOCK)} scales, got {c.numel()} and "
+                           f"{s.numel()}")
+    if c.device != device or s.device != device:
+        raise SFShapeError(f"{what}: the moment is not on {device}")
+    if not (c.is_contiguous() and s.is_contiguous()):
+        raise SFShapeError(f"{what}: codes and scales must be contiguous")
+    if n and c.data_ptr() % 4:
+        raise SFShapeError(f"{what}: the codes must start on a 4-byte boundary")
+
+
+def _check_rates(lr, betas, eps, weight_decay):
+    for name, v in (("lr", lr), ("eps", eps), ("weight_decay", weight_decay)):
+        if isinstance(v, torch.Tensor):
+            raise SFTypeError(f"{name} must be a number, not a tensor")
+        if not (v >= 0 and math.isfinite(v)):
+            raise ValueError(f"{name} must be a finite number of at least 0, got {v!r}")
+    if len(betas) != 2 or not all(0 <= b < 1 for b in betas):
+        raise ValueError(f"betas must be two numbers in [0, 1), got {betas!r}")
+
+
+def _buckets(params, grads, exp_avg, exp_avg_sq):
+    """{(device index, element type, sf8): [table words]}, one entry for each
+    tensor, after the checks; and the gradients that had to be laid out."""
+    buckets, kept = {}, []
+    for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avg, exp_avg_sq)):
+        dt = _ELEMENT.get(p.dtype)
+        if dt is None:
+            raise SFTypeError(f"adamw: tensor {i} is {p.dtype}; float32, bfloat16 and float16 are supported")
+        if g.dtype != p.dtype:
+            raise SFTypeError(f"adamw: tensor {i} is {p.dtype} and its gradient {g.dtype}")
+        if not p.is_cuda or g.device != p.device:
+            raise SFShapeError(f"adamw: tensor {i} and its gradient must be on one CUDA device, got {p.device} and "
+                               f"{g.device}")
+        if g.is_sparse or g.layout != torch.strided:
+            raise SFUnsupportedError(f"adamw: tensor {i} has a gradient that is not strided")
+        if g.shape != p.shape:
+            raise SFShapeError(f"adamw: tensor {i} has shape {tuple(p.shape)}, its gradient {tuple(g.shape)}")
+        if not _dense(p):
+            raise SFShapeError(f"adamw: tensor {i} has gaps or overlaps in memory (shape {tuple(p.shape)}, strides "
+                               f"{p.stride()})")
+        if not _same_layout(p, g):
+            g = torch.empty_strided(p.shape, p.stride(), dtype=g.dtype, device=g.device).copy_(g)
+            kept.append(g)
+        n = p.numel()
+        sf8 = isinstance(m, SF8Moment)
+        if sf8 != isinstance(v, SF8Moment):
+            raise SFTypeError(f"adamw: tensor {i} has one moment in sf8 and one that is not")
+        if sf8:
+            _check_sf8(m, n, p.device, f"adamw: first moment of tensor {i}")
+            _check_sf8(v, n, p.device, f"adamw: second moment of tensor {i}")
+            words = (p.data_ptr(), g.data_ptr(), m.codes.data_ptr(), v.codes.data_ptr(), m.scale.data_ptr(),
+                     v.scale.data_ptr(), n, (i * _SEED_STEP) & 0xFFFFFFFF)
+        else:
+            for t in (m, v):
+                if t.dtype != torch.float32:
+                    raise SFTypeError(f"adamw: tensor {i} has a moment of {t.dtype}; float32 or SF8Moment")
+                if t.device != p.device or not _same_layout(p, t):
+                    raise SFShapeError(f"adamw: tensor {i} has a moment of another shape, layout or device")
+            words = (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, n, 0)
+        key = (p.get_device(), dt, sf8)
+        if key not in buckets:
+            buckets[key] = array("q")
+        buckets[key].extend(words)
+    return buckets, kept
+
+
+def _launch(buckets, lr, betas, eps, weight_decay, step, dither, constants=None):
+    for (index, dt, sf8), words in buckets.items():
+        with _lib.on_device(index) as d:
+            _lib.adamw(words.buffer_info()[0], len(words) // _lib.ADAMW_WORDS, dt, sf8, float(lr),
+                       (float(betas[0]), float(betas[1])), float(eps), float(weight_decay), int(step),
+                       dither & 0xFFFFFFFF, constants, d.stream)
+
+
+@torch.no_grad()
+def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step: int, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 0.0, dither: int = 0) -> None:
+    """One AdamW step on lists of CUDA tensors, in place, on each device's
+    current stream.
+
+    ``params`` and ``grads``: float32, bfloat16 or float16 tensors without gaps
+    in memory (a gradient of another layout is copied).  ``exp_avg`` and
+    ``exp_avg_sq``: float32 tensors of the parameter's layout, or
+    :class:`SF8Moment`; both of a parameter's moments are of one kind.  ``step``
+    counts from 1.  ``dither`` seeds the rounding of sf8 moments: another number
+    each step (the step will do).  The arithmetic is float32; a 16-bit parameter
+    is rounded to nearest once.  A tensor that is given twice, or overlaps
+    another that the step writes, is refused."""
+    if not len(params) == len(grads) == len(exp_avg) == len(exp_avg_sq):
+        raise SFShapeError(f"adamw: {len(params)} parameters, {len(grads)} gradients, {len(exp_avg)} and "
+                           f"{len(exp_avg_sq)} moments")
+    if isinstance(step, bool) or not isinstance(step, int) or step < 1:
+        raise ValueError(f"step must be an int of at least 1, got {step!r}")
+    _check_rates(lr, betas, eps, weight_decay)
+    buckets, _kept = _buckets(params, grads, exp_avg, exp_avg_sq)
+    _launch(buckets, lr, betas, eps, weight_decay, step, dither)
+
+
+@torch.no_grad()
+def moment_values(moments, kind: str) -> list:
+    """The float32 values of moments: what the codes of each
+    :class:`SF8Moment` stand for, flat in storage order, and float32 moments as
+    they are.  ``kind``: "first" or "second"."""
+    if kind not in _POWER:
+        raise ValueError(f"kind must be \"first\" or \"second\", got {kind!r}")
+    out, tables = [], {}
+    for i, m in enumerate(moments):
+        if not isinstance(m, SF8Moment):
+            out.append(m)
+            continue
+        n = m.codes.numel()
+        if not m.codes.is_cuda:
+            raise SFShapeError(f"moment {i} must be on a CUDA device, got {m.codes.device}")
+        _check_sf8(m, n, m.codes.device, f"moment {i}")
+        out.append(torch.empty(n, dtype=torch.float32, device=m.codes.device))
+        tables.setdefault(m.codes.get_device(), array("q")).extend(
+            (out[-1].data_ptr(), m.codes.data_ptr(), 0, 0, m.scale.data_ptr(), 0, n, 0))
+    for index, words in tables.items():
+        with _lib.on_device(index) as d:
+            _lib.sf8_values(words.buffer_info()[0], len(words) // _lib.ADAMW_WORDS, _POWER[kind], d.stream)
+    return out
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW whose step is one launch for the tensors of each type.
+
+    ``state``: "float32", or "sf8" for moments of one byte an element (tensors
+    below 4096 elements, biases and norms mostly, keep float32 moments).
+    ``dither_seed`` sets the rounding of sf8 moments apart from another run's.
+    ``capturable=True`` keeps the step count on the device, so that ``step()``
+    can be captured into a CUDA graph and replayed; the other settings are
+    then those of the capture.  Every parameter needs its gradient then.
+
+    >>> opt = sft.AdamW(model.parameters(), lr=1e-4, state="sf8")
+    >>> loss.backward(); opt.step(); opt.zero_grad()
+    """
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01, *,
+                 state: str = "float32", dither_seed: int = 0, capturable: bool = False):
+        _check_rates(lr, betas, eps, weight_decay)
+        if state not in ("float32", "sf8"):
+            raise ValueError(f"state must be \"float32\" or \"sf8\", got {state!r}")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state=state,
+                                      dither_seed=int(dither_seed), capturable=bool(capturable)))
+
+    @staticmethod
+    def _check_param(p):
+        if _ELEMENT.get(p.dtype) is None or not p.is_cuda:
+            raise SFTypeError(f"AdamW: a parameter of {p.dtype} on {p.device}; float32, bfloat16 and float16 on a "
+                              f"CUDA device are supported")
+
+    def _begin(self, p, group):
+        st = self.state[p]
+        if st:
+            return st
+        if group["state"] == "sf8" and p.numel() >= SF8_FROM:
+            m, v = SF8Moment.zeros(p.numel(), p.device), SF8Moment.zeros(p.numel(), p.device)
+            st["exp_avg"], st["exp_avg_scale"] = m.codes, m.scale
+            st["exp_avg_sq"], st["exp_avg_sq_scale"] = v.codes, v.scale
+        else:
+            st["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+            st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+        st["step"] = 0
+        return st
+
+    @staticmethod
+    def _moments(st):
+        if "exp_avg_scale" in st:
+            return (SF8Moment(st["exp_avg"], st["exp_avg_scale"]),
+                    SF8Moment(st["exp_avg_sq"], st["exp_avg_sq_scale"]))
+        return st["exp_avg"], st["exp_avg_sq"]
+
+    def _counter(self, group):
+        """The group's step counter and constants on the device (capturable)."""
+        c = group.get("_counter")
+        device = group["params"][0].device
+        if c is None or c[0].device != device:
+            if torch.cuda.is_current_stream_capturing():
+                raise SFUnsupportedError("AdamW: take one step before the capture, so that the moments and the step "
+                                         "counter exist")
+            done = max((self.state[p].get("step", 0) for p in group["params"] if p in self.state), default=0)
+            c = (torch.full((1,), done, dtype=torch.int64, device=device),
+                 torch.zeros(_lib.ADAMW_CONSTANTS, dtype=torch.uint8, device=device))
+            group["_counter"] = c
+        return c
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            _check_rates(group["lr"], group["betas"], group["eps"], group["weight_decay"])
+            with_grad = [p for p in group["params"] if p.grad is not None]
+            if not with_grad:
+                continue
+            for p in with_grad:
+                self._check_param(p)
+            capturing = torch.cuda.is_current_stream_capturing()
+            if capturing and not group["capturable"]:
+                raise SFUnsupportedError("AdamW: a captured step needs capturable=True (the step count is on the "
+                                         "host otherwise, and every replay would repeat it)")
+            if capturing and any(not self.state.get(p) for p in with_grad):
+                raise SFUnsupportedError("AdamW: take one step before the capture, so that the moments and the step "
+                                         "counter exist")
+            if group["capturable"]:
+                self._device_step(group, with_grad)
+            else:
+                self._host_step(group, with_grad)
+        return loss
+
+    def _host_step(self, group, with_grad):
+        by_step = {}
+        for p in with_grad:
+            st = self._begin(p, group)
+            by_step.setdefault(st["step"] + 1, []).append((p, st))
+        for step, items in by_step.items():
+            moments = [self._moments(st) for _, st in items]
+            buckets, _kept = _buckets([p for p, _ in items], [p.grad for p, _ in items], [m for m, _ in moments],
+                                      [v for _, v in moments])
+            _launch(buckets, group["lr"], group["betas"], group["eps"], group["weight_decay"], step,
+                    group["dither_seed"] + step)
+            for _, st in items:
+                st["step"] = step
+
+    def _device_step(self, group, with_grad):
+        if len(with_grad) != len(group["params"]):
+            raise SFUnsupportedError("AdamW: with capturable=True every parameter of the group needs its gradient "
+                                     "(one step count serves the group)")
+        if len({p.device for p in with_grad}) != 1:
+            raise SFUnsupportedError("AdamW: with capturable=True a group's parameters are on one device")
+        states = [self._begin(p, group) for p in with_grad]
+        counter, constants = self._counter(group)
+        moments = [self._moments(st) for st in states]
+        buckets, _kept = _buckets(with_grad, [p.grad for p in with_grad], [m for m, _ in moments],
+                                  [v for _, v in moments])
+        with _lib.on_device(counter.get_device()) as d:
+            _lib.adamw_advance(counter.data_ptr(), constants.data_ptr(), float(group["lr"]),
+                               tuple(map(float, group["betas"])), float(group["eps"]), float(group["weight_decay"]),
+                               group["dither_seed"] & 0xFFFFFFFF, d.stream)
+        _launch(buckets, group["lr"], group["betas"], group["eps"], group["weight_decay"], 1, 0,
+                constants.data_ptr())
+
+    def moments(self, p) -> tuple:
+        """The float32 values of a parameter's two moments, in its shape."""
+        st = self.state.get(p)
+        if not st:
+            raise ValueError("the parameter has not been stepped yet")
+        m, v = self._moments(st)
+        if isinstance(m, SF8Moment):
+            m, v = moment_values([m], "first")[0], moment_values([v], "second")[0]
+            m, v = (torch.as_strided(t, p.shape, p.stride()) for t in (m, v))
+        return m, v
+
+    def steps_done(self, p) -> int:
+        """How many steps the parameter has taken (reads the device with capturable=True)."""
+        for group in self.param_groups:
+            if any(q is p for q in group["params"]) and group.get("_counter") is not None:
+                return int(group["_counter"][0])
+        return self.state[p]["step"] if self.state.get(p) else 0
+
+    def state_dict(self):
+        """As torch's; a group's device counter is saved as its step count."""
+        for group in self.param_groups:
+            if group.get("_counter") is not None:
+                done = int(group["_counter"][0])
+                for p in group["params"]:
+                    if self.state.get(p):
+                        self.state[p]["step"] = done
+        d = super().state_dict()
+        for g in d["param_groups"]:
+            g.pop("_counter", None)
+        return d
+
+    def load_state_dict(self, state_dict):
+        """As torch's, but the moments keep their own types (torch would cast them to the parameter's)."""
+        groups = state_dict["param_groups"]
+        super().load_state_dict({**state_dict, "state": {}})
+        own = [p for g in self.param_groups for p in g["params"]]
+        saved = [i for g in groups for i in g["params"]]
+        self.state.clear()
+        for p, i in zip(own, saved):
+            st = state_dict["state"].get(i)
+            if not st:
+                continue
+            self.state[p] = {k: t.to(device=p.device, copy=True) if isinstance(t, torch.Tensor) else t
+                             for k, t in st.items()}
+        for g in self.param_groups:
+            g["_counter"] = None
