@@ -82,6 +82,14 @@ typedef void *sfb_stream; /* a cudaStream_t */
 /* and of the tensor-core linear and the AdamW step */
 #define SFB_BF16 2
 #define SFB_F16 3
+#define SFB_I8 4 /* codes */
+
+/* activations of the tensor-core linear */
+#define SFB_ACT_NONE 0
+#define SFB_ACT_RELU 1
+#define SFB_ACT_GELU 2      /* z Phi(z) */
+#define SFB_ACT_GELU_TANH 3 /* its tanh form */
+#define SFB_ACT_SILU 4
 
 /* Statistics of a float tensor and of its quantization (device memory; the
  * caller zeroes it): scan -> nan_count, inf_count, absmax (largest finite |x|);
@@ -364,6 +372,51 @@ SFB_API int sfb_elementwise_signmag(int op, int bits, const uint16_t *a, const u
  * Device buffers. */
 SFB_API int sfb_sweep(int op, int bits, int64_t a_lo, int64_t a_hi, uint32_t *row_digest, sfb_counts *counts,
                       sfb_stream stream);
+
+/* The tensor-core linear: y = act(x Wq^T + b) + r over sf4..sf8 codes, Wq[n, k]
+ * = codes[n, k] 2^-(bits-1) scale[n], summed in float32.  The reference computes
+ * a converted layer on the chip's integer units (src/sf/torch/_core.py:336-433);
+ * these have no counterpart there.  x, y, r: dtype, SFB_BF16 or SFB_F16.
+ *
+ * sfb_code_quantize: the codes of a float weight (N rows of K, ldw apart, any of
+ * SFB_F32 / BF16 / F16) and their scales: scale = max|w| / m over the row or, with
+ * per_channel 0, over the matrix (1 where that is 0), code = rint(w / scale
+ * 2^(bits-1)) within +-M.  codes_dtype SFB_I8 packs them, SFB_BF16 / F16 writes
+ * the product's operand.  work: 4 N bytes.  A row with a NaN or an infinity gets
+ * it as its scale.
+ *
+ * sfb_code_expand: packed codes as the product's operand.
+ *
+ * sfb_tensor_linear: the forward product.  codes of type dtype.  z (nullable)
+ * receives the pre-activation in fp16 for the backward pass.
+ * sfb_slope: dz = dy act'(z) and / or dzs = dz scale / top (top NULL: dz scale
+ * 2^-(bits-1)), rows ldd apart (a multiple of 8, padding written as 0), and db =
+ * sum of dz over the rows.  work: sfb_slope_workspace(M, N) bytes when db is wanted.
+ * sfb_tensor_grad_x: dx = dzs codes (top as in sfb_slope).
+ * sfb_tensor_grad_w: dw = dz^T x.
+ *
+ * Operands of the products start on 16-byte boundaries and their row strides are
+ * multiples of 8 elements; outputs, residual and bias may start anywhere.
+ * sfb_tensor_failures: how many CTAs of these products have given up a bounded
+ * wait on the current device since the library was loaded (their outputs are
+ * NaN); it waits for the device.  sfb_wide_wait_limit bounds these waits too. */
+SFB_API int sfb_code_quantize(const void *w, int dtype, int64_t N, int64_t K, int64_t ldw, int bits, int per_channel,
+                              void *codes, int64_t ldc, int codes_dtype, float *scale, void *work, sfb_stream stream);
+SFB_API int sfb_code_expand(const int8_t *codes, int64_t N, int64_t K, int64_t ldc, void *out, int64_t ldo, int dtype,
+                            sfb_stream stream);
+SFB_API int sfb_tensor_linear(int dtype, const void *x, int64_t ldx, const void *codes, int64_t ldw, const float *scale,
+                              int bits, const void *bias, int bias_dtype, int act, const void *residual, int64_t ldr,
+                              void *y, int64_t ldy, void *z, int64_t ldz, int64_t M, int64_t N, int64_t K,
+                              sfb_stream stream);
+SFB_API int64_t sfb_slope_workspace(int64_t M, int64_t N);
+SFB_API int sfb_slope(int dtype, int act, const void *dy, int64_t ldy, const void *z, int64_t ldz, int64_t M, int64_t N,
+                      const float *scale, int bits, const float *top, void *dz, void *dzs, int64_t ldd, void *db,
+                      int db_dtype, void *work, sfb_stream stream);
+SFB_API int sfb_tensor_grad_x(int dtype, const void *dzs, int64_t ldd, const void *codes, int64_t ldw, const float *top,
+                              int bits, void *dx, int64_t ldy, int64_t M, int64_t N, int64_t K, sfb_stream stream);
+SFB_API int sfb_tensor_grad_w(int dtype, const void *dz, int64_t ldd, const void *x, int64_t ldx, void *dw,
+                              int dw_dtype, int64_t ldy, int64_t M, int64_t N, int64_t K, sfb_stream stream);
+SFB_API int sfb_tensor_failures(int64_t *count);
 
 /* One AdamW step over `count` tensors.  No counterpart in the reference, whose
  * straight-through training uses torch's optimizers.  `table` is HOST memory,

@@ -68,6 +68,15 @@ SIGNATURES = {
                                    _i64, _p, _i64, _p, _p]),
     "sfb_wide_finish": (_i32, [_i32, _i32, _p, _i64, _i64, _p, _p, _p, _p, _i32, _i32, _i32, _p, _p, _p, _p, _p,
                                _p, _p]),
+    "sfb_code_quantize": (_i32, [_p, _i32, _i64, _i64, _i64, _i32, _i32, _p, _i64, _i32, _p, _p, _p]),
+    "sfb_code_expand": (_i32, [_p, _i64, _i64, _i64, _p, _i64, _i32, _p]),
+    "sfb_tensor_linear": (_i32, [_i32, _p, _i64, _p, _i64, _p, _i32, _p, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _i64,
+                                 _i64, _i64, _p]),
+    "sfb_slope_workspace": (_i64, [_i64, _i64]),
+    "sfb_slope": (_i32, [_i32, _i32, _p, _i64, _p, _i64, _i64, _i64, _p, _i32, _p, _p, _p, _i64, _p, _i32, _p, _p]),
+    "sfb_tensor_grad_x": (_i32, [_i32, _p, _i64, _p, _i64, _p, _i32, _p, _i64, _i64, _i64, _i64, _p]),
+    "sfb_tensor_grad_w": (_i32, [_i32, _p, _i64, _p, _i64, _p, _i32, _i64, _i64, _i64, _i64, _p]),
+    "sfb_tensor_failures": (_i32, [_p]),
     "sfb_adamw": (_i32, [_p, _i32, _i32, _i32, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
                          ctypes.c_double, _i64, ctypes.c_uint, _p, _p]),
     "sfb_adamw_advance": (_i32, [_p, _p, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
@@ -396,3 +405,47 @@ def adamw_advance(step, constants, lr, betas, eps, weight_decay, seed, stream) -
 
 def sf8_values(table, count, power, stream) -> None:
     check(load().sfb_sf8_values(table, count, power, stream), "sf8 moment values")
+
+
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+I8 = 4                                     # SFB_I8: packed codes
+
+
+def code_quantize(w, dtype, N, K, ldw, bits, per_channel, codes, ldc, codes_dtype, scale, work, stream) -> None:
+    check(load().sfb_code_quantize(w, dtype, N, K, ldw, bits, int(per_channel), codes, ldc, codes_dtype, scale, work,
+                                   stream), "sf tensor linear (weight codes)")
+
+
+def code_expand(codes, N, K, ldc, out, ldo, dtype, stream) -> None:
+    check(load().sfb_code_expand(codes, N, K, ldc, out, ldo, dtype, stream), "sf tensor linear (packed codes)")
+
+
+def tensor_linear(dtype, x, ldx, codes, ldw, scale, bits, bias, bias_dtype, act, residual, ldr, y, ldy, z, ldz, M, N,
+                  K, stream) -> None:
+    check(load().sfb_tensor_linear(dtype, x, ldx, codes, ldw, scale, bits, bias, bias_dtype, act, residual, ldr, y,
+                                   ldy, z, ldz, M, N, K, stream), "sf tensor linear")
+
+
+def slope_workspace(M, N) -> int:
+    return int(load().sfb_slope_workspace(M, N))
+
+
+def slope(dtype, act, dy, ldy, z, ldz, M, N, scale, bits, top, dz, dzs, ldd, db, db_dtype, work, stream) -> None:
+    check(load().sfb_slope(dtype, act, dy, ldy, z, ldz, M, N, scale, bits, top, dz, dzs, ldd, db, db_dtype, work,
+                           stream), "sf tensor linear (activation's gradient)")
+
+
+def tensor_grad_x(dtype, dzs, ldd, codes, ldw, top, bits, dx, ldy, M, N, K, stream) -> None:
+    check(load().sfb_tensor_grad_x(dtype, dzs, ldd, codes, ldw, top, bits, dx, ldy, M, N, K, stream),
+          "sf tensor linear (gradient of x)")
+
+
+def tensor_grad_w(dtype, dz, ldd, x, ldx, dw, dw_dtype, ldy, M, N, K, stream) -> None:
+    check(load().sfb_tensor_grad_w(dtype, dz, ldd, x, ldx, dw, dw_dtype, ldy, M, N, K, stream),
+          "sf tensor linear (gradient of the weight)")
+
+
+def tensor_failures() -> int:
+    n = ctypes.c_int64()
+    check(load().sfb_tensor_failures(ctypes.addressof(n)), "sf tensor linear")
+    return n.value

@@ -26,15 +26,13 @@
 // A CTA takes one chunk of one tensor, found by bisection over the chunk counts.
 // Memory bound: 28 bytes an element with float32 p, g and moments, 16.06 with sf8
 // moments, 10.06 with 16-bit p and g besides.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <math.h>
 
 #include <algorithm>
 #include <exception>
 #include <vector>
 
-#include "sfb_common.cuh"
+#include "sfb_tensor.cuh"
 
 namespace sfb {
 namespace {
@@ -67,22 +65,11 @@ struct Table {
     Entry e[CAP];
 };
 
-template <typename T> __device__ __forceinline__ float to_f(T v);
-template <> __device__ __forceinline__ float to_f(float v) { return v; }
-template <> __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <typename T> __device__ __forceinline__ T from_f(float v);
-template <> __device__ __forceinline__ float from_f(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
-
-template <typename T> struct alignas(4 * sizeof(T)) Four { T v[4]; };
-
 // elements i .. i + 3 (those below n) as float
 template <typename T>
 __device__ __forceinline__ void load4(const T *x, int64_t i, int64_t n, bool vec, float (&r)[4]) {
     if (vec && i + 4 <= n) {
-        const Four<T> q = *reinterpret_cast<const Four<T> *>(x + i);
+        const Vec<T, 4> q = *reinterpret_cast<const Vec<T, 4> *>(x + i);
 #pragma unroll
         for (int j = 0; j < 4; j++) r[j] = to_f(q.v[j]);
     } else {
@@ -94,10 +81,10 @@ __device__ __forceinline__ void load4(const T *x, int64_t i, int64_t n, bool vec
 template <typename T>
 __device__ __forceinline__ void store4(T *x, int64_t i, int64_t n, bool vec, const float (&r)[4]) {
     if (vec && i + 4 <= n) {
-        Four<T> q;
+        Vec<T, 4> q;
 #pragma unroll
         for (int j = 0; j < 4; j++) q.v[j] = from_f<T>(r[j]);
-        *reinterpret_cast<Four<T> *>(x + i) = q;
+        *reinterpret_cast<Vec<T, 4> *>(x + i) = q;
     } else {
 #pragma unroll
         for (int j = 0; j < 4; j++)

@@ -1083,6 +1083,9 @@ int make_map(CUtensorMap *map, void *base, int64_t rows_pad, int64_t Kp, int box
 
 }  // namespace
 
+unsigned wait_polls() { return t_wait_polls; }
+int wait_stall() { return t_wait_stall; }
+
 int64_t wide_tc_workspace(int bits, int mx, int64_t batch, int64_t M, int64_t N, int64_t K) {
     (void)batch;
     if (!eligible(bits, mx, M, N, K)) return 0;

@@ -19,6 +19,7 @@ from ._modules import (ConversionReport, SFConfig, SFConv2d, SFHFConv1D, SFLinea
                        find_lm_heads, is_hf_conv1d)
 from ._optim import AdamW, SF8Moment, adamw_step, moment_values
 from ._status import SFLayerStatus, capture_status, last_status, reset_status
+from ._tensor import SFPackedWeight, pack_weight, tensor_failures, tensor_linear
 
 
 def _bits(dtype) -> int:
@@ -63,4 +64,4 @@ def matmul(a, b, dtype="sf16", headroom="bound", name="matmul", *, accumulate="c
 __all__ = ["quantize", "linear", "matmul", "SFLinear", "SFConv2d", "SFHFConv1D", "SFConfig", "convert",
            "find_lm_heads", "is_hf_conv1d", "conversion_report", "ConversionReport", "last_status",
            "reset_status", "capture_status", "SFLayerStatus", "compile_report", "compile_reports", "GraphReport",
-           "AdamW", "SF8Moment", "adamw_step", "moment_values"]
+           "SFPackedWeight", "pack_weight", "tensor_linear", "tensor_failures", "AdamW", "SF8Moment", "adamw_step", "moment_values"]
