@@ -408,6 +408,13 @@ SFB_API int sfb_tensor_linear(int dtype, const void *x, int64_t ldx, const void 
                               int bits, const void *bias, int bias_dtype, int act, const void *residual, int64_t ldr,
                               void *y, int64_t ldy, void *z, int64_t ldz, int64_t M, int64_t N, int64_t K,
                               sfb_stream stream);
+/* the same from packed codes (rows anywhere, ldc apart) for at most
+ * SFB_SMALL_ROWS rows of x: the codes are read once and not expanded */
+#define SFB_SMALL_ROWS 64
+SFB_API int sfb_tensor_linear_small(int dtype, const void *x, int64_t ldx, const int8_t *codes, int64_t ldc,
+                                    const float *scale, int bits, const void *bias, int bias_dtype, int act,
+                                    const void *residual, int64_t ldr, void *y, int64_t ldy, int64_t M, int64_t N,
+                                    int64_t K, sfb_stream stream);
 SFB_API int64_t sfb_slope_workspace(int64_t M, int64_t N);
 SFB_API int sfb_slope(int dtype, int act, const void *dy, int64_t ldy, const void *z, int64_t ldz, int64_t M, int64_t N,
                       const float *scale, int bits, const float *top, void *dz, void *dzs, int64_t ldd, void *db,

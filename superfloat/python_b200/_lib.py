@@ -72,6 +72,8 @@ SIGNATURES = {
     "sfb_code_expand": (_i32, [_p, _i64, _i64, _i64, _p, _i64, _i32, _p]),
     "sfb_tensor_linear": (_i32, [_i32, _p, _i64, _p, _i64, _p, _i32, _p, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _i64,
                                  _i64, _i64, _p]),
+    "sfb_tensor_linear_small": (_i32, [_i32, _p, _i64, _p, _i64, _p, _i32, _p, _i32, _i32, _p, _i64, _p, _i64, _i64, _i64,
+                                       _i64, _p]),
     "sfb_slope_workspace": (_i64, [_i64, _i64]),
     "sfb_slope": (_i32, [_i32, _i32, _p, _i64, _p, _i64, _i64, _i64, _p, _i32, _p, _p, _p, _i64, _p, _i32, _p, _p]),
     "sfb_tensor_grad_x": (_i32, [_i32, _p, _i64, _p, _i64, _p, _i32, _p, _i64, _i64, _i64, _i64, _p]),
@@ -424,6 +426,15 @@ def tensor_linear(dtype, x, ldx, codes, ldw, scale, bits, bias, bias_dtype, act,
                   K, stream) -> None:
     check(load().sfb_tensor_linear(dtype, x, ldx, codes, ldw, scale, bits, bias, bias_dtype, act, residual, ldr, y,
                                    ldy, z, ldz, M, N, K, stream), "sf tensor linear")
+
+
+SMALL_ROWS = 64                            # SFB_SMALL_ROWS
+
+
+def tensor_linear_small(dtype, x, ldx, codes, ldc, scale, bits, bias, bias_dtype, act, residual, ldr, y, ldy, M, N, K,
+                        stream) -> None:
+    check(load().sfb_tensor_linear_small(dtype, x, ldx, codes, ldc, scale, bits, bias, bias_dtype, act, residual, ldr,
+                                         y, ldy, M, N, K, stream), "sf tensor linear (few rows)")
 
 
 def slope_workspace(M, N) -> int:

@@ -81,13 +81,31 @@ __global__ void __launch_bounds__(QT) code_kernel(const W *__restrict__ w, int64
 
 // --- packed codes in the activations' type -----------------------------------------------------------
 
+// A thread turns 16 codes of a row at a time; where rows do not start on 16
+// bytes it loads them one by one (the stores are aligned: the rows of `out` are).
 template <typename O>
-__global__ void __launch_bounds__(QT) expand_kernel(const int8_t *__restrict__ codes, int64_t K, int64_t ldc,
-                                                    O *__restrict__ out, int64_t ldo) {
-    const int8_t *row = codes + (int64_t)blockIdx.y * ldc;
-    O *to = out + (int64_t)blockIdx.y * ldo;
-    for (int64_t k = (int64_t)blockIdx.x * QT + threadIdx.x; k < K; k += (int64_t)gridDim.x * QT)
-        to[k] = from_f<O>((float)row[k]);
+__global__ void __launch_bounds__(QT) expand_kernel(const int8_t *__restrict__ codes, int64_t N, int64_t K, int64_t ldc,
+                                                    O *__restrict__ out, int64_t ldo, bool vec) {
+    const int64_t per = (K + 15) / 16, total = N * per;
+    for (int64_t i = (int64_t)blockIdx.x * QT + threadIdx.x; i < total; i += (int64_t)gridDim.x * QT) {
+        const int64_t n = i / per, k = (i - n * per) * 16;
+        const int8_t *from = codes + n * ldc + k;
+        O *to = out + n * ldo + k;
+        Vec<int8_t, 16> q;
+        if (vec && k + 16 <= K) {
+            q = *reinterpret_cast<const Vec<int8_t, 16> *>(from);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++) q.v[j] = k + j < K ? from[j] : (int8_t)0;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            Vec<O, 8> r;
+#pragma unroll
+            for (int j = 0; j < 8; j++) r.v[j] = from_f<O>((float)q.v[8 * h + j]);
+            if (k + 8 * h < K) *reinterpret_cast<Vec<O, 8> *>(to + 8 * h) = r;   // a row's padding may be written
+        }
+    }
 }
 
 // --- the gradient of the pre-activation --------------------------------------------------------------
@@ -236,15 +254,16 @@ extern "C" int sfb_code_expand(const int8_t *codes, int64_t N, int64_t K, int64_
     if (N < 0 || K < 0 || ldc < K || ldo < K) return set_error(SFB_EINVAL, "sfb_code_expand: bad shape");
     if (N == 0 || K == 0) return SFB_OK;
     if (!codes || !out) return set_error(SFB_EINVAL, "sfb_code_expand: null pointer");
+    if ((reinterpret_cast<uintptr_t>(out) & 15) || ldo % 8)
+        return set_error(SFB_EINVAL, "sfb_code_expand: the rows of the result must be aligned to 16 bytes");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const unsigned gx = (unsigned)std::min<int64_t>((K + QT - 1) / QT, 64);
-    for (int64_t n = 0; n < N; n += 65535) {
-        const dim3 grid(gx, (unsigned)std::min<int64_t>(N - n, 65535));
-        if (dtype == SFB_BF16)
-            expand_kernel<<<grid, QT, 0, st>>>(codes + n * ldc, K, ldc, static_cast<__nv_bfloat16 *>(out) + n * ldo, ldo);
-        else
-            expand_kernel<<<grid, QT, 0, st>>>(codes + n * ldc, K, ldc, static_cast<__half *>(out) + n * ldo, ldo);
-    }
+    const int64_t total = N * ((K + 15) / 16);
+    const unsigned grid = (unsigned)std::min<int64_t>((total + QT - 1) / QT, 16ll * sm_count());
+    const bool vec = ldc % 16 == 0 && (reinterpret_cast<uintptr_t>(codes) & 15) == 0;
+    if (dtype == SFB_BF16)
+        expand_kernel<<<grid, QT, 0, st>>>(codes, N, K, ldc, static_cast<__nv_bfloat16 *>(out), ldo, vec);
+    else
+        expand_kernel<<<grid, QT, 0, st>>>(codes, N, K, ldc, static_cast<__half *>(out), ldo, vec);
     return check_launch("sfb_code_expand");
 }
 

@@ -1,0 +1,233 @@
+// The forward product for few rows, straight from the packed codes.
+//
+//   y = act((x code^T) s[n] 2^-(bits-1) + b[n]) + r,  at most 64 rows
+//
+// Bound by the codes' bytes: each is read once, and turned into the activations'
+// type in registers (exact: a code has at most 7 bits).  The products go to the
+// warps' matrix instruction with the CODES as its 16-row operand and x as its
+// 8-column one, so one row of x wastes 7 of 8 columns of a pipe that is idle
+// anyway, where a tile of 128 rows on tcgen05 would need the codes in 16 bits in
+// shared memory first.  The contraction index may be permuted freely as long as
+// both operands agree: a lane takes 16 consecutive codes of a row with one load
+// and the same 16 elements of x, and four steps of 16 use four of each.
+// A CTA of 8 warps covers 8 / ks groups of 16 channels; ks warps share a group,
+// each every ks-th segment of 64, and their sums are added in a fixed order.
+#include <algorithm>
+
+#include "sfb_tensor.cuh"
+
+namespace sfb {
+namespace {
+
+constexpr int WARPS = 8, SEG = 64;
+
+// four codes as two pairs of the activations' type
+template <typename T> __device__ __forceinline__ void widen(uint32_t w, uint32_t &lo, uint32_t &hi);
+
+// 0x43cc as bf16 is 128 + (c mod 128), or twice that form's 128 where bit 7 is set: the
+// difference of the two is c in two's complement, exactly
+template <>
+__device__ __forceinline__ void widen<__nv_bfloat16>(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    const uint32_t a = __byte_perm(w, 0x43434343u, 0x4140), b = __byte_perm(w, 0x43434343u, 0x4342);
+    const uint32_t a0 = a & 0xFF7FFF7Fu, a1 = a & 0xFF80FF80u, b0 = b & 0xFF7FFF7Fu, b1 = b & 0xFF80FF80u;
+    __nv_bfloat162 x = __hsub2(reinterpret_cast<const __nv_bfloat162 &>(a0), reinterpret_cast<const __nv_bfloat162 &>(a1));
+    __nv_bfloat162 y = __hsub2(reinterpret_cast<const __nv_bfloat162 &>(b0), reinterpret_cast<const __nv_bfloat162 &>(b1));
+    lo = reinterpret_cast<uint32_t &>(x);
+    hi = reinterpret_cast<uint32_t &>(y);
+}
+
+// 0x64uu as fp16 is 1024 + u; with u = c + 128 less 1152 it is c
+template <>
+__device__ __forceinline__ void widen<__half>(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    w ^= 0x80808080u;
+    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 c = __half2half2(__ushort_as_half((unsigned short)0x6480));
+    __half2 x = __hsub2(reinterpret_cast<const __half2 &>(a), c), y = __hsub2(reinterpret_cast<const __half2 &>(b), c);
+    lo = reinterpret_cast<uint32_t &>(x);
+    hi = reinterpret_cast<uint32_t &>(y);
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                      uint32_t b1) {
+    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16 codes of a row from k on, those at or past K as 0
+template <bool ALIGNED>
+__device__ __forceinline__ uint4 load_codes(const int8_t *row, int64_t k, int64_t K) {
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (k >= K) return make_uint4(0, 0, 0, 0);
+    if constexpr (ALIGNED) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4 *>(row + k));
+        if (k + 16 <= K) return q;
+        w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+    } else {
+        // whole words around the row's bytes, each holding at least one of the row's codes, shifted into place
+        const uintptr_t at = reinterpret_cast<uintptr_t>(row + k), end = reinterpret_cast<uintptr_t>(row + K);
+        const uint32_t *from = reinterpret_cast<const uint32_t *>(at & ~(uintptr_t)3);
+        const uint32_t shift = 8 * (uint32_t)(at & 3);
+        uint32_t a = __ldg(from);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t b = reinterpret_cast<uintptr_t>(from + i + 1) < end ? __ldg(from + i + 1) : 0u;
+            w[i] = __funnelshift_r(a, b, shift);
+            a = b;
+        }
+        if (k + 16 <= K) return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    const int left = (int)(K - k);                   // 1 .. 15 codes are the row's
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int keep = left - 4 * i;
+        w[i] &= keep >= 4 ? 0xFFFFFFFFu : keep <= 0 ? 0u : (1u << (8 * keep)) - 1u;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// 16 elements of a row of x from k on, those at or past K as 0; rows start on 16 bytes
+template <typename T>
+__device__ __forceinline__ void load_x(const T *row, int64_t k, int64_t K, uint32_t (&x)[8]) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        uint4 q = make_uint4(0, 0, 0, 0);
+        const int64_t at = k + 8 * h;
+        if (at < K) {
+            q = __ldg(reinterpret_cast<const uint4 *>(row + at));
+            if (at + 8 > K) {
+                uint32_t w[4] = {q.x, q.y, q.z, q.w};
+                const int left = (int)(K - at);
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] &= left >= 2 * i + 2 ? 0xFFFFFFFFu : left == 2 * i + 1 ? 0xFFFFu : 0u;
+                q = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+        x[4 * h] = q.x, x[4 * h + 1] = q.y, x[4 * h + 2] = q.z, x[4 * h + 3] = q.w;
+    }
+}
+
+struct Small {
+    const void *x;
+    const int8_t *codes;
+    const float *scale;
+    const void *bias, *residual;
+    void *y;
+    int64_t ldx, ldc, ldr, ldy, N, K;
+    float unit;
+    int M, ks, bias_dtype;
+};
+
+template <typename T, int MT, bool ALIGNED, int ACT>
+__global__ void __launch_bounds__(32 * WARPS) small_kernel(Small p) {
+    __shared__ float s_sum[WARPS][16][8 * MT];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int groups = WARPS / p.ks, group = warp / p.ks, part = warp % p.ks;
+    const int64_t n0 = ((int64_t)blockIdx.x * groups + group) * 16;
+    // channels past the last read the last one's codes; their sums are not stored
+    const int8_t *row0 = p.codes + min(n0 + g, p.N - 1) * p.ldc, *row1 = p.codes + min(n0 + g + 8, p.N - 1) * p.ldc;
+    const T *x = static_cast<const T *>(p.x);
+    float d[MT][4] = {};
+    const int64_t segs = (p.K + SEG - 1) / SEG;
+    if (n0 < p.N) {
+#pragma unroll(MT == 1 ? 4 : MT == 2 ? 2 : 1)
+        for (int64_t s = part; s < segs; s += p.ks) {
+            const int64_t k = s * SEG + t * 16;
+            const uint4 c0 = load_codes<ALIGNED>(row0, k, p.K), c1 = load_codes<ALIGNED>(row1, k, p.K);
+            uint32_t b[MT][8];
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+                const int m = i * 8 + g;
+                if (m < p.M) {
+                    load_x(x + m * p.ldx, k, p.K, b[i]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) b[i][j] = 0;
+                }
+            }
+            const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t a0, a1, a2, a3;
+                widen<T>(w0[j], a0, a2);
+                widen<T>(w1[j], a1, a3);
+#pragma unroll
+                for (int i = 0; i < MT; i++) mma16<T>(d[i], a0, a1, a2, a3, b[i][2 * j], b[i][2 * j + 1]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        s_sum[warp][g][i * 8 + 2 * t] = d[i][0];
+        s_sum[warp][g][i * 8 + 2 * t + 1] = d[i][1];
+        s_sum[warp][g + 8][i * 8 + 2 * t] = d[i][2];
+        s_sum[warp][g + 8][i * 8 + 2 * t + 1] = d[i][3];
+    }
+    __syncthreads();
+    for (int o = threadIdx.x; o < groups * 16 * p.M; o += 32 * WARPS) {
+        const int c = o % (groups * 16), m = o / (groups * 16);
+        const int64_t n = (int64_t)blockIdx.x * groups * 16 + c;
+        if (n >= p.N) continue;
+        float v = 0.0f;
+        for (int i = 0; i < p.ks; i++) v += s_sum[(c / 16) * p.ks + i][c % 16][m];
+        v = fmaf(v, p.scale[n] * p.unit, p.bias ? load_as(p.bias, n, p.bias_dtype) : 0.0f);
+        v = activate<ACT>(v);
+        if (p.residual) v += to_f(static_cast<const T *>(p.residual)[m * p.ldr + n]);
+        static_cast<T *>(p.y)[m * p.ldy + n] = from_f<T>(v);
+    }
+}
+
+template <typename T, int MT, bool ALIGNED>
+int launch(const Small &p, int act, cudaStream_t st) {
+    const int64_t groups = (p.N + 15) / 16;
+    const int per = WARPS / p.ks;
+    const unsigned grid = (unsigned)((groups + per - 1) / per);
+    return with_activation(act, [&](auto a) {
+        small_kernel<T, MT, ALIGNED, decltype(a)::value><<<grid, 32 * WARPS, 0, st>>>(p);
+        return check_launch("sfb_tensor_linear_small");
+    });
+}
+
+template <typename T>
+int by_rows(const Small &p, int act, cudaStream_t st) {
+    const bool al = p.ldc % 16 == 0 && (reinterpret_cast<uintptr_t>(p.codes) & 15) == 0;
+    if (p.M <= 8) return al ? launch<T, 1, true>(p, act, st) : launch<T, 1, false>(p, act, st);
+    if (p.M <= 16) return al ? launch<T, 2, true>(p, act, st) : launch<T, 2, false>(p, act, st);
+    if (p.M <= 32) return al ? launch<T, 4, true>(p, act, st) : launch<T, 4, false>(p, act, st);
+    return al ? launch<T, 8, true>(p, act, st) : launch<T, 8, false>(p, act, st);
+}
+
+}  // namespace
+}  // namespace sfb
+
+extern "C" int sfb_tensor_linear_small(int dtype, const void *x, int64_t ldx, const int8_t *codes, int64_t ldc,
+                                       const float *scale, int bits, const void *bias, int bias_dtype, int act,
+                                       const void *residual, int64_t ldr, void *y, int64_t ldy, int64_t M, int64_t N,
+                                       int64_t K, sfb_stream stream) {
+    using namespace sfb;
+    if (dtype != SFB_BF16 && dtype != SFB_F16) return set_error(SFB_EINVAL, "sfb_tensor_linear_small: element type %d", dtype);
+    if (bits < 4 || bits > 8) return set_error(SFB_EINVAL, "sfb_tensor_linear_small: width %d is not in 4..8", bits);
+    if (M < 0 || N < 0 || K < 1 || ldx < K || ldc < K || ldy < N || (residual && ldr < N))
+        return set_error(SFB_EINVAL, "sfb_tensor_linear_small: bad shape");
+    if (M > SFB_SMALL_ROWS) return set_error(SFB_ERANGE, "sfb_tensor_linear_small: %lld rows", (long long)M);
+    if (N >= (1ll << 34)) return set_error(SFB_ERANGE, "sfb_tensor_linear_small: %lld channels", (long long)N);
+    if (bias && bias_dtype != SFB_F32 && bias_dtype != SFB_BF16 && bias_dtype != SFB_F16)
+        return set_error(SFB_EINVAL, "sfb_tensor_linear_small: bias type %d", bias_dtype);
+    if (M == 0 || N == 0) return SFB_OK;
+    if (!x || !codes || !scale || !y) return set_error(SFB_EINVAL, "sfb_tensor_linear_small: null pointer");
+    if ((reinterpret_cast<uintptr_t>(x) & 15) || ldx % 8)
+        return set_error(SFB_EINVAL, "sfb_tensor_linear_small: x and its rows must be aligned to 16 bytes");
+    Small p{x, codes, scale, bias, residual, y, ldx, ldc, ldr, ldy, N, K, 1.0f / (float)(1 << (bits - 1)), (int)M, 8,
+            bias_dtype};
+    // warps that share a group of channels: as many as fill the SMs, each with two segments at least
+    const int64_t groups = (N + 15) / 16, segs = (K + SEG - 1) / SEG;
+    while (p.ks > 1 && (segs < 2 * p.ks || groups * p.ks > 32ll * sm_count())) p.ks /= 2;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return dtype == SFB_BF16 ? by_rows<__nv_bfloat16>(p, act, st) : by_rows<__half>(p, act, st);
+}

@@ -287,16 +287,27 @@ def tensor_linear(x: torch.Tensor, weight, bias=None, *, activation: str | None 
 
 
 def _no_grad(x, weight, packed, bias, residual, bits, wscale, act):
+    N, K = weight.shape
     with _lib.on_device(x.get_device()) as d:
-        N = weight.shape[0]
-        xa = _operand(x.detach().reshape(-1, x.shape[-1]))
+        xa = _operand(x.detach().reshape(-1, K))
+        M = xa.shape[0]
+        small = M <= _lib.SMALL_ROWS
         if packed is None:
-            codes, scale = _quantize(weight.detach(), bits, wscale, x.dtype, d.stream)
+            codes, scale = _quantize(weight.detach(), bits, wscale, None if small else x.dtype, d.stream)
+        elif small:
+            codes, scale = _rows(packed.codes), packed.scale.contiguous()
         else:
             codes, scale = _expand(packed, x.dtype, d.stream), packed.scale.contiguous()
         r = None if residual is None else _rows(residual.detach().reshape(-1, N))
         b = None if bias is None else bias.detach().contiguous()
-        y, _ = _forward(xa, codes, scale, bits, b, act, r, False, d.stream)
+        if small:
+            y = torch.empty(M, N, dtype=x.dtype, device=x.device)
+            _lib.tensor_linear_small(_TYPES[x.dtype], xa.data_ptr(), max(xa.stride(0), _up8(K)), codes.data_ptr(),
+                                     max(codes.stride(0), K), scale.data_ptr(), bits, _ptr(b),
+                                     0 if b is None else _FLOATS[b.dtype], act, _ptr(r),
+                                     0 if r is None else max(r.stride(0), N), y.data_ptr(), N, M, N, K, d.stream)
+        else:
+            y, _ = _forward(xa, codes, scale, bits, b, act, r, False, d.stream)
     return y.view(*x.shape[:-1], N)
 
 
