@@ -8,11 +8,16 @@
 // operands of the forward product are exact; the sums are held in float32 in
 // TMEM and rounded once, when they are stored.
 //
-// One CTA per SM walks output tiles of 128 x BN.  Warp 0 lane 0 issues the TMA
-// loads (64 elements of the contraction a stage, 128-byte swizzle), warp 1 lane
-// 0 the MMAs, warps 2..9 read the accumulator out of TMEM, two warps to each
-// group of 32 lanes, each half of the columns.  Two accumulators (2 BN TMEM
-// columns) let a tile's epilogue run under the next tile's products.
+// One CTA per SM walks output tiles; warp 0 lane 0 issues the TMA loads (64
+// elements of the contraction a stage, 128-byte swizzle), warp 1 lane 0 the MMAs,
+// warps 2..9 read the accumulator out of TMEM, two warps to each group of 32
+// lanes, each half of the columns.  Two accumulators (2 BN TMEM columns) let a
+// tile's epilogue run under the next tile's products.
+// CTAS = 2: a pair of SMs shares a tile of 256 x BN.  Each holds 128 rows of A,
+// half of B's columns and the sums of its own rows; the first one's thread issues
+// the products of both (cta_group::2).  B crosses into shared memory once for
+// the pair, which a single SM's tile of 128 x 256 has to load and read twice.
+// CTAS = 1: tiles of 128 x BN, for problems with too few tiles for the pairs.
 // An operand whose contraction index is contiguous in memory is loaded K-major
 // (rows of 64); one whose row index is contiguous MN-major (64 rows wide, 64
 // deep), so that no operand of the backward products is transposed beforehand.
@@ -37,7 +42,7 @@ namespace {
 constexpr int BM = 128, BK = 64, THREADS = 320, EPI_WARPS = 8;
 constexpr unsigned kSpinLimit = 1u << 26;     // polls of one wait, some seconds
 constexpr int SMEM_OPERANDS = 196608;         // of the stages
-constexpr int GROUP_M = 8;                    // row tiles that sweep the columns together, for L2
+constexpr int GROUP_ROWS = 1024;              // rows that sweep the columns together, for L2
 
 __device__ unsigned long long g_failures;
 
@@ -57,13 +62,44 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// one lane of the warp, the same each time.  The warps that issue copies and
+// products run their loops as a whole and only the issue is one lane's: descriptors
+// and addresses then stay in uniform registers.  With the loops inside `if
+// (threadIdx.x == 32)` a stage of 4 products took 750 cycles to issue, whatever
+// their size (timestamps around the issue; 128 x 128 and 256 x 256 tiles alike).
+__device__ __forceinline__ bool elected() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+
+// the same barrier of the pair's first CTA
+__device__ __forceinline__ uint32_t of_leader(uint32_t bar) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(bar));
+    return r;
+}
+
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // false once `limit` polls have not seen the phase of this parity end
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, unsigned limit) {
     for (unsigned i = 0; i < limit; i++) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(ok)
             : "r"(bar), "r"(parity)
@@ -73,8 +109,22 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, unsigne
     return false;
 }
 
+// the same wait by all lanes of a warp, with one answer
+__device__ __forceinline__ bool all_wait(uint32_t bar, uint32_t parity, unsigned limit) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, limit));
+}
+
+// into this CTA's shared memory; the barrier is the pair's first CTA's with CTAS = 2
+template <int CTAS>
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
-    asm volatile(
+    if constexpr (CTAS == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
+            "{%2, %3}], [%4];" ::"r"(dst),
+            "l"(map), "r"(c0), "r"(c1), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
         "[%4];" ::"r"(dst),
         "l"(map), "r"(c0), "r"(c1), "r"(bar)
@@ -103,25 +153,51 @@ template <typename T> struct Kind;
 template <> struct Kind<__half> { static constexpr uint32_t id = 0; };
 template <> struct Kind<__nv_bfloat16> { static constexpr uint32_t id = 1; };
 
-// kind::f16: float32 accumulator, both operands of type T, M = 128, N = BN
-template <typename T, bool A_MN, bool B_MN, int BN>
+// kind::f16: float32 accumulator, both operands of type T, M = 128 CTAS, N = BN
+template <typename T, bool A_MN, bool B_MN, int BN, int CTAS>
 __host__ __device__ constexpr uint32_t instruction() {
     return (1u << 4) | (Kind<T>::id << 7) | (Kind<T>::id << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) |
-           ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+           ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(CTAS * BM >> 4) << 24);
 }
 
+template <int CTAS>
 __device__ __forceinline__ void mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                     uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
+    if constexpr (CTAS == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
 }
 
+// arrives on this CTA's barrier once the products issued so far are done
+template <int CTAS>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    if constexpr (CTAS == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// on that barrier of both CTAs of a pair
+template <int CTAS>
+__device__ __forceinline__ void mma_commit_all(uint32_t bar) {
+    if constexpr (CTAS == 2)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        mma_commit<1>(bar);
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
@@ -212,33 +288,37 @@ struct Tiles {
     int mt, nt, total;
 };
 
+template <int CTAS>
 __device__ __forceinline__ void tile_of(const Tiles &t, int i, int &tm, int &tn) {
+    constexpr int GROUP_M = GROUP_ROWS / (CTAS * BM);
     const int gsize = GROUP_M * t.nt, g = i / gsize, m0 = g * GROUP_M;
     const int gm = min(GROUP_M, t.mt - m0), r = i - g * gsize;
     tm = m0 + r % gm;
     tn = r / gm;
 }
 
-template <int BN>
+template <int BN, int CTAS>
 struct Shape {
-    static constexpr int A = BM * BK * 2, B = BN * BK * 2, STAGE = A + B, STAGES = SMEM_OPERANDS / STAGE;
+    static constexpr int BNL = BN / CTAS;                            // columns of B that a CTA loads
+    static constexpr int A = BM * BK * 2, B = BNL * BK * 2, STAGE = A + B, STAGES = SMEM_OPERANDS / STAGE;
     static constexpr int COLS = 2 * BN;                              // TMEM columns
     static constexpr int FACTORS = EPI_WARPS * 2 * (BN / 2) * 4;     // each warp's scales and biases
     static constexpr int SMEM = STAGES * STAGE + FACTORS + 512 + 1024;
 };
 
-template <typename T, bool A_MN, bool B_MN, int BN, int ACT>
+template <typename T, bool A_MN, bool B_MN, int BN, int CTAS, int ACT>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, int nkb, int64_t M,
             int64_t N, Tiles tiles, const __grid_constant__ Epilogue e, unsigned spin, int stall) {
-    using S = Shape<BN>;
+    using S = Shape<BN, CTAS>;
     constexpr int STAGES = S::STAGES;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     float *factors = reinterpret_cast<float *>(smem + STAGES * S::STAGE);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + STAGES * S::STAGE + S::FACTORS);
     // full [0, S), empty [S, 2 S), accumulator full 2 S + {0, 1}, accumulator empty 2 S + {2, 3}, all done 2 S + 4,
-    // and one that nothing arrives on (the tests' stall)
+    // and one that nothing arrives on (the tests' stall).  Of a pair, the first CTA's full, accumulator empty and
+    // done barriers serve both; each has its own empty and accumulator full ones.
     auto full = [&](int s) { return smem_u32(&bars[s]); };
     auto empty = [&](int s) { return smem_u32(&bars[STAGES + s]); };
     auto acc_full = [&](int a) { return smem_u32(&bars[2 * STAGES + a]); };
@@ -248,7 +328,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     __shared__ int s_fail;
     volatile int *failed = &s_fail;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
     if (threadIdx.x == 0) {
         s_fail = 0;
         for (int s = 0; s < STAGES; s++) {
@@ -257,94 +338,115 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         }
         for (int a = 0; a < 2; a++) {
             mbar_init(acc_full(a), 1);
-            mbar_init(acc_empty(a), EPI_WARPS);
+            mbar_init(acc_empty(a), CTAS * EPI_WARPS);
         }
         mbar_init(done, 1);
         mbar_init(never, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "n"(S::COLS)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (CTAS == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                         "n"(S::COLS)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                         "n"(S::COLS)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (CTAS == 2) cluster_sync();           // the barriers of both are set
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
     int issued = 0;
-    if (threadIdx.x == 0) {
-        for (int t = blockIdx.x; t < tiles.total && !*failed; t += gridDim.x) {
+    if (warp == 0) {
+        for (int t = first; t < tiles.total; t += step) {
             int tm, tn;
-            tile_of(tiles, t, tm, tn);
+            tile_of<CTAS>(tiles, t, tm, tn);
+            const int m0 = (tm * CTAS + rank) * BM, n0 = tn * BN + rank * S::BNL;
             for (int kb = 0; kb < nkb; kb++, issued++) {
                 const int s = issued % STAGES, round = issued / STAGES;
-                if (round > 0 && !mbar_wait(empty(s), (round - 1) & 1, spin)) {
+                if (round > 0 && !all_wait(empty(s), (round - 1) & 1, spin)) {
                     *failed = 1;
                     break;
                 }
-                if (*failed) break;
+                if (__any_sync(0xffffffffu, *failed)) break;
                 const uint32_t a = smem_u32(smem + s * S::STAGE), b = a + S::A;
-                mbar_expect_tx(full(s), S::STAGE);
-                if constexpr (A_MN) {
+                const uint32_t bar = CTAS == 2 ? of_leader(full(s)) : full(s);
+                if (elected()) {
+                    if (rank == 0) mbar_expect_tx(full(s), CTAS * S::STAGE);
+                    if constexpr (A_MN) {
 #pragma unroll
-                    for (int i = 0; i < BM / 64; i++) tma_load_2d(a + i * 8192, &tmA, tm * BM + i * 64, kb * BK, full(s));
-                } else {
-                    tma_load_2d(a, &tmA, kb * BK, tm * BM, full(s));
-                }
-                if constexpr (B_MN) {
+                        for (int i = 0; i < BM / 64; i++) tma_load_2d<CTAS>(a + i * 8192, &tmA, m0 + i * 64, kb * BK, bar);
+                    } else {
+                        tma_load_2d<CTAS>(a, &tmA, kb * BK, m0, bar);
+                    }
+                    if constexpr (B_MN) {
 #pragma unroll
-                    for (int i = 0; i < BN / 64; i++) tma_load_2d(b + i * 8192, &tmB, tn * BN + i * 64, kb * BK, full(s));
-                } else {
-                    tma_load_2d(b, &tmB, kb * BK, tn * BN, full(s));
+                        for (int i = 0; i < S::BNL / 64; i++)
+                            tma_load_2d<CTAS>(b + i * 8192, &tmB, n0 + i * 64, kb * BK, bar);
+                    } else {
+                        tma_load_2d<CTAS>(b, &tmB, kb * BK, n0, bar);
+                    }
                 }
+                __syncwarp();
             }
-            if (*failed) break;
+            if (__any_sync(0xffffffffu, *failed)) break;
         }
-    } else if (threadIdx.x == 32) {
-        constexpr uint32_t id = instruction<T, A_MN, B_MN, BN>();
-        bool ok = !(stall && !mbar_wait(never, 0, spin));
+    } else if (warp == 1 && rank == 0) {
+        constexpr uint32_t id = instruction<T, A_MN, B_MN, BN, CTAS>();
+        bool ok = !(stall && !all_wait(never, 0, spin));
         int it = 0, i = 0;
-        for (int t = blockIdx.x; t < tiles.total && ok; t += gridDim.x, i++) {
+        for (int t = first; t < tiles.total && ok; t += step, i++) {
             const int acc = i & 1;
-            if (i >= 2 && !mbar_wait(acc_empty(acc), ((i >> 1) - 1) & 1, spin)) {
+            if (i >= 2 && !all_wait(acc_empty(acc), ((i >> 1) - 1) & 1, spin)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
             for (int kb = 0; kb < nkb; kb++, it++) {
                 const int s = it % STAGES;
-                if (!mbar_wait(full(s), (it / STAGES) & 1, spin) || *failed) {
+                if (!all_wait(full(s), (it / STAGES) & 1, spin) || __any_sync(0xffffffffu, *failed)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
                 const uint32_t a = smem_u32(smem + s * S::STAGE), b = a + S::A;
+                if (elected()) {
 #pragma unroll
-                for (int kk = 0; kk < BK / 16; kk++)
-                    mma(tmem + acc * BN, smem_desc<A_MN>(a + kk * (A_MN ? 2048 : 32)),
-                        smem_desc<B_MN>(b + kk * (B_MN ? 2048 : 32)), id, kb == 0 && kk == 0 ? 0u : 1u);
-                mma_commit(empty(s));
+                    for (int kk = 0; kk < BK / 16; kk++)
+                        mma<CTAS>(tmem + acc * BN, smem_desc<A_MN>(a + kk * (A_MN ? 2048 : 32)),
+                                  smem_desc<B_MN>(b + kk * (B_MN ? 2048 : 32)), id, kb == 0 && kk == 0 ? 0u : 1u);
+                    mma_commit_all<CTAS>(empty(s));
+                }
+                __syncwarp();
             }
-            if (ok) mma_commit(acc_full(acc));
+            if (ok && elected()) mma_commit_all<CTAS>(acc_full(acc));
+            __syncwarp();
         }
-        if (!ok) {
-            *failed = 1;
-            mma_commit(acc_full(0));         // release the epilogue: it sees that the CTA failed
-            mma_commit(acc_full(1));
+        if (!ok) *failed = 1;
+        if (elected()) {
+            if (!ok) {
+                // release this CTA's epilogue, which sees that the CTA failed; the other CTA's waits run out by themselves
+                mma_commit<CTAS>(acc_full(0));
+                mma_commit<CTAS>(acc_full(1));
+            }
+            mma_commit<CTAS>(done);
         }
-        mma_commit(done);
     } else if (warp >= 2) {
         const int half = (warp - 2) >> 2, quad = warp & 3;        // a warp reaches the TMEM lanes 32 (warp % 4) ..
         const uint32_t lanes = (uint32_t)(32 * quad) << 16;
         float *scale = factors + (warp - 2) * BN, *bias = scale + BN / 2;
         const float alpha = e.alpha ? *e.alpha * e.unit : e.unit;
         int i = 0;
-        for (int t = blockIdx.x; t < tiles.total; t += gridDim.x, i++) {
+        for (int t = first; t < tiles.total; t += step, i++) {
             int tm, tn;
-            tile_of(tiles, t, tm, tn);
+            tile_of<CTAS>(tiles, t, tm, tn);
             const int acc = i & 1;
             const int64_t n0 = (int64_t)tn * BN + half * (BN / 2);
             __syncwarp();
@@ -352,11 +454,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 scale[c] = n0 + c < N && e.scale ? e.scale[n0 + c] * alpha : alpha;
                 bias[c] = n0 + c < N && e.bias ? load_as(e.bias, n0 + c, e.bias_dtype) : 0.0f;
             }
-            bool fine = !*failed && mbar_wait(acc_full(acc), (i >> 1) & 1, spin) && !*failed;
-            fine = __all_sync(0xffffffffu, fine);        // TMEM loads are the whole warp's
+            // one lane polls: 256 of them would crowd the copies' and products' issue out of the memory pipe
+            int fine = 0;
+            if (lane == 0) fine = !*failed && mbar_wait(acc_full(acc), (i >> 1) & 1, spin) && !*failed;
+            fine = __shfl_sync(0xffffffffu, fine, 0);    // TMEM loads are the whole warp's
             if (!fine) *failed = 1;
             tc_fence_after();
-            const int64_t m = (int64_t)tm * BM + quad * 32 + lane;
+            const int64_t m = (int64_t)(tm * CTAS + rank) * BM + quad * 32 + lane;
             for (int c = 0; c < BN / 2; c += 32) {
                 if (n0 + c >= N) break;
                 float v[32];
@@ -377,7 +481,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty(acc));
+            if (lane == 0) {
+                if constexpr (CTAS == 2) mbar_arrive_cluster(of_leader(acc_empty(acc)));
+                else mbar_arrive(acc_empty(acc));
+            }
         }
     }
     __syncwarp();
@@ -385,17 +492,25 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     __syncthreads();
     if (s_fail && threadIdx.x == 0) {
         atomicAdd(&g_failures, 1ull);
-        // this CTA's copies land before its shared memory is released, its products (the commit on `done`
-        // follows them) end before its TMEM is freed: full-length waits, whatever `spin` was
-        for (int it = issued > STAGES ? issued - STAGES : 0; it < issued; it++)
-            (void)mbar_wait(full(it % STAGES), (it / STAGES) & 1, kSpinLimit);
-        (void)mbar_wait(done, 0, kSpinLimit);
+        // the copies land before their shared memory is released (a pair's complete on the first CTA's barriers; the
+        // other CTA waits for it below), the products (the commit on `done` follows them) end before TMEM is freed:
+        // full-length waits, whatever `spin` was
+        if (rank == 0) {
+            for (int it = issued > STAGES ? issued - STAGES : 0; it < issued; it++)
+                (void)mbar_wait(full(it % STAGES), (it / STAGES) & 1, kSpinLimit);
+            (void)mbar_wait(done, 0, kSpinLimit);
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (CTAS == 2) cluster_sync();           // neither leaves while the other's copies or arrivals may come
     tc_fence_after();
-    if (warp == 0)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::COLS) : "memory");
+    if (warp == 0) {
+        if constexpr (CTAS == 2)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::COLS) : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::COLS) : "memory");
+    }
 }
 
 // --- launches ------------------------------------------------------------------------------------------------
@@ -439,10 +554,10 @@ struct Problem {
     int dtype;
 };
 
-template <typename T, bool A_MN, bool B_MN, int BN, int ACT>
+template <typename T, bool A_MN, bool B_MN, int BN, int CTAS, int ACT>
 int launch(const Problem &p, const Epilogue &e, cudaStream_t st) {
-    using S = Shape<BN>;
-    auto *kernel = gemm_kernel<T, A_MN, B_MN, BN, ACT>;
+    using S = Shape<BN, CTAS>;
+    auto *kernel = gemm_kernel<T, A_MN, B_MN, BN, CTAS, ACT>;
     static std::mutex lock;
     static unsigned long long ready[64] = {};          // the CUDA context whose attribute is set, per device
     int dev = 0;
@@ -460,31 +575,36 @@ int launch(const Problem &p, const Epilogue &e, cudaStream_t st) {
     CUtensorMap tmA, tmB;
     int rc = A_MN ? make_map(&tmA, p.A, p.dtype, p.K, p.M, p.lda, BK) : make_map(&tmA, p.A, p.dtype, p.M, p.K, p.lda, BM);
     if (rc) return rc;
-    rc = B_MN ? make_map(&tmB, p.B, p.dtype, p.K, p.N, p.ldb, BK) : make_map(&tmB, p.B, p.dtype, p.N, p.K, p.ldb, BN);
+    rc = B_MN ? make_map(&tmB, p.B, p.dtype, p.K, p.N, p.ldb, BK) : make_map(&tmB, p.B, p.dtype, p.N, p.K, p.ldb, S::BNL);
     if (rc) return rc;
     Tiles t;
-    t.mt = (int)((p.M + BM - 1) / BM);
+    t.mt = (int)((p.M + CTAS * BM - 1) / (CTAS * BM));
     t.nt = (int)((p.N + BN - 1) / BN);
     t.total = t.mt * t.nt;
-    kernel<<<std::min(t.total, sm_count()), THREADS, S::SMEM, st>>>(
-        tmA, tmB, (int)((p.K + BK - 1) / BK), p.M, p.N, t, e, wait_polls() ? wait_polls() : kSpinLimit, wait_stall());
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute pair;
+    pair.id = cudaLaunchAttributeClusterDimension;
+    pair.val.clusterDim.x = CTAS;
+    pair.val.clusterDim.y = pair.val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(CTAS * std::min(t.total, sm_count() / CTAS)));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = st;
+    cfg.attrs = &pair;
+    cfg.numAttrs = CTAS > 1 ? 1 : 0;
+    const unsigned spin = wait_polls() ? wait_polls() : kSpinLimit;
+    if (cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, (int)((p.K + BK - 1) / BK), p.M, p.N, t, e, spin, wait_stall()) !=
+        cudaSuccess)
+        return check_launch("sf tensor linear");
     return check_launch("sf tensor linear");
 }
 
-// Columns of a tile: the fewest passes over the SMs weigh more than the larger
-// tile's better reuse, until its products are bound by the operands' loads.
-int columns(int64_t M, int64_t N) {
-    const int64_t mt = (M + BM - 1) / BM, sms = sm_count();
-    int best = 256;
-    double least = 0;
-    for (int bn : {256, 128}) {
-        const double cost = (double)((mt * ((N + bn - 1) / bn) + sms - 1) / sms) * (bn == 256 ? 256 : 150);
-        if (bn == 256 || cost < least) {
-            best = bn;
-            least = cost;
-        }
-    }
-    return best;
+// The tile: passes over the SMs times what a pass costs.  A pair's tile of 256 x
+// 256 keeps its two SMs as busy as 128 x 128 keeps one for 0.6 of that time.
+bool pairs(int64_t M, int64_t N) {
+    const int64_t sms = sm_count(), two = ((M + 255) / 256) * ((N + 255) / 256),
+                  one = ((M + BM - 1) / BM) * ((N + 127) / 128);
+    return (double)((two + sms / 2 - 1) / (sms / 2)) <= 0.6 * (double)((one + sms - 1) / sms);
 }
 
 int check(const Problem &p, const char *what) {
@@ -507,11 +627,11 @@ bool aligned16(const void *p, int64_t ld, int size) {
 
 template <bool A_MN, bool B_MN, int ACT>
 int launch_typed(const Problem &p, const Epilogue &e, cudaStream_t st) {
-    const bool wide = columns(p.M, p.N) == 256;
+    const bool two = pairs(p.M, p.N);
     if (p.dtype == SFB_BF16)
-        return wide ? launch<__nv_bfloat16, A_MN, B_MN, 256, ACT>(p, e, st)
-                    : launch<__nv_bfloat16, A_MN, B_MN, 128, ACT>(p, e, st);
-    return wide ? launch<__half, A_MN, B_MN, 256, ACT>(p, e, st) : launch<__half, A_MN, B_MN, 128, ACT>(p, e, st);
+        return two ? launch<__nv_bfloat16, A_MN, B_MN, 256, 2, ACT>(p, e, st)
+                   : launch<__nv_bfloat16, A_MN, B_MN, 128, 1, ACT>(p, e, st);
+    return two ? launch<__half, A_MN, B_MN, 256, 2, ACT>(p, e, st) : launch<__half, A_MN, B_MN, 128, 1, ACT>(p, e, st);
 }
 
 }  // namespace

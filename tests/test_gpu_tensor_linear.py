@@ -287,6 +287,25 @@ def test_training(gpu, m, n, k, dtype, wscale):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_large_products(gpu, dtype):
+    """Sizes at which tiles are shared by pairs of SMs in all three products, ragged in each direction."""
+    m, n, k = 4100, 4107, 4201
+    x = randn(m, k, seed=1, dtype=dtype).requires_grad_()
+    w = randn(n, k, seed=2, std=k ** -0.5, dtype=dtype).requires_grad_()
+    b = randn(n, seed=3, std=0.3).requires_grad_()
+    r, dy = randn(m, n, seed=4, dtype=dtype), randn(m, n, seed=5, dtype=dtype)
+    codes, s = codes64(w, 8, "per_channel")
+    want, tol, _, _ = forward64(x, codes, s, 8, b, "gelu", r)
+    y = sft.tensor_linear(x, w, b, activation="gelu", residual=r)
+    close(y.detach(), want, tol, dtype)
+    y.backward(dy)
+    gx, gw, gb = backward64(x, codes, s, 8, b, "gelu", dy, dtype, w.dtype, None)
+    close_grad(x.grad, gx, dtype)
+    close_grad(w.grad, gw, dtype)
+    close_grad(b.grad, gb, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_packed_weight_passes_gradients_to_the_rest(gpu, dtype):
     x = randn(33, 40, dtype=dtype).requires_grad_()
     p = sft.pack_weight(randn(24, 40, seed=2, std=0.2))
@@ -475,11 +494,12 @@ def test_runs_repeat(gpu):
         assert all(torch.equal(a, c) for a, c in zip(first, step()))
 
 
-def test_a_wait_that_runs_out_leaves_nan(gpu):
+@pytest.mark.parametrize("m,n", [(300, 200), (4100, 4100)])        # one SM to a tile, and pairs
+def test_a_wait_that_runs_out_leaves_nan(gpu, m, n):
     """With every wait of the products bounded by 1000 polls and the first made on a barrier that nothing arrives
     on, the call returns, its outputs are NaN, the CTAs are counted, and the next call is whole."""
-    x = randn(300, 256, dtype=torch.bfloat16)
-    w = sft.pack_weight(randn(200, 256, seed=1, std=0.1))
+    x = randn(m, 256, dtype=torch.bfloat16)
+    w = sft.pack_weight(randn(n, 256, seed=1, std=0.1))
     want = sft.tensor_linear(x, w)
     before = sft.tensor_failures()
     try:
