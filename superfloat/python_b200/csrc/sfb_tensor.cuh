@@ -106,14 +106,19 @@ __device__ __forceinline__ float slope(float z) {
     }
 }
 
-// The pre-activation as the backward pass reads it: fp16 whatever the type of x
+// Two pre-activations as the backward pass reads them: fp16 whatever the type of x
 // (2^-12 of the value against bf16's 2^-9, at the same two bytes), held within
-// fp16's range, where every activation has long reached its asymptote; a positive
-// value never becomes 0, which relu's slope would tell from it.
-__device__ __forceinline__ __half kept(float z) {
-    const float c = z > 65504.0f ? 65504.0f : z < -65504.0f ? -65504.0f : z;
-    const __half h = __float2half_rn(c);
-    return z > 0.0f && __half2float(h) == 0.0f ? __ushort_as_half((unsigned short)1) : h;
+// fp16's range, where every activation has long reached its asymptote.  For relu a
+// positive value must not become 0, which its slope would tell from it.
+template <int ACT>
+__device__ __forceinline__ uint32_t kept2(float a, float b) {
+    if constexpr (ACT == SFB_ACT_RELU) {
+        a = a > 0.0f ? fmaxf(a, 0x1p-24f) : a;
+        b = b > 0.0f ? fmaxf(b, 0x1p-24f) : b;
+    }
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
 }
 
 // runs f with the activation as a compile-time constant

@@ -8,16 +8,22 @@
 // operands of the forward product are exact; the sums are held in float32 in
 // TMEM and rounded once, when they are stored.
 //
-// One CTA per SM walks output tiles; warp 0 lane 0 issues the TMA loads (64
-// elements of the contraction a stage, 128-byte swizzle), warp 1 lane 0 the MMAs,
-// warps 2..9 read the accumulator out of TMEM, two warps to each group of 32
-// lanes, each half of the columns.  Two accumulators (2 BN TMEM columns) let a
-// tile's epilogue run under the next tile's products.
-// CTAS = 2: a pair of SMs shares a tile of 256 x BN.  Each holds 128 rows of A,
-// half of B's columns and the sums of its own rows; the first one's thread issues
-// the products of both (cta_group::2).  B crosses into shared memory once for
-// the pair, which a single SM's tile of 128 x 256 has to load and read twice.
-// CTAS = 1: tiles of 128 x BN, for problems with too few tiles for the pairs.
+// A pair of SMs (a cluster of two CTAs) shares an output tile of 256 x BN: each
+// holds 128 rows of A, half of B's columns and the sums of its own rows, and the
+// first one's warp 1 issues the products of both (cta_group::2).  Products read
+// their operands from shared memory at the rate at which copies write them, and
+// that is what bounds a smaller tile: 256 x 256 of bf16 moves 64 KB an SM and
+// stage of 64 against 512 cycles of products, at the 128 bytes a cycle that it
+// has; 128 x 128 on one SM needs 64 KB for 256 cycles (577 were measured).
+// Warp 0 issues the TMA loads (64 elements of the contraction a stage, 128-byte
+// swizzle), warps 2..9 are the epilogue, two to each group of 32 rows, each half
+// of the columns.  Two accumulators (2 BN TMEM columns) let a tile's epilogue run
+// under the next tile's products.
+// The epilogue takes 32 columns at a time through a box of 32 rows in shared
+// memory, loaded (residual) and stored (y, z) by TMA: a lane has a row, and 16-byte
+// accesses of 32 rows cost 32 lines each (a tile's took 9500 cycles, two thirds of
+// them on stores, where K = 768 gives its products 6100).  Rows that TMA cannot
+// address (odd sizes, odd offsets) pass through the same box, element by element.
 // An operand whose contraction index is contiguous in memory is loaded K-major
 // (rows of 64); one whose row index is contiguous MN-major (64 rows wide, 64
 // deep), so that no operand of the backward products is transposed beforehand.
@@ -41,8 +47,9 @@ namespace {
 
 constexpr int BM = 128, BK = 64, THREADS = 320, EPI_WARPS = 8;
 constexpr unsigned kSpinLimit = 1u << 26;     // polls of one wait, some seconds
-constexpr int SMEM_OPERANDS = 196608;         // of the stages
-constexpr int GROUP_ROWS = 1024;              // rows that sweep the columns together, for L2
+constexpr int SMEM_OPERANDS = 172032;         // of the stages: what hides a copy's 1500 cycles or so under load
+constexpr int SMEM_BOXES = EPI_WARPS * 4096;  // of the epilogue
+constexpr int GROUP_M = 4;                    // row tiles that sweep the columns together, for L2
 
 __device__ unsigned long long g_failures;
 
@@ -56,10 +63,6 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // one lane of the warp, the same each time.  The warps that issue copies and
@@ -85,7 +88,7 @@ __device__ __forceinline__ uint32_t of_leader(uint32_t bar) {
 }
 
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ void cluster_sync() {
@@ -114,22 +117,35 @@ __device__ __forceinline__ bool all_wait(uint32_t bar, uint32_t parity, unsigned
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, limit));
 }
 
-// into this CTA's shared memory; the barrier is the pair's first CTA's with CTAS = 2
-template <int CTAS>
+// an operand's box into this CTA's shared memory; the barrier is the pair's first CTA's
+__device__ __forceinline__ void tma_load_operand(uint32_t dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
+        "{%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
-    if constexpr (CTAS == 2)
-        asm volatile(
-            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
-            "{%2, %3}], [%4];" ::"r"(dst),
-            "l"(map), "r"(c0), "r"(c1), "r"(bar)
-            : "memory");
-    else
-        asm volatile(
+    asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
         "[%4];" ::"r"(dst),
         "l"(map), "r"(c0), "r"(c1), "r"(bar)
         : "memory");
 }
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, int c0, int c1, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(c0),
+                 "r"(c1), "r"(src)
+                 : "memory");
+}
+
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// all but the last N groups of this thread's stores have read their shared memory
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -153,51 +169,34 @@ template <typename T> struct Kind;
 template <> struct Kind<__half> { static constexpr uint32_t id = 0; };
 template <> struct Kind<__nv_bfloat16> { static constexpr uint32_t id = 1; };
 
-// kind::f16: float32 accumulator, both operands of type T, M = 128 CTAS, N = BN
-template <typename T, bool A_MN, bool B_MN, int BN, int CTAS>
+// kind::f16: float32 accumulator, both operands of type T, M = 256, N = BN
+template <typename T, bool A_MN, bool B_MN, int BN>
 __host__ __device__ constexpr uint32_t instruction() {
     return (1u << 4) | (Kind<T>::id << 7) | (Kind<T>::id << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) |
-           ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(CTAS * BM >> 4) << 24);
+           ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(2 * BM >> 4) << 24);
 }
 
-template <int CTAS>
 __device__ __forceinline__ void mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                     uint32_t accumulate) {
-    if constexpr (CTAS == 2)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-            : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "setp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-            : "memory");
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
 }
 
 // arrives on this CTA's barrier once the products issued so far are done
-template <int CTAS>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-    if constexpr (CTAS == 2)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-    else
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// on that barrier of both CTAs of a pair
-template <int CTAS>
-__device__ __forceinline__ void mma_commit_all(uint32_t bar) {
-    if constexpr (CTAS == 2)
-        asm volatile(
-            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-            "h"((uint16_t)3)
-            : "memory");
-    else
-        mma_commit<1>(bar);
+// on that barrier of both CTAs of the pair
+__device__ __forceinline__ void mma_commit_both(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
@@ -227,109 +226,100 @@ struct Epilogue {
     float unit;                  // 2^-(bits-1) where a scale or alpha stands for codes, else 1
     int bias_dtype, y_dtype;
     int64_t ldr, ldz, ldy;
-    bool vec;                    // rows of y, r and z are aligned to 16 bytes
+    bool r_tma, z_tma, y_tma;    // rows on 16-byte boundaries
 };
 
-template <typename Y>
-__device__ __forceinline__ void put8(Y *to, const float *v) {
-    Vec<Y, 8> q;
-#pragma unroll
-    for (int j = 0; j < 8; j++) q.v[j] = from_f<Y>(v[j]);
-    *reinterpret_cast<Vec<Y, 8> *>(to) = q;
+// A box is 32 rows of 32 columns, swizzled as TMA reads and writes it: 16-byte
+// pieces of a row change places with (row / 2) mod 4 where it has 64 bytes, with
+// row mod 8 where it has 128, so that 8 lanes' pieces fall into distinct banks.
+template <typename E>
+__device__ __forceinline__ uint32_t box_at(int row, int piece) {
+    return sizeof(E) == 4 ? row * 128 + ((piece ^ (row & 7)) << 4) : row * 64 + ((piece ^ ((row >> 1) & 3)) << 4);
 }
 
-// 8 columns n .. n + 7 of one row
-template <typename T, int ACT>
-__device__ __forceinline__ void finish8(const Epilogue &e, float (&v)[8], const float *scale, const float *bias,
-                                        int64_t m, int64_t n, int64_t N) {
+// 32 values of a lane's row
+template <typename E>
+__device__ __forceinline__ void box_put(uint8_t *box, int row, const float (&v)[32]) {
+    constexpr int P = 16 / sizeof(E);
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = fmaf(v[j], scale[j], bias[j]);
-    const bool vec = e.vec && n + 8 <= N;
-    if (e.z) {
-        __half *to = e.z + m * e.ldz + n;
-        if (vec) {
-            Vec<__half, 8> q;
+    for (int i = 0; i < 32 / P; i++) {
+        Vec<E, P> q;
 #pragma unroll
-            for (int j = 0; j < 8; j++) q.v[j] = kept(v[j]);
-            *reinterpret_cast<Vec<__half, 8> *>(to) = q;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (n + j < N) to[j] = kept(v[j]);
-        }
+        for (int j = 0; j < P; j++) q.v[j] = from_f<E>(v[i * P + j]);
+        *reinterpret_cast<Vec<E, P> *>(box + box_at<E>(row, i)) = q;
     }
-#pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = activate<ACT>(v[j]);
-    if (e.residual) {
-        const T *from = static_cast<const T *>(e.residual) + m * e.ldr + n;
-        if (vec) {
-            const Vec<T, 8> q = *reinterpret_cast<const Vec<T, 8> *>(from);
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] += to_f(q.v[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (n + j < N) v[j] += to_f(from[j]);
-        }
-    }
-    const int64_t at = m * e.ldy + n;
-    if (vec) {
-        if (e.y_dtype == SFB_F32) put8(static_cast<float *>(e.y) + at, v);
-        else if (e.y_dtype == SFB_BF16) put8(static_cast<__nv_bfloat16 *>(e.y) + at, v);
-        else put8(static_cast<__half *>(e.y) + at, v);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (n + j < N) store_as(e.y, at + j, e.y_dtype, v[j]);
-    }
+}
+
+// a box element by element: a row at a time, a column a lane
+template <typename E>
+__device__ __forceinline__ void box_store(const uint8_t *box, E *to, int64_t ld, int64_t m0, int64_t n, int64_t M,
+                                          int64_t N, int lane) {
+    constexpr int P = 16 / sizeof(E);
+    const int rows = (int)min((int64_t)32, M - m0);
+    if (n + lane < N)
+        for (int r = 0; r < rows; r++)
+            to[(m0 + r) * ld + n + lane] =
+                *reinterpret_cast<const E *>(box + box_at<E>(r, lane / P) + (lane % P) * sizeof(E));
+}
+
+template <typename E>
+__device__ __forceinline__ void box_load(uint8_t *box, const E *from, int64_t ld, int64_t m0, int64_t n, int64_t M,
+                                         int64_t N, int lane) {
+    constexpr int P = 16 / sizeof(E);
+    const int rows = (int)min((int64_t)32, M - m0);
+    if (n + lane < N)
+#pragma unroll 8
+        for (int r = 0; r < rows; r++)
+            *reinterpret_cast<E *>(box + box_at<E>(r, lane / P) + (lane % P) * sizeof(E)) = from[(m0 + r) * ld + n + lane];
 }
 
 struct Tiles {
     int mt, nt, total;
 };
 
-template <int CTAS>
 __device__ __forceinline__ void tile_of(const Tiles &t, int i, int &tm, int &tn) {
-    constexpr int GROUP_M = GROUP_ROWS / (CTAS * BM);
     const int gsize = GROUP_M * t.nt, g = i / gsize, m0 = g * GROUP_M;
     const int gm = min(GROUP_M, t.mt - m0), r = i - g * gsize;
     tm = m0 + r % gm;
     tn = r / gm;
 }
 
-template <int BN, int CTAS>
+template <int BN>
 struct Shape {
-    static constexpr int BNL = BN / CTAS;                            // columns of B that a CTA loads
+    static constexpr int BNL = BN / 2;                               // columns of B that a CTA loads
     static constexpr int A = BM * BK * 2, B = BNL * BK * 2, STAGE = A + B, STAGES = SMEM_OPERANDS / STAGE;
     static constexpr int COLS = 2 * BN;                              // TMEM columns
     static constexpr int FACTORS = EPI_WARPS * 2 * (BN / 2) * 4;     // each warp's scales and biases
-    static constexpr int SMEM = STAGES * STAGE + FACTORS + 512 + 1024;
+    static constexpr int SMEM = STAGES * STAGE + SMEM_BOXES + FACTORS + 512 + 1024;
 };
 
-template <typename T, bool A_MN, bool B_MN, int BN, int CTAS, int ACT>
-__global__ void __launch_bounds__(THREADS, 1)
-gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, int nkb, int64_t M,
-            int64_t N, Tiles tiles, const __grid_constant__ Epilogue e, unsigned spin, int stall) {
-    using S = Shape<BN, CTAS>;
+template <typename T, bool A_MN, bool B_MN, int BN, int ACT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+            const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmR,
+            const __grid_constant__ CUtensorMap tmZ, int nkb, int64_t M, int64_t N, Tiles tiles,
+            const __grid_constant__ Epilogue e, unsigned spin, int stall) {
+    using S = Shape<BN>;
     constexpr int STAGES = S::STAGES;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    float *factors = reinterpret_cast<float *>(smem + STAGES * S::STAGE);
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + STAGES * S::STAGE + S::FACTORS);
+    uint8_t *boxes = smem + STAGES * S::STAGE;
+    float *factors = reinterpret_cast<float *>(boxes + SMEM_BOXES);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(boxes + SMEM_BOXES + S::FACTORS);
     // full [0, S), empty [S, 2 S), accumulator full 2 S + {0, 1}, accumulator empty 2 S + {2, 3}, all done 2 S + 4,
-    // and one that nothing arrives on (the tests' stall).  Of a pair, the first CTA's full, accumulator empty and
-    // done barriers serve both; each has its own empty and accumulator full ones.
+    // one that nothing arrives on (the tests' stall), the epilogue warps' residual boxes from 2 S + 6.  The first
+    // CTA's full, accumulator empty and done barriers serve both; each has its own empty and accumulator full ones.
     auto full = [&](int s) { return smem_u32(&bars[s]); };
     auto empty = [&](int s) { return smem_u32(&bars[STAGES + s]); };
     auto acc_full = [&](int a) { return smem_u32(&bars[2 * STAGES + a]); };
     auto acc_empty = [&](int a) { return smem_u32(&bars[2 * STAGES + 2 + a]); };
     const uint32_t done = smem_u32(&bars[2 * STAGES + 4]), never = smem_u32(&bars[2 * STAGES + 5]);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 6);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 6 + 2 * EPI_WARPS);
     __shared__ int s_fail;
     volatile int *failed = &s_fail;
 
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-    const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0, first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
+    const int rank = (int)(blockIdx.x & 1), first = blockIdx.x / 2, step = gridDim.x / 2;
     if (threadIdx.x == 0) {
         s_fail = 0;
         for (int s = 0; s < STAGES; s++) {
@@ -338,28 +328,20 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         }
         for (int a = 0; a < 2; a++) {
             mbar_init(acc_full(a), 1);
-            mbar_init(acc_empty(a), CTAS * EPI_WARPS);
+            mbar_init(acc_empty(a), 2 * EPI_WARPS);
         }
-        mbar_init(done, 1);
-        mbar_init(never, 1);
+        for (int i = 4; i < 6 + 2 * EPI_WARPS; i++) mbar_init(smem_u32(&bars[2 * STAGES + i]), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
-        if constexpr (CTAS == 2) {
-            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                         "n"(S::COLS)
-                         : "memory");
-            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-        } else {
-            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                         "n"(S::COLS)
-                         : "memory");
-            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-        }
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "n"(S::COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
-    if constexpr (CTAS == 2) cluster_sync();           // the barriers of both are set
+    cluster_sync();                                    // the barriers of both are set
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
@@ -367,8 +349,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     if (warp == 0) {
         for (int t = first; t < tiles.total; t += step) {
             int tm, tn;
-            tile_of<CTAS>(tiles, t, tm, tn);
-            const int m0 = (tm * CTAS + rank) * BM, n0 = tn * BN + rank * S::BNL;
+            tile_of(tiles, t, tm, tn);
+            const int m0 = (tm * 2 + rank) * BM, n0 = tn * BN + rank * S::BNL;
             for (int kb = 0; kb < nkb; kb++, issued++) {
                 const int s = issued % STAGES, round = issued / STAGES;
                 if (round > 0 && !all_wait(empty(s), (round - 1) & 1, spin)) {
@@ -376,22 +358,21 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     break;
                 }
                 if (__any_sync(0xffffffffu, *failed)) break;
-                const uint32_t a = smem_u32(smem + s * S::STAGE), b = a + S::A;
-                const uint32_t bar = CTAS == 2 ? of_leader(full(s)) : full(s);
+                const uint32_t a = smem_u32(smem + s * S::STAGE), b = a + S::A, bar = of_leader(full(s));
                 if (elected()) {
-                    if (rank == 0) mbar_expect_tx(full(s), CTAS * S::STAGE);
+                    if (rank == 0) mbar_expect_tx(full(s), 2 * S::STAGE);
                     if constexpr (A_MN) {
 #pragma unroll
-                        for (int i = 0; i < BM / 64; i++) tma_load_2d<CTAS>(a + i * 8192, &tmA, m0 + i * 64, kb * BK, bar);
+                        for (int i = 0; i < BM / 64; i++) tma_load_operand(a + i * 8192, &tmA, m0 + i * 64, kb * BK, bar);
                     } else {
-                        tma_load_2d<CTAS>(a, &tmA, kb * BK, m0, bar);
+                        tma_load_operand(a, &tmA, kb * BK, m0, bar);
                     }
                     if constexpr (B_MN) {
 #pragma unroll
                         for (int i = 0; i < S::BNL / 64; i++)
-                            tma_load_2d<CTAS>(b + i * 8192, &tmB, n0 + i * 64, kb * BK, bar);
+                            tma_load_operand(b + i * 8192, &tmB, n0 + i * 64, kb * BK, bar);
                     } else {
-                        tma_load_2d<CTAS>(b, &tmB, kb * BK, n0, bar);
+                        tma_load_operand(b, &tmB, kb * BK, n0, bar);
                     }
                 }
                 __syncwarp();
@@ -399,7 +380,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             if (__any_sync(0xffffffffu, *failed)) break;
         }
     } else if (warp == 1 && rank == 0) {
-        constexpr uint32_t id = instruction<T, A_MN, B_MN, BN, CTAS>();
+        constexpr uint32_t id = instruction<T, A_MN, B_MN, BN>();
         bool ok = !(stall && !all_wait(never, 0, spin));
         int it = 0, i = 0;
         for (int t = first; t < tiles.total && ok; t += step, i++) {
@@ -420,80 +401,164 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 if (elected()) {
 #pragma unroll
                     for (int kk = 0; kk < BK / 16; kk++)
-                        mma<CTAS>(tmem + acc * BN, smem_desc<A_MN>(a + kk * (A_MN ? 2048 : 32)),
-                                  smem_desc<B_MN>(b + kk * (B_MN ? 2048 : 32)), id, kb == 0 && kk == 0 ? 0u : 1u);
-                    mma_commit_all<CTAS>(empty(s));
+                        mma(tmem + acc * BN, smem_desc<A_MN>(a + kk * (A_MN ? 2048 : 32)),
+                            smem_desc<B_MN>(b + kk * (B_MN ? 2048 : 32)), id, kb == 0 && kk == 0 ? 0u : 1u);
+                    mma_commit_both(empty(s));
                 }
                 __syncwarp();
             }
-            if (ok && elected()) mma_commit_all<CTAS>(acc_full(acc));
+            if (ok && elected()) mma_commit_both(acc_full(acc));
             __syncwarp();
         }
         if (!ok) *failed = 1;
         if (elected()) {
             if (!ok) {
                 // release this CTA's epilogue, which sees that the CTA failed; the other CTA's waits run out by themselves
-                mma_commit<CTAS>(acc_full(0));
-                mma_commit<CTAS>(acc_full(1));
+                mma_commit(acc_full(0));
+                mma_commit(acc_full(1));
             }
-            mma_commit<CTAS>(done);
+            mma_commit(done);
         }
     } else if (warp >= 2) {
-        const int half = (warp - 2) >> 2, quad = warp & 3;        // a warp reaches the TMEM lanes 32 (warp % 4) ..
+        const int w = warp - 2, half = w >> 2, quad = warp & 3;   // a warp reaches the TMEM lanes 32 (warp % 4) ..
         const uint32_t lanes = (uint32_t)(32 * quad) << 16;
-        float *scale = factors + (warp - 2) * BN, *bias = scale + BN / 2;
+        float *scale = factors + w * BN, *bias = scale + BN / 2;
+        // Two boxes of 16-bit elements: y's in turn, the residual coming in where y goes out; or z's and y's, or one of
+        // float32.  Only y's in turn let a box be filled while TMA reads the other.
+        uint8_t *box = boxes + w * 4096;
+        const bool turns = !e.z && e.y_dtype != SFB_F32;
+        auto loaded = [&](int k) { return smem_u32(&bars[2 * STAGES + 6 + 2 * w + k]); };
         const float alpha = e.alpha ? *e.alpha * e.unit : e.unit;
-        int i = 0;
+        const bool wide = e.y_dtype == SFB_F32;
+        const T *res = static_cast<const T *>(e.residual);
+        int i = 0, q = 0;                             // tiles, boxes so far
         for (int t = first; t < tiles.total; t += step, i++) {
             int tm, tn;
-            tile_of<CTAS>(tiles, t, tm, tn);
+            tile_of(tiles, t, tm, tn);
             const int acc = i & 1;
             const int64_t n0 = (int64_t)tn * BN + half * (BN / 2);
+            const int64_t m0 = (int64_t)(tm * 2 + rank) * BM + quad * 32;
+            const int count = m0 < M && n0 < N ? (int)min((int64_t)(BN / 64), (N - n0 + 31) / 32) : 0;
+            const int q0 = q;
+            // the residual's box c into its buffer, once the stores before have read it
+            auto fetch = [&](int c) {
+                const int k = turns ? (q0 + c) & 1 : 1;
+                uint8_t *to = box + k * 2048;
+                proxy_fence();
+                if (elected()) bulk_wait_read<0>();
+                __syncwarp();
+                if (e.r_tma) {
+                    if (elected()) {
+                        mbar_expect_tx(loaded(k), 2048);
+                        tma_load_2d(smem_u32(to), &tmR, (int)n0 + 32 * c, (int)m0, loaded(k));
+                    }
+                } else {
+                    box_load(to, res, e.ldr, m0, n0 + 32 * c, M, N, lane);
+                }
+            };
+            if (res && count) fetch(0);
             __syncwarp();
             for (int c = lane; c < BN / 2; c += 32) {
                 scale[c] = n0 + c < N && e.scale ? e.scale[n0 + c] * alpha : alpha;
                 bias[c] = n0 + c < N && e.bias ? load_as(e.bias, n0 + c, e.bias_dtype) : 0.0f;
             }
-            // one lane polls: 256 of them would crowd the copies' and products' issue out of the memory pipe
             int fine = 0;
             if (lane == 0) fine = !*failed && mbar_wait(acc_full(acc), (i >> 1) & 1, spin) && !*failed;
             fine = __shfl_sync(0xffffffffu, fine, 0);    // TMEM loads are the whole warp's
             if (!fine) *failed = 1;
             tc_fence_after();
-            const int64_t m = (int64_t)(tm * CTAS + rank) * BM + quad * 32 + lane;
-            for (int c = 0; c < BN / 2; c += 32) {
-                if (n0 + c >= N) break;
+            for (int c = 0; c < count; c++) {
                 float v[32];
                 if (fine) {
-                    tmem_ld32(tmem + lanes + acc * BN + half * (BN / 2) + c, v);
+                    tmem_ld32(tmem + lanes + acc * BN + half * (BN / 2) + 32 * c, v);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 32; j++) v[j] = __int_as_float(0x7FC00000);
                 }
-                if (m < M) {
-#pragma unroll
-                    for (int j = 0; j < 32; j += 8)
-                        if (n0 + c + j < N)
-                            finish8<T, ACT>(e, *reinterpret_cast<float(*)[8]>(v + j), scale + c + j, bias + c + j, m,
-                                            n0 + c + j, N);
+                if (c + 1 == count) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(of_leader(acc_empty(acc)));
                 }
+                if (res && turns && c + 1 < count) {
+                    fetch(c + 1);
+                } else if (res && !turns && c > 0) {
+                    fetch(c);
+                } else {
+                    if (elected()) {
+                        if (turns) bulk_wait_read<1>();
+                        else bulk_wait_read<0>();
+                    }
+                    __syncwarp();
+                }
+                uint8_t *yb = box + (turns ? (q & 1) * 2048 : e.z ? 2048 : 0), *zb = box;
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                    const float4 s4 = *reinterpret_cast<const float4 *>(scale + 32 * c + j);
+                    const float4 b4 = *reinterpret_cast<const float4 *>(bias + 32 * c + j);
+                    v[j] = fmaf(v[j], s4.x, b4.x);
+                    v[j + 1] = fmaf(v[j + 1], s4.y, b4.y);
+                    v[j + 2] = fmaf(v[j + 2], s4.z, b4.z);
+                    v[j + 3] = fmaf(v[j + 3], s4.w, b4.w);
+                }
+                if (e.z) {
+#pragma unroll
+                    for (int p = 0; p < 4; p++) {
+                        uint4 h;
+                        h.x = kept2<ACT>(v[8 * p], v[8 * p + 1]);
+                        h.y = kept2<ACT>(v[8 * p + 2], v[8 * p + 3]);
+                        h.z = kept2<ACT>(v[8 * p + 4], v[8 * p + 5]);
+                        h.w = kept2<ACT>(v[8 * p + 6], v[8 * p + 7]);
+                        *reinterpret_cast<uint4 *>(zb + box_at<__half>(lane, p)) = h;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 32; j++) v[j] = activate<ACT>(v[j]);
+                if (res) {
+                    if (e.r_tma) (void)mbar_wait(loaded(turns ? q & 1 : 1), (turns ? q >> 1 : q) & 1, kSpinLimit);
+                    __syncwarp();
+#pragma unroll
+                    for (int p = 0; p < 4; p++) {
+                        const Vec<T, 8> r = *reinterpret_cast<const Vec<T, 8> *>(yb + box_at<T>(lane, p));
+#pragma unroll
+                        for (int j = 0; j < 8; j++) v[8 * p + j] += to_f(r.v[j]);
+                    }
+                }
+                if (wide) box_put<float>(yb, lane, v);
+                else if (e.y_dtype == SFB_BF16) box_put<__nv_bfloat16>(yb, lane, v);
+                else box_put<__half>(yb, lane, v);
+                proxy_fence();
                 __syncwarp();
+                const int64_t n = n0 + 32 * c;
+                if (elected()) {
+                    if (e.y_tma) tma_store_2d(&tmY, (int)n, (int)m0, smem_u32(yb));
+                    if (e.z && e.z_tma) tma_store_2d(&tmZ, (int)n, (int)m0, smem_u32(zb));
+                    bulk_commit();
+                }
+                if (!e.y_tma) {
+                    if (wide) box_store(yb, static_cast<float *>(e.y), e.ldy, m0, n, M, N, lane);
+                    else if (e.y_dtype == SFB_BF16) box_store(yb, static_cast<__nv_bfloat16 *>(e.y), e.ldy, m0, n, M, N, lane);
+                    else box_store(yb, static_cast<__half *>(e.y), e.ldy, m0, n, M, N, lane);
+                }
+                if (e.z && !e.z_tma) box_store(zb, e.z, e.ldz, m0, n, M, N, lane);
+                __syncwarp();
+                q++;
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if constexpr (CTAS == 2) mbar_arrive_cluster(of_leader(acc_empty(acc)));
-                else mbar_arrive(acc_empty(acc));
+            if (count == 0) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(of_leader(acc_empty(acc)));
             }
         }
+        if (elected()) bulk_wait_all();
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
     if (s_fail && threadIdx.x == 0) {
         atomicAdd(&g_failures, 1ull);
-        // the copies land before their shared memory is released (a pair's complete on the first CTA's barriers; the
-        // other CTA waits for it below), the products (the commit on `done` follows them) end before TMEM is freed:
+        // the copies land before their shared memory is released (both CTAs' complete on the first one's barriers; the
+        // other waits for it below), the products (the commit on `done` follows them) end before TMEM is freed:
         // full-length waits, whatever `spin` was
         if (rank == 0) {
             for (int it = issued > STAGES ? issued - STAGES : 0; it < issued; it++)
@@ -503,14 +568,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     }
     tc_fence_before();
     __syncthreads();
-    if constexpr (CTAS == 2) cluster_sync();           // neither leaves while the other's copies or arrivals may come
+    cluster_sync();                                    // neither leaves while the other's copies or arrivals may come
     tc_fence_after();
-    if (warp == 0) {
-        if constexpr (CTAS == 2)
-            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::COLS) : "memory");
-        else
-            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::COLS) : "memory");
-    }
+    if (warp == 0)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::COLS) : "memory");
 }
 
 // --- launches ------------------------------------------------------------------------------------------------
@@ -532,20 +593,26 @@ EncodeTiled encoder() {
     return fn;
 }
 
-// a matrix of `rows` lines of `cols` elements, ld apart, read in boxes of 64 columns
-int make_map(CUtensorMap *map, const void *base, int dtype, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+// a matrix of `rows` lines of `cols` elements of `size` bytes, ld apart, in boxes
+int make_map(CUtensorMap *map, const void *base, CUtensorMapDataType type, int size, CUtensorMapSwizzle swizzle,
+             int64_t rows, int64_t cols, int64_t ld, int box_cols, int box_rows) {
     EncodeTiled enc = encoder();
     if (!enc) return set_error(SFB_ECUDA, "sf tensor linear: cuTensorMapEncodeTiled is unavailable");
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld * size};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
     const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = enc(map, dtype == SFB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                           2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    const CUresult r = enc(map, type, 2, const_cast<void *>(base), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(SFB_ECUDA, "sf tensor linear: tensor map encoding failed (%d)", (int)r);
     return SFB_OK;
+}
+
+CUtensorMapDataType map_type(int dtype) {
+    return dtype == SFB_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+           : dtype == SFB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
 }
 
 struct Problem {
@@ -554,10 +621,25 @@ struct Problem {
     int dtype;
 };
 
-template <typename T, bool A_MN, bool B_MN, int BN, int CTAS, int ACT>
-int launch(const Problem &p, const Epilogue &e, cudaStream_t st) {
-    using S = Shape<BN, CTAS>;
-    auto *kernel = gemm_kernel<T, A_MN, B_MN, BN, CTAS, ACT>;
+// an operand in boxes of 64 columns
+int operand_map(CUtensorMap *map, const void *base, int dtype, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+    return make_map(map, base, map_type(dtype), 2, CU_TENSOR_MAP_SWIZZLE_128B, rows, cols, ld, 64, box_rows);
+}
+
+// an output or residual in boxes of 32 x 32
+int box_map(CUtensorMap *map, const void *base, int dtype, int64_t rows, int64_t cols, int64_t ld) {
+    return make_map(map, base, map_type(dtype), dtype == SFB_F32 ? 4 : 2,
+                    dtype == SFB_F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, rows, cols, ld, 32, 32);
+}
+
+bool aligned16(const void *p, int64_t ld, int size) {
+    return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * size) % 16 == 0;
+}
+
+template <typename T, bool A_MN, bool B_MN, int BN, int ACT>
+int launch(const Problem &p, Epilogue e, cudaStream_t st) {
+    using S = Shape<BN>;
+    auto *kernel = gemm_kernel<T, A_MN, B_MN, BN, ACT>;
     static std::mutex lock;
     static unsigned long long ready[64] = {};          // the CUDA context whose attribute is set, per device
     int dev = 0;
@@ -572,39 +654,35 @@ int launch(const Problem &p, const Epilogue &e, cudaStream_t st) {
             ready[dev] = context_id();
         }
     }
-    CUtensorMap tmA, tmB;
-    int rc = A_MN ? make_map(&tmA, p.A, p.dtype, p.K, p.M, p.lda, BK) : make_map(&tmA, p.A, p.dtype, p.M, p.K, p.lda, BM);
-    if (rc) return rc;
-    rc = B_MN ? make_map(&tmB, p.B, p.dtype, p.K, p.N, p.ldb, BK) : make_map(&tmB, p.B, p.dtype, p.N, p.K, p.ldb, S::BNL);
+    e.r_tma = aligned16(e.residual, e.ldr, 2);
+    e.z_tma = aligned16(e.z, e.ldz, 2);
+    e.y_tma = aligned16(e.y, e.ldy, e.y_dtype == SFB_F32 ? 4 : 2);
+    CUtensorMap tmA, tmB, tmY = {}, tmR = {}, tmZ = {};
+    int rc = A_MN ? operand_map(&tmA, p.A, p.dtype, p.K, p.M, p.lda, BK) : operand_map(&tmA, p.A, p.dtype, p.M, p.K, p.lda, BM);
+    if (!rc)
+        rc = B_MN ? operand_map(&tmB, p.B, p.dtype, p.K, p.N, p.ldb, BK)
+                  : operand_map(&tmB, p.B, p.dtype, p.N, p.K, p.ldb, S::BNL);
+    if (!rc && e.y_tma) rc = box_map(&tmY, e.y, e.y_dtype, p.M, p.N, e.ldy);
+    if (!rc && e.r_tma) rc = box_map(&tmR, e.residual, p.dtype, p.M, p.N, e.ldr);
+    if (!rc && e.z_tma) rc = box_map(&tmZ, e.z, SFB_F16, p.M, p.N, e.ldz);
     if (rc) return rc;
     Tiles t;
-    t.mt = (int)((p.M + CTAS * BM - 1) / (CTAS * BM));
+    t.mt = (int)((p.M + 2 * BM - 1) / (2 * BM));
     t.nt = (int)((p.N + BN - 1) / BN);
     t.total = t.mt * t.nt;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute pair;
-    pair.id = cudaLaunchAttributeClusterDimension;
-    pair.val.clusterDim.x = CTAS;
-    pair.val.clusterDim.y = pair.val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)(CTAS * std::min(t.total, sm_count() / CTAS)));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = S::SMEM;
-    cfg.stream = st;
-    cfg.attrs = &pair;
-    cfg.numAttrs = CTAS > 1 ? 1 : 0;
-    const unsigned spin = wait_polls() ? wait_polls() : kSpinLimit;
-    if (cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, (int)((p.K + BK - 1) / BK), p.M, p.N, t, e, spin, wait_stall()) !=
-        cudaSuccess)
-        return check_launch("sf tensor linear");
+    kernel<<<2 * std::min(t.total, sm_count() / 2), THREADS, S::SMEM, st>>>(
+        tmA, tmB, tmY, tmR, tmZ, (int)((p.K + BK - 1) / BK), p.M, p.N, t, e, wait_polls() ? wait_polls() : kSpinLimit,
+        wait_stall());
     return check_launch("sf tensor linear");
 }
 
-// The tile: passes over the SMs times what a pass costs.  A pair's tile of 256 x
-// 256 keeps its two SMs as busy as 128 x 128 keeps one for 0.6 of that time.
-bool pairs(int64_t M, int64_t N) {
-    const int64_t sms = sm_count(), two = ((M + 255) / 256) * ((N + 255) / 256),
-                  one = ((M + BM - 1) / BM) * ((N + 127) / 128);
-    return (double)((two + sms / 2 - 1) / (sms / 2)) <= 0.6 * (double)((one + sms - 1) / sms);
+// Columns of a tile.  A stage of 256 columns takes its 512 cycles of products, one
+// of 128 about 390 (48 KB of shared memory's traffic against 256 cycles of products),
+// so the wider tile wins unless it leaves pairs without one.
+int columns(int64_t M, int64_t N) {
+    const int64_t mt = (M + 2 * BM - 1) / (2 * BM), n = sm_count() / 2;
+    const int64_t wide = (mt * ((N + 255) / 256) + n - 1) / n, narrow = (mt * ((N + 127) / 128) + n - 1) / n;
+    return 512 * wide <= 390 * narrow ? 256 : 128;
 }
 
 int check(const Problem &p, const char *what) {
@@ -621,17 +699,13 @@ int check(const Problem &p, const char *what) {
     return SFB_OK;
 }
 
-bool aligned16(const void *p, int64_t ld, int size) {
-    return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * size) % 16 == 0);
-}
-
 template <bool A_MN, bool B_MN, int ACT>
 int launch_typed(const Problem &p, const Epilogue &e, cudaStream_t st) {
-    const bool two = pairs(p.M, p.N);
+    const bool wide = columns(p.M, p.N) == 256;
     if (p.dtype == SFB_BF16)
-        return two ? launch<__nv_bfloat16, A_MN, B_MN, 256, 2, ACT>(p, e, st)
-                   : launch<__nv_bfloat16, A_MN, B_MN, 128, 1, ACT>(p, e, st);
-    return two ? launch<__half, A_MN, B_MN, 256, 2, ACT>(p, e, st) : launch<__half, A_MN, B_MN, 128, 1, ACT>(p, e, st);
+        return wide ? launch<__nv_bfloat16, A_MN, B_MN, 256, ACT>(p, e, st)
+                    : launch<__nv_bfloat16, A_MN, B_MN, 128, ACT>(p, e, st);
+    return wide ? launch<__half, A_MN, B_MN, 256, ACT>(p, e, st) : launch<__half, A_MN, B_MN, 128, ACT>(p, e, st);
 }
 
 }  // namespace
@@ -664,7 +738,6 @@ extern "C" int sfb_tensor_linear(int dtype, const void *x, int64_t ldx, const vo
     e.ldr = ldr;
     e.ldz = ldz;
     e.ldy = ldy;
-    e.vec = aligned16(y, ldy, 2) && aligned16(residual, ldr, 2) && aligned16(z, ldz, 2);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return with_activation(act, [&](auto a) { return launch_typed<false, false, decltype(a)::value>(p, e, st); });
 }
@@ -687,7 +760,6 @@ extern "C" int sfb_tensor_grad_x(int dtype, const void *dzs, int64_t ldd, const 
     e.unit = top ? 1.0f / (float)(1 << (bits - 1)) : 1.0f;
     e.y_dtype = dtype;
     e.ldy = ldy;
-    e.vec = aligned16(dx, ldy, 2);
     return launch_typed<false, true, SFB_ACT_NONE>(p, e, static_cast<cudaStream_t>(stream));
 }
 
@@ -708,7 +780,6 @@ extern "C" int sfb_tensor_grad_w(int dtype, const void *dz, int64_t ldd, const v
     e.unit = 1.0f;
     e.y_dtype = dw_dtype;
     e.ldy = ldy;
-    e.vec = aligned16(dw, ldy, dw_dtype == SFB_F32 ? 4 : 2);
     return launch_typed<true, true, SFB_ACT_NONE>(p, e, static_cast<cudaStream_t>(stream));
 }
 
