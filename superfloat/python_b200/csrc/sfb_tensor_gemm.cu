@@ -19,11 +19,12 @@
 // swizzle), warps 2..9 are the epilogue, two to each group of 32 rows, each half
 // of the columns.  Two accumulators (2 BN TMEM columns) let a tile's epilogue run
 // under the next tile's products.
-// The epilogue takes 32 columns at a time through a box of 32 rows in shared
-// memory, loaded (residual) and stored (y, z) by TMA: a lane has a row, and 16-byte
-// accesses of 32 rows cost 32 lines each (a tile's took 9500 cycles, two thirds of
-// them on stores, where K = 768 gives its products 6100).  Rows that TMA cannot
-// address (odd sizes, odd offsets) pass through the same box, element by element.
+// The epilogue has a row to a lane and 32 columns at a time, the next ones' TMEM
+// load and residual in flight.  It stores from registers, 32 bytes a lane: whole
+// sectors, and nothing to wait for.  (Through shared memory and TMA stores a warp
+// spent 550 of a box's 1400 cycles on fences and waits.)  Rows that do not start
+// on 16 bytes pass through a box of 32 x 32 in shared memory instead, so that a
+// row's elements are stored together.
 // An operand whose contraction index is contiguous in memory is loaded K-major
 // (rows of 64); one whose row index is contiguous MN-major (64 rows wide, 64
 // deep), so that no operand of the backward products is transposed beforehand.
@@ -47,8 +48,8 @@ namespace {
 
 constexpr int BM = 128, BK = 64, THREADS = 320, EPI_WARPS = 8;
 constexpr unsigned kSpinLimit = 1u << 26;     // polls of one wait, some seconds
-constexpr int SMEM_OPERANDS = 172032;         // of the stages: what hides a copy's 1500 cycles or so under load
-constexpr int SMEM_BOXES = EPI_WARPS * 4096;  // of the epilogue
+constexpr int SMEM_OPERANDS = 196608;         // of the stages: what hides a copy's 1500 cycles or so under load
+constexpr int SMEM_BOXES = EPI_WARPS * 2048;  // of the epilogue
 constexpr int GROUP_M = 4;                    // row tiles that sweep the columns together, for L2
 
 __device__ unsigned long long g_failures;
@@ -96,19 +97,22 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 // false once `limit` polls have not seen the phase of this parity end
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, unsigned limit) {
-    for (unsigned i = 0; i < limit; i++) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (ok) return true;
-    }
+    for (unsigned i = 0; i < limit; i++)
+        if (mbar_try(bar, parity)) return true;
     return false;
 }
 
@@ -125,27 +129,6 @@ __device__ __forceinline__ void tma_load_operand(uint32_t dst, const CUtensorMap
         "l"(map), "r"(c0), "r"(c1), "r"(bar)
         : "memory");
 }
-
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-        "[%4];" ::"r"(dst),
-        "l"(map), "r"(c0), "r"(c1), "r"(bar)
-        : "memory");
-}
-
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, int c0, int c1, uint32_t src) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(c0),
-                 "r"(c1), "r"(src)
-                 : "memory");
-}
-
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-// all but the last N groups of this thread's stores have read their shared memory
-template <int N>
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -199,8 +182,8 @@ __device__ __forceinline__ void mma_commit_both(uint32_t bar) {
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
-    uint32_t r[32];
+// 32 columns of this lane's row: in flight until tmem_landed
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
         "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -209,9 +192,28 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
           "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+
+// waits for the loads; the registers pass through, so that nothing reads them before
+__device__ __forceinline__ void tmem_landed(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                   "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
+// 32 bytes
+__device__ __forceinline__ void store32(void *to, const uint32_t (&w)[8], bool whole) {
+    if (whole) {
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                     "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                     : "memory");
+    } else {
+        static_cast<uint4 *>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        static_cast<uint4 *>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
 }
 
 // --- the epilogue --------------------------------------------------------------------------------------------
@@ -226,51 +228,115 @@ struct Epilogue {
     float unit;                  // 2^-(bits-1) where a scale or alpha stands for codes, else 1
     int bias_dtype, y_dtype;
     int64_t ldr, ldz, ldy;
-    bool r_tma, z_tma, y_tma;    // rows on 16-byte boundaries
+    bool direct;                 // rows of y, r and z start on 16 bytes
+    bool sectors;                // and those of y and z on 32
 };
 
-// A box is 32 rows of 32 columns, swizzled as TMA reads and writes it: 16-byte
-// pieces of a row change places with (row / 2) mod 4 where it has 64 bytes, with
-// row mod 8 where it has 128, so that 8 lanes' pieces fall into distinct banks.
-template <typename E>
-__device__ __forceinline__ uint32_t box_at(int row, int piece) {
-    return sizeof(E) == 4 ? row * 128 + ((piece ^ (row & 7)) << 4) : row * 64 + ((piece ^ ((row >> 1) & 3)) << 4);
+// two values in 16 bits each
+template <typename E> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return reinterpret_cast<uint32_t &>(h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    __half2 h = __floats2half2_rn(a, b);
+    return reinterpret_cast<uint32_t &>(h);
+}
+template <typename E> __device__ __forceinline__ void unpack2(uint32_t w, float &a, float &b);
+template <> __device__ __forceinline__ void unpack2<__nv_bfloat16>(uint32_t w, float &a, float &b) {
+    a = __uint_as_float(w << 16);
+    b = __uint_as_float(w & 0xFFFF0000u);
+}
+template <> __device__ __forceinline__ void unpack2<__half>(uint32_t w, float &a, float &b) {
+    const float2 f = __half22float2(reinterpret_cast<__half2 &>(w));
+    a = f.x;
+    b = f.y;
 }
 
-// 32 values of a lane's row
-template <typename E>
-__device__ __forceinline__ void box_put(uint8_t *box, int row, const float (&v)[32]) {
-    constexpr int P = 16 / sizeof(E);
+// 32 columns of one row, from 16 packed words: columns past `left` are not the matrix's
+__device__ __forceinline__ void row_store(uint16_t *to, const uint32_t (&w)[16], int left, bool sectors) {
 #pragma unroll
-    for (int i = 0; i < 32 / P; i++) {
-        Vec<E, P> q;
+    for (int i = 0; i < 2; i++) {
+        if (left >= 16 * i + 16) {
+            store32(to + 16 * i, *reinterpret_cast<const uint32_t(*)[8]>(w + 8 * i), sectors);
+        } else {
 #pragma unroll
-        for (int j = 0; j < P; j++) q.v[j] = from_f<E>(v[i * P + j]);
-        *reinterpret_cast<Vec<E, P> *>(box + box_at<E>(row, i)) = q;
+            for (int j = 0; j < 16; j++)
+                if (16 * i + j < left) to[16 * i + j] = (uint16_t)(w[8 * i + j / 2] >> (16 * (j & 1)));
+        }
     }
 }
 
-// a box element by element: a row at a time, a column a lane
-template <typename E>
-__device__ __forceinline__ void box_store(const uint8_t *box, E *to, int64_t ld, int64_t m0, int64_t n, int64_t M,
-                                          int64_t N, int lane) {
-    constexpr int P = 16 / sizeof(E);
-    const int rows = (int)min((int64_t)32, M - m0);
-    if (n + lane < N)
-        for (int r = 0; r < rows; r++)
-            to[(m0 + r) * ld + n + lane] =
-                *reinterpret_cast<const E *>(box + box_at<E>(r, lane / P) + (lane % P) * sizeof(E));
+__device__ __forceinline__ void row_store(float *to, const float (&v)[32], int left, bool sectors) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (left >= 8 * i + 8) {
+            store32(to + 8 * i, *reinterpret_cast<const uint32_t(*)[8]>(v + 8 * i), sectors);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (8 * i + j < left) to[8 * i + j] = v[8 * i + j];
+        }
+    }
 }
 
-template <typename E>
-__device__ __forceinline__ void box_load(uint8_t *box, const E *from, int64_t ld, int64_t m0, int64_t n, int64_t M,
-                                         int64_t N, int lane) {
-    constexpr int P = 16 / sizeof(E);
-    const int rows = (int)min((int64_t)32, M - m0);
-    if (n + lane < N)
+// 32 columns of one row into 16 packed words, the rows starting on 16 bytes
+__device__ __forceinline__ void row_load(const uint16_t *from, uint32_t (&w)[16], int left) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (left >= 8 * i + 8) {
+            q = __ldg(reinterpret_cast<const uint4 *>(from) + i);
+        } else {
+            uint32_t h[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (8 * i + j < left) h[j / 2] |= (uint32_t)from[8 * i + j] << (16 * (j & 1));
+            q = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
+    }
+}
+
+// A box of 32 rows of 64 bytes: pieces of 16 bytes change places with (row / 2) mod 4,
+// so that 8 lanes' pieces of a column fall into distinct banks.
+__device__ __forceinline__ uint32_t box_at(int row, int byte) {
+    return row * 64 + ((((byte >> 4) ^ (row >> 1)) & 3) << 4) + (byte & 15);
+}
+
+__device__ __forceinline__ void box_put(uint8_t *box, int row, const uint32_t (&w)[16]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        *reinterpret_cast<uint4 *>(box + box_at(row, 16 * i)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+}
+
+__device__ __forceinline__ void box_get(const uint8_t *box, int row, uint32_t (&w)[16]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint4 q = *reinterpret_cast<const uint4 *>(box + box_at(row, 16 * i));
+        w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
+    }
+}
+
+// a box of 16-bit elements to `rows` rows of memory, or from them: a column a lane
+__device__ __forceinline__ void box_out(const uint8_t *box, uint16_t *to, int64_t ld, int rows, int left, int lane) {
+    if (lane < left)
+#pragma unroll 4
+        for (int r = 0; r < rows; r++) to[r * ld + lane] = *reinterpret_cast<const uint16_t *>(box + box_at(r, 2 * lane));
+}
+
+__device__ __forceinline__ void box_in(uint8_t *box, const uint16_t *from, int64_t ld, int rows, int left, int lane) {
+    if (lane < left)
 #pragma unroll 8
-        for (int r = 0; r < rows; r++)
-            *reinterpret_cast<E *>(box + box_at<E>(r, lane / P) + (lane % P) * sizeof(E)) = from[(m0 + r) * ld + n + lane];
+        for (int r = 0; r < rows; r++) *reinterpret_cast<uint16_t *>(box + box_at(r, 2 * lane)) = from[r * ld + lane];
+}
+
+// a box of 16 float32 columns: two rows at a time
+__device__ __forceinline__ void box_out(const uint8_t *box, float *to, int64_t ld, int rows, int left, int lane) {
+    const int c = lane & 15;
+    if (c < left)
+#pragma unroll 4
+        for (int r = lane >> 4; r < rows; r += 2) to[r * ld + c] = *reinterpret_cast<const float *>(box + box_at(r, 4 * c));
 }
 
 struct Tiles {
@@ -295,10 +361,8 @@ struct Shape {
 
 template <typename T, bool A_MN, bool B_MN, int BN, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-            const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmR,
-            const __grid_constant__ CUtensorMap tmZ, int nkb, int64_t M, int64_t N, Tiles tiles,
-            const __grid_constant__ Epilogue e, unsigned spin, int stall) {
+gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, int nkb, int64_t M,
+            int64_t N, Tiles tiles, const __grid_constant__ Epilogue e, unsigned spin, int stall) {
     using S = Shape<BN>;
     constexpr int STAGES = S::STAGES;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -307,14 +371,14 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     float *factors = reinterpret_cast<float *>(boxes + SMEM_BOXES);
     uint64_t *bars = reinterpret_cast<uint64_t *>(boxes + SMEM_BOXES + S::FACTORS);
     // full [0, S), empty [S, 2 S), accumulator full 2 S + {0, 1}, accumulator empty 2 S + {2, 3}, all done 2 S + 4,
-    // one that nothing arrives on (the tests' stall), the epilogue warps' residual boxes from 2 S + 6.  The first
-    // CTA's full, accumulator empty and done barriers serve both; each has its own empty and accumulator full ones.
+    // and one that nothing arrives on (the tests' stall).  The first CTA's full, accumulator empty and done barriers
+    // serve both; each has its own empty and accumulator full ones.
     auto full = [&](int s) { return smem_u32(&bars[s]); };
     auto empty = [&](int s) { return smem_u32(&bars[STAGES + s]); };
     auto acc_full = [&](int a) { return smem_u32(&bars[2 * STAGES + a]); };
     auto acc_empty = [&](int a) { return smem_u32(&bars[2 * STAGES + 2 + a]); };
     const uint32_t done = smem_u32(&bars[2 * STAGES + 4]), never = smem_u32(&bars[2 * STAGES + 5]);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 6 + 2 * EPI_WARPS);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 6);
     __shared__ int s_fail;
     volatile int *failed = &s_fail;
 
@@ -330,7 +394,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             mbar_init(acc_full(a), 1);
             mbar_init(acc_empty(a), 2 * EPI_WARPS);
         }
-        for (int i = 4; i < 6 + 2 * EPI_WARPS; i++) mbar_init(smem_u32(&bars[2 * STAGES + i]), 1);
+        mbar_init(done, 1);
+        mbar_init(never, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -357,7 +422,6 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     *failed = 1;
                     break;
                 }
-                if (__any_sync(0xffffffffu, *failed)) break;
                 const uint32_t a = smem_u32(smem + s * S::STAGE), b = a + S::A, bar = of_leader(full(s));
                 if (elected()) {
                     if (rank == 0) mbar_expect_tx(full(s), 2 * S::STAGE);
@@ -382,7 +446,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     } else if (warp == 1 && rank == 0) {
         constexpr uint32_t id = instruction<T, A_MN, B_MN, BN>();
         bool ok = !(stall && !all_wait(never, 0, spin));
-        int it = 0, i = 0;
+        // The next stage's barrier is polled under this one's products, and nothing else is asked in the loop: a stage
+        // took 480 cycles to issue (115 the wait on a barrier that was ready, 150 a look at s_fail and a fence, 190
+        // the products and their commit), as long as 256 columns' products take and twice as long as 128's.
+        int s = 0, parity = 0, i = 0;
+        bool ready = mbar_try(full(0), 0);
         for (int t = first; t < tiles.total && ok; t += step, i++) {
             const int acc = i & 1;
             if (i >= 2 && !all_wait(acc_empty(acc), ((i >> 1) - 1) & 1, spin)) {
@@ -390,20 +458,21 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 break;
             }
             tc_fence_after();
-            for (int kb = 0; kb < nkb; kb++, it++) {
-                const int s = it % STAGES;
-                if (!all_wait(full(s), (it / STAGES) & 1, spin) || __any_sync(0xffffffffu, *failed)) {
+            for (int kb = 0; kb < nkb; kb++) {
+                if (!__all_sync(0xffffffffu, ready) && !all_wait(full(s), parity, spin)) {
                     ok = false;
                     break;
                 }
-                tc_fence_after();
-                const uint32_t a = smem_u32(smem + s * S::STAGE), b = a + S::A;
+                const uint32_t a = smem_u32(smem + s * S::STAGE), b = a + S::A, free = empty(s);
+                if (++s == STAGES) s = 0, parity ^= 1;
+                ready = mbar_try(full(s), parity);
                 if (elected()) {
+                    const uint64_t da = smem_desc<A_MN>(a), db = smem_desc<B_MN>(b);
 #pragma unroll
                     for (int kk = 0; kk < BK / 16; kk++)
-                        mma(tmem + acc * BN, smem_desc<A_MN>(a + kk * (A_MN ? 2048 : 32)),
-                            smem_desc<B_MN>(b + kk * (B_MN ? 2048 : 32)), id, kb == 0 && kk == 0 ? 0u : 1u);
-                    mma_commit_both(empty(s));
+                        mma(tmem + acc * BN, da + kk * (A_MN ? 128 : 2), db + kk * (B_MN ? 128 : 2), id,
+                            kb == 0 && kk == 0 ? 0u : 1u);
+                    mma_commit_both(free);
                 }
                 __syncwarp();
             }
@@ -423,75 +492,52 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         const int w = warp - 2, half = w >> 2, quad = warp & 3;   // a warp reaches the TMEM lanes 32 (warp % 4) ..
         const uint32_t lanes = (uint32_t)(32 * quad) << 16;
         float *scale = factors + w * BN, *bias = scale + BN / 2;
-        // Two boxes of 16-bit elements: y's in turn, the residual coming in where y goes out; or z's and y's, or one of
-        // float32.  Only y's in turn let a box be filled while TMA reads the other.
-        uint8_t *box = boxes + w * 4096;
-        const bool turns = !e.z && e.y_dtype != SFB_F32;
-        auto loaded = [&](int k) { return smem_u32(&bars[2 * STAGES + 6 + 2 * w + k]); };
+        uint8_t *box = boxes + w * 2048;
         const float alpha = e.alpha ? *e.alpha * e.unit : e.unit;
-        const bool wide = e.y_dtype == SFB_F32;
-        const T *res = static_cast<const T *>(e.residual);
-        int i = 0, q = 0;                             // tiles, boxes so far
+        const uint16_t *res = static_cast<const uint16_t *>(e.residual);
+        int i = 0;
         for (int t = first; t < tiles.total; t += step, i++) {
             int tm, tn;
             tile_of(tiles, t, tm, tn);
             const int acc = i & 1;
             const int64_t n0 = (int64_t)tn * BN + half * (BN / 2);
-            const int64_t m0 = (int64_t)(tm * 2 + rank) * BM + quad * 32;
-            const int count = m0 < M && n0 < N ? (int)min((int64_t)(BN / 64), (N - n0 + 31) / 32) : 0;
-            const int q0 = q;
-            // the residual's box c into its buffer, once the stores before have read it
-            auto fetch = [&](int c) {
-                const int k = turns ? (q0 + c) & 1 : 1;
-                uint8_t *to = box + k * 2048;
-                proxy_fence();
-                if (elected()) bulk_wait_read<0>();
-                __syncwarp();
-                if (e.r_tma) {
-                    if (elected()) {
-                        mbar_expect_tx(loaded(k), 2048);
-                        tma_load_2d(smem_u32(to), &tmR, (int)n0 + 32 * c, (int)m0, loaded(k));
-                    }
-                } else {
-                    box_load(to, res, e.ldr, m0, n0 + 32 * c, M, N, lane);
-                }
-            };
-            if (res && count) fetch(0);
+            const int64_t m0 = (int64_t)(tm * 2 + rank) * BM + quad * 32, m = m0 + lane;
+            const int rows = (int)min((int64_t)32, M - m0), cols = (int)min((int64_t)(BN / 2), N - n0);
+            const int count = rows > 0 && cols > 0 ? (cols + 31) / 32 : 0;
+            uint32_t rnext[16];
+            if (res && e.direct && count && lane < rows) row_load(res + m * e.ldr + n0, rnext, cols);
             __syncwarp();
             for (int c = lane; c < BN / 2; c += 32) {
-                scale[c] = n0 + c < N && e.scale ? e.scale[n0 + c] * alpha : alpha;
-                bias[c] = n0 + c < N && e.bias ? load_as(e.bias, n0 + c, e.bias_dtype) : 0.0f;
+                scale[c] = c < cols && e.scale ? e.scale[n0 + c] * alpha : alpha;
+                bias[c] = c < cols && e.bias ? load_as(e.bias, n0 + c, e.bias_dtype) : 0.0f;
             }
+            // one lane polls: 256 of them would crowd the memory pipe
             int fine = 0;
             if (lane == 0) fine = !*failed && mbar_wait(acc_full(acc), (i >> 1) & 1, spin) && !*failed;
             fine = __shfl_sync(0xffffffffu, fine, 0);    // TMEM loads are the whole warp's
             if (!fine) *failed = 1;
             tc_fence_after();
+            const uint32_t from = tmem + lanes + acc * BN + half * (BN / 2);
+            uint32_t next[32];
+            if (fine && count) tmem_load(from, next);
             for (int c = 0; c < count; c++) {
                 float v[32];
-                if (fine) {
-                    tmem_ld32(tmem + lanes + acc * BN + half * (BN / 2) + 32 * c, v);
-                } else {
+                uint32_t r[16];
+                if (fine) tmem_landed(next);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) v[j] = __int_as_float(0x7FC00000);
-                }
-                if (c + 1 == count) {
+                for (int j = 0; j < 32; j++) v[j] = fine ? __uint_as_float(next[j]) : __int_as_float(0x7FC00000);
+#pragma unroll
+                for (int j = 0; j < 16; j++) r[j] = rnext[j];
+                const int left = cols - 32 * c;
+                const int64_t n = n0 + 32 * c;
+                if (c + 1 < count) {
+                    if (fine) tmem_load(from + 32 * (c + 1), next);
+                    if (res && e.direct && lane < rows) row_load(res + m * e.ldr + n + 32, rnext, left - 32);
+                } else {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(of_leader(acc_empty(acc)));
                 }
-                if (res && turns && c + 1 < count) {
-                    fetch(c + 1);
-                } else if (res && !turns && c > 0) {
-                    fetch(c);
-                } else {
-                    if (elected()) {
-                        if (turns) bulk_wait_read<1>();
-                        else bulk_wait_read<0>();
-                    }
-                    __syncwarp();
-                }
-                uint8_t *yb = box + (turns ? (q & 1) * 2048 : e.z ? 2048 : 0), *zb = box;
 #pragma unroll
                 for (int j = 0; j < 32; j += 4) {
                     const float4 s4 = *reinterpret_cast<const float4 *>(scale + 32 * c + j);
@@ -501,48 +547,71 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     v[j + 2] = fmaf(v[j + 2], s4.z, b4.z);
                     v[j + 3] = fmaf(v[j + 3], s4.w, b4.w);
                 }
+                uint32_t h[16];
                 if (e.z) {
 #pragma unroll
-                    for (int p = 0; p < 4; p++) {
-                        uint4 h;
-                        h.x = kept2<ACT>(v[8 * p], v[8 * p + 1]);
-                        h.y = kept2<ACT>(v[8 * p + 2], v[8 * p + 3]);
-                        h.z = kept2<ACT>(v[8 * p + 4], v[8 * p + 5]);
-                        h.w = kept2<ACT>(v[8 * p + 6], v[8 * p + 7]);
-                        *reinterpret_cast<uint4 *>(zb + box_at<__half>(lane, p)) = h;
+                    for (int j = 0; j < 16; j++) h[j] = kept2<ACT>(v[2 * j], v[2 * j + 1]);
+                    uint16_t *z = reinterpret_cast<uint16_t *>(e.z);
+                    if (e.direct) {
+                        if (lane < rows) row_store(z + m * e.ldz + n, h, left, e.sectors);
+                    } else {
+                        box_put(box, lane, h);
+                        __syncwarp();
+                        box_out(box, z + m0 * e.ldz + n, e.ldz, rows, left, lane);
+                        __syncwarp();
                     }
                 }
 #pragma unroll
                 for (int j = 0; j < 32; j++) v[j] = activate<ACT>(v[j]);
                 if (res) {
-                    if (e.r_tma) (void)mbar_wait(loaded(turns ? q & 1 : 1), (turns ? q >> 1 : q) & 1, kSpinLimit);
-                    __syncwarp();
+                    if (!e.direct) {
+                        box_in(box, res + m0 * e.ldr + n, e.ldr, rows, left, lane);
+                        __syncwarp();
+                        box_get(box, lane, r);
+                        __syncwarp();
+                    }
 #pragma unroll
-                    for (int p = 0; p < 4; p++) {
-                        const Vec<T, 8> r = *reinterpret_cast<const Vec<T, 8> *>(yb + box_at<T>(lane, p));
-#pragma unroll
-                        for (int j = 0; j < 8; j++) v[8 * p + j] += to_f(r.v[j]);
+                    for (int j = 0; j < 16; j++) {
+                        float a, b;
+                        unpack2<T>(r[j], a, b);
+                        v[2 * j] += a;
+                        v[2 * j + 1] += b;
                     }
                 }
-                if (wide) box_put<float>(yb, lane, v);
-                else if (e.y_dtype == SFB_BF16) box_put<__nv_bfloat16>(yb, lane, v);
-                else box_put<__half>(yb, lane, v);
-                proxy_fence();
-                __syncwarp();
-                const int64_t n = n0 + 32 * c;
-                if (elected()) {
-                    if (e.y_tma) tma_store_2d(&tmY, (int)n, (int)m0, smem_u32(yb));
-                    if (e.z && e.z_tma) tma_store_2d(&tmZ, (int)n, (int)m0, smem_u32(zb));
-                    bulk_commit();
+                if (e.y_dtype == SFB_F32) {
+                    float *y = static_cast<float *>(e.y);
+                    if (e.direct) {
+                        if (lane < rows) row_store(y + m * e.ldy + n, v, left, e.sectors);
+                    } else {
+#pragma unroll
+                        for (int p = 0; p < 2; p++) {
+#pragma unroll
+                            for (int j = 0; j < 16; j++) h[j] = __float_as_uint(v[16 * p + j]);
+                            box_put(box, lane, h);
+                            __syncwarp();
+                            box_out(box, y + m0 * e.ldy + n + 16 * p, e.ldy, rows, left - 16 * p, lane);
+                            __syncwarp();
+                        }
+                    }
+                } else {
+                    uint16_t *y = static_cast<uint16_t *>(e.y);
+                    if (e.y_dtype == SFB_BF16) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++) h[j] = pack2<__nv_bfloat16>(v[2 * j], v[2 * j + 1]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; j++) h[j] = pack2<__half>(v[2 * j], v[2 * j + 1]);
+                    }
+                    if (e.direct) {
+                        if (lane < rows) row_store(y + m * e.ldy + n, h, left, e.sectors);
+                    } else {
+                        box_put(box, lane, h);
+                        __syncwarp();
+                        box_out(box, y + m0 * e.ldy + n, e.ldy, rows, left, lane);
+                        __syncwarp();
+                    }
                 }
-                if (!e.y_tma) {
-                    if (wide) box_store(yb, static_cast<float *>(e.y), e.ldy, m0, n, M, N, lane);
-                    else if (e.y_dtype == SFB_BF16) box_store(yb, static_cast<__nv_bfloat16 *>(e.y), e.ldy, m0, n, M, N, lane);
-                    else box_store(yb, static_cast<__half *>(e.y), e.ldy, m0, n, M, N, lane);
-                }
-                if (e.z && !e.z_tma) box_store(zb, e.z, e.ldz, m0, n, M, N, lane);
                 __syncwarp();
-                q++;
             }
             if (count == 0) {
                 tc_fence_before();
@@ -550,7 +619,6 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 if (lane == 0) mbar_arrive_cluster(of_leader(acc_empty(acc)));
             }
         }
-        if (elected()) bulk_wait_all();
     }
     __syncwarp();
     tc_fence_before();
@@ -593,47 +661,31 @@ EncodeTiled encoder() {
     return fn;
 }
 
-// a matrix of `rows` lines of `cols` elements of `size` bytes, ld apart, in boxes
-int make_map(CUtensorMap *map, const void *base, CUtensorMapDataType type, int size, CUtensorMapSwizzle swizzle,
-             int64_t rows, int64_t cols, int64_t ld, int box_cols, int box_rows) {
-    EncodeTiled enc = encoder();
-    if (!enc) return set_error(SFB_ECUDA, "sf tensor linear: cuTensorMapEncodeTiled is unavailable");
-    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)ld * size};
-    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = enc(map, type, 2, const_cast<void *>(base), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return set_error(SFB_ECUDA, "sf tensor linear: tensor map encoding failed (%d)", (int)r);
-    return SFB_OK;
-}
-
-CUtensorMapDataType map_type(int dtype) {
-    return dtype == SFB_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-           : dtype == SFB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-}
-
 struct Problem {
     const void *A, *B;
     int64_t lda, ldb, M, N, K;
     int dtype;
 };
 
-// an operand in boxes of 64 columns
+// an operand, `rows` lines of `cols` elements, ld apart, read in boxes of 64 columns
 int operand_map(CUtensorMap *map, const void *base, int dtype, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
-    return make_map(map, base, map_type(dtype), 2, CU_TENSOR_MAP_SWIZZLE_128B, rows, cols, ld, 64, box_rows);
+    EncodeTiled enc = encoder();
+    if (!enc) return set_error(SFB_ECUDA, "sf tensor linear: cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = enc(map, dtype == SFB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                           2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(SFB_ECUDA, "sf tensor linear: tensor map encoding failed (%d)", (int)r);
+    return SFB_OK;
 }
 
-// an output or residual in boxes of 32 x 32
-int box_map(CUtensorMap *map, const void *base, int dtype, int64_t rows, int64_t cols, int64_t ld) {
-    return make_map(map, base, map_type(dtype), dtype == SFB_F32 ? 4 : 2,
-                    dtype == SFB_F32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, rows, cols, ld, 32, 32);
-}
-
-bool aligned16(const void *p, int64_t ld, int size) {
-    return p != nullptr && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * size) % 16 == 0;
+// whether the rows of a matrix start on `bytes`
+bool rows_on(const void *p, int64_t ld, int size, int bytes) {
+    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && (ld * size) % bytes == 0);
 }
 
 template <typename T, bool A_MN, bool B_MN, int BN, int ACT>
@@ -654,24 +706,21 @@ int launch(const Problem &p, Epilogue e, cudaStream_t st) {
             ready[dev] = context_id();
         }
     }
-    e.r_tma = aligned16(e.residual, e.ldr, 2);
-    e.z_tma = aligned16(e.z, e.ldz, 2);
-    e.y_tma = aligned16(e.y, e.ldy, e.y_dtype == SFB_F32 ? 4 : 2);
-    CUtensorMap tmA, tmB, tmY = {}, tmR = {}, tmZ = {};
+    const int size = e.y_dtype == SFB_F32 ? 4 : 2;
+    e.direct = rows_on(e.y, e.ldy, size, 16) && rows_on(e.z, e.ldz, 2, 16) && rows_on(e.residual, e.ldr, 2, 16);
+    e.sectors = rows_on(e.y, e.ldy, size, 32) && rows_on(e.z, e.ldz, 2, 32);
+    CUtensorMap tmA, tmB;
     int rc = A_MN ? operand_map(&tmA, p.A, p.dtype, p.K, p.M, p.lda, BK) : operand_map(&tmA, p.A, p.dtype, p.M, p.K, p.lda, BM);
     if (!rc)
         rc = B_MN ? operand_map(&tmB, p.B, p.dtype, p.K, p.N, p.ldb, BK)
                   : operand_map(&tmB, p.B, p.dtype, p.N, p.K, p.ldb, S::BNL);
-    if (!rc && e.y_tma) rc = box_map(&tmY, e.y, e.y_dtype, p.M, p.N, e.ldy);
-    if (!rc && e.r_tma) rc = box_map(&tmR, e.residual, p.dtype, p.M, p.N, e.ldr);
-    if (!rc && e.z_tma) rc = box_map(&tmZ, e.z, SFB_F16, p.M, p.N, e.ldz);
     if (rc) return rc;
     Tiles t;
     t.mt = (int)((p.M + 2 * BM - 1) / (2 * BM));
     t.nt = (int)((p.N + BN - 1) / BN);
     t.total = t.mt * t.nt;
     kernel<<<2 * std::min(t.total, sm_count() / 2), THREADS, S::SMEM, st>>>(
-        tmA, tmB, tmY, tmR, tmZ, (int)((p.K + BK - 1) / BK), p.M, p.N, t, e, wait_polls() ? wait_polls() : kSpinLimit,
+        tmA, tmB, (int)((p.K + BK - 1) / BK), p.M, p.N, t, e, wait_polls() ? wait_polls() : kSpinLimit,
         wait_stall());
     return check_launch("sf tensor linear");
 }
