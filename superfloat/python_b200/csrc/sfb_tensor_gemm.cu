@@ -109,6 +109,19 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 
+// the same without a wait: try_wait may hold the thread some microseconds
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 // false once `limit` polls have not seen the phase of this parity end
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, unsigned limit) {
     for (unsigned i = 0; i < limit; i++)
@@ -446,11 +459,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     } else if (warp == 1 && rank == 0) {
         constexpr uint32_t id = instruction<T, A_MN, B_MN, BN>();
         bool ok = !(stall && !all_wait(never, 0, spin));
-        // The next stage's barrier is polled under this one's products, and nothing else is asked in the loop: a stage
+        // The next stage's barrier is tested under this one's products, and nothing else is asked in the loop: a stage
         // took 480 cycles to issue (115 the wait on a barrier that was ready, 150 a look at s_fail and a fence, 190
         // the products and their commit), as long as 256 columns' products take and twice as long as 128's.
         int s = 0, parity = 0, i = 0;
-        bool ready = mbar_try(full(0), 0);
+        bool ready = mbar_test(full(0), 0);
         for (int t = first; t < tiles.total && ok; t += step, i++) {
             const int acc = i & 1;
             if (i >= 2 && !all_wait(acc_empty(acc), ((i >> 1) - 1) & 1, spin)) {
@@ -465,7 +478,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 }
                 const uint32_t a = smem_u32(smem + s * S::STAGE), b = a + S::A, free = empty(s);
                 if (++s == STAGES) s = 0, parity ^= 1;
-                ready = mbar_try(full(s), parity);
+                ready = mbar_test(full(s), parity);
                 if (elected()) {
                     const uint64_t da = smem_desc<A_MN>(a), db = smem_desc<B_MN>(b);
 #pragma unroll
