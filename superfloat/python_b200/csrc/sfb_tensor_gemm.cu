@@ -8,6 +8,15 @@
 // operands of the forward product are exact; the sums are held in float32 in
 // TMEM and rounded once, when they are stored.
 //
+// A tile's rows (TMEM lanes) run along the result's contiguous index, its columns
+// along the other: operand A is the codes (forward), the codes again (x grad) or x
+// (w grad).  A lane then has one channel, with its scale and bias in registers.
+// (With a row of the result to a lane they came from shared memory, 16 wide loads
+// a lane for 32 columns, and a tile's epilogue took 7500 cycles where K = 768 gives
+// its products 6100.)  A store of two bytes a lane costs the memory pipe as much as
+// one of 16 (about 8 cycles), so 32 x 32 values are packed and turned around in
+// shared memory, written a channel to a lane and read by ldmatrix with its rows
+// chosen so that a lane gets 8 neighbouring channels of one column.
 // A pair of SMs (a cluster of two CTAs) shares an output tile of 256 x BN: each
 // holds 128 rows of A, half of B's columns and the sums of its own rows, and the
 // first one's warp 1 issues the products of both (cta_group::2).  Products read
@@ -15,18 +24,12 @@
 // that is what bounds a smaller tile: 256 x 256 of bf16 moves 64 KB an SM and
 // stage of 64 against 512 cycles of products, at the 128 bytes a cycle that it
 // has; 128 x 128 on one SM needs 64 KB for 256 cycles (577 were measured).
-// Warp 0 issues the TMA loads (64 elements of the contraction a stage, 128-byte
-// swizzle), warps 2..9 are the epilogue, two to each group of 32 rows, each half
-// of the columns.  Two accumulators (2 BN TMEM columns) let a tile's epilogue run
-// under the next tile's products.
-// The epilogue has a row to a lane and 32 columns at a time, the next ones' TMEM
-// load and residual in flight.  It stores from registers, 32 bytes a lane: whole
-// sectors, and nothing to wait for.  (Through shared memory and TMA stores a warp
-// spent 550 of a box's 1400 cycles on fences and waits.)  Rows that do not start
-// on 16 bytes pass through a box of 32 x 32 in shared memory instead, so that a
-// row's elements are stored together.
+// Warp 0 issues the TMA loads (128-byte swizzle), warps 2..9 are the epilogue, two
+// to each group of 32 rows, each half of the columns, 32 at a time, the next ones'
+// TMEM load and residual in flight.  Two accumulators (2 BN TMEM columns) let a
+// tile's epilogue run under the next tile's products.
 // An operand whose contraction index is contiguous in memory is loaded K-major
-// (rows of 64); one whose row index is contiguous MN-major (64 rows wide, 64
+// (lines of 64), one whose row index is contiguous MN-major (64 rows wide, 64
 // deep), so that no operand of the backward products is transposed beforehand.
 //
 // Every wait is bounded; one that runs out is counted in g_failures, the CTA's
@@ -46,11 +49,11 @@ int wait_stall();
 
 namespace {
 
-constexpr int BM = 128, BK = 64, THREADS = 320, EPI_WARPS = 8;
+constexpr int BM = 128, THREADS = 320, EPI_WARPS = 8;
 constexpr unsigned kSpinLimit = 1u << 26;     // polls of one wait, some seconds
 constexpr int SMEM_OPERANDS = 196608;         // of the stages: what hides a copy's 1500 cycles or so under load
 constexpr int SMEM_BOXES = EPI_WARPS * 2048;  // of the epilogue
-constexpr int GROUP_M = 4;                    // row tiles that sweep the columns together, for L2
+constexpr int GROUP = 4;                      // row tiles that sweep the columns together, for L2
 
 __device__ unsigned long long g_failures;
 
@@ -217,23 +220,11 @@ __device__ __forceinline__ void tmem_landed(uint32_t (&r)[32]) {
                    "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
-// 32 bytes
-__device__ __forceinline__ void store32(void *to, const uint32_t (&w)[8], bool whole) {
-    if (whole) {
-        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                     "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                     : "memory");
-    } else {
-        static_cast<uint4 *>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        static_cast<uint4 *>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-    }
-}
-
 // --- the epilogue --------------------------------------------------------------------------------------------
 
 struct Epilogue {
-    const float *scale;          // per column (forward), or null
-    const void *bias;            // per column, or null
+    const float *scale;          // per row of the tile, a channel (forward), or null
+    const void *bias;            // likewise
     const void *residual;        // of the operands' type, or null
     const float *alpha;          // one factor for all, in device memory, or null
     __half *z;                   // the pre-activation for the backward pass, or null
@@ -241,20 +232,9 @@ struct Epilogue {
     float unit;                  // 2^-(bits-1) where a scale or alpha stands for codes, else 1
     int bias_dtype, y_dtype;
     int64_t ldr, ldz, ldy;
-    bool direct;                 // rows of y, r and z start on 16 bytes
-    bool sectors;                // and those of y and z on 32
+    bool vec;                    // y (of 16 bits), z and r start on 16 bytes, and so do their rows
 };
 
-// two values in 16 bits each
-template <typename E> __device__ __forceinline__ uint32_t pack2(float a, float b);
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return reinterpret_cast<uint32_t &>(h);
-}
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-    __half2 h = __floats2half2_rn(a, b);
-    return reinterpret_cast<uint32_t &>(h);
-}
 template <typename E> __device__ __forceinline__ void unpack2(uint32_t w, float &a, float &b);
 template <> __device__ __forceinline__ void unpack2<__nv_bfloat16>(uint32_t w, float &a, float &b) {
     a = __uint_as_float(w << 16);
@@ -266,123 +246,137 @@ template <> __device__ __forceinline__ void unpack2<__half>(uint32_t w, float &a
     b = f.y;
 }
 
-// 32 columns of one row, from 16 packed words: columns past `left` are not the matrix's
-__device__ __forceinline__ void row_store(uint16_t *to, const uint32_t (&w)[16], int left, bool sectors) {
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        if (left >= 16 * i + 16) {
-            store32(to + 16 * i, *reinterpret_cast<const uint32_t(*)[8]>(w + 8 * i), sectors);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; j++)
-                if (16 * i + j < left) to[16 * i + j] = (uint16_t)(w[8 * i + j / 2] >> (16 * (j & 1)));
-        }
-    }
+// two values in 16 bits each
+template <typename E> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return reinterpret_cast<uint32_t &>(h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    __half2 h = __floats2half2_rn(a, b);
+    return reinterpret_cast<uint32_t &>(h);
 }
 
-__device__ __forceinline__ void row_store(float *to, const float (&v)[32], int left, bool sectors) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if (left >= 8 * i + 8) {
-            store32(to + 8 * i, *reinterpret_cast<const uint32_t(*)[8]>(v + 8 * i), sectors);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (8 * i + j < left) to[8 * i + j] = v[8 * i + j];
-        }
-    }
+// A box: 32 channels (rows of 64 bytes) by 32 columns of 16 bits.  A row's four
+// pieces of 16 bytes change places so that neither 8 neighbouring rows (a channel
+// to a lane) nor the rows 2 i, 2 i + 1 and those 8, 16 and 24 on (ldmatrix below)
+// meet in a bank.
+__device__ __forceinline__ uint32_t box_at(int row, int piece) {
+    return row * 64 + (((piece ^ (row >> 1) ^ (row >> 3)) & 3) << 4);
 }
 
-// 32 columns of one row into 16 packed words, the rows starting on 16 bytes
-__device__ __forceinline__ void row_load(const uint16_t *from, uint32_t (&w)[16], int left) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        uint4 q = make_uint4(0, 0, 0, 0);
-        if (left >= 8 * i + 8) {
-            q = __ldg(reinterpret_cast<const uint4 *>(from) + i);
-        } else {
-            uint32_t h[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (8 * i + j < left) h[j / 2] |= (uint32_t)from[8 * i + j] << (16 * (j & 1));
-            q = make_uint4(h[0], h[1], h[2], h[3]);
-        }
-        w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
-    }
-}
-
-// A box of 32 rows of 64 bytes: pieces of 16 bytes change places with (row / 2) mod 4,
-// so that 8 lanes' pieces of a column fall into distinct banks.
-__device__ __forceinline__ uint32_t box_at(int row, int byte) {
-    return row * 64 + ((((byte >> 4) ^ (row >> 1)) & 3) << 4) + (byte & 15);
-}
-
-__device__ __forceinline__ void box_put(uint8_t *box, int row, const uint32_t (&w)[16]) {
+__device__ __forceinline__ void box_put(uint32_t box, int row, const uint32_t (&w)[16]) {
 #pragma unroll
     for (int i = 0; i < 4; i++)
-        *reinterpret_cast<uint4 *>(box + box_at(row, 16 * i)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + box_at(row, i)), "r"(w[4 * i]),
+                     "r"(w[4 * i + 1]), "r"(w[4 * i + 2]), "r"(w[4 * i + 3])
+                     : "memory");
 }
 
-__device__ __forceinline__ void box_get(const uint8_t *box, int row, uint32_t (&w)[16]) {
+__device__ __forceinline__ void box_get(uint32_t box, int row, uint32_t (&w)[16]) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint4 q = *reinterpret_cast<const uint4 *>(box + box_at(row, 16 * i));
-        w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
+    for (int i = 0; i < 4; i++)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3])
+                     : "r"(box + box_at(row, i))
+                     : "memory");
+}
+
+// Columns 8 p .. 8 p + 7 turned around: lane l has channels 8 (l mod 4) .. + 7 of
+// column 8 p + l / 4.  Matrix i's line q is the channel 8 (q / 2) + 2 i + q mod 2,
+// of which a lane gets lines 2 (l mod 4) and one on.
+__device__ __forceinline__ uint32_t turn_at(uint32_t box, int p, int lane) {
+    const int i = lane >> 3, q = lane & 7;
+    return box + box_at(8 * (q >> 1) + 2 * i + (q & 1), p);
+}
+
+__device__ __forceinline__ uint4 box_turn(uint32_t box, int p, int lane) {
+    uint4 o;
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(o.x), "=r"(o.y), "=r"(o.z), "=r"(o.w)
+                 : "r"(turn_at(box, p, lane))
+                 : "memory");
+    return o;
+}
+
+__device__ __forceinline__ void box_turn_in(uint32_t box, int p, int lane, uint4 o) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(turn_at(box, p, lane)),
+                 "r"(o.x), "r"(o.y), "r"(o.z), "r"(o.w)
+                 : "memory");
+}
+
+// 8 channels of a column, those past `left` not the matrix's
+__device__ __forceinline__ void store8(uint16_t *to, uint4 o, int left) {
+    if (left >= 8) {
+        *reinterpret_cast<uint4 *>(to) = o;
+    } else {
+        const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (j < left) to[j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
     }
 }
 
-// a box of 16-bit elements to `rows` rows of memory, or from them: a column a lane
-__device__ __forceinline__ void box_out(const uint8_t *box, uint16_t *to, int64_t ld, int rows, int left, int lane) {
-    if (lane < left)
-#pragma unroll 4
-        for (int r = 0; r < rows; r++) to[r * ld + lane] = *reinterpret_cast<const uint16_t *>(box + box_at(r, 2 * lane));
+__device__ __forceinline__ uint4 load8(const uint16_t *from, int left) {
+    if (left >= 8) return __ldg(reinterpret_cast<const uint4 *>(from));
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        if (j < left) w[j / 2] |= (uint32_t)from[j] << (16 * (j & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__device__ __forceinline__ void box_in(uint8_t *box, const uint16_t *from, int64_t ld, int rows, int left, int lane) {
-    if (lane < left)
-#pragma unroll 8
-        for (int r = 0; r < rows; r++) *reinterpret_cast<uint16_t *>(box + box_at(r, 2 * lane)) = from[r * ld + lane];
-}
-
-// a box of 16 float32 columns: two rows at a time
-__device__ __forceinline__ void box_out(const uint8_t *box, float *to, int64_t ld, int rows, int left, int lane) {
-    const int c = lane & 15;
-    if (c < left)
-#pragma unroll 4
-        for (int r = lane >> 4; r < rows; r += 2) to[r * ld + c] = *reinterpret_cast<const float *>(box + box_at(r, 4 * c));
+// A box of 16-bit values to memory.  `to` is the warp's first channel in the box's
+// first column; `cols` and `chans` are what the matrix has from there on.
+__device__ __forceinline__ void box_out(uint32_t box, const uint32_t (&w)[16], uint16_t *to, int64_t ld, int cols,
+                                        int chans, bool vec, int lane) {
+    if (vec) {
+        box_put(box, lane, w);
+        __syncwarp();
+        const int part = 8 * (lane & 3), c = lane >> 2;
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+            const uint4 o = box_turn(box, p, lane);
+            if (8 * p + c < cols) store8(to + (8 * p + c) * ld + part, o, chans - part);
+        }
+        __syncwarp();
+    } else if (lane < chans) {
+        to += lane;
+#pragma unroll
+        for (int j = 0; j < 32; j++, to += ld)
+            if (j < cols) *to = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+    }
 }
 
 struct Tiles {
-    int mt, nt, total;
+    int rt, ct, total;               // of rows, of columns
 };
 
-__device__ __forceinline__ void tile_of(const Tiles &t, int i, int &tm, int &tn) {
-    const int gsize = GROUP_M * t.nt, g = i / gsize, m0 = g * GROUP_M;
-    const int gm = min(GROUP_M, t.mt - m0), r = i - g * gsize;
-    tm = m0 + r % gm;
-    tn = r / gm;
+__device__ __forceinline__ void tile_of(const Tiles &t, int i, int &tr, int &tc) {
+    const int gsize = GROUP * t.ct, g = i / gsize, r0 = g * GROUP;
+    const int gr = min(GROUP, t.rt - r0), r = i - g * gsize;
+    tr = r0 + r % gr;
+    tc = r / gr;
 }
 
 template <int BN>
 struct Shape {
     static constexpr int BNL = BN / 2;                               // columns of B that a CTA loads
+    static constexpr int BK = BN == 256 ? 64 : 128;                  // of the contraction, a stage
     static constexpr int A = BM * BK * 2, B = BNL * BK * 2, STAGE = A + B, STAGES = SMEM_OPERANDS / STAGE;
     static constexpr int COLS = 2 * BN;                              // TMEM columns
-    static constexpr int FACTORS = EPI_WARPS * 2 * (BN / 2) * 4;     // each warp's scales and biases
-    static constexpr int SMEM = STAGES * STAGE + SMEM_BOXES + FACTORS + 512 + 1024;
+    static constexpr int SMEM = STAGES * STAGE + SMEM_BOXES + 512 + 1024;
 };
 
 template <typename T, bool A_MN, bool B_MN, int BN, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, int nkb, int64_t M,
-            int64_t N, Tiles tiles, const __grid_constant__ Epilogue e, unsigned spin, int stall) {
+gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, int nkb, int64_t R,
+            int64_t C, Tiles tiles, const __grid_constant__ Epilogue e, unsigned spin, int stall) {
     using S = Shape<BN>;
-    constexpr int STAGES = S::STAGES;
+    constexpr int STAGES = S::STAGES, BK = S::BK;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint8_t *boxes = smem + STAGES * S::STAGE;
-    float *factors = reinterpret_cast<float *>(boxes + SMEM_BOXES);
-    uint64_t *bars = reinterpret_cast<uint64_t *>(boxes + SMEM_BOXES + S::FACTORS);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + STAGES * S::STAGE + SMEM_BOXES);
     // full [0, S), empty [S, 2 S), accumulator full 2 S + {0, 1}, accumulator empty 2 S + {2, 3}, all done 2 S + 4,
     // and one that nothing arrives on (the tests' stall).  The first CTA's full, accumulator empty and done barriers
     // serve both; each has its own empty and accumulator full ones.
@@ -426,9 +420,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     int issued = 0;
     if (warp == 0) {
         for (int t = first; t < tiles.total; t += step) {
-            int tm, tn;
-            tile_of(tiles, t, tm, tn);
-            const int m0 = (tm * 2 + rank) * BM, n0 = tn * BN + rank * S::BNL;
+            int tr, tc;
+            tile_of(tiles, t, tr, tc);
+            const int r0 = (tr * 2 + rank) * BM, c0 = tc * BN + rank * S::BNL;
             for (int kb = 0; kb < nkb; kb++, issued++) {
                 const int s = issued % STAGES, round = issued / STAGES;
                 if (round > 0 && !all_wait(empty(s), (round - 1) & 1, spin)) {
@@ -438,18 +432,23 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 const uint32_t a = smem_u32(smem + s * S::STAGE), b = a + S::A, bar = of_leader(full(s));
                 if (elected()) {
                     if (rank == 0) mbar_expect_tx(full(s), 2 * S::STAGE);
-                    if constexpr (A_MN) {
 #pragma unroll
-                        for (int i = 0; i < BM / 64; i++) tma_load_operand(a + i * 8192, &tmA, m0 + i * 64, kb * BK, bar);
-                    } else {
-                        tma_load_operand(a, &tmA, kb * BK, m0, bar);
-                    }
-                    if constexpr (B_MN) {
+                    for (int h = 0; h < BK / 64; h++) {              // 64 of the contraction at a time
+                        const int k = kb * BK + h * 64;
+                        const uint32_t ah = a + h * (BM * 128), bh = b + h * (S::BNL * 128);
+                        if constexpr (A_MN) {
 #pragma unroll
-                        for (int i = 0; i < S::BNL / 64; i++)
-                            tma_load_operand(b + i * 8192, &tmB, n0 + i * 64, kb * BK, bar);
-                    } else {
-                        tma_load_operand(b, &tmB, kb * BK, n0, bar);
+                            for (int i = 0; i < BM / 64; i++) tma_load_operand(ah + i * 8192, &tmA, r0 + i * 64, k, bar);
+                        } else {
+                            tma_load_operand(ah, &tmA, k, r0, bar);
+                        }
+                        if constexpr (B_MN) {
+#pragma unroll
+                            for (int i = 0; i < S::BNL / 64; i++)
+                                tma_load_operand(bh + i * 8192, &tmB, c0 + i * 64, k, bar);
+                        } else {
+                            tma_load_operand(bh, &tmB, k, c0, bar);
+                        }
                     }
                 }
                 __syncwarp();
@@ -480,11 +479,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 if (++s == STAGES) s = 0, parity ^= 1;
                 ready = mbar_test(full(s), parity);
                 if (elected()) {
-                    const uint64_t da = smem_desc<A_MN>(a), db = smem_desc<B_MN>(b);
 #pragma unroll
-                    for (int kk = 0; kk < BK / 16; kk++)
-                        mma(tmem + acc * BN, da + kk * (A_MN ? 128 : 2), db + kk * (B_MN ? 128 : 2), id,
+                    for (int kk = 0; kk < BK / 16; kk++) {
+                        const int h = kk / 4, q = kk % 4;
+                        const uint64_t da = smem_desc<A_MN>(a + h * (BM * 128)), db = smem_desc<B_MN>(b + h * (S::BNL * 128));
+                        mma(tmem + acc * BN, da + q * (A_MN ? 128 : 2), db + q * (B_MN ? 128 : 2), id,
                             kb == 0 && kk == 0 ? 0u : 1u);
+                    }
                     mma_commit_both(free);
                 }
                 __syncwarp();
@@ -502,28 +503,46 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             mma_commit(done);
         }
     } else if (warp >= 2) {
-        const int w = warp - 2, half = w >> 2, quad = warp & 3;   // a warp reaches the TMEM lanes 32 (warp % 4) ..
-        const uint32_t lanes = (uint32_t)(32 * quad) << 16;
-        float *scale = factors + w * BN, *bias = scale + BN / 2;
-        uint8_t *box = boxes + w * 2048;
+        const int half = (warp - 2) >> 2, quad = warp & 3;   // a warp reaches the TMEM lanes 32 (warp % 4) ..
+        const uint32_t lanes = (uint32_t)(32 * quad) << 16, box = smem_u32(smem + STAGES * S::STAGE) + (warp - 2) * 2048;
         const float alpha = e.alpha ? *e.alpha * e.unit : e.unit;
         const uint16_t *res = static_cast<const uint16_t *>(e.residual);
+        uint16_t *z = reinterpret_cast<uint16_t *>(e.z);
         int i = 0;
         for (int t = first; t < tiles.total; t += step, i++) {
-            int tm, tn;
-            tile_of(tiles, t, tm, tn);
+            int tr, tc;
+            tile_of(tiles, t, tr, tc);
             const int acc = i & 1;
-            const int64_t n0 = (int64_t)tn * BN + half * (BN / 2);
-            const int64_t m0 = (int64_t)(tm * 2 + rank) * BM + quad * 32, m = m0 + lane;
-            const int rows = (int)min((int64_t)32, M - m0), cols = (int)min((int64_t)(BN / 2), N - n0);
-            const int count = rows > 0 && cols > 0 ? (cols + 31) / 32 : 0;
+            const int64_t r0 = (int64_t)(tr * 2 + rank) * BM + quad * 32, c0 = (int64_t)tc * BN + half * (BN / 2);
+            const int chans = (int)min((int64_t)32, R - r0), cols = (int)min((int64_t)(BN / 2), C - c0);
+            const int count = chans > 0 && cols > 0 ? (cols + 31) / 32 : 0;
+            const bool mine = lane < chans;
+            const float scale = mine && e.scale ? e.scale[r0 + lane] * alpha : alpha;
+            const float bias = mine && e.bias ? load_as(e.bias, r0 + lane, e.bias_dtype) : 0.0f;
+            // the residual of box b: as box_turn has it or, unaligned, the lane's channel in 32 columns
             uint32_t rnext[16];
-            if (res && e.direct && count && lane < rows) row_load(res + m * e.ldr + n0, rnext, cols);
-            __syncwarp();
-            for (int c = lane; c < BN / 2; c += 32) {
-                scale[c] = c < cols && e.scale ? e.scale[n0 + c] * alpha : alpha;
-                bias[c] = c < cols && e.bias ? load_as(e.bias, n0 + c, e.bias_dtype) : 0.0f;
-            }
+            auto fetch = [&](int b) {
+                const int left = cols - 32 * b;
+                const uint16_t *from = res + (c0 + 32 * b) * e.ldr + r0;
+                if (e.vec) {
+                    const int part = 8 * (lane & 3), c = lane >> 2;
+#pragma unroll
+                    for (int p = 0; p < 4; p++) {
+                        uint4 q = make_uint4(0, 0, 0, 0);
+                        if (8 * p + c < left) q = load8(from + (8 * p + c) * e.ldr + part, chans - part);
+                        rnext[4 * p] = q.x, rnext[4 * p + 1] = q.y, rnext[4 * p + 2] = q.z, rnext[4 * p + 3] = q.w;
+                    }
+                } else {
+                    from += lane;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2, from += 2 * e.ldr) {
+                        const uint32_t lo = mine && j < left ? __ldg(from) : 0;
+                        const uint32_t hi = mine && j + 1 < left ? __ldg(from + e.ldr) : 0;
+                        rnext[j / 2] = lo | hi << 16;
+                    }
+                }
+            };
+            if (res && count) fetch(0);
             // one lane polls: 256 of them would crowd the memory pipe
             int fine = 0;
             if (lane == 0) fine = !*failed && mbar_wait(acc_full(acc), (i >> 1) & 1, spin) && !*failed;
@@ -533,98 +552,66 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             const uint32_t from = tmem + lanes + acc * BN + half * (BN / 2);
             uint32_t next[32];
             if (fine && count) tmem_load(from, next);
-            for (int c = 0; c < count; c++) {
+            for (int b = 0; b < count; b++) {
                 float v[32];
-                uint32_t r[16];
+                uint32_t w[16], rr[16];
                 if (fine) tmem_landed(next);
 #pragma unroll
                 for (int j = 0; j < 32; j++) v[j] = fine ? __uint_as_float(next[j]) : __int_as_float(0x7FC00000);
 #pragma unroll
-                for (int j = 0; j < 16; j++) r[j] = rnext[j];
-                const int left = cols - 32 * c;
-                const int64_t n = n0 + 32 * c;
-                if (c + 1 < count) {
-                    if (fine) tmem_load(from + 32 * (c + 1), next);
-                    if (res && e.direct && lane < rows) row_load(res + m * e.ldr + n + 32, rnext, left - 32);
+                for (int j = 0; j < 16; j++) rr[j] = rnext[j];
+                const int left = cols - 32 * b;
+                const int64_t c = c0 + 32 * b;
+                if (b + 1 < count) {
+                    if (fine) tmem_load(from + 32 * (b + 1), next);
+                    if (res) fetch(b + 1);
                 } else {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(of_leader(acc_empty(acc)));
                 }
 #pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    const float4 s4 = *reinterpret_cast<const float4 *>(scale + 32 * c + j);
-                    const float4 b4 = *reinterpret_cast<const float4 *>(bias + 32 * c + j);
-                    v[j] = fmaf(v[j], s4.x, b4.x);
-                    v[j + 1] = fmaf(v[j + 1], s4.y, b4.y);
-                    v[j + 2] = fmaf(v[j + 2], s4.z, b4.z);
-                    v[j + 3] = fmaf(v[j + 3], s4.w, b4.w);
-                }
-                uint32_t h[16];
-                if (e.z) {
+                for (int j = 0; j < 32; j++) v[j] = fmaf(v[j], scale, bias);
+                if (z) {
 #pragma unroll
-                    for (int j = 0; j < 16; j++) h[j] = kept2<ACT>(v[2 * j], v[2 * j + 1]);
-                    uint16_t *z = reinterpret_cast<uint16_t *>(e.z);
-                    if (e.direct) {
-                        if (lane < rows) row_store(z + m * e.ldz + n, h, left, e.sectors);
-                    } else {
-                        box_put(box, lane, h);
-                        __syncwarp();
-                        box_out(box, z + m0 * e.ldz + n, e.ldz, rows, left, lane);
-                        __syncwarp();
-                    }
+                    for (int j = 0; j < 16; j++) w[j] = kept2<ACT>(v[2 * j], v[2 * j + 1]);
+                    box_out(box, w, z + c * e.ldz + r0, e.ldz, left, chans, e.vec, lane);
                 }
 #pragma unroll
                 for (int j = 0; j < 32; j++) v[j] = activate<ACT>(v[j]);
                 if (res) {
-                    if (!e.direct) {
-                        box_in(box, res + m0 * e.ldr + n, e.ldr, rows, left, lane);
+                    if (e.vec) {
+#pragma unroll
+                        for (int p = 0; p < 4; p++)
+                            box_turn_in(box, p, lane, make_uint4(rr[4 * p], rr[4 * p + 1], rr[4 * p + 2], rr[4 * p + 3]));
                         __syncwarp();
-                        box_get(box, lane, r);
+                        box_get(box, lane, rr);
                         __syncwarp();
                     }
 #pragma unroll
                     for (int j = 0; j < 16; j++) {
-                        float a, b;
-                        unpack2<T>(r[j], a, b);
-                        v[2 * j] += a;
-                        v[2 * j + 1] += b;
+                        float lo, hi;
+                        unpack2<T>(rr[j], lo, hi);
+                        v[2 * j] += lo;
+                        v[2 * j + 1] += hi;
                     }
                 }
                 if (e.y_dtype == SFB_F32) {
-                    float *y = static_cast<float *>(e.y);
-                    if (e.direct) {
-                        if (lane < rows) row_store(y + m * e.ldy + n, v, left, e.sectors);
-                    } else {
+                    float *y = static_cast<float *>(e.y) + c * e.ldy + r0 + lane;
+                    if (mine)
 #pragma unroll
-                        for (int p = 0; p < 2; p++) {
-#pragma unroll
-                            for (int j = 0; j < 16; j++) h[j] = __float_as_uint(v[16 * p + j]);
-                            box_put(box, lane, h);
-                            __syncwarp();
-                            box_out(box, y + m0 * e.ldy + n + 16 * p, e.ldy, rows, left - 16 * p, lane);
-                            __syncwarp();
-                        }
-                    }
+                        for (int j = 0; j < 32; j++, y += e.ldy)
+                            if (j < left) *y = v[j];
                 } else {
-                    uint16_t *y = static_cast<uint16_t *>(e.y);
                     if (e.y_dtype == SFB_BF16) {
 #pragma unroll
-                        for (int j = 0; j < 16; j++) h[j] = pack2<__nv_bfloat16>(v[2 * j], v[2 * j + 1]);
+                        for (int j = 0; j < 16; j++) w[j] = pack2<__nv_bfloat16>(v[2 * j], v[2 * j + 1]);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 16; j++) h[j] = pack2<__half>(v[2 * j], v[2 * j + 1]);
+                        for (int j = 0; j < 16; j++) w[j] = pack2<__half>(v[2 * j], v[2 * j + 1]);
                     }
-                    if (e.direct) {
-                        if (lane < rows) row_store(y + m * e.ldy + n, h, left, e.sectors);
-                    } else {
-                        box_put(box, lane, h);
-                        __syncwarp();
-                        box_out(box, y + m0 * e.ldy + n, e.ldy, rows, left, lane);
-                        __syncwarp();
-                    }
+                    box_out(box, w, static_cast<uint16_t *>(e.y) + c * e.ldy + r0, e.ldy, left, chans, e.vec, lane);
                 }
-                __syncwarp();
             }
             if (count == 0) {
                 tc_fence_before();
@@ -674,9 +661,10 @@ EncodeTiled encoder() {
     return fn;
 }
 
+// rows of A, columns (rows of B in memory where it is K-major), contraction
 struct Problem {
     const void *A, *B;
-    int64_t lda, ldb, M, N, K;
+    int64_t lda, ldb, R, C, K;
     int dtype;
 };
 
@@ -696,9 +684,9 @@ int operand_map(CUtensorMap *map, const void *base, int dtype, int64_t rows, int
     return SFB_OK;
 }
 
-// whether the rows of a matrix start on `bytes`
-bool rows_on(const void *p, int64_t ld, int size, int bytes) {
-    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && (ld * size) % bytes == 0);
+// whether a matrix of 16-bit elements and its rows start on 16 bytes
+bool rows_on16(const void *p, int64_t ld) {
+    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0);
 }
 
 template <typename T, bool A_MN, bool B_MN, int BN, int ACT>
@@ -719,21 +707,19 @@ int launch(const Problem &p, Epilogue e, cudaStream_t st) {
             ready[dev] = context_id();
         }
     }
-    const int size = e.y_dtype == SFB_F32 ? 4 : 2;
-    e.direct = rows_on(e.y, e.ldy, size, 16) && rows_on(e.z, e.ldz, 2, 16) && rows_on(e.residual, e.ldr, 2, 16);
-    e.sectors = rows_on(e.y, e.ldy, size, 32) && rows_on(e.z, e.ldz, 2, 32);
+    e.vec = (e.y_dtype == SFB_F32 || rows_on16(e.y, e.ldy)) && rows_on16(e.z, e.ldz) && rows_on16(e.residual, e.ldr);
     CUtensorMap tmA, tmB;
-    int rc = A_MN ? operand_map(&tmA, p.A, p.dtype, p.K, p.M, p.lda, BK) : operand_map(&tmA, p.A, p.dtype, p.M, p.K, p.lda, BM);
+    int rc = A_MN ? operand_map(&tmA, p.A, p.dtype, p.K, p.R, p.lda, 64) : operand_map(&tmA, p.A, p.dtype, p.R, p.K, p.lda, BM);
     if (!rc)
-        rc = B_MN ? operand_map(&tmB, p.B, p.dtype, p.K, p.N, p.ldb, BK)
-                  : operand_map(&tmB, p.B, p.dtype, p.N, p.K, p.ldb, S::BNL);
+        rc = B_MN ? operand_map(&tmB, p.B, p.dtype, p.K, p.C, p.ldb, 64)
+                  : operand_map(&tmB, p.B, p.dtype, p.C, p.K, p.ldb, S::BNL);
     if (rc) return rc;
     Tiles t;
-    t.mt = (int)((p.M + 2 * BM - 1) / (2 * BM));
-    t.nt = (int)((p.N + BN - 1) / BN);
-    t.total = t.mt * t.nt;
+    t.rt = (int)((p.R + 2 * BM - 1) / (2 * BM));
+    t.ct = (int)((p.C + BN - 1) / BN);
+    t.total = t.rt * t.ct;
     kernel<<<2 * std::min(t.total, sm_count() / 2), THREADS, S::SMEM, st>>>(
-        tmA, tmB, (int)((p.K + BK - 1) / BK), p.M, p.N, t, e, wait_polls() ? wait_polls() : kSpinLimit,
+        tmA, tmB, (int)((p.K + S::BK - 1) / S::BK), p.R, p.C, t, e, wait_polls() ? wait_polls() : kSpinLimit,
         wait_stall());
     return check_launch("sf tensor linear");
 }
@@ -741,20 +727,20 @@ int launch(const Problem &p, Epilogue e, cudaStream_t st) {
 // Columns of a tile.  A stage of 256 columns takes its 512 cycles of products, one
 // of 128 about 390 (48 KB of shared memory's traffic against 256 cycles of products),
 // so the wider tile wins unless it leaves pairs without one.
-int columns(int64_t M, int64_t N) {
-    const int64_t mt = (M + 2 * BM - 1) / (2 * BM), n = sm_count() / 2;
-    const int64_t wide = (mt * ((N + 255) / 256) + n - 1) / n, narrow = (mt * ((N + 127) / 128) + n - 1) / n;
+int columns(int64_t R, int64_t C) {
+    const int64_t rt = (R + 2 * BM - 1) / (2 * BM), n = sm_count() / 2;
+    const int64_t wide = (rt * ((C + 255) / 256) + n - 1) / n, narrow = (rt * ((C + 127) / 128) + n - 1) / n;
     return 512 * wide <= 390 * narrow ? 256 : 128;
 }
 
 int check(const Problem &p, const char *what) {
     if (p.dtype != SFB_BF16 && p.dtype != SFB_F16) return set_error(SFB_EINVAL, "%s: element type %d", what, p.dtype);
-    if (p.M < 0 || p.N < 0 || p.K < 1) return set_error(SFB_EINVAL, "%s: bad shape", what);
-    if (p.M >= (1ll << 31) || p.N >= (1ll << 31) || p.K >= (1ll << 31) || p.lda >= (1ll << 36) || p.ldb >= (1ll << 36) ||
-        ((p.M + BM - 1) / BM) * ((p.N + 127) / 128) >= (1ll << 31))
-        return set_error(SFB_ERANGE, "%s: a size of %lld x %lld x %lld", what, (long long)p.M, (long long)p.N,
+    if (p.R < 0 || p.C < 0 || p.K < 1) return set_error(SFB_EINVAL, "%s: bad shape", what);
+    if (p.R >= (1ll << 31) - 512 || p.C >= (1ll << 31) - 512 || p.K >= (1ll << 31) - 512 || p.lda >= (1ll << 36) ||
+        p.ldb >= (1ll << 36) || ((p.R + 2 * BM - 1) / (2 * BM)) * ((p.C + 127) / 128) >= (1ll << 31) - 512)
+        return set_error(SFB_ERANGE, "%s: a size of %lld x %lld x %lld", what, (long long)p.R, (long long)p.C,
                          (long long)p.K);
-    if (p.M == 0 || p.N == 0) return SFB_OK;
+    if (p.R == 0 || p.C == 0) return SFB_OK;
     if (!p.A || !p.B) return set_error(SFB_EINVAL, "%s: null pointer", what);
     if (((reinterpret_cast<uintptr_t>(p.A) | reinterpret_cast<uintptr_t>(p.B)) & 15) || p.lda % 8 || p.ldb % 8)
         return set_error(SFB_EINVAL, "%s: operands and their rows must be aligned to 16 bytes", what);
@@ -763,7 +749,7 @@ int check(const Problem &p, const char *what) {
 
 template <bool A_MN, bool B_MN, int ACT>
 int launch_typed(const Problem &p, const Epilogue &e, cudaStream_t st) {
-    const bool wide = columns(p.M, p.N) == 256;
+    const bool wide = columns(p.R, p.C) == 256;
     if (p.dtype == SFB_BF16)
         return wide ? launch<__nv_bfloat16, A_MN, B_MN, 256, ACT>(p, e, st)
                     : launch<__nv_bfloat16, A_MN, B_MN, 128, ACT>(p, e, st);
@@ -778,7 +764,7 @@ extern "C" int sfb_tensor_linear(int dtype, const void *x, int64_t ldx, const vo
                                  const void *residual, int64_t ldr, void *y, int64_t ldy, void *z, int64_t ldz,
                                  int64_t M, int64_t N, int64_t K, sfb_stream stream) {
     using namespace sfb;
-    const Problem p{x, codes, ldx, ldw, M, N, K, dtype};
+    const Problem p{codes, x, ldw, ldx, N, M, K, dtype};
     const int rc = check(p, "sfb_tensor_linear");
     if (rc) return rc;
     if (bits < 4 || bits > 8) return set_error(SFB_EINVAL, "sfb_tensor_linear: width %d is not in 4..8", bits);
@@ -809,7 +795,7 @@ extern "C" int sfb_tensor_grad_x(int dtype, const void *dzs, int64_t ldd, const 
                                  sfb_stream stream) {
     using namespace sfb;
     if (N < 1) return set_error(SFB_EINVAL, "sfb_tensor_grad_x: no channels");
-    const Problem p{dzs, codes, ldd, ldw, M, K, N, dtype};
+    const Problem p{codes, dzs, ldw, ldd, K, M, N, dtype};
     const int rc = check(p, "sfb_tensor_grad_x");
     if (rc) return rc;
     if (bits < 4 || bits > 8) return set_error(SFB_EINVAL, "sfb_tensor_grad_x: width %d is not in 4..8", bits);
@@ -822,14 +808,14 @@ extern "C" int sfb_tensor_grad_x(int dtype, const void *dzs, int64_t ldd, const 
     e.unit = top ? 1.0f / (float)(1 << (bits - 1)) : 1.0f;
     e.y_dtype = dtype;
     e.ldy = ldy;
-    return launch_typed<false, true, SFB_ACT_NONE>(p, e, static_cast<cudaStream_t>(stream));
+    return launch_typed<true, false, SFB_ACT_NONE>(p, e, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int sfb_tensor_grad_w(int dtype, const void *dz, int64_t ldd, const void *x, int64_t ldx, void *dw,
                                  int dw_dtype, int64_t ldy, int64_t M, int64_t N, int64_t K, sfb_stream stream) {
     using namespace sfb;
     if (M < 1) return set_error(SFB_EINVAL, "sfb_tensor_grad_w: no rows");
-    const Problem p{dz, x, ldd, ldx, N, K, M, dtype};
+    const Problem p{x, dz, ldx, ldd, K, N, M, dtype};
     const int rc = check(p, "sfb_tensor_grad_w");
     if (rc) return rc;
     if (dw_dtype != SFB_F32 && dw_dtype != SFB_BF16 && dw_dtype != SFB_F16)
