@@ -24,8 +24,11 @@
 // One launch takes a table of tensors as its parameter (no table in device
 // memory: nothing to copy, and nothing that two captured graphs could share).
 // A CTA takes one chunk of one tensor, found by bisection over the chunk counts.
-// Memory bound: 28 bytes an element with float32 p, g and moments, 16.06 with sf8
-// moments, 10.06 with 16-bit p and g besides.
+// Float32 moments: bound by memory, 28 bytes an element with float32 p and g, 6430
+// GB/s for 46.5 M elements (202 us).  sf8 moments: 16.06 bytes an element with float32
+// p and g, 10.06 with 16-bit ones, against about 88 instructions of arithmetic: 136
+// us for 46.5 M float32 elements (5500 GB/s), 328 us for 117 M of bf16 (3590 GB/s,
+// bound by instruction issue).
 #include <math.h>
 
 #include <algorithm>
@@ -37,9 +40,10 @@
 namespace sfb {
 namespace {
 
-constexpr int AT = 256;                       // threads of a CTA
+constexpr int AT = 128;                       // threads of a CTA: 8 of them an SM were faster than 4 of 256 (136 against 155 us)
 constexpr int AB = 256;                       // elements of one sf8 block
-constexpr int CHUNK = 4096;                   // elements of one CTA
+// elements of one CTA: sf8 blocks in turn to its warps
+template <bool SF8> constexpr int CHUNK = SF8 ? 8192 : 4096;
 constexpr float UNIT2 = (float)(1.0 / 16129.0), UNIT4 = (float)(1.0 / 260144641.0);
 constexpr float TOP2 = 16129.0f, TOP4 = 260144641.0f;
 
@@ -118,33 +122,105 @@ __device__ __forceinline__ uint32_t mixed(uint32_t i, uint32_t seed) {
     return h;
 }
 
-template <int POWER>
-__device__ __forceinline__ float level(float c) {
-    const float c2 = __fmul_rn(c, c);
-    return POWER == 2 ? c2 : __fmul_rn(c2, c2);
+// Two elements at a time: one instruction for both, each result rounded as the
+// scalar operation's.  Unlike the scalar forms, a mul2 whose result is added may be
+// contracted with the addition: products that are summed are scalar (`once`).
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\t"
+        "mov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\t"
+        "mov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// a - b: b (-1) + a, the product exact
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return fma2(b, both(-1.0f), a); }
+
+__device__ __forceinline__ float2 once(float2 a, float2 b) { return make_float2(__fmul_rn(a.x, b.x), __fmul_rn(a.y, b.y)); }
+
+// 1 where a < b, else 0
+__device__ __forceinline__ float less(float a, float b) {
+    float r;
+    asm("set.lt.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 less2(float2 a, float2 b) { return make_float2(less(a.x, b.x), less(a.y, b.y)); }
+
+__device__ __forceinline__ float root_ftz(float x) {
+    float r;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 
-// the code of t = |value| * top / s: the largest c with level(c) <= t, or the next one by the dither
-template <int POWER>
-__device__ __forceinline__ int code_of(float t, float u) {
-    float r = sqrt_fast(t);
-    if (POWER == 4) r = sqrt_fast(r);
-    int k = t < 3.0e38f ? (int)r : 127;               // NaN and infinity: any code, the scale tells
-    float c = (float)k;
-    if (level<POWER>(c) > t) c -= 1.0f;
-    else if (level<POWER>(c + 1.0f) <= t) c += 1.0f;
-    if (c >= 127.0f) return 127;
-    const float low = level<POWER>(c), wide = __fsub_rn(level<POWER>(c + 1.0f), low);
-    if (__fmul_rn(u, wide) < __fsub_rn(t, low)) c += 1.0f;
-    if (POWER == 4 && t > 0.0f) c = fmaxf(c, 1.0f);
-    return (int)c;
+__device__ __forceinline__ float top_nan(float a, float b) {           // NaN above all
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
-__device__ __forceinline__ uint32_t warp_top(const float (&x)[8]) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(x[j]) & 0x7FFFFFFFu);
-    return __reduce_max_sync(0xffffffffu, top);       // magnitudes order as their bits, NaN above all
+template <int POWER>
+__device__ __forceinline__ float2 level(float2 c) {
+    const float2 c2 = mul2(c, c);
+    return POWER == 2 ? c2 : mul2(c2, c2);
+}
+
+// the level of c + 1, its last product not to be contracted
+template <int POWER>
+__device__ __forceinline__ float2 above(float2 c) {
+    const float2 d = add2(c, both(1.0f)), d2 = mul2(d, d);
+    return POWER == 2 ? once(d, d) : once(d2, d2);
+}
+
+// Conversions between integers and floats share a unit of 16 lanes with the square
+// roots, and ten of them an element made the kernel wait for it (281 us for 46.5 M
+// float32 elements; 199 without them, 136 with two elements to an instruction).  Adding 2^23 to a float in [0, 2^23) leaves the nearest
+// integer in its low bits, and putting an integer there and subtracting is the way back.
+constexpr float MAGIC = 8388608.0f;
+
+// bytes J and J + 1 of a word of codes, exactly
+template <int J>
+__device__ __forceinline__ float2 code_values(uint32_t biased) {        // each byte c + 128
+    return add2(make_float2(__uint_as_float(__byte_perm(biased, 0x4B000000u, 0x7650 | J)),
+                            __uint_as_float(__byte_perm(biased, 0x4B000000u, 0x7650 | (J + 1)))),
+                both(-MAGIC - 128.0f));
+}
+
+// The codes of t = |value| * top / s as floats in [0, 127]: the largest c with
+// level(c) <= t, or the next one by the dither u.  `root` is t^(1/POWER) to within a few
+// units, so its nearest integer is that c or one more.  Where t is not finite the
+// code is any: the scale tells.
+template <int POWER>
+__device__ __forceinline__ float2 codes_of(float2 t, float2 root, float2 u) {
+    float2 c = add2(add2(root, both(MAGIC)), both(-MAGIC));
+    c = sub2(c, less2(t, level<POWER>(c)));
+    const float2 low = POWER == 2 ? once(c, c) : once(mul2(c, c), mul2(c, c));
+    // the step to the next level: 2 c + 1 of the squares, exactly
+    const float2 wide = POWER == 2 ? fma2(c, both(2.0f), both(1.0f)) : sub2(above<POWER>(c), low);
+    c = add2(c, less2(mul2(u, wide), sub2(t, low)));
+    c.x = fminf(c.x, 127.0f);
+    c.y = fminf(c.y, 127.0f);
+    if (POWER == 4) {
+        if (t.x > 0.0f) c.x = fmaxf(c.x, 1.0f);
+        if (t.y > 0.0f) c.y = fmaxf(c.y, 1.0f);
+    }
+    return c;
 }
 
 __device__ __forceinline__ float scale_of(uint32_t bits) {
@@ -152,76 +228,143 @@ __device__ __forceinline__ float scale_of(uint32_t bits) {
     return s < 1e-30f ? 0.0f : s;
 }
 
-// a block of 256 elements by one warp: lane l has elements 4 l .. 4 l + 3 of each half
+// the low bytes of four floats c + 1.5 2^23
+__device__ __forceinline__ uint32_t bytes_of(const float (&c)[4]) {
+    const float m = 1.5f * MAGIC;
+    const uint32_t a = __byte_perm(__float_as_uint(__fadd_rn(c[0], m)), __float_as_uint(__fadd_rn(c[1], m)), 0x0040);
+    const uint32_t b = __byte_perm(__float_as_uint(__fadd_rn(c[2], m)), __float_as_uint(__fadd_rn(c[3], m)), 0x0040);
+    return __byte_perm(a, b, 0x5410);
+}
+
+// A block of 256 elements by one warp: lane l has elements 4 l .. 4 l + 3 of each half.
+// What it loads.  (Loading the next block under this one's arithmetic was slower: 22
+// registers more leave 3 CTAs an SM and spill, 157 and 411 us against 151 and 342
+// for 46.5 M float32 and 117 M bf16 elements.)
 template <typename T>
-__device__ __forceinline__ void block_sf8(const Entry &e, int64_t blk, const Coefs &c, int lane) {
+struct Loaded {
+    Vec<T, 4> p[2], g[2];
+    uint32_t cm[2], cv[2];
+    float sm, sv;
+};
+
+template <typename T>
+__device__ __forceinline__ void load_block(const Entry &e, int64_t blk, int lane, Loaded<T> &q) {
     const int64_t base = blk * AB;
-    T *p = static_cast<T *>(e.p);
-    const T *g = static_cast<const T *>(e.g);
-    int8_t *mc = static_cast<int8_t *>(e.m), *vc = static_cast<int8_t *>(e.v);
-    const bool whole = base + AB <= e.n;
-    float P[8], G[8], M[8], V[8];
-    char4 cm[2], cv[2];
-    const float sm = e.ms[blk], sv = e.vs[blk];
+    const T *p = static_cast<const T *>(e.p), *g = static_cast<const T *>(e.g);
+    const uint8_t *mc = static_cast<const uint8_t *>(e.m), *vc = static_cast<const uint8_t *>(e.v);
+    q.sm = e.ms[blk];
+    q.sv = e.vs[blk];
+    if (base + AB <= e.n && e.vec) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int64_t i = base + h * 128 + lane * 4;
+            q.g[h] = *reinterpret_cast<const Vec<T, 4> *>(g + i);
+            q.cm[h] = *reinterpret_cast<const uint32_t *>(mc + i);
+            q.cv[h] = *reinterpret_cast<const uint32_t *>(vc + i);
+            q.p[h] = *reinterpret_cast<const Vec<T, 4> *>(p + i);
+        }
+        return;
+    }
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         const int64_t i = base + h * 128 + lane * 4;
-        load4(g, i, e.n, e.vec, *reinterpret_cast<float(*)[4]>(G + 4 * h));
-        if (whole) {
-            cm[h] = *reinterpret_cast<const char4 *>(mc + i);
-            cv[h] = *reinterpret_cast<const char4 *>(vc + i);
-        } else {
-            signed char a[4], b[4];
+        q.cm[h] = q.cv[h] = 0;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                a[j] = i + j < e.n ? mc[i + j] : (signed char)0;
-                b[j] = i + j < e.n ? vc[i + j] : (signed char)0;
+        for (int j = 0; j < 4; j++) {
+            const bool in = i + j < e.n;
+            q.g[h].v[j] = in ? g[i + j] : from_f<T>(0.0f);
+            q.p[h].v[j] = in ? p[i + j] : from_f<T>(0.0f);
+            if (in) {
+                q.cm[h] |= (uint32_t)mc[i + j] << (8 * j);
+                q.cv[h] |= (uint32_t)vc[i + j] << (8 * j);
             }
-            cm[h] = make_char4(a[0], a[1], a[2], a[3]);
-            cv[h] = make_char4(b[0], b[1], b[2], b[3]);
         }
-        load4(p, i, e.n, e.vec, *reinterpret_cast<float(*)[4]>(P + 4 * h));
     }
-    const float um = __fmul_rn(sm, UNIT2), uv = __fmul_rn(sv, UNIT4);
+}
+
+template <typename T>
+__device__ __forceinline__ void block_sf8(const Entry &e, int64_t blk, const Coefs &c, int lane, const Loaded<T> &q) {
+    const int64_t base = blk * AB;
+    T *p = static_cast<T *>(e.p);
+    uint8_t *mc = static_cast<uint8_t *>(e.m), *vc = static_cast<uint8_t *>(e.v);
+    const bool whole = base + AB <= e.n;
+    const uint32_t *cm = q.cm, *cv = q.cv;
+    const float sm = q.sm, sv = q.sv;
+    float P[8], G[8];
+    float2 M[4], V[4], S[4];                        // pairs of elements
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        const char4 a = cm[j / 4], b = cv[j / 4];
-        const int x = j % 4 == 0 ? a.x : j % 4 == 1 ? a.y : j % 4 == 2 ? a.z : a.w;
-        const int y = j % 4 == 0 ? b.x : j % 4 == 1 ? b.y : j % 4 == 2 ? b.z : b.w;
-        M[j] = __fmul_rn((float)(x * abs(x)), um);
-        const float y2 = (float)(y * y);
-        V[j] = __fmul_rn(__fmul_rn(y2, y2), uv);
-        moments(M[j], V[j], G[j], c);
-        P[j] = stepped(P[j], M[j], V[j], c);
+        P[j] = to_f(q.p[j / 4].v[j % 4]);
+        G[j] = to_f(q.g[j / 4].v[j % 4]);
     }
-    const float sm1 = scale_of(warp_top(M)), sv1 = scale_of(warp_top(V));
+    const float um = __fmul_rn(sm, UNIT2), uv = __fmul_rn(sv, UNIT4);
+    float tm = 0.0f, tv = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t a = cm[j / 2] ^ 0x80808080u, b = cv[j / 2] ^ 0x80808080u;
+        const float2 x = j % 2 ? code_values<2>(a) : code_values<0>(a), y = j % 2 ? code_values<2>(b) : code_values<0>(b);
+        const float2 gg = make_float2(G[2 * j], G[2 * j + 1]);
+        const float2 m0 = mul2(mul2(x, make_float2(fabsf(x.x), fabsf(x.y))), both(um)), v0 = mul2(level<4>(y), both(uv));
+        M[j] = add2(once(m0, both(c.b1)), once(gg, both(c.a1)));
+        V[j] = add2(once(v0, both(c.b2)), once(mul2(gg, both(c.a2)), gg));
+        tm = top_nan(tm, top_nan(fabsf(M[j].x), fabsf(M[j].y)));
+        tv = top_nan(tv, top_nan(V[j].x, V[j].y));
+        // (2^-126 more, so that a v below float32's normal range is not taken for 0; its root is far below any eps)
+        const float2 vv = add2(V[j], both(0x1p-126f));
+        S[j] = make_float2(root_ftz(vv.x), root_ftz(vv.y));
+        const float2 d = fma2(S[j], both(c.root), both(c.eps));
+        const float2 by = mul2(M[j], make_float2(rcp_fast(d.x), rcp_fast(d.y)));
+        const float2 r = fma2(by, both(-c.size), mul2(make_float2(P[2 * j], P[2 * j + 1]), both(c.shrink)));
+        P[2 * j] = r.x;
+        P[2 * j + 1] = r.y;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+        store4(p, base + h * 128 + lane * 4, e.n, e.vec, *reinterpret_cast<float(*)[4]>(P + 4 * h));
+    // magnitudes order as their bits, NaN above all
+    const float sm1 = scale_of(__reduce_max_sync(0xffffffffu, __float_as_uint(tm) & 0x7FFFFFFFu));
+    const float sv1 = scale_of(__reduce_max_sync(0xffffffffu, __float_as_uint(tv) & 0x7FFFFFFFu));
     const float im = sm1 != 0.0f ? __fdiv_rn(TOP2, sm1) : 0.0f, iv = sv1 != 0.0f ? __fdiv_rn(TOP4, sv1) : 0.0f;
+    const float siv = sqrt_fast(iv);
     if (lane == 0) {
         e.ms[blk] = sm1;
         e.vs[blk] = sv1;
     }
+    const uint32_t seed = e.seed + c.dither, i0 = (uint32_t)base + lane * 4;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const int64_t i = base + h * 128 + lane * 4;
-        store4(p, i, e.n, e.vec, *reinterpret_cast<float(*)[4]>(P + 4 * h));
-        int a[4], b[4];
+        float a[4], b[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t r = mixed((uint32_t)(i + j), e.seed + c.dither);
-            const float m = M[4 * h + j];
-            const int k = code_of<2>(__fmul_rn(fabsf(m), im), (float)(r & 0xFFFFu) * 0x1p-16f);
-            a[j] = m < 0.0f ? -k : k;
-            b[j] = code_of<4>(__fmul_rn(V[4 * h + j], iv), (float)(r >> 16) * 0x1p-16f);
+        for (int k = 0; k < 2; k++) {
+            const int j = 2 * h + k;
+            const uint32_t r0 = mixed(i0 + h * 128 + 2 * k, seed), r1 = mixed(i0 + h * 128 + 2 * k + 1, seed);
+            // a 16-bit number u under 2^23 as a float, then (2^23 + u) 2^-16 - 2^7 = u 2^-16 exactly
+            const float2 lo = fma2(make_float2(__uint_as_float(__byte_perm(r0, 0x4B000000u, 0x7610)),
+                                               __uint_as_float(__byte_perm(r1, 0x4B000000u, 0x7610))),
+                                   both(0x1p-16f), both(-128.0f));
+            const float2 hi = fma2(make_float2(__uint_as_float(__byte_perm(r0, 0x4B000000u, 0x7632)),
+                                               __uint_as_float(__byte_perm(r1, 0x4B000000u, 0x7632))),
+                                   both(0x1p-16f), both(-128.0f));
+            const float2 t = mul2(make_float2(fabsf(M[j].x), fabsf(M[j].y)), both(im)), tq = mul2(V[j], both(iv));
+            const float2 rq = mul2(S[j], both(siv));
+            const float2 x = codes_of<2>(t, make_float2(root_ftz(t.x), root_ftz(t.y)), lo);
+            const float2 y = codes_of<4>(tq, make_float2(root_ftz(rq.x), root_ftz(rq.y)), hi);
+            a[2 * k] = copysignf(x.x, M[j].x);
+            a[2 * k + 1] = copysignf(x.y, M[j].y);
+            b[2 * k] = y.x;
+            b[2 * k + 1] = y.y;
         }
+        const int64_t i = base + h * 128 + lane * 4;
+        const uint32_t x = bytes_of(a), y = bytes_of(b);
         if (whole) {
-            *reinterpret_cast<char4 *>(mc + i) = make_char4(a[0], a[1], a[2], a[3]);
-            *reinterpret_cast<char4 *>(vc + i) = make_char4(b[0], b[1], b[2], b[3]);
+            *reinterpret_cast<uint32_t *>(mc + i) = x;
+            *reinterpret_cast<uint32_t *>(vc + i) = y;
         } else {
 #pragma unroll
             for (int j = 0; j < 4; j++)
                 if (i + j < e.n) {
-                    mc[i + j] = (int8_t)a[j];
-                    vc[i + j] = (int8_t)b[j];
+                    mc[i + j] = (uint8_t)(x >> (8 * j));
+                    vc[i + j] = (uint8_t)(y >> (8 * j));
                 }
         }
     }
@@ -259,15 +402,20 @@ __device__ __forceinline__ int tensor_of(const Table<CAP> &t, uint32_t chunk) {
 }
 
 template <typename T, bool SF8, int CAP>
-__global__ void __launch_bounds__(AT) adamw_kernel(const __grid_constant__ Table<CAP> t, Coefs given,
+__global__ void __launch_bounds__(AT, SF8 ? 8 : 12) adamw_kernel(const __grid_constant__ Table<CAP> t, Coefs given,
                                                    const Coefs *__restrict__ on_device) {
     const int k = tensor_of(t, blockIdx.x);
     const Entry &e = t.e[k];
     const Coefs c = on_device ? *on_device : given;
-    const int64_t first = (int64_t)(blockIdx.x - t.start[k]) * CHUNK, last = min(e.n, first + CHUNK);
+    const int64_t first = (int64_t)(blockIdx.x - t.start[k]) * CHUNK<SF8>, last = min(e.n, first + CHUNK<SF8>);
     if constexpr (SF8) {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        for (int64_t b = first / AB + warp; b * AB < last; b += AT / 32) block_sf8<T>(e, b, c, lane);
+#pragma unroll 1
+        for (int64_t b = first / AB + warp; b * AB < last; b += AT / 32) {
+            Loaded<T> q;
+            load_block(e, b, lane, q);
+            block_sf8<T>(e, b, c, lane, q);
+        }
     } else {
 #pragma unroll 2
         for (int64_t i = first + 4 * threadIdx.x; i < last; i += 4 * AT) four_f32<T>(e, i, c);
@@ -310,9 +458,10 @@ template <int CAP>
 __global__ void __launch_bounds__(AT) values_kernel(const __grid_constant__ Table<CAP> t, int power) {
     const int k = tensor_of(t, blockIdx.x);
     const Entry &e = t.e[k];
-    const int64_t first = (int64_t)(blockIdx.x - t.start[k]) * CHUNK, last = min(e.n, first + CHUNK);
+    const int64_t first = (int64_t)(blockIdx.x - t.start[k]) * CHUNK<false>, last = min(e.n, first + CHUNK<false>);
     const int8_t *code = static_cast<const int8_t *>(e.g);
     float *out = static_cast<float *>(e.p);
+#pragma unroll 4
     for (int64_t i = first + 4 * threadIdx.x; i < last; i += 4 * AT) {
         const float s = e.ms[i / AB], u = __fmul_rn(s, power == 2 ? UNIT2 : UNIT4);
         float r[4];
@@ -337,7 +486,7 @@ __global__ void __launch_bounds__(AT) values_kernel(const __grid_constant__ Tabl
 constexpr int WORDS = 8;                      // of one table entry as the caller gives it
 constexpr int MAX_CAP = 448;
 
-template <int CAP, typename F>
+template <int CAP, bool SF8, typename F>
 int each_table(const int64_t *rows, int count, F launch) {
     // one launch for every CAP tensors, or sooner where the grid would pass 2^30 chunks
     Table<CAP> t;
@@ -349,7 +498,7 @@ int each_table(const int64_t *rows, int count, F launch) {
             const int64_t *r = rows + (int64_t)at * WORDS;
             const int64_t n = r[6];
             if (n == 0) continue;
-            const uint64_t need = (uint64_t)((n + CHUNK - 1) / CHUNK);
+            const uint64_t need = (uint64_t)((n + CHUNK<SF8> - 1) / CHUNK<SF8>);
             if (need > (1u << 30)) return set_error(SFB_ERANGE, "sfb_adamw: a tensor of %lld elements", (long long)n);
             if (chunks + need > (1u << 30)) break;
             Entry &e = t.e[t.count];
@@ -407,7 +556,7 @@ int check_overlap(const int64_t *rows, int count, int size, bool sf8) {
 
 template <typename T, bool SF8, int CAP>
 int run_adamw(const int64_t *rows, int count, const Coefs &c, const Coefs *dev, cudaStream_t st) {
-    return each_table<CAP>(rows, count, [&](Table<CAP> &t, unsigned grid) {
+    return each_table<CAP, SF8>(rows, count, [&](Table<CAP> &t, unsigned grid) {
         for (int i = 0; i < t.count; i++) {
             Entry &e = t.e[i];
             const uintptr_t a = reinterpret_cast<uintptr_t>(e.p) | reinterpret_cast<uintptr_t>(e.g);
@@ -488,11 +637,11 @@ extern "C" int sfb_sf8_values(const int64_t *table, int count, int power, sfb_st
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (count <= 16)
-        return each_table<16>(table, count, [&](Table<16> &t, unsigned grid) {
+        return each_table<16, false>(table, count, [&](Table<16> &t, unsigned grid) {
             values_kernel<16><<<grid, AT, 0, st>>>(t, power);
             return check_launch("sfb_sf8_values");
         });
-    return each_table<MAX_CAP>(table, count, [&](Table<MAX_CAP> &t, unsigned grid) {
+    return each_table<MAX_CAP, false>(table, count, [&](Table<MAX_CAP> &t, unsigned grid) {
         values_kernel<MAX_CAP><<<grid, AT, 0, st>>>(t, power);
         return check_launch("sfb_sf8_values");
     });
