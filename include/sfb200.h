@@ -376,53 +376,61 @@ SFB_API int sfb_sweep(int op, int bits, int64_t a_lo, int64_t a_hi, uint32_t *ro
 /* The tensor-core linear: y = act(x Wq^T + b) + r over sf4..sf8 codes, Wq[n, k]
  * = codes[n, k] 2^-(bits-1) scale[n], summed in float32.  The reference computes
  * a converted layer on the chip's integer units (src/sf/torch/_core.py:336-433);
- * these have no counterpart there.  x, y, r: dtype, SFB_BF16 or SFB_F16.
+ * these have no counterpart there.
  *
- * sfb_code_quantize: the codes of a float weight (N rows of K, ldw apart, any of
- * SFB_F32 / BF16 / F16) and their scales: scale = max|w| / m over the row or, with
- * per_channel 0, over the matrix (1 where that is 0), code = rint(w / scale
- * 2^(bits-1)) within +-M.  codes_dtype SFB_I8 packs them, SFB_BF16 / F16 writes
- * the product's operand.  work: 4 N bytes.  A row with a NaN or an infinity gets
- * it as its scale.
- *
- * sfb_code_expand: packed codes as the product's operand.
- *
- * sfb_tensor_linear: the forward product.  codes of type dtype.  z (nullable)
- * receives the pre-activation in fp16 for the backward pass.
- * sfb_slope: dz = dy act'(z) and / or dzs = dz scale / top (top NULL: dz scale
- * 2^-(bits-1)), rows ldd apart (a multiple of 8, padding written as 0), and db =
- * sum of dz over the rows.  work: sfb_slope_workspace(M, N) bytes when db is wanted.
- * sfb_tensor_grad_x: dx = dzs codes (top as in sfb_slope).
- * sfb_tensor_grad_w: dw = dz^T x.
- *
- * Operands of the products start on 16-byte boundaries and their row strides are
- * multiples of 8 elements; outputs, residual and bias may start anywhere.
- * sfb_tensor_failures: how many CTAs of these products have given up a bounded
- * wait on the current device since the library was loaded (their outputs are
- * NaN); it waits for the device.  sfb_wide_wait_limit bounds these waits too. */
-SFB_API int sfb_code_quantize(const void *w, int dtype, int64_t N, int64_t K, int64_t ldw, int bits, int per_channel,
-                              void *codes, int64_t ldc, int codes_dtype, float *scale, void *work, sfb_stream stream);
-SFB_API int sfb_code_expand(const int8_t *codes, int64_t N, int64_t K, int64_t ldc, void *out, int64_t ldo, int dtype,
-                            sfb_stream stream);
-SFB_API int sfb_tensor_linear(int dtype, const void *x, int64_t ldx, const void *codes, int64_t ldw, const float *scale,
-                              int bits, const void *bias, int bias_dtype, int act, const void *residual, int64_t ldr,
-                              void *y, int64_t ldy, void *z, int64_t ldz, int64_t M, int64_t N, int64_t K,
-                              sfb_stream stream);
-/* the same from packed codes (rows anywhere, ldc apart) for at most
- * SFB_SMALL_ROWS rows of x: the codes are read once and not expanded */
+ * One struct describes a call; every field has 8 bytes.  Matrices are row-major
+ * with a row stride in elements (ld*).  x, y, residual and their gradients are of
+ * `dtype` (SFB_BF16 or SFB_F16) and may start anywhere, but the backward pass
+ * reads x (or the forward pass's xpad), codes and its scratch on 16-byte
+ * boundaries with row strides that are multiples of 8. */
+typedef struct sfb_tensor_call {
+    int64_t dtype, bits, act, M, N, K;      /* x is M x K, the weight N x K */
+    const void *x;
+    int64_t ldx;
+    void *xpad;                             /* M x ldp of dtype, where x's rows do not start on 16 bytes */
+    int64_t ldp;
+    const void *w;                          /* float weight of w_dtype, or packed codes (SFB_I8) */
+    int64_t ldw, w_dtype, per_channel;
+    void *codes;                            /* N x ldc of dtype: written by the forward pass, read by the backward */
+    int64_t ldc;
+    const float *scale;                     /* N: written where the weight is float */
+    const void *bias;                       /* N of bias_dtype, or NULL */
+    int64_t bias_dtype;
+    const void *residual;
+    int64_t ldr;
+    void *y;                                /* the result; in the backward pass its gradient, which is read */
+    int64_t ldy;
+    void *z;                                /* M x N in fp16: the pre-activation, kept for the backward pass (nullable) */
+    int64_t ldz;
+    void *work;                             /* forward, one scale: 4 N bytes; backward with db: sfb_tensor_sums bytes */
+    float *top;                             /* backward, fp16 and a scale a channel: one float */
+    void *dz, *dzs;                         /* backward: M x ldd of dtype */
+    int64_t ldd;
+    void *dx, *dw, *db;                     /* the gradients that are wanted: M x K, N x K of w_dtype, N of db_dtype */
+    int64_t db_dtype;
+} sfb_tensor_call;
+
+/* The forward pass.  A float weight is quantized first (by sfb_code_quantize's rule);
+ * packed codes are expanded into `codes`, or where that is NULL, for at most
+ * SFB_SMALL_ROWS rows and no z, read as they are. */
 #define SFB_SMALL_ROWS 64
-SFB_API int sfb_tensor_linear_small(int dtype, const void *x, int64_t ldx, const int8_t *codes, int64_t ldc,
-                                    const float *scale, int bits, const void *bias, int bias_dtype, int act,
-                                    const void *residual, int64_t ldr, void *y, int64_t ldy, int64_t M, int64_t N,
-                                    int64_t K, sfb_stream stream);
-SFB_API int64_t sfb_slope_workspace(int64_t M, int64_t N);
-SFB_API int sfb_slope(int dtype, int act, const void *dy, int64_t ldy, const void *z, int64_t ldz, int64_t M, int64_t N,
-                      const float *scale, int bits, const float *top, void *dz, void *dzs, int64_t ldd, void *db,
-                      int db_dtype, void *work, sfb_stream stream);
-SFB_API int sfb_tensor_grad_x(int dtype, const void *dzs, int64_t ldd, const void *codes, int64_t ldw, const float *top,
-                              int bits, void *dx, int64_t ldy, int64_t M, int64_t N, int64_t K, sfb_stream stream);
-SFB_API int sfb_tensor_grad_w(int dtype, const void *dz, int64_t ldd, const void *x, int64_t ldx, void *dw,
-                              int dw_dtype, int64_t ldy, int64_t M, int64_t N, int64_t K, sfb_stream stream);
+SFB_API int sfb_tensor_forward(const sfb_tensor_call *call, sfb_stream stream);
+
+/* The backward pass: dz = dy act'(z), dx = (dz scale) codes, dw = dz^T x (straight
+ * through the rounding), db = the sum of dz over the rows. */
+SFB_API int64_t sfb_tensor_sums(int64_t M, int64_t N);
+SFB_API int sfb_tensor_backward(const sfb_tensor_call *call, sfb_stream stream);
+
+/* The packed int8 codes of a float weight (N rows of K, ldw apart; SFB_F32 / BF16 /
+ * F16) and their scales: scale = max|w| / m over the row or, with per_channel 0, over the
+ * matrix (1 where that is 0), code = rint(w / scale 2^(bits-1)) within +-M.  work:
+ * 4 N bytes (per_channel 0).  A row with a NaN or an infinity gets it as its scale. */
+SFB_API int sfb_code_quantize(const void *w, int dtype, int64_t N, int64_t K, int64_t ldw, int bits, int per_channel,
+                              void *codes, int64_t ldc, float *scale, void *work, sfb_stream stream);
+
+/* How many CTAs of these products have given up a bounded wait on the current
+ * device since the library was loaded (their outputs are NaN); waits for the
+ * device.  sfb_wide_wait_limit bounds these waits too. */
 SFB_API int sfb_tensor_failures(int64_t *count);
 
 /* One AdamW step over `count` tensors.  No counterpart in the reference, whose

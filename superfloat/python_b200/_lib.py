@@ -68,16 +68,10 @@ SIGNATURES = {
                                    _i64, _p, _i64, _p, _p]),
     "sfb_wide_finish": (_i32, [_i32, _i32, _p, _i64, _i64, _p, _p, _p, _p, _i32, _i32, _i32, _p, _p, _p, _p, _p,
                                _p, _p]),
-    "sfb_code_quantize": (_i32, [_p, _i32, _i64, _i64, _i64, _i32, _i32, _p, _i64, _i32, _p, _p, _p]),
-    "sfb_code_expand": (_i32, [_p, _i64, _i64, _i64, _p, _i64, _i32, _p]),
-    "sfb_tensor_linear": (_i32, [_i32, _p, _i64, _p, _i64, _p, _i32, _p, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _i64,
-                                 _i64, _i64, _p]),
-    "sfb_tensor_linear_small": (_i32, [_i32, _p, _i64, _p, _i64, _p, _i32, _p, _i32, _i32, _p, _i64, _p, _i64, _i64, _i64,
-                                       _i64, _p]),
-    "sfb_slope_workspace": (_i64, [_i64, _i64]),
-    "sfb_slope": (_i32, [_i32, _i32, _p, _i64, _p, _i64, _i64, _i64, _p, _i32, _p, _p, _p, _i64, _p, _i32, _p, _p]),
-    "sfb_tensor_grad_x": (_i32, [_i32, _p, _i64, _p, _i64, _p, _i32, _p, _i64, _i64, _i64, _i64, _p]),
-    "sfb_tensor_grad_w": (_i32, [_i32, _p, _i64, _p, _i64, _p, _i32, _i64, _i64, _i64, _i64, _p]),
+    "sfb_code_quantize": (_i32, [_p, _i32, _i64, _i64, _i64, _i32, _i32, _p, _i64, _p, _p, _p]),
+    "sfb_tensor_forward": (_i32, [_p, _p]),
+    "sfb_tensor_sums": (_i64, [_i64, _i64]),
+    "sfb_tensor_backward": (_i32, [_p, _p]),
     "sfb_tensor_failures": (_i32, [_p]),
     "sfb_adamw": (_i32, [_p, _i32, _i32, _i32, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
                          ctypes.c_double, _i64, ctypes.c_uint, _p, _p]),
@@ -362,25 +356,41 @@ ADAMW_WORDS, ADAMW_CONSTANTS = 8, 64       # words of a table entry, bytes of th
 ELEMENT = {"float32": 0, "bfloat16": 2, "float16": 3}
 
 
+_torch = None
+_raw_stream = None
+
+
+def _bind_torch():
+    """torch, and the address of a device's current stream (torch.cuda.current_stream's, without its object)."""
+    global _torch, _raw_stream
+    import torch
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda i: torch.cuda.current_stream(i).cuda_stream)
+    _torch = torch
+    return torch
+
+
 class on_device:
     """The launches inside go to CUDA device ``index``, on its current stream (the attribute ``stream``)."""
+
+    __slots__ = ("index", "before", "stream")
 
     def __init__(self, index: int):
         self.index = index
 
     def __enter__(self):
-        import torch
+        torch = _torch or _bind_torch()
         self.before = torch.cuda.current_device()
-        ensure_current(self.index)
+        if self.index not in _ready_devices:
+            ensure_current(self.index)
         if self.before != self.index:
             torch.cuda.set_device(self.index)
-        self.stream = torch.cuda.current_stream(self.index).cuda_stream
+        self.stream = _raw_stream(self.index)
         return self
 
     def __exit__(self, *exc):
         if self.before != self.index:
-            import torch
-            torch.cuda.set_device(self.before)
+            _torch.cuda.set_device(self.before)
 
 
 def ensure_current(index: int) -> None:
@@ -413,47 +423,33 @@ ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 I8 = 4                                     # SFB_I8: packed codes
 
 
-def code_quantize(w, dtype, N, K, ldw, bits, per_channel, codes, ldc, codes_dtype, scale, work, stream) -> None:
-    check(load().sfb_code_quantize(w, dtype, N, K, ldw, bits, int(per_channel), codes, ldc, codes_dtype, scale, work,
-                                   stream), "sf tensor linear (weight codes)")
-
-
-def code_expand(codes, N, K, ldc, out, ldo, dtype, stream) -> None:
-    check(load().sfb_code_expand(codes, N, K, ldc, out, ldo, dtype, stream), "sf tensor linear (packed codes)")
-
-
-def tensor_linear(dtype, x, ldx, codes, ldw, scale, bits, bias, bias_dtype, act, residual, ldr, y, ldy, z, ldz, M, N,
-                  K, stream) -> None:
-    check(load().sfb_tensor_linear(dtype, x, ldx, codes, ldw, scale, bits, bias, bias_dtype, act, residual, ldr, y,
-                                   ldy, z, ldz, M, N, K, stream), "sf tensor linear")
-
-
 SMALL_ROWS = 64                            # SFB_SMALL_ROWS
+# the fields of sfb_tensor_call, in order: 8 bytes each
+TENSOR_CALL = ("dtype", "bits", "act", "M", "N", "K", "x", "ldx", "xpad", "ldp", "w", "ldw", "w_dtype", "per_channel",
+               "codes", "ldc", "scale", "bias", "bias_dtype", "residual", "ldr", "y", "ldy", "z", "ldz", "work", "top",
+               "dz", "dzs", "ldd", "dx", "dw", "db", "db_dtype")
 
 
-def tensor_linear_small(dtype, x, ldx, codes, ldc, scale, bits, bias, bias_dtype, act, residual, ldr, y, ldy, M, N, K,
-                        stream) -> None:
-    check(load().sfb_tensor_linear_small(dtype, x, ldx, codes, ldc, scale, bits, bias, bias_dtype, act, residual, ldr,
-                                         y, ldy, M, N, K, stream), "sf tensor linear (few rows)")
+def code_quantize(w, dtype, N, K, ldw, bits, per_channel, codes, ldc, scale, work, stream) -> None:
+    check(load().sfb_code_quantize(w, dtype, N, K, ldw, bits, int(per_channel), codes, ldc, scale, work, stream),
+          "sf weight codes")
 
 
-def slope_workspace(M, N) -> int:
-    return int(load().sfb_slope_workspace(M, N))
+def tensor_forward(call, stream) -> None:
+    """``call``: an array("q") of TENSOR_CALL's fields."""
+    rc = load().sfb_tensor_forward(call.buffer_info()[0], stream)
+    if rc:
+        check(rc, "sf tensor linear")
 
 
-def slope(dtype, act, dy, ldy, z, ldz, M, N, scale, bits, top, dz, dzs, ldd, db, db_dtype, work, stream) -> None:
-    check(load().sfb_slope(dtype, act, dy, ldy, z, ldz, M, N, scale, bits, top, dz, dzs, ldd, db, db_dtype, work,
-                           stream), "sf tensor linear (activation's gradient)")
+def tensor_sums(M, N) -> int:
+    return int(load().sfb_tensor_sums(M, N))
 
 
-def tensor_grad_x(dtype, dzs, ldd, codes, ldw, top, bits, dx, ldy, M, N, K, stream) -> None:
-    check(load().sfb_tensor_grad_x(dtype, dzs, ldd, codes, ldw, top, bits, dx, ldy, M, N, K, stream),
-          "sf tensor linear (gradient of x)")
-
-
-def tensor_grad_w(dtype, dz, ldd, x, ldx, dw, dw_dtype, ldy, M, N, K, stream) -> None:
-    check(load().sfb_tensor_grad_w(dtype, dz, ldd, x, ldx, dw, dw_dtype, ldy, M, N, K, stream),
-          "sf tensor linear (gradient of the weight)")
+def tensor_backward(call, stream) -> None:
+    rc = load().sfb_tensor_backward(call.buffer_info()[0], stream)
+    if rc:
+        check(rc, "sf tensor linear (backward)")
 
 
 def tensor_failures() -> int:

@@ -5,7 +5,7 @@
 
 #include <algorithm>
 
-#include "sfb_tensor.cuh"
+#include "sfb_tensor_parts.cuh"
 
 namespace sfb {
 namespace {
@@ -15,67 +15,108 @@ constexpr int QT = 256;
 // --- codes of a float weight -------------------------------------------------------------------------
 //
 // s = amax / m (m = M / 2^(N-1), 1 where amax is 0) in float64, kept as float32;
-// code = rint(w / s 2^(N-1)), held within +-M.  The quotient is taken as a
-// product with 2^(N-1) / s in float64, 1e-16 off the true one; only where that
-// lies within 1e-9 of a border of two codes is the division itself made, so the
-// codes are those of the division.  A row that holds a NaN or an infinity gets
-// that as its scale and its outputs are NaN.
-// Memory bound: a row is read twice, the second time from L1 / L2.
+// code = rint(w / s 2^(N-1)), held within +-M.  The quotient is first taken in
+// float32, off by at most 2^-16 of a code; where that lies within 2^-10 of a border of two
+// codes it is made again as a float64 division, so the codes are those of the
+// division.  A row that holds a NaN or an infinity gets that as its scale and its
+// outputs are NaN.
+// A warp has a row and reads it twice, the second time from L1 or L2; 8 elements a lane
+// at a time where rows start on 16 bytes.  (A CTA to a row, an element a thread and
+// every quotient in float64: 51 us for 4096 x 4096 of fp16.)
 
 __device__ __forceinline__ float scale_from(uint32_t amax_bits, double m) {
     const float amax = __uint_as_float(amax_bits);
     return amax == 0.0f ? 1.0f : (float)((double)amax / m);
 }
 
-__device__ __forceinline__ int code_from(float w, double s, double inv, int M, double unit) {
-    double t = (double)w * inv;
-    if (fabs(t - rint(t)) > 0.5 - 1e-9) t = (double)w / s * unit;
-    const double r = rint(t);
-    return r >= M ? M : r <= -M ? -M : r == r ? (int)r : 0;
+__device__ __forceinline__ float code_from(float w, float s, float inv, float M, double unit) {
+    const float t = w * inv, r = rintf(t);
+    if (fabsf(t - r) <= 0.4990234375f) return r > M ? M : r < -M ? -M : r;
+    const double d = rint((double)w / (double)s * unit);            // near a border, or not finite
+    return d >= M ? M : d <= -M ? -M : d == d ? (float)d : 0.0f;
+}
+
+// 8 elements from k on, those past K as 0
+template <typename W>
+__device__ __forceinline__ void load8f(const W *row, int64_t k, int64_t K, bool vec, float (&v)[8]) {
+    if (vec && k + 8 <= K) {
+        constexpr int P = 16 / sizeof(W);
+#pragma unroll
+        for (int i = 0; i < 8 / P; i++) {
+            const Vec<W, P> q = *reinterpret_cast<const Vec<W, P> *>(row + k + i * P);
+#pragma unroll
+            for (int j = 0; j < P; j++) v[i * P + j] = to_f(q.v[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = k + j < K ? to_f(row[k + j]) : 0.0f;
+    }
 }
 
 // magnitudes order as their bits, NaN above infinity
 template <typename W>
-__global__ void __launch_bounds__(QT) amax_kernel(const W *__restrict__ w, int64_t K, int64_t ldw, uint32_t *amax) {
-    __shared__ uint32_t s_top[QT / 32];
-    const W *row = w + (int64_t)blockIdx.x * ldw;
+__device__ __forceinline__ uint32_t row_top(const W *row, int64_t K, bool vec, int lane) {
     uint32_t top = 0;
-    for (int64_t k = threadIdx.x; k < K; k += QT) top = max(top, __float_as_uint(to_f(row[k])) & 0x7FFFFFFFu);
-    top = __reduce_max_sync(0xffffffffu, top);
-    if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < QT / 32; i++) top = max(top, s_top[i]);
-        amax[blockIdx.x] = top;
+#pragma unroll 4
+    for (int64_t k = lane * 8; k < K; k += 256) {
+        float v[8];
+        load8f(row, k, K, vec, v);
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
     }
+    return __reduce_max_sync(0xffffffffu, top);
 }
 
+template <typename W>
+__global__ void __launch_bounds__(QT) amax_kernel(const W *__restrict__ w, int64_t N, int64_t K, int64_t ldw, bool vec,
+                                                  uint32_t *amax) {
+    const int64_t n = (int64_t)blockIdx.x * (QT / 32) + threadIdx.x / 32;
+    if (n >= N) return;
+    const uint32_t top = row_top(w + n * ldw, K, vec, threadIdx.x & 31);
+    if ((threadIdx.x & 31) == 0) amax[n] = top;
+}
+
+// amax: of the rows, for one scale; null for a scale a row
 template <typename W, typename O>
-__global__ void __launch_bounds__(QT) code_kernel(const W *__restrict__ w, int64_t N, int64_t K, int64_t ldw, int bits,
-                                                  const uint32_t *__restrict__ amax, int per_channel, O *codes,
-                                                  int64_t ldc, float *scale) {
+__global__ void __launch_bounds__(QT) code_kernel(const W *__restrict__ w, int64_t N, int64_t K, int64_t ldw, bool vec,
+                                                  int bits, const uint32_t *__restrict__ amax, O *codes, int64_t ldc,
+                                                  bool whole, float *scale) {
     __shared__ uint32_t s_top[QT / 32];
-    const int M = (1 << (bits - 1)) - 1;
-    const double unit = (double)(1 << (bits - 1)), m = M / unit;
+    const int lane = threadIdx.x & 31;
+    const int64_t n = (int64_t)blockIdx.x * (QT / 32) + threadIdx.x / 32;
     uint32_t top = 0;
-    if (per_channel) {
-        top = amax[blockIdx.x];
-    } else {
-        for (int64_t n = threadIdx.x; n < N; n += QT) top = max(top, amax[n]);
+    if (amax) {
+        for (int64_t i = threadIdx.x; i < N; i += QT) top = max(top, amax[i]);
         top = __reduce_max_sync(0xffffffffu, top);
-        if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+        if (lane == 0) s_top[threadIdx.x >> 5] = top;
         __syncthreads();
         for (int i = 0; i < QT / 32; i++) top = max(top, s_top[i]);
     }
-    const float s = scale_from(top, m);
-    if (threadIdx.x == 0) scale[blockIdx.x] = s;
-    const double inv = unit / (double)s;
-    const W *row = w + (int64_t)blockIdx.x * ldw;
-    O *out = codes + (int64_t)blockIdx.x * ldc;
-    for (int64_t k = threadIdx.x; k < K; k += QT) {
-        const int c = code_from(to_f(row[k]), (double)s, inv, M, unit);
-        if constexpr (sizeof(O) == 1) out[k] = (O)c;
-        else out[k] = from_f<O>((float)c);
+    if (n >= N) return;
+    const W *row = w + n * ldw;
+    if (!amax) top = row_top(row, K, vec, lane);
+    const double unit = (double)(1 << (bits - 1));
+    const float M = (float)((1 << (bits - 1)) - 1), s = scale_from(top, (double)M / unit), inv = (float)(unit / (double)s);
+    if (lane == 0) scale[n] = s;
+    O *out = codes + n * ldc;
+#pragma unroll 2
+    for (int64_t k = lane * 8; k < K; k += 256) {
+        float v[8];
+        load8f(row, k, K, vec, v);
+        Vec<O, 8> q;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float c = code_from(v[j], s, inv, M, unit);
+            if constexpr (sizeof(O) == 1) q.v[j] = (O)(int)c;
+            else q.v[j] = from_f<O>(c);
+        }
+        if (whole) {
+            *reinterpret_cast<Vec<O, 8> *>(out + k) = q;         // a row's padding may be written
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (k + j < K) out[k + j] = q.v[j];
+        }
     }
 }
 
@@ -108,17 +149,41 @@ __global__ void __launch_bounds__(QT) expand_kernel(const int8_t *__restrict__ c
     }
 }
 
+// --- rows on 16-byte boundaries ----------------------------------------------------------------------
+
+__global__ void __launch_bounds__(QT) pad_kernel(const uint16_t *__restrict__ x, int64_t M, int64_t K, int64_t ldx,
+                                                 uint16_t *__restrict__ out, int64_t ldo) {
+    const int64_t per = (K + 7) / 8, total = M * per;
+    for (int64_t i = (int64_t)blockIdx.x * QT + threadIdx.x; i < total; i += (int64_t)gridDim.x * QT) {
+        const int64_t m = i / per, k = (i - m * per) * 8;
+        Vec<uint16_t, 8> q;
+#pragma unroll
+        for (int j = 0; j < 8; j++) q.v[j] = k + j < K ? x[m * ldx + k + j] : (uint16_t)0;
+        *reinterpret_cast<Vec<uint16_t, 8> *>(out + m * ldo + k) = q;
+    }
+}
+
 // --- the gradient of the pre-activation --------------------------------------------------------------
 //
 // dz = dy act'(z); written as dz (the operand of the weight's gradient) and
 // as dz[n] s[n] / top (the operand of x's gradient: the channel's scale cannot
 // wait for the product, which sums over channels; top keeps fp16 within its range),
 // each rounded once from float32.  db = sum over rows, in a fixed order: every
-// CTA sums its 128 rows, and a second kernel the CTAs' sums.
-// Memory bound: dy and z read, dz and / or dz s written.
+// CTA sums its 64 rows, and a second kernel the CTAs' sums.
+// Memory bound: dy and z read, dz and / or dz s written; a thread has 8 columns and
+// four rows' loads in flight.
 
-constexpr int BR = 128;                  // rows of a CTA
+constexpr int BR = 64;                   // rows of a CTA
 constexpr int BC = 256;                  // columns: 32 threads of 8
+
+template <typename T>
+__device__ __forceinline__ Vec<T, 8> load8t(const T *from, int64_t left, bool vec) {
+    if (vec && left >= 8) return *reinterpret_cast<const Vec<T, 8> *>(from);
+    Vec<T, 8> q;
+#pragma unroll
+    for (int j = 0; j < 8; j++) q.v[j] = j < left ? from[j] : from_f<T>(0.0f);
+    return q;
+}
 
 template <typename T, int ACT>
 __global__ void __launch_bounds__(256) slope_kernel(const T *__restrict__ dy, int64_t ldy, const __half *__restrict__ z,
@@ -127,55 +192,54 @@ __global__ void __launch_bounds__(256) slope_kernel(const T *__restrict__ dy, in
                                                     T *__restrict__ dzs, int64_t ldd, float *__restrict__ sums) {
     __shared__ float s_sum[8][BC];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int64_t n0 = (int64_t)blockIdx.x * BC + tx * 8;
-    const int64_t r0 = (int64_t)blockIdx.y * BR, r1 = min(M, r0 + BR);
-    const bool whole = n0 + 8 <= N;
-    const bool vy = whole && ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(dy) & 15) == 0;
-    const bool vz = ACT != SFB_ACT_NONE && whole && ldz % 8 == 0 && (reinterpret_cast<uintptr_t>(z) & 15) == 0;
+    const int64_t n0 = (int64_t)blockIdx.x * BC + tx * 8, left = N - n0;
+    const int64_t r0 = (int64_t)blockIdx.y * BR + ty;
+    const bool vy = ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(dy) & 15) == 0;
+    const bool vz = ldz % 8 == 0 && (reinterpret_cast<uintptr_t>(z) & 15) == 0;
     float acc[8] = {}, f[8];
     if (dzs) {
         const float by = top ? __fdiv_rn(1.0f, *top) : unit;
 #pragma unroll
-        for (int j = 0; j < 8; j++) f[j] = n0 + j < N ? scale[n0 + j] * by : 0.0f;
+        for (int j = 0; j < 8; j++) f[j] = j < left ? scale[n0 + j] * by : 0.0f;
     }
-    if (n0 < N) {
-        for (int64_t r = r0 + ty; r < r1; r += 8) {
-            float g[8], d[8];
-            if (vy) {
-                const Vec<T, 8> q = *reinterpret_cast<const Vec<T, 8> *>(dy + r * ldy + n0);
+    if (left > 0) {
+        for (int i = 0; i < BR / 8; i += 4) {
+            Vec<T, 8> g[4];
+            Vec<__half, 8> h[4];
 #pragma unroll
-                for (int j = 0; j < 8; j++) g[j] = to_f(q.v[j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) g[j] = n0 + j < N ? to_f(dy[r * ldy + n0 + j]) : 0.0f;
-            }
-            if constexpr (ACT != SFB_ACT_NONE) {
-                if (vz) {
-                    const Vec<__half, 8> q = *reinterpret_cast<const Vec<__half, 8> *>(z + r * ldz + n0);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) d[j] = g[j] * slope<ACT>(to_f(q.v[j]));
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) d[j] = n0 + j < N ? g[j] * slope<ACT>(to_f(z[r * ldz + n0 + j])) : 0.0f;
+            for (int u = 0; u < 4; u++) {
+                const int64_t r = r0 + 8 * (i + u);
+                if (r < M) {
+                    g[u] = load8t(dy + r * ldy + n0, left, vy);
+                    if constexpr (ACT != SFB_ACT_NONE) h[u] = load8t(z + r * ldz + n0, left, vz);
                 }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) d[j] = g[j];
             }
 #pragma unroll
-            for (int j = 0; j < 8; j++) acc[j] += d[j];
-            // ldd is a multiple of 8 and the buffers are aligned: the vector's tail lands in the row's padding
-            if (dz) {
-                Vec<T, 8> q;
+            for (int u = 0; u < 4; u++) {
+                const int64_t r = r0 + 8 * (i + u);
+                if (r >= M) break;
+                float d[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) q.v[j] = from_f<T>(d[j]);
-                *reinterpret_cast<Vec<T, 8> *>(dz + r * ldd + n0) = q;
-            }
-            if (dzs) {
-                Vec<T, 8> q;
+                for (int j = 0; j < 8; j++) {
+                    d[j] = to_f(g[u].v[j]);
+                    // (one rounding, whatever else is wanted: contracted with the sum it would be none)
+                    if constexpr (ACT != SFB_ACT_NONE) d[j] = __fmul_rn(d[j], slope<ACT>(to_f(h[u].v[j])));
+                    if (j >= left) d[j] = 0.0f;
+                    acc[j] += d[j];
+                }
+                // ldd is a multiple of 8 and the buffers are aligned: the vector's tail lands in the row's padding
+                if (dz) {
+                    Vec<T, 8> q;
 #pragma unroll
-                for (int j = 0; j < 8; j++) q.v[j] = from_f<T>(d[j] * f[j]);
-                *reinterpret_cast<Vec<T, 8> *>(dzs + r * ldd + n0) = q;
+                    for (int j = 0; j < 8; j++) q.v[j] = from_f<T>(d[j]);
+                    *reinterpret_cast<Vec<T, 8> *>(dz + r * ldd + n0) = q;
+                }
+                if (dzs) {
+                    Vec<T, 8> q;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) q.v[j] = from_f<T>(d[j] * f[j]);
+                    *reinterpret_cast<Vec<T, 8> *>(dzs + r * ldd + n0) = q;
+                }
             }
         }
     }
@@ -193,49 +257,64 @@ __global__ void __launch_bounds__(256) slope_kernel(const T *__restrict__ dy, in
     }
 }
 
+// 32 columns a CTA, 8 threads to a column, each every 8th part
 __global__ void __launch_bounds__(QT) sum_kernel(const float *__restrict__ sums, int64_t parts, int64_t N, void *db,
                                                  int dtype) {
-    const int64_t n = (int64_t)blockIdx.x * QT + threadIdx.x;
-    if (n >= N) return;
+    __shared__ float s_sum[8][32];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int64_t n = (int64_t)blockIdx.x * 32 + tx;
     float v = 0.0f;
-    for (int64_t i = 0; i < parts; i++) v += sums[i * N + n];
-    store_as(db, n, dtype, v);
+    if (n < N)
+#pragma unroll 8
+        for (int64_t i = ty; i < parts; i += 8) v += sums[i * N + n];
+    s_sum[ty][tx] = v;
+    __syncthreads();
+    if (ty == 0 && n < N) {
+#pragma unroll
+        for (int i = 1; i < 8; i++) v += s_sum[i][tx];
+        store_as(db, n, dtype, v);
+    }
 }
 
-bool is_float(int dtype) { return dtype == SFB_F32 || dtype == SFB_BF16 || dtype == SFB_F16; }
+// the largest of the scales
+__global__ void __launch_bounds__(1024) top_kernel(const float *__restrict__ scale, int64_t N, float *top) {
+    __shared__ uint32_t s_top[32];
+    uint32_t t = 0;                                    // scales are above 0, and NaN above all
+    for (int64_t n = threadIdx.x; n < N; n += 1024) t = max(t, __float_as_uint(scale[n]) & 0x7FFFFFFFu);
+    t = __reduce_max_sync(0xffffffffu, t);
+    if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = t;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        t = __reduce_max_sync(0xffffffffu, s_top[threadIdx.x]);
+        if (threadIdx.x == 0) *top = __uint_as_float(t);
+    }
+}
 
 template <typename W>
-int quantize_from(const W *w, int64_t N, int64_t K, int64_t ldw, int bits, int per_channel, void *codes, int64_t ldc,
+int quantize_from(const W *w, int64_t N, int64_t K, int64_t ldw, int bits, bool per_channel, void *codes, int64_t ldc,
                   int out, float *scale, uint32_t *amax, cudaStream_t st) {
-    amax_kernel<W><<<(unsigned)N, QT, 0, st>>>(w, K, ldw, amax);
+    const bool vec = (reinterpret_cast<uintptr_t>(w) & 15) == 0 && ldw * sizeof(W) % 16 == 0;
+    const unsigned grid = (unsigned)((N + QT / 32 - 1) / (QT / 32));
+    if (!per_channel) amax_kernel<W><<<grid, QT, 0, st>>>(w, N, K, ldw, vec, amax);
+    const uint32_t *top = per_channel ? nullptr : amax;
+    // a row of 16-bit codes is padded to a multiple of 8; one of int8 only where the caller's stride says so
     if (out == SFB_I8)
-        code_kernel<W, int8_t><<<(unsigned)N, QT, 0, st>>>(w, N, K, ldw, bits, amax, per_channel,
-                                                           static_cast<int8_t *>(codes), ldc, scale);
+        code_kernel<W, int8_t><<<grid, QT, 0, st>>>(w, N, K, ldw, vec, bits, top, static_cast<int8_t *>(codes), ldc,
+                                                    K % 8 == 0 && ldc % 8 == 0 && (reinterpret_cast<uintptr_t>(codes) & 7) == 0,
+                                                    scale);
     else if (out == SFB_BF16)
-        code_kernel<W, __nv_bfloat16><<<(unsigned)N, QT, 0, st>>>(w, N, K, ldw, bits, amax, per_channel,
-                                                                  static_cast<__nv_bfloat16 *>(codes), ldc, scale);
+        code_kernel<W, __nv_bfloat16><<<grid, QT, 0, st>>>(w, N, K, ldw, vec, bits, top,
+                                                           static_cast<__nv_bfloat16 *>(codes), ldc, true, scale);
     else
-        code_kernel<W, __half><<<(unsigned)N, QT, 0, st>>>(w, N, K, ldw, bits, amax, per_channel,
-                                                           static_cast<__half *>(codes), ldc, scale);
-    return check_launch("sfb_code_quantize");
+        code_kernel<W, __half><<<grid, QT, 0, st>>>(w, N, K, ldw, vec, bits, top, static_cast<__half *>(codes), ldc,
+                                                    true, scale);
+    return check_launch("sf weight codes");
 }
 
 }  // namespace
-}  // namespace sfb
 
-extern "C" int sfb_code_quantize(const void *w, int dtype, int64_t N, int64_t K, int64_t ldw, int bits,
-                                 int per_channel, void *codes, int64_t ldc, int codes_dtype, float *scale, void *work,
-                                 sfb_stream stream) {
-    using namespace sfb;
-    if (bits < 4 || bits > 8) return set_error(SFB_EINVAL, "sfb_code_quantize: width %d is not in 4..8", bits);
-    if (!is_float(dtype)) return set_error(SFB_EINVAL, "sfb_code_quantize: element type %d", dtype);
-    if (codes_dtype != SFB_I8 && codes_dtype != SFB_BF16 && codes_dtype != SFB_F16)
-        return set_error(SFB_EINVAL, "sfb_code_quantize: codes of type %d", codes_dtype);
-    if (N < 0 || K < 0 || ldw < K || ldc < K) return set_error(SFB_EINVAL, "sfb_code_quantize: bad shape");
-    if (N >= (1ll << 31)) return set_error(SFB_ERANGE, "sfb_code_quantize: %lld rows", (long long)N);
-    if (N == 0 || K == 0) return SFB_OK;
-    if (!w || !codes || !scale || !work) return set_error(SFB_EINVAL, "sfb_code_quantize: null pointer");
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
+int tensor_quantize(const void *w, int dtype, int64_t N, int64_t K, int64_t ldw, int bits, bool per_channel, void *codes,
+                    int64_t ldc, int codes_dtype, float *scale, void *work, cudaStream_t st) {
     uint32_t *amax = static_cast<uint32_t *>(work);
     if (dtype == SFB_F32)
         return quantize_from(static_cast<const float *>(w), N, K, ldw, bits, per_channel, codes, ldc, codes_dtype,
@@ -247,16 +326,8 @@ extern "C" int sfb_code_quantize(const void *w, int dtype, int64_t N, int64_t K,
                          amax, st);
 }
 
-extern "C" int sfb_code_expand(const int8_t *codes, int64_t N, int64_t K, int64_t ldc, void *out, int64_t ldo,
-                               int dtype, sfb_stream stream) {
-    using namespace sfb;
-    if (dtype != SFB_BF16 && dtype != SFB_F16) return set_error(SFB_EINVAL, "sfb_code_expand: element type %d", dtype);
-    if (N < 0 || K < 0 || ldc < K || ldo < K) return set_error(SFB_EINVAL, "sfb_code_expand: bad shape");
-    if (N == 0 || K == 0) return SFB_OK;
-    if (!codes || !out) return set_error(SFB_EINVAL, "sfb_code_expand: null pointer");
-    if ((reinterpret_cast<uintptr_t>(out) & 15) || ldo % 8)
-        return set_error(SFB_EINVAL, "sfb_code_expand: the rows of the result must be aligned to 16 bytes");
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
+int tensor_expand(const int8_t *codes, int64_t N, int64_t K, int64_t ldc, void *out, int64_t ldo, int dtype,
+                  cudaStream_t st) {
     const int64_t total = N * ((K + 15) / 16);
     const unsigned grid = (unsigned)std::min<int64_t>((total + QT - 1) / QT, 16ll * sm_count());
     const bool vec = ldc % 16 == 0 && (reinterpret_cast<uintptr_t>(codes) & 15) == 0;
@@ -264,49 +335,61 @@ extern "C" int sfb_code_expand(const int8_t *codes, int64_t N, int64_t K, int64_
         expand_kernel<<<grid, QT, 0, st>>>(codes, N, K, ldc, static_cast<__nv_bfloat16 *>(out), ldo, vec);
     else
         expand_kernel<<<grid, QT, 0, st>>>(codes, N, K, ldc, static_cast<__half *>(out), ldo, vec);
-    return check_launch("sfb_code_expand");
+    return check_launch("sf tensor linear (packed codes)");
 }
 
-extern "C" int64_t sfb_slope_workspace(int64_t M, int64_t N) { return 4 * ((M + sfb::BR - 1) / sfb::BR) * N; }
+int tensor_pad(const void *x, int64_t M, int64_t K, int64_t ldx, void *out, int64_t ldo, cudaStream_t st) {
+    const int64_t total = M * ((K + 7) / 8);
+    const unsigned grid = (unsigned)std::min<int64_t>((total + QT - 1) / QT, 16ll * sm_count());
+    pad_kernel<<<grid, QT, 0, st>>>(static_cast<const uint16_t *>(x), M, K, ldx, static_cast<uint16_t *>(out), ldo);
+    return check_launch("sf tensor linear (rows of x)");
+}
 
-extern "C" int sfb_slope(int dtype, int act, const void *dy, int64_t ldy, const void *z, int64_t ldz, int64_t M,
-                         int64_t N, const float *scale, int bits, const float *top, void *dz, void *dzs, int64_t ldd,
-                         void *db, int db_dtype, void *work, sfb_stream stream) {
-    using namespace sfb;
-    if (dtype != SFB_BF16 && dtype != SFB_F16) return set_error(SFB_EINVAL, "sfb_slope: element type %d", dtype);
-    if (bits < 4 || bits > 8) return set_error(SFB_EINVAL, "sfb_slope: width %d is not in 4..8", bits);
-    if (M < 0 || N < 0 || ldy < N || (act != SFB_ACT_NONE && ldz < N) || ((dz || dzs) && (ldd < N || ldd % 8)))
-        return set_error(SFB_EINVAL, "sfb_slope: bad shape");
-    if ((reinterpret_cast<uintptr_t>(dz) | reinterpret_cast<uintptr_t>(dzs)) & 15)
-        return set_error(SFB_EINVAL, "sfb_slope: the outputs must be aligned to 16 bytes");
-    if (db && !is_float(db_dtype)) return set_error(SFB_EINVAL, "sfb_slope: bias type %d", db_dtype);
-    if (N == 0) return SFB_OK;
-    if ((M > 0 && (!dy || (act != SFB_ACT_NONE && !z))) || (dzs && !scale) || (db && M > 0 && !work))
-        return set_error(SFB_EINVAL, "sfb_slope: null pointer");
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
+int tensor_top(const float *scale, int64_t N, float *top, cudaStream_t st) {
+    top_kernel<<<1, 1024, 0, st>>>(scale, N, top);
+    return check_launch("sf tensor linear (largest scale)");
+}
+
+int64_t tensor_slope_workspace(int64_t M, int64_t N) { return 4 * ((M + BR - 1) / BR) * N; }
+
+int tensor_slope(int dtype, int act, const void *dy, int64_t ldy, const void *z, int64_t ldz, int64_t M, int64_t N,
+                 const float *scale, int bits, const float *top, void *dz, void *dzs, int64_t ldd, void *db,
+                 int db_dtype, void *work, cudaStream_t st) {
     const int64_t parts = (M + BR - 1) / BR;
-    if (parts > 65535) return set_error(SFB_ERANGE, "sfb_slope: %lld rows", (long long)M);
+    if (parts > 65535) return set_error(SFB_ERANGE, "sf tensor linear: %lld rows", (long long)M);
     float *sums = db ? static_cast<float *>(work) : nullptr;
     const float unit = 1.0f / (float)(1 << (bits - 1));
-    if (M > 0) {
-        const dim3 grid((unsigned)((N + BC - 1) / BC), (unsigned)parts);
-        const int rc = with_activation(act, [&](auto a) {
-            constexpr int A = decltype(a)::value;
-            if (dtype == SFB_BF16)
-                slope_kernel<__nv_bfloat16, A><<<grid, 256, 0, st>>>(
-                    static_cast<const __nv_bfloat16 *>(dy), ldy, static_cast<const __half *>(z), ldz, M, N, scale,
-                    unit, top, static_cast<__nv_bfloat16 *>(dz), static_cast<__nv_bfloat16 *>(dzs), ldd, sums);
-            else
-                slope_kernel<__half, A><<<grid, 256, 0, st>>>(
-                    static_cast<const __half *>(dy), ldy, static_cast<const __half *>(z), ldz, M, N, scale, unit, top,
-                    static_cast<__half *>(dz), static_cast<__half *>(dzs), ldd, sums);
-            return check_launch("sfb_slope");
-        });
-        if (rc) return rc;
-    }
-    if (db) {
-        sum_kernel<<<(unsigned)((N + QT - 1) / QT), QT, 0, st>>>(sums, parts, N, db, db_dtype);
-        return check_launch("sfb_slope (bias)");
-    }
-    return SFB_OK;
+    const dim3 grid((unsigned)((N + BC - 1) / BC), (unsigned)parts);
+    const int rc = with_activation(act, [&](auto a) {
+        constexpr int A = decltype(a)::value;
+        if (dtype == SFB_BF16)
+            slope_kernel<__nv_bfloat16, A><<<grid, 256, 0, st>>>(
+                static_cast<const __nv_bfloat16 *>(dy), ldy, static_cast<const __half *>(z), ldz, M, N, scale, unit,
+                top, static_cast<__nv_bfloat16 *>(dz), static_cast<__nv_bfloat16 *>(dzs), ldd, sums);
+        else
+            slope_kernel<__half, A><<<grid, 256, 0, st>>>(static_cast<const __half *>(dy), ldy,
+                                                          static_cast<const __half *>(z), ldz, M, N, scale, unit, top,
+                                                          static_cast<__half *>(dz), static_cast<__half *>(dzs), ldd, sums);
+        return check_launch("sf tensor linear (activation's gradient)");
+    });
+    if (rc || !db) return rc;
+    sum_kernel<<<(unsigned)((N + 31) / 32), QT, 0, st>>>(sums, parts, N, db, db_dtype);
+    return check_launch("sf tensor linear (bias's gradient)");
+}
+
+}  // namespace sfb
+
+extern "C" int sfb_code_quantize(const void *w, int dtype, int64_t N, int64_t K, int64_t ldw, int bits,
+                                 int per_channel, void *codes, int64_t ldc, float *scale, void *work,
+                                 sfb_stream stream) {
+    using namespace sfb;
+    if (bits < 4 || bits > 8) return set_error(SFB_EINVAL, "sfb_code_quantize: width %d is not in 4..8", bits);
+    if (dtype != SFB_F32 && dtype != SFB_BF16 && dtype != SFB_F16)
+        return set_error(SFB_EINVAL, "sfb_code_quantize: element type %d", dtype);
+    if (N < 0 || K < 0 || ldw < K || ldc < K) return set_error(SFB_EINVAL, "sfb_code_quantize: bad shape");
+    if (N >= (1ll << 31)) return set_error(SFB_ERANGE, "sfb_code_quantize: %lld rows", (long long)N);
+    if (N == 0 || K == 0) return SFB_OK;
+    if (!w || !codes || !scale || (!per_channel && !work)) return set_error(SFB_EINVAL, "sfb_code_quantize: null pointer");
+    return tensor_quantize(w, dtype, N, K, ldw, bits, per_channel != 0, codes, ldc, SFB_I8, scale, work,
+                           static_cast<cudaStream_t>(stream));
 }

@@ -40,7 +40,7 @@
 #include <algorithm>
 #include <mutex>
 
-#include "sfb_tensor.cuh"
+#include "sfb_tensor_parts.cuh"
 
 namespace sfb {
 
@@ -733,20 +733,6 @@ int columns(int64_t R, int64_t C) {
     return 512 * wide <= 390 * narrow ? 256 : 128;
 }
 
-int check(const Problem &p, const char *what) {
-    if (p.dtype != SFB_BF16 && p.dtype != SFB_F16) return set_error(SFB_EINVAL, "%s: element type %d", what, p.dtype);
-    if (p.R < 0 || p.C < 0 || p.K < 1) return set_error(SFB_EINVAL, "%s: bad shape", what);
-    if (p.R >= (1ll << 31) - 512 || p.C >= (1ll << 31) - 512 || p.K >= (1ll << 31) - 512 || p.lda >= (1ll << 36) ||
-        p.ldb >= (1ll << 36) || ((p.R + 2 * BM - 1) / (2 * BM)) * ((p.C + 127) / 128) >= (1ll << 31) - 512)
-        return set_error(SFB_ERANGE, "%s: a size of %lld x %lld x %lld", what, (long long)p.R, (long long)p.C,
-                         (long long)p.K);
-    if (p.R == 0 || p.C == 0) return SFB_OK;
-    if (!p.A || !p.B) return set_error(SFB_EINVAL, "%s: null pointer", what);
-    if (((reinterpret_cast<uintptr_t>(p.A) | reinterpret_cast<uintptr_t>(p.B)) & 15) || p.lda % 8 || p.ldb % 8)
-        return set_error(SFB_EINVAL, "%s: operands and their rows must be aligned to 16 bytes", what);
-    return SFB_OK;
-}
-
 template <bool A_MN, bool B_MN, int ACT>
 int launch_typed(const Problem &p, const Epilogue &e, cudaStream_t st) {
     const bool wide = columns(p.R, p.C) == 256;
@@ -757,23 +743,11 @@ int launch_typed(const Problem &p, const Epilogue &e, cudaStream_t st) {
 }
 
 }  // namespace
-}  // namespace sfb
 
-extern "C" int sfb_tensor_linear(int dtype, const void *x, int64_t ldx, const void *codes, int64_t ldw,
-                                 const float *scale, int bits, const void *bias, int bias_dtype, int act,
-                                 const void *residual, int64_t ldr, void *y, int64_t ldy, void *z, int64_t ldz,
-                                 int64_t M, int64_t N, int64_t K, sfb_stream stream) {
-    using namespace sfb;
+int tensor_product(int dtype, const void *x, int64_t ldx, const void *codes, int64_t ldw, const float *scale, int bits,
+                   const void *bias, int bias_dtype, int act, const void *residual, int64_t ldr, void *y, int64_t ldy,
+                   void *z, int64_t ldz, int64_t M, int64_t N, int64_t K, cudaStream_t st) {
     const Problem p{codes, x, ldw, ldx, N, M, K, dtype};
-    const int rc = check(p, "sfb_tensor_linear");
-    if (rc) return rc;
-    if (bits < 4 || bits > 8) return set_error(SFB_EINVAL, "sfb_tensor_linear: width %d is not in 4..8", bits);
-    if (ldx < K || ldw < K || ldy < N || (residual && ldr < N) || (z && ldz < N))
-        return set_error(SFB_EINVAL, "sfb_tensor_linear: a row stride is shorter than its row");
-    if (bias && bias_dtype != SFB_F32 && bias_dtype != SFB_BF16 && bias_dtype != SFB_F16)
-        return set_error(SFB_EINVAL, "sfb_tensor_linear: bias type %d", bias_dtype);
-    if (M == 0 || N == 0) return SFB_OK;
-    if (!scale || !y) return set_error(SFB_EINVAL, "sfb_tensor_linear: null pointer");
     Epilogue e{};
     e.scale = scale;
     e.bias = bias;
@@ -786,50 +760,33 @@ extern "C" int sfb_tensor_linear(int dtype, const void *x, int64_t ldx, const vo
     e.ldr = ldr;
     e.ldz = ldz;
     e.ldy = ldy;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
     return with_activation(act, [&](auto a) { return launch_typed<false, false, decltype(a)::value>(p, e, st); });
 }
 
-extern "C" int sfb_tensor_grad_x(int dtype, const void *dzs, int64_t ldd, const void *codes, int64_t ldw,
-                                 const float *top, int bits, void *dx, int64_t ldy, int64_t M, int64_t N, int64_t K,
-                                 sfb_stream stream) {
-    using namespace sfb;
-    if (N < 1) return set_error(SFB_EINVAL, "sfb_tensor_grad_x: no channels");
+int tensor_grad_x(int dtype, const void *dzs, int64_t ldd, const void *codes, int64_t ldw, const float *top, int bits,
+                  void *dx, int64_t ldx, int64_t M, int64_t N, int64_t K, cudaStream_t st) {
     const Problem p{codes, dzs, ldw, ldd, K, M, N, dtype};
-    const int rc = check(p, "sfb_tensor_grad_x");
-    if (rc) return rc;
-    if (bits < 4 || bits > 8) return set_error(SFB_EINVAL, "sfb_tensor_grad_x: width %d is not in 4..8", bits);
-    if (ldd < N || ldw < K || ldy < K) return set_error(SFB_EINVAL, "sfb_tensor_grad_x: a row stride is shorter than its row");
-    if (M == 0 || K == 0) return SFB_OK;
-    if (!dx) return set_error(SFB_EINVAL, "sfb_tensor_grad_x: null pointer");
     Epilogue e{};
     e.alpha = top;
     e.y = dx;
     e.unit = top ? 1.0f / (float)(1 << (bits - 1)) : 1.0f;
     e.y_dtype = dtype;
-    e.ldy = ldy;
-    return launch_typed<true, false, SFB_ACT_NONE>(p, e, static_cast<cudaStream_t>(stream));
+    e.ldy = ldx;
+    return launch_typed<true, false, SFB_ACT_NONE>(p, e, st);
 }
 
-extern "C" int sfb_tensor_grad_w(int dtype, const void *dz, int64_t ldd, const void *x, int64_t ldx, void *dw,
-                                 int dw_dtype, int64_t ldy, int64_t M, int64_t N, int64_t K, sfb_stream stream) {
-    using namespace sfb;
-    if (M < 1) return set_error(SFB_EINVAL, "sfb_tensor_grad_w: no rows");
+int tensor_grad_w(int dtype, const void *dz, int64_t ldd, const void *x, int64_t ldx, void *dw, int dw_dtype,
+                  int64_t ldw, int64_t M, int64_t N, int64_t K, cudaStream_t st) {
     const Problem p{x, dz, ldx, ldd, K, N, M, dtype};
-    const int rc = check(p, "sfb_tensor_grad_w");
-    if (rc) return rc;
-    if (dw_dtype != SFB_F32 && dw_dtype != SFB_BF16 && dw_dtype != SFB_F16)
-        return set_error(SFB_EINVAL, "sfb_tensor_grad_w: weight type %d", dw_dtype);
-    if (ldd < N || ldx < K || ldy < K) return set_error(SFB_EINVAL, "sfb_tensor_grad_w: a row stride is shorter than its row");
-    if (N == 0 || K == 0) return SFB_OK;
-    if (!dw) return set_error(SFB_EINVAL, "sfb_tensor_grad_w: null pointer");
     Epilogue e{};
     e.y = dw;
     e.unit = 1.0f;
     e.y_dtype = dw_dtype;
-    e.ldy = ldy;
-    return launch_typed<true, true, SFB_ACT_NONE>(p, e, static_cast<cudaStream_t>(stream));
+    e.ldy = ldw;
+    return launch_typed<true, true, SFB_ACT_NONE>(p, e, st);
 }
+
+}  // namespace sfb
 
 extern "C" int sfb_tensor_failures(int64_t *count) {
     using namespace sfb;

@@ -1,0 +1,33 @@
+// The launches that the tensor-core linear is made of.  Arguments are checked by
+// its entry points (sfb_tensor.cu).
+#pragma once
+
+#include "sfb_tensor.cuh"
+
+namespace sfb {
+
+// codes and scales of a float weight; work: 4 N bytes, for one scale only
+int tensor_quantize(const void *w, int dtype, int64_t N, int64_t K, int64_t ldw, int bits, bool per_channel, void *codes,
+                    int64_t ldc, int codes_dtype, float *scale, void *work, cudaStream_t st);
+// packed codes as the products' operand
+int tensor_expand(const int8_t *codes, int64_t N, int64_t K, int64_t ldc, void *out, int64_t ldo, int dtype,
+                  cudaStream_t st);
+// a matrix of 16-bit elements with its rows on 16-byte boundaries
+int tensor_pad(const void *x, int64_t M, int64_t K, int64_t ldx, void *out, int64_t ldo, cudaStream_t st);
+int tensor_top(const float *scale, int64_t N, float *top, cudaStream_t st);
+int tensor_small(int dtype, const void *x, int64_t ldx, const int8_t *codes, int64_t ldc, const float *scale, int bits,
+                 const void *bias, int bias_dtype, int act, const void *residual, int64_t ldr, void *y, int64_t ldy,
+                 int64_t M, int64_t N, int64_t K, cudaStream_t st);
+int tensor_product(int dtype, const void *x, int64_t ldx, const void *codes, int64_t ldw, const float *scale, int bits,
+                   const void *bias, int bias_dtype, int act, const void *residual, int64_t ldr, void *y, int64_t ldy,
+                   void *z, int64_t ldz, int64_t M, int64_t N, int64_t K, cudaStream_t st);
+int64_t tensor_slope_workspace(int64_t M, int64_t N);
+int tensor_slope(int dtype, int act, const void *dy, int64_t ldy, const void *z, int64_t ldz, int64_t M, int64_t N,
+                 const float *scale, int bits, const float *top, void *dz, void *dzs, int64_t ldd, void *db,
+                 int db_dtype, void *work, cudaStream_t st);
+int tensor_grad_x(int dtype, const void *dzs, int64_t ldd, const void *codes, int64_t ldw, const float *top, int bits,
+                  void *dx, int64_t ldx, int64_t M, int64_t N, int64_t K, cudaStream_t st);
+int tensor_grad_w(int dtype, const void *dz, int64_t ldd, const void *x, int64_t ldx, void *dw, int dw_dtype,
+                  int64_t ldw, int64_t M, int64_t N, int64_t K, cudaStream_t st);
+
+}  // namespace sfb

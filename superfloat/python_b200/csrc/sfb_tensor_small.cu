@@ -14,7 +14,7 @@
 // each every ks-th segment of 64, and their sums are added in a fixed order.
 #include <algorithm>
 
-#include "sfb_tensor.cuh"
+#include "sfb_tensor_parts.cuh"
 
 namespace sfb {
 namespace {
@@ -190,7 +190,7 @@ int launch(const Small &p, int act, cudaStream_t st) {
     const unsigned grid = (unsigned)((groups + per - 1) / per);
     return with_activation(act, [&](auto a) {
         small_kernel<T, MT, ALIGNED, decltype(a)::value><<<grid, 32 * WARPS, 0, st>>>(p);
-        return check_launch("sfb_tensor_linear_small");
+        return check_launch("sf tensor linear (few rows)");
     });
 }
 
@@ -204,30 +204,16 @@ int by_rows(const Small &p, int act, cudaStream_t st) {
 }
 
 }  // namespace
-}  // namespace sfb
 
-extern "C" int sfb_tensor_linear_small(int dtype, const void *x, int64_t ldx, const int8_t *codes, int64_t ldc,
-                                       const float *scale, int bits, const void *bias, int bias_dtype, int act,
-                                       const void *residual, int64_t ldr, void *y, int64_t ldy, int64_t M, int64_t N,
-                                       int64_t K, sfb_stream stream) {
-    using namespace sfb;
-    if (dtype != SFB_BF16 && dtype != SFB_F16) return set_error(SFB_EINVAL, "sfb_tensor_linear_small: element type %d", dtype);
-    if (bits < 4 || bits > 8) return set_error(SFB_EINVAL, "sfb_tensor_linear_small: width %d is not in 4..8", bits);
-    if (M < 0 || N < 0 || K < 1 || ldx < K || ldc < K || ldy < N || (residual && ldr < N))
-        return set_error(SFB_EINVAL, "sfb_tensor_linear_small: bad shape");
-    if (M > SFB_SMALL_ROWS) return set_error(SFB_ERANGE, "sfb_tensor_linear_small: %lld rows", (long long)M);
-    if (N >= (1ll << 34)) return set_error(SFB_ERANGE, "sfb_tensor_linear_small: %lld channels", (long long)N);
-    if (bias && bias_dtype != SFB_F32 && bias_dtype != SFB_BF16 && bias_dtype != SFB_F16)
-        return set_error(SFB_EINVAL, "sfb_tensor_linear_small: bias type %d", bias_dtype);
-    if (M == 0 || N == 0) return SFB_OK;
-    if (!x || !codes || !scale || !y) return set_error(SFB_EINVAL, "sfb_tensor_linear_small: null pointer");
-    if ((reinterpret_cast<uintptr_t>(x) & 15) || ldx % 8)
-        return set_error(SFB_EINVAL, "sfb_tensor_linear_small: x and its rows must be aligned to 16 bytes");
+int tensor_small(int dtype, const void *x, int64_t ldx, const int8_t *codes, int64_t ldc, const float *scale, int bits,
+                 const void *bias, int bias_dtype, int act, const void *residual, int64_t ldr, void *y, int64_t ldy,
+                 int64_t M, int64_t N, int64_t K, cudaStream_t st) {
     Small p{x, codes, scale, bias, residual, y, ldx, ldc, ldr, ldy, N, K, 1.0f / (float)(1 << (bits - 1)), (int)M, 8,
             bias_dtype};
     // warps that share a group of channels: as many as fill the SMs, each with two segments at least
     const int64_t groups = (N + 15) / 16, segs = (K + SEG - 1) / SEG;
     while (p.ks > 1 && (segs < 2 * p.ks || groups * p.ks > 32ll * sm_count())) p.ks /= 2;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
     return dtype == SFB_BF16 ? by_rows<__nv_bfloat16>(p, act, st) : by_rows<__half>(p, act, st);
 }
+
+}  // namespace sfb

@@ -14,6 +14,7 @@ gradient, or an :class:`SFPackedWeight`, codes and scales laid out once.
 """
 from __future__ import annotations
 
+from array import array
 from dataclasses import dataclass
 
 import torch
@@ -57,14 +58,6 @@ class SFPackedWeight:
         return self.codes.float() * (self.scale * 2.0 ** (1 - self.bits))[:, None]
 
 
-def _up8(n: int) -> int:
-    return -(-n // 8) * 8
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
 def _check_width(bits: int) -> None:
     if bits not in BITS:
         raise SFUnsupportedError(f"the tensor-core linear takes sf4..sf8, whose codes are exact in 16-bit floats; got "
@@ -78,35 +71,34 @@ def _check_weight(w: torch.Tensor) -> None:
         raise SFTypeError(f"the weight is {w.dtype}; float32, bfloat16 and float16 are supported")
     if not w.is_cuda:
         raise SFShapeError(f"the weight must be on a CUDA device, got {w.device}")
+    if w.numel() == 0:
+        raise SFShapeError(f"a weight has at least one row and one column, got {tuple(w.shape)}")
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t (2-D) with its rows contiguous, one after another."""
-    if t.shape[0] <= 1 and t.stride(1) == 1:
-        return t
-    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+def _rows(t: torch.Tensor, width: int):
+    """(t, row stride): t (2-D) with each row contiguous and the rows one after another."""
+    ld, inner = t.stride()
+    if (inner == 1 or width == 1) and (ld >= width or t.shape[0] <= 1):
+        return t, max(ld, width)
+    return t.contiguous(), width
 
 
-def _operand(t: torch.Tensor) -> torch.Tensor:
-    """t (2-D) as an operand of the products: rows on 16-byte boundaries."""
-    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1]:
-        return t
-    out = torch.empty(t.shape[0], _up8(t.shape[1]), dtype=t.dtype, device=t.device)[:, :t.shape[1]]
-    return out.copy_(t)
+def _two_d(t: torch.Tensor, width: int):
+    return _rows(t if t.dim() == 2 else t.reshape(-1, width), width)
 
 
-def _quantize(w, bits, wscale, dtype, stream):
-    """(codes, scale): int8 codes for a dtype of None, else the product's operand."""
-    N, K = w.shape
-    w = _rows(w)
-    if dtype is None:
-        codes, kind = torch.empty(N, K, dtype=torch.int8, device=w.device), _lib.I8
-    else:
-        codes, kind = torch.empty(N, _up8(K), dtype=dtype, device=w.device)[:, :K], _TYPES[dtype]
-    both = torch.empty(2, N, dtype=torch.float32, device=w.device)       # the scales; the rows' maxima
-    _lib.code_quantize(w.data_ptr(), _FLOATS[w.dtype], N, K, max(w.stride(0), K), bits, wscale == "per_channel",
-                       codes.data_ptr(), max(codes.stride(0), K), kind, both[0].data_ptr(), both[1].data_ptr(), stream)
-    return codes, both[0]
+class _Room:
+    """Places in one buffer, each on 256 bytes."""
+
+    __slots__ = ("size",)
+
+    def __init__(self):
+        self.size = 0
+
+    def take(self, nbytes: int) -> int:
+        at = self.size
+        self.size = at + (nbytes + 255 & -256)
+        return at
 
 
 @torch.no_grad()
@@ -116,38 +108,22 @@ def pack_weight(weight: torch.Tensor, dtype="sf8", scale: str = "per_channel") -
     the codes are rounded to nearest, ties to even, as the other modes quantize a
     weight; a row that holds a NaN or an infinity has it as its scale."""
     from .._array import resolve_dtype
-    bits = resolve_dtype(dtype).bits
+    bits, scale_kind = resolve_dtype(dtype).bits, scale
     _check_width(bits)
-    _core.check_args(bits, scale)
+    _core.check_args(bits, scale_kind)
     weight = weight.detach()
     _check_weight(weight)
+    (N, K), (weight, ldw) = weight.shape, _rows(weight, weight.shape[1])
+    dev = weight.device
+    # rows on 16 bytes: what the few-rows product reads a row's codes in
+    codes = torch.empty(N, K + 15 & -16, dtype=torch.int8, device=dev)[:, :K]
+    scale, work = torch.empty(N, dtype=torch.float32, device=dev), None
+    if scale_of_all := scale_kind == "per_tensor":
+        work = torch.empty(N, dtype=torch.float32, device=dev)
     with _lib.on_device(weight.get_device()) as d:
-        if weight.numel() == 0:
-            raise SFShapeError(f"a weight has at least one element, got {tuple(weight.shape)}")
-        return SFPackedWeight(*_quantize(weight, bits, scale, None, d.stream), bits)
-
-
-def _expand(packed: SFPackedWeight, dtype, stream):
-    N, K = packed.shape
-    codes = _rows(packed.codes)
-    out = torch.empty(N, _up8(K), dtype=dtype, device=codes.device)[:, :K]
-    _lib.code_expand(codes.data_ptr(), N, K, max(codes.stride(0), K), out.data_ptr(), max(out.stride(0), K),
-                     _TYPES[dtype], stream)
-    return out
-
-
-def _forward(x, codes, scale, bits, bias, act, residual, keep_z, stream):
-    """(y, z) of operands laid out as the product takes them."""
-    (M, K), N = x.shape, codes.shape[0]
-    y = torch.empty(M, N, dtype=x.dtype, device=x.device)
-    z = torch.empty(M, N, dtype=torch.float16, device=x.device) if keep_z else None
-    if y.numel():
-        _lib.tensor_linear(_TYPES[x.dtype], x.data_ptr(), max(x.stride(0), _up8(K)), codes.data_ptr(),
-                           max(codes.stride(0), _up8(K)), scale.data_ptr(), bits, _ptr(bias),
-                           0 if bias is None else _FLOATS[bias.dtype], act, _ptr(residual),
-                           0 if residual is None else max(residual.stride(0), N), y.data_ptr(), N, _ptr(z), N, M, N,
-                           K, stream)
-    return y, z
+        _lib.code_quantize(weight.data_ptr(), _FLOATS[weight.dtype], N, K, ldw, bits, not scale_of_all, codes.data_ptr(),
+                           codes.stride(0), scale.data_ptr(), work.data_ptr() if scale_of_all else None, d.stream)
+    return SFPackedWeight(codes, scale, bits)
 
 
 def _check_operands(x, weight, bias, activation, residual):
@@ -156,103 +132,122 @@ def _check_operands(x, weight, bias, activation, residual):
     if x.dtype not in _TYPES:
         raise SFTypeError(f"the input is {x.dtype}: the tensor cores take bfloat16 or float16 (accumulate=\"chain\" "
                           f"and \"wide\" take float32)")
-    if x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        raise SFShapeError(f"the input has shape {tuple(x.shape)}, the weight expects {weight.shape[1]} features")
-    if weight.shape[1] < 1 or weight.shape[0] < 1:
+    N, K = weight.shape
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise SFShapeError(f"the input has shape {tuple(x.shape)}, the weight expects {K} features")
+    if N < 1 or K < 1:
         raise SFShapeError(f"a weight has at least one row and one column, got {tuple(weight.shape)}")
     device = weight.codes.device if isinstance(weight, SFPackedWeight) else weight.device
-    N = weight.shape[0]
-    for name, t in (("input", x), ("bias", bias), ("residual", residual)):
-        if t is not None and (t.device != device or not t.is_cuda):
-            raise SFShapeError(f"the {name} is on {t.device}, the weight on {device}; both must be on one CUDA device")
+    if x.device != device or not x.is_cuda:
+        raise SFShapeError(f"the input is on {x.device}, the weight on {device}; both must be on one CUDA device")
     if bias is not None:
         if bias.shape != (N,):
             raise SFShapeError(f"the bias has shape {tuple(bias.shape)}, expected ({N},)")
         if bias.dtype not in _FLOATS:
             raise SFTypeError(f"the bias is {bias.dtype}; float32, bfloat16 and float16 are supported")
+        if bias.device != device:
+            raise SFShapeError(f"the bias is on {bias.device}, the weight on {device}")
     if residual is not None:
         if residual.shape != (*x.shape[:-1], N):
             raise SFShapeError(f"the residual has shape {tuple(residual.shape)}, expected {(*x.shape[:-1], N)}")
         if residual.dtype != x.dtype:
             raise SFTypeError(f"the residual is {residual.dtype}, the input {x.dtype}")
+        if residual.device != device:
+            raise SFShapeError(f"the residual is on {residual.device}, the weight on {device}")
 
 
-def _backward(g, x, codes, scale, z, bits, act, top, want_x, want_w, w_dtype, want_b, b_dtype, stream):
-    """Gradients (x, weight, bias) from the output's, all 2-D."""
-    (M, K), N = x.shape, codes.shape[0]
-    kind, dev = _TYPES[x.dtype], x.device
-    g = _rows(g)
-    dx = dw = db = None
-    # per-tensor scales: top is that scale and dz s / top = dz, one operand for both products
-    one_scale = top is not None and top.data_ptr() == scale.data_ptr()
-    direct = act == 0 and g.data_ptr() % 16 == 0 and g.stride(0) % 8 == 0 and g.stride(0) >= N
-    need_dz = (want_w or (want_x and one_scale)) and not direct
-    need_dzs = want_x and not one_scale
-    ldd = _up8(N)
-    dz = torch.empty(M, ldd, dtype=x.dtype, device=dev)[:, :N] if need_dz else None
-    dzs = torch.empty(M, ldd, dtype=x.dtype, device=dev)[:, :N] if need_dzs else None
-    if want_b:
-        db = torch.empty(N, dtype=b_dtype, device=dev)
-    if M and (need_dz or need_dzs or want_b):
-        work = torch.empty(_lib.slope_workspace(M, N), dtype=torch.uint8, device=dev) if want_b else None
-        _lib.slope(kind, act, g.data_ptr(), max(g.stride(0), N), _ptr(z), N, M, N, scale.data_ptr(), bits, _ptr(top),
-                   _ptr(dz), _ptr(dzs), ldd, _ptr(db), _FLOATS[b_dtype] if want_b else 0, _ptr(work), stream)
-    elif want_b:
-        db.zero_()
-    if direct:
-        dz = g
-    if want_x:
-        d = dz if one_scale else dzs
-        dx = torch.empty(M, K, dtype=x.dtype, device=dev)
-        if M:
-            _lib.tensor_grad_x(kind, d.data_ptr(), max(d.stride(0), ldd), codes.data_ptr(),
-                               max(codes.stride(0), _up8(K)), _ptr(top), bits, dx.data_ptr(), K, M, N, K, stream)
-    if want_w:
-        dw = torch.empty(N, K, dtype=w_dtype, device=dev)
-        if M:
-            _lib.tensor_grad_w(kind, dz.data_ptr(), max(dz.stride(0), ldd), x.data_ptr(), max(x.stride(0), _up8(K)),
-                               dw.data_ptr(), _FLOATS[w_dtype], K, M, N, K, stream)
-        else:
-            dw.zero_()
-    return dx, dw, db
+def _forward(x, weight, packed, bias, residual, bits, wscale, act, train):
+    """The result and, with ``train``, what the backward pass reads: (x, its
+    row stride), the pre-activation, the buffer of codes and scales and their
+    places in it.  One library call, all scratch in one buffer."""
+    (N, K), kind = weight.shape, _TYPES[x.dtype]
+    out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    x, ldx = _two_d(x, K)
+    M = x.shape[0]
+    ldk = K + 7 & -8
+    if M <= 1:
+        ldx = max(ldx, ldk) if ldx % 8 == 0 else ldk
+    small = packed is not None and M <= _lib.SMALL_ROWS and not train
+    room = _Room()
+    codes = 0 if small else room.take(2 * N * ldk)
+    if packed is None:
+        w, ldw = _rows(weight, K)
+        w_ptr, w_kind = w.data_ptr(), _FLOATS[w.dtype]
+        scale_at, work = room.take(4 * N), room.take(4 * N) if wscale == "per_tensor" else None
+    else:
+        w, ldw = _rows(packed.codes, K)
+        w_ptr, w_kind, scale = w.data_ptr(), _lib.I8, packed.scale.contiguous()
+    xpad = room.take(2 * M * ldk) if x.data_ptr() % 16 or ldx % 8 else None
+    buf = torch.empty(room.size, dtype=torch.uint8, device=x.device) if room.size else None
+    base = buf.data_ptr() if buf is not None else 0
+    scale_ptr = base + scale_at if packed is None else scale.data_ptr()
+    z = torch.empty(M, N, dtype=torch.float16, device=x.device) if train and act else None
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    r_ptr, ldr = 0, 0
+    if residual is not None:
+        residual, ldr = _two_d(residual, N)
+        r_ptr = residual.data_ptr()
+    with _lib.on_device(x.get_device()) as d:
+        _lib.tensor_forward(array("q", (
+            kind, bits, act, M, N, K, x.data_ptr(), ldx, 0 if xpad is None else base + xpad, ldk, w_ptr, ldw, w_kind,
+            wscale == "per_channel", 0 if small else base + codes, ldk, scale_ptr,
+            0 if bias is None else bias.data_ptr(), 0 if bias is None else _FLOATS[bias.dtype], r_ptr, ldr,
+            out.data_ptr(), N, 0 if z is None else z.data_ptr(), N, 0 if packed or work is None else base + work,
+            0, 0, 0, 0, 0, 0, 0, 0)), d.stream)
+    if not train:
+        return out
+    if xpad is not None:
+        x, ldx, x_at = buf, ldk, xpad
+    else:
+        x_at = 0
+    return out, x, z, buf, (scale if packed is not None else buf), (M, N, K, ldx, x_at, codes,
+                                                                    0 if packed is not None else scale_at)
 
 
 class _TensorLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, packed, bias, residual, bits, wscale, act):
-        with _lib.on_device(x.get_device()) as d:
-            ctx.lead, N = x.shape[:-1], (packed or weight).shape[0]
-            xa = _operand(x.detach().reshape(-1, x.shape[-1]))
-            if packed is None:
-                codes, scale = _quantize(weight.detach(), bits, wscale, x.dtype, d.stream)
-            else:
-                codes, scale = _expand(packed, x.dtype, d.stream), packed.scale.contiguous()
-            r = None if residual is None else _rows(residual.detach().reshape(-1, N))
-            b = None if bias is None else bias.detach().contiguous()
-            y, z = _forward(xa, codes, scale, bits, b, act, r, act != 0, d.stream)
-        ctx.save_for_backward(xa, codes, scale, z)
-        ctx.bits, ctx.act = bits, act
-        ctx.wscale = wscale if packed is None else "per_channel"
+        y, xs, z, buf, scales, ctx.layout = _forward(x, packed or weight, packed, bias, residual, bits, wscale, act, True)
+        ctx.save_for_backward(xs, z, buf, scales)
+        ctx.x_shape, ctx.kind, ctx.dtype, ctx.bits, ctx.act = x.shape, _TYPES[x.dtype], x.dtype, bits, act
+        ctx.per_channel = packed is not None or wscale == "per_channel"
         ctx.w_dtype = None if packed is not None else weight.dtype
         ctx.b_dtype = None if bias is None else bias.dtype
-        return y.view(*ctx.lead, N)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        xa, codes, scale, z = ctx.saved_tensors
         want_x, want_w, _, want_b, want_r = ctx.needs_input_grad[:5]
-        with _lib.on_device(xa.get_device()) as d:
-            top = None
-            if want_x and ctx.wscale == "per_tensor":
-                top = scale[:1]
-            elif want_x and xa.dtype == torch.float16:
-                # dz s would leave fp16's range where the scales are small: s / max s is within it
-                top = scale.amax().view(1)
-            dx, dw, db = _backward(g.reshape(-1, codes.shape[0]), xa, codes, scale, z, ctx.bits, ctx.act, top, want_x,
-                                   want_w, ctx.w_dtype, want_b, ctx.b_dtype, d.stream)
-        if dx is not None:
-            dx = dx.view(*ctx.lead, xa.shape[1])
+        if not (want_x or want_w or want_b):
+            return None, None, None, None, g if want_r else None, None, None, None
+        xs, z, buf, scales = ctx.saved_tensors
+        M, N, K, ldx, x_at, codes, scale_at = ctx.layout
+        dev, dt = buf.device, ctx.dtype
+        dx = torch.empty(ctx.x_shape, dtype=dt, device=dev) if want_x else None
+        dw = torch.empty(N, K, dtype=ctx.w_dtype, device=dev) if want_w else None
+        db = torch.empty(N, dtype=ctx.b_dtype, device=dev) if want_b else None
+        if M == 0:
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+            return dx, dw, None, db, g if want_r else None, None, None, None
+        g2, ldg = _two_d(g, N)
+        room, ldn, ldk = _Room(), N + 7 & -8, K + 7 & -8
+        sums = room.take(_lib.tensor_sums(M, N)) if want_b else 0
+        top = room.take(4)
+        dz = room.take(2 * M * ldn) if want_w or not ctx.per_channel else 0
+        dzs = room.take(2 * M * ldn) if want_x and ctx.per_channel else 0
+        work = torch.empty(room.size, dtype=torch.uint8, device=dev)
+        at, base = work.data_ptr(), buf.data_ptr()
+        with _lib.on_device(work.get_device()) as d:
+            _lib.tensor_backward(array("q", (
+                ctx.kind, ctx.bits, ctx.act, M, N, K, xs.data_ptr() + x_at, ldx, 0, 0, 0, 0,
+                _FLOATS[ctx.w_dtype] if want_w else 0, ctx.per_channel, base + codes, ldk, scales.data_ptr() + scale_at,
+                0, 0, 0, 0, g2.data_ptr(), ldg, 0 if z is None else z.data_ptr(), N, at + sums, at + top, at + dz,
+                at + dzs, ldn, 0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
+                0 if db is None else db.data_ptr(), _FLOATS[ctx.b_dtype] if want_b else 0)), d.stream)
         return dx, dw, None, db, g if want_r else None, None, None, None
 
 
@@ -268,7 +263,8 @@ def tensor_linear(x: torch.Tensor, weight, bias=None, *, activation: str | None 
     ``activation``: None, "relu", "gelu" (erf), "gelu_tanh" or "silu".
     Sums are float32; the result is rounded once.  Everything is on one CUDA
     device; the work is queued on its current stream.  Differentiable once, in
-    x, a float weight, bias and residual."""
+    x, a float weight, bias and residual; the backward pass keeps x, the codes
+    and the pre-activation (in fp16)."""
     packed = weight if isinstance(weight, SFPackedWeight) else None
     if packed is None:
         from .._array import resolve_dtype
@@ -280,35 +276,15 @@ def tensor_linear(x: torch.Tensor, weight, bias=None, *, activation: str | None 
         bits = packed.bits
     _check_operands(x, weight, bias, activation, residual)
     act = _lib.ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in
-                                       (x, None if packed else weight, bias, residual)):
-        return _TensorLinear.apply(x, None if packed else weight, packed, bias, residual, bits, scale, act)
-    return _no_grad(x, weight, packed, bias, residual, bits, scale, act)
-
-
-def _no_grad(x, weight, packed, bias, residual, bits, wscale, act):
-    N, K = weight.shape
-    with _lib.on_device(x.get_device()) as d:
-        xa = _operand(x.detach().reshape(-1, K))
-        M = xa.shape[0]
-        small = M <= _lib.SMALL_ROWS
-        if packed is None:
-            codes, scale = _quantize(weight.detach(), bits, wscale, None if small else x.dtype, d.stream)
-        elif small:
-            codes, scale = _rows(packed.codes), packed.scale.contiguous()
-        else:
-            codes, scale = _expand(packed, x.dtype, d.stream), packed.scale.contiguous()
-        r = None if residual is None else _rows(residual.detach().reshape(-1, N))
-        b = None if bias is None else bias.detach().contiguous()
-        if small:
-            y = torch.empty(M, N, dtype=x.dtype, device=x.device)
-            _lib.tensor_linear_small(_TYPES[x.dtype], xa.data_ptr(), max(xa.stride(0), _up8(K)), codes.data_ptr(),
-                                     max(codes.stride(0), K), scale.data_ptr(), bits, _ptr(b),
-                                     0 if b is None else _FLOATS[b.dtype], act, _ptr(r),
-                                     0 if r is None else max(r.stride(0), N), y.data_ptr(), N, M, N, K, d.stream)
-        else:
-            y, _ = _forward(xa, codes, scale, bits, b, act, r, False, d.stream)
-    return y.view(*x.shape[:-1], N)
+    if torch.is_grad_enabled() and (x.requires_grad or (packed is None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
+        return _TensorLinear.apply(x, None if packed is not None else weight, packed, bias, residual, bits, scale, act)
+    if packed is None and x.numel() <= _lib.SMALL_ROWS * x.shape[-1]:
+        # few rows: int8 codes are half the bytes of the product's operand, and the product reads them as they are
+        weight = packed = pack_weight(weight, bits, scale)
+    with torch.no_grad():
+        return _forward(x, weight, packed, bias, residual, bits, scale, act, False)
 
 
 def tensor_failures() -> int:
