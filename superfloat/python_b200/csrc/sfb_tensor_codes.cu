@@ -170,77 +170,77 @@ __global__ void __launch_bounds__(QT) pad_kernel(const uint16_t *__restrict__ x,
 // wait for the product, which sums over channels; top keeps fp16 within its range),
 // each rounded once from float32.  db = sum over rows, in a fixed order: every
 // CTA sums its 64 rows, and a second kernel the CTAs' sums.
-// Memory bound: dy and z read, dz and / or dz s written; a thread has 8 columns and
-// four rows' loads in flight.
+// Memory bound: dy and z read, dz and / or dz s written.
 
 constexpr int BR = 64;                   // rows of a CTA
 constexpr int BC = 256;                  // columns: 32 threads of 8
 
-template <typename T>
-__device__ __forceinline__ Vec<T, 8> load8t(const T *from, int64_t left, bool vec) {
-    if (vec && left >= 8) return *reinterpret_cast<const Vec<T, 8> *>(from);
+template <bool VEC, typename T>
+__device__ __forceinline__ Vec<T, 8> load8t(const T *from, int64_t left) {
+    if constexpr (VEC) return *reinterpret_cast<const Vec<T, 8> *>(from);
     Vec<T, 8> q;
 #pragma unroll
     for (int j = 0; j < 8; j++) q.v[j] = j < left ? from[j] : from_f<T>(0.0f);
     return q;
 }
 
-template <typename T, int ACT>
-__global__ void __launch_bounds__(256) slope_kernel(const T *__restrict__ dy, int64_t ldy, const __half *__restrict__ z,
-                                                    int64_t ldz, int64_t M, int64_t N, const float *__restrict__ scale,
-                                                    float unit, const float *__restrict__ top, T *__restrict__ dz,
-                                                    T *__restrict__ dzs, int64_t ldd, float *__restrict__ sums) {
+// VEC: N is a multiple of 8 and the rows of dy and z start on 16 bytes
+template <typename T, int ACT, bool VEC>
+__global__ void __launch_bounds__(256, VEC ? 4 : 2)
+slope_kernel(const T *__restrict__ dy, int64_t ldy, const __half *__restrict__ z, int64_t ldz, int64_t M, int64_t N,
+             const float *__restrict__ scale, float unit, const float *__restrict__ top, T *__restrict__ dz,
+             T *__restrict__ dzs, int64_t ldd, float *__restrict__ sums) {
     __shared__ float s_sum[8][BC];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int64_t n0 = (int64_t)blockIdx.x * BC + tx * 8, left = N - n0;
-    const int64_t r0 = (int64_t)blockIdx.y * BR + ty;
-    const bool vy = ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(dy) & 15) == 0;
-    const bool vz = ldz % 8 == 0 && (reinterpret_cast<uintptr_t>(z) & 15) == 0;
+    const int64_t r1 = min(M, (int64_t)(blockIdx.y + 1) * BR);
     float acc[8] = {}, f[8];
     if (dzs) {
         const float by = top ? __fdiv_rn(1.0f, *top) : unit;
 #pragma unroll
         for (int j = 0; j < 8; j++) f[j] = j < left ? scale[n0 + j] * by : 0.0f;
     }
+    auto row = [&](int64_t r, const Vec<T, 8> &g, const Vec<__half, 8> &h) {
+        float d[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            d[j] = to_f(g.v[j]);
+            // (one rounding, whatever else is wanted: contracted with the sum it would be none)
+            if constexpr (ACT != SFB_ACT_NONE) d[j] = __fmul_rn(d[j], slope<ACT>(to_f(h.v[j])));
+            acc[j] += d[j];
+        }
+        // ldd is a multiple of 8 and the buffers are aligned: the vector's tail lands in the row's padding
+        if (dz) {
+            Vec<T, 8> q;
+#pragma unroll
+            for (int j = 0; j < 8; j++) q.v[j] = from_f<T>(d[j]);
+            *reinterpret_cast<Vec<T, 8> *>(dz + r * ldd + n0) = q;
+        }
+        if (dzs) {
+            Vec<T, 8> q;
+#pragma unroll
+            for (int j = 0; j < 8; j++) q.v[j] = from_f<T>(d[j] * f[j]);
+            *reinterpret_cast<Vec<T, 8> *>(dzs + r * ldd + n0) = q;
+        }
+    };
     if (left > 0) {
-        for (int i = 0; i < BR / 8; i += 4) {
-            Vec<T, 8> g[4];
-            Vec<__half, 8> h[4];
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int64_t r = r0 + 8 * (i + u);
-                if (r < M) {
-                    g[u] = load8t(dy + r * ldy + n0, left, vy);
-                    if constexpr (ACT != SFB_ACT_NONE) h[u] = load8t(z + r * ldz + n0, left, vz);
-                }
+        int64_t r = (int64_t)blockIdx.y * BR + ty;
+#pragma unroll 1
+        for (; r + 8 < r1; r += 16) {                     // two rows' loads in flight
+            const Vec<T, 8> g0 = load8t<VEC>(dy + r * ldy + n0, left), g1 = load8t<VEC>(dy + (r + 8) * ldy + n0, left);
+            Vec<__half, 8> h0, h1;
+            if constexpr (ACT != SFB_ACT_NONE) {
+                h0 = load8t<VEC>(z + r * ldz + n0, left);
+                h1 = load8t<VEC>(z + (r + 8) * ldz + n0, left);
             }
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int64_t r = r0 + 8 * (i + u);
-                if (r >= M) break;
-                float d[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    d[j] = to_f(g[u].v[j]);
-                    // (one rounding, whatever else is wanted: contracted with the sum it would be none)
-                    if constexpr (ACT != SFB_ACT_NONE) d[j] = __fmul_rn(d[j], slope<ACT>(to_f(h[u].v[j])));
-                    if (j >= left) d[j] = 0.0f;
-                    acc[j] += d[j];
-                }
-                // ldd is a multiple of 8 and the buffers are aligned: the vector's tail lands in the row's padding
-                if (dz) {
-                    Vec<T, 8> q;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) q.v[j] = from_f<T>(d[j]);
-                    *reinterpret_cast<Vec<T, 8> *>(dz + r * ldd + n0) = q;
-                }
-                if (dzs) {
-                    Vec<T, 8> q;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) q.v[j] = from_f<T>(d[j] * f[j]);
-                    *reinterpret_cast<Vec<T, 8> *>(dzs + r * ldd + n0) = q;
-                }
-            }
+            row(r, g0, h0);
+            row(r + 8, g1, h1);
+        }
+        if (r < r1) {
+            const Vec<T, 8> g = load8t<VEC>(dy + r * ldy + n0, left);
+            Vec<__half, 8> h;
+            if constexpr (ACT != SFB_ACT_NONE) h = load8t<VEC>(z + r * ldz + n0, left);
+            row(r, g, h);
         }
     }
     if (sums) {
@@ -360,16 +360,19 @@ int tensor_slope(int dtype, int act, const void *dy, int64_t ldy, const void *z,
     float *sums = db ? static_cast<float *>(work) : nullptr;
     const float unit = 1.0f / (float)(1 << (bits - 1));
     const dim3 grid((unsigned)((N + BC - 1) / BC), (unsigned)parts);
+    const bool vec = N % 8 == 0 && ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(dy) & 15) == 0 &&
+                     (act == SFB_ACT_NONE || (ldz % 8 == 0 && (reinterpret_cast<uintptr_t>(z) & 15) == 0));
     const int rc = with_activation(act, [&](auto a) {
         constexpr int A = decltype(a)::value;
+        auto go = [&](auto *kernel, auto type) {
+            using T = decltype(type);
+            kernel<<<grid, 256, 0, st>>>(static_cast<const T *>(dy), ldy, static_cast<const __half *>(z), ldz, M, N, scale,
+                                         unit, top, static_cast<T *>(dz), static_cast<T *>(dzs), ldd, sums);
+        };
         if (dtype == SFB_BF16)
-            slope_kernel<__nv_bfloat16, A><<<grid, 256, 0, st>>>(
-                static_cast<const __nv_bfloat16 *>(dy), ldy, static_cast<const __half *>(z), ldz, M, N, scale, unit,
-                top, static_cast<__nv_bfloat16 *>(dz), static_cast<__nv_bfloat16 *>(dzs), ldd, sums);
+            vec ? go(slope_kernel<__nv_bfloat16, A, true>, __nv_bfloat16()) : go(slope_kernel<__nv_bfloat16, A, false>, __nv_bfloat16());
         else
-            slope_kernel<__half, A><<<grid, 256, 0, st>>>(static_cast<const __half *>(dy), ldy,
-                                                          static_cast<const __half *>(z), ldz, M, N, scale, unit, top,
-                                                          static_cast<__half *>(dz), static_cast<__half *>(dzs), ldd, sums);
+            vec ? go(slope_kernel<__half, A, true>, __half()) : go(slope_kernel<__half, A, false>, __half());
         return check_launch("sf tensor linear (activation's gradient)");
     });
     if (rc || !db) return rc;
