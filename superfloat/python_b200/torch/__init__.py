@@ -7,6 +7,13 @@ reference's ``sf.torch`` surface for the chain accumulation).
 >>> with torch.no_grad():
 ...     out = fast(x)
 >>> sft.last_status()                                  # exact events per layer
+
+Training and serving on the tensor cores, with the same quantized weights:
+
+>>> model = sft.convert(model.bfloat16(), dtype="sf8", accumulate="tensor")
+>>> opt = sft.AdamW(model.parameters(), lr=1e-4, state="sf8")
+>>> loss(model(x)).backward(); opt.step()              # straight-through gradients
+>>> served = sft.pack(model)                           # weights as int8 codes
 """
 from __future__ import annotations
 
@@ -15,8 +22,8 @@ import torch
 from . import _ops  # noqa: F401  (registers the sf:: custom ops)
 from ._backend import GraphReport, compile_report, compile_reports, superfloat  # noqa: F401
 from ._core import weight_cache  # noqa: F401
-from ._modules import (ConversionReport, SFConfig, SFConv2d, SFHFConv1D, SFLinear, conversion_report, convert,
-                       find_lm_heads, is_hf_conv1d)
+from ._modules import (ConversionReport, SFConfig, SFConv2d, SFHFConv1D, SFLinear, SFPackedLinear, conversion_report,
+                       convert, find_lm_heads, is_hf_conv1d, pack)
 from ._optim import AdamW, SF8Moment, adamw_step, moment_values
 from ._status import SFLayerStatus, capture_status, last_status, reset_status
 from ._tensor import SFPackedWeight, pack_weight, tensor_failures, tensor_linear
@@ -64,4 +71,4 @@ def matmul(a, b, dtype="sf16", headroom="bound", name="matmul", *, accumulate="c
 __all__ = ["quantize", "linear", "matmul", "SFLinear", "SFConv2d", "SFHFConv1D", "SFConfig", "convert",
            "find_lm_heads", "is_hf_conv1d", "conversion_report", "ConversionReport", "last_status",
            "reset_status", "capture_status", "SFLayerStatus", "compile_report", "compile_reports", "GraphReport",
-           "SFPackedWeight", "pack_weight", "tensor_linear", "tensor_failures", "AdamW", "SF8Moment", "adamw_step", "moment_values"]
+           "SFPackedLinear", "pack", "SFPackedWeight", "pack_weight", "tensor_linear", "tensor_failures", "AdamW", "SF8Moment", "adamw_step", "moment_values"]

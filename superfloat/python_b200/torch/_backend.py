@@ -15,7 +15,8 @@ from dataclasses import dataclass, field
 import torch
 from torch._dynamo import register_backend
 
-from ._ops import SF_OP_ARGS, SF_OPS, linear_impl, linear_wide_impl, matmul_impl, matmul_wide_impl
+from ._ops import (SF_OP_ARGS, SF_OPS, linear_impl, linear_tensor_impl, linear_wide_impl, matmul_impl,
+                   matmul_wide_impl)
 
 # float linear algebra that convert() did not turn into SF ops: reported as
 # "not converted" (it runs in float, off the device)
@@ -94,7 +95,7 @@ def _inference_only(tensors) -> None:
 
 # op -> (the function the node is retargeted to, how many leading tensor arguments it checks)
 _DEVICE_IMPLS = {"linear": (linear_impl, 3), "matmul": (matmul_impl, 2), "linear_wide": (linear_wide_impl, 3),
-                 "matmul_wide": (matmul_wide_impl, 2)}
+                 "matmul_wide": (matmul_wide_impl, 2), "linear_tensor": (linear_tensor_impl, 3)}
 
 
 def _on_device(op: str, device_name: str):

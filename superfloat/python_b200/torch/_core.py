@@ -35,7 +35,7 @@ from .._format import FORMATS, SFFormat
 
 WSCALES = ("per_tensor", "per_channel")
 HEADROOMS = ("bound", "none")
-ACCUMULATES = ("chain", "wide")
+ACCUMULATES = ("chain", "wide", "tensor")
 _MAX_ITER = 32
 
 

@@ -13,10 +13,11 @@ from __future__ import annotations
 import copy
 from dataclasses import dataclass, field
 
+import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import _core
+from . import _core, _tensor
 from ._ops import call_linear
 
 
@@ -28,7 +29,10 @@ def _bits_of(dtype) -> int:
 @dataclass
 class SFConfig:
     """How an SF layer computes: width, weight scale ("per_tensor" |
-    "per_channel"), headroom ("bound": no saturation, provable | "none")."""
+    "per_channel"), headroom ("bound": no saturation, provable | "none").
+    ``accumulate``: "chain" and "wide" compute as the chip does; "tensor" takes
+    the weights' sf4..sf8 codes to the tensor cores, with bfloat16 or float16
+    activations and float32 sums (headroom and shift do not apply)."""
 
     bits: int = 16
     scale: str = "per_tensor"
@@ -38,6 +42,8 @@ class SFConfig:
 
     def __post_init__(self):
         _core.check_args(self.bits, self.scale, self.headroom, self.accumulate)
+        if self.accumulate == "tensor":
+            _tensor._check_width(self.bits)
         if self.shift is not None:
             if self.accumulate != "wide":
                 raise ValueError("shift= only applies to accumulate=\"wide\"")
@@ -53,6 +59,8 @@ class SFConfig:
     def describe(self) -> str:
         if self.accumulate == "wide":
             return f"dtype={self.dtype_name}, accumulate=wide" + ("" if self.shift is None else f", shift={self.shift}")
+        if self.accumulate == "tensor":
+            return f"dtype={self.dtype_name}, scale={self.scale}, accumulate=tensor"
         return f"dtype={self.dtype_name}, scale={self.scale}, headroom={self.headroom}"
 
 
@@ -358,6 +366,65 @@ class _Converter:
         return model
 
 
+class SFPackedLinear(nn.Module):
+    """A linear layer whose weight is packed sf codes (buffers ``codes`` int8 and
+    ``scale`` float32): an SF layer of accumulate="tensor" laid out once for
+    serving.  Its weight does not train; gradients pass to x and the bias."""
+
+    def __init__(self, packed: "_tensor.SFPackedWeight", bias=None, name: str = ""):
+        super().__init__()
+        self.bits, self.sf_name = packed.bits, name
+        self.out_features, self.in_features = packed.shape
+        self.register_buffer("codes", packed.codes)
+        self.register_buffer("scale", packed.scale)
+        self.bias = bias
+
+    def forward(self, x, *, activation=None, residual=None):
+        return _tensor.tensor_linear(x, _tensor.SFPackedWeight(self.codes, self.scale, self.bits), self.bias,
+                                     activation=activation, residual=residual)
+
+    def _apply(self, fn, recurse=True):
+        # .to(dtype), .half() and the like move the layer; its scales stay float32
+        scale = self.scale
+        super()._apply(fn, recurse)
+        if self.scale.dtype != torch.float32:
+            self.scale = scale.to(self.scale.device)
+        return self
+
+    def extra_repr(self):
+        return (f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, "
+                f"dtype=sf{self.bits}, name={self.sf_name!r}")
+
+
+def pack(model: nn.Module, inplace: bool = False) -> nn.Module:
+    """Replace the SF linear layers of accumulate="tensor" (SFLinear, SFHFConv1D)
+    by :class:`SFPackedLinear`: their weights' codes are made once, and a weight
+    takes one byte an element.  Other layers stay as they are; a layer that the
+    model reaches twice is packed once."""
+    if not inplace:
+        model = copy.deepcopy(model)
+    done = {}
+
+    def packed(m):
+        if id(m) not in done:
+            w = m.weight.t() if isinstance(m, SFHFConv1D) else m.weight
+            p = _tensor.pack_weight(w, m.sf.bits, m.sf.scale)
+            # (the layer itself is kept, so that its id stays its own)
+            done[id(m)] = (m, SFPackedLinear(p, m.bias, m.sf_name).train(m.training))
+        return done[id(m)][1]
+
+    def wanted(m):
+        return isinstance(m, (SFLinear, SFHFConv1D)) and m.sf.accumulate == "tensor"
+
+    if wanted(model):
+        return packed(model)
+    for parent in list(model.modules()):
+        for name, child in list(parent._modules.items()):
+            if child is not None and wanted(child):
+                setattr(parent, name, packed(child))
+    return model
+
+
 def _keep_plan(model, keep_sf16, bits):
     """(LM heads by id, module names) that stay at sf16 when ``bits`` < 16."""
     if keep_sf16 == "auto":
@@ -379,7 +446,9 @@ def convert(model: nn.Module, dtype="sf16", scale: str = "per_tensor", headroom:
     """Swap ``nn.Linear``, ``nn.Conv2d`` and Hugging Face ``Conv1D`` for SF
     layers (src/sf/torch/_modules.py:295-537).  ``keep_sf16`` ("auto": the LM
     head; False; or module names) keeps layers at sf16 when ``dtype`` is
-    narrower; ``widths`` ({name: dtype}) gives layers their own width."""
+    narrower; ``widths`` ({name: dtype}) gives layers their own width.
+    ``accumulate="tensor"`` runs the layers on the tensor cores, for a model in
+    bfloat16 or float16; it ends at sf8, so "auto" keeps nothing there."""
     if calibration not in ("heuristic",):
         raise ValueError(f"calibration must be 'heuristic', got {calibration!r}")
     if attention not in ("auto", False, None):
@@ -393,6 +462,10 @@ def convert(model: nn.Module, dtype="sf16", scale: str = "per_tensor", headroom:
                                  "on the MX engine, which is not built here; pass attention=False to keep "
                                  "attention in float (the layers still run wide)")
     cfg = SFConfig(_bits_of(dtype), scale, headroom, accumulate, shift)
+    if accumulate == "tensor":
+        if keep_sf16 not in ("auto", False, None):
+            raise ValueError("accumulate=\"tensor\" has no sf16 for keep_sf16 to keep layers at")
+        keep_sf16 = False
     if not inplace:
         model = copy.deepcopy(model)
     keep_ids, keep_names = _keep_plan(model, keep_sf16, cfg.bits)
@@ -400,7 +473,7 @@ def convert(model: nn.Module, dtype="sf16", scale: str = "per_tensor", headroom:
     if widths:
         _unknown_names(model, widths, "widths")
         per_layer = {n: SFConfig(_bits_of(d), scale, headroom, accumulate, shift) for n, d in widths.items()}
-    cfg16 = SFConfig(16, scale, headroom, accumulate, shift)
+    cfg16 = cfg if accumulate == "tensor" else SFConfig(16, scale, headroom, accumulate, shift)
     return _Converter(cfg, cfg16, per_layer, keep_ids, keep_names).run(model)
 
 

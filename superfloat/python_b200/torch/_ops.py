@@ -7,6 +7,9 @@ the reference's (src/sf/torch/_ops.py:184-417):
   with the scale policy;
 * ``sf::matmul(a, b, bits, headroom, name)``: the SF matmul of two
   activations;
+* ``sf::linear_tensor(x, weight, bias, bits, wscale, name)``: the linear over
+  sf4..sf8 codes on the tensor cores (``accumulate="tensor"``, no counterpart
+  in the reference): bfloat16 or float16 in and out;
 * ``sf::linear_wide(x, weight, bias, bits, shift, name)`` and
   ``sf::matmul_wide(a, b, bits, shift, name)``: the same on the MX engine
   (``accumulate="wide"``) with the wide-mode shift rule; ``shift`` (an int)
@@ -26,7 +29,7 @@ from typing import Optional
 
 import torch
 
-from . import _core, _wide
+from . import _core, _tensor, _wide
 from ._status import SFLayerStatus, record
 
 if hasattr(torch.ops, "sf") and hasattr(torch.ops.sf, "linear"):
@@ -94,6 +97,12 @@ def matmul_wide_impl(a, b, bits, shift, name):
     r = _wide.wide_matmul(a, b, bits, shift, dev, out_dtype=od)
     _record(name, "matmul", dev.name, bits, r)
     return r.y.to(device=a.device, dtype=od)
+
+
+def linear_tensor_impl(x, weight, bias, bits, wscale, name):
+    # no fixed-point step can saturate or flush here, so there are no events and no status
+    with torch.no_grad():
+        return _tensor.tensor_linear(x, weight, bias, dtype=bits, scale=wscale)
 
 
 # --- sf::quantize -------------------------------------------------------------------------
@@ -275,13 +284,53 @@ torch.library.register_autograd("sf::matmul_wide", lambda ctx, g: _matmul_backwa
                                 setup_context=lambda ctx, inputs, output: ctx.save_for_backward(inputs[0], inputs[1]))
 
 
+# --- the tensor cores: sf::linear_tensor -------------------------------------------------------
+
+@torch.library.custom_op("sf::linear_tensor", mutates_args=())
+def linear_tensor(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], bits: int, wscale: str,
+                  name: str) -> torch.Tensor:
+    return linear_tensor_impl(x, weight, bias, bits, wscale, name)
+
+
+@linear_tensor.register_fake
+def _(x, weight, bias, bits, wscale, name):
+    return x.new_empty(tuple(x.shape[:-1]) + (weight.shape[0],))
+
+
+def _linear_tensor_setup(ctx, inputs, output):
+    ctx.save_for_backward(*(t for t in inputs[:3] if t is not None))
+    ctx.bits, ctx.wscale = inputs[3], inputs[4]
+
+
+def _linear_tensor_backward(ctx, g):
+    """The layer again, differentiated by its own backward pass: the op keeps only its inputs."""
+    inputs = [t.detach().requires_grad_(need) for t, need in zip(ctx.saved_tensors, ctx.needs_input_grad)]
+    with torch.enable_grad():
+        y = _tensor.tensor_linear(*inputs, dtype=ctx.bits, scale=ctx.wscale)
+    wanted = [t for t in inputs if t.requires_grad]
+    grads = iter(torch.autograd.grad(y, wanted, g))
+    out = [next(grads) if t.requires_grad else None for t in inputs]
+    return (*out, *[None] * (6 - len(out)))
+
+
+torch.library.register_autograd("sf::linear_tensor", _linear_tensor_backward, setup_context=_linear_tensor_setup)
+
+
 def call_linear(x, weight, bias, cfg, name):
+    if cfg.accumulate == "tensor":
+        if torch.compiler.is_compiling():                   # one opaque node, as the other modes are
+            return torch.ops.sf.linear_tensor(x, weight, bias, cfg.bits, cfg.scale, name)
+        return _tensor.tensor_linear(x, weight, bias, dtype=cfg.bits, scale=cfg.scale)
     if cfg.accumulate == "wide":
         return torch.ops.sf.linear_wide(x, weight, bias, cfg.bits, cfg.shift, name)
     return torch.ops.sf.linear(x, weight, bias, cfg.bits, cfg.scale, cfg.headroom, name)
 
 
 def call_matmul(a, b, cfg, name):
+    if cfg.accumulate == "tensor":
+        from .._errors import SFUnsupportedError
+        raise SFUnsupportedError("accumulate=\"tensor\" is for linear layers, whose weights are quantized; a matmul of "
+                                 "two activations runs in \"chain\" or \"wide\"")
     if cfg.accumulate == "wide":
         return torch.ops.sf.matmul_wide(a, b, cfg.bits, cfg.shift, name)
     return torch.ops.sf.matmul(a, b, cfg.bits, cfg.headroom, name)
@@ -289,5 +338,7 @@ def call_matmul(a, b, cfg, name):
 
 SF_OPS = {"sf.linear": "linear", "sf.linear.default": "linear", "sf.matmul": "matmul",
           "sf.matmul.default": "matmul", "sf.linear_wide": "linear_wide", "sf.linear_wide.default": "linear_wide",
-          "sf.matmul_wide": "matmul_wide", "sf.matmul_wide.default": "matmul_wide"}
-SF_OP_ARGS = {"linear": (3, 6), "matmul": (2, 4), "linear_wide": (3, 5), "matmul_wide": (2, 4)}
+          "sf.matmul_wide": "matmul_wide", "sf.matmul_wide.default": "matmul_wide",
+          "sf.linear_tensor": "linear_tensor", "sf.linear_tensor.default": "linear_tensor"}
+SF_OP_ARGS = {"linear": (3, 6), "matmul": (2, 4), "linear_wide": (3, 5), "matmul_wide": (2, 4),
+              "linear_tensor": (3, 5)}

@@ -58,23 +58,19 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
-    return a.shape == b.shape and (a.stride() == b.stride() or (a.is_contiguous() and b.is_contiguous()))
-
-
-def _check_sf8(m: SF8Moment, n: int, device, what: str) -> None:
+def _check_sf8(m: SF8Moment, n: int, device, what: str, i: int) -> None:
     c, s = m.codes, m.scale
     if c.dtype != torch.int8 or s.dtype != torch.float32:
-        raise SFTypeError(f"{what}: an sf8 moment has int8 codes and float32 scales, got {c.dtype} and {s.dtype}")
+        raise SFTypeError(f"{what} {i}: an sf8 moment has int8 codes and float32 scales, got {c.dtype} and {s.dtype}")
     if c.numel() != n or s.numel() != -(-n // BLOCK):
-        raise SFShapeError(f"{what}: {n} elements need {n} codes and {-(-n // BLOCK)} scales, got {c.numel()} and "
+        raise SFShapeError(f"{what} {i}: {n} elements need {n} codes and {-(-n // BLOCK)} scales, got {c.numel()} and "
                            f"{s.numel()}")
     if c.device != device or s.device != device:
-        raise SFShapeError(f"{what}: the moment is not on {device}")
+        raise SFShapeError(f"{what} {i}: the moment is not on {device}")
     if not (c.is_contiguous() and s.is_contiguous()):
-        raise SFShapeError(f"{what}: codes and scales must be contiguous")
+        raise SFShapeError(f"{what} {i}: codes and scales must be contiguous")
     if n and c.data_ptr() % 4:
-        raise SFShapeError(f"{what}: the codes must start on a 4-byte boundary")
+        raise SFShapeError(f"{what} {i}: the codes must start on a 4-byte boundary")
 
 
 def _check_rates(lr, betas, eps, weight_decay):
@@ -92,38 +88,40 @@ def _buckets(params, grads, exp_avg, exp_avg_sq):
     tensor, after the checks; and the gradients that had to be laid out."""
     buckets, kept = {}, []
     for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avg, exp_avg_sq)):
-        dt = _ELEMENT.get(p.dtype)
+        dt, shape, device = _ELEMENT.get(p.dtype), p.shape, p.device
         if dt is None:
             raise SFTypeError(f"adamw: tensor {i} is {p.dtype}; float32, bfloat16 and float16 are supported")
         if g.dtype != p.dtype:
             raise SFTypeError(f"adamw: tensor {i} is {p.dtype} and its gradient {g.dtype}")
-        if not p.is_cuda or g.device != p.device:
-            raise SFShapeError(f"adamw: tensor {i} and its gradient must be on one CUDA device, got {p.device} and "
+        if not p.is_cuda or g.device != device:
+            raise SFShapeError(f"adamw: tensor {i} and its gradient must be on one CUDA device, got {device} and "
                                f"{g.device}")
-        if g.is_sparse or g.layout != torch.strided:
+        if g.layout != torch.strided:
             raise SFUnsupportedError(f"adamw: tensor {i} has a gradient that is not strided")
-        if g.shape != p.shape:
-            raise SFShapeError(f"adamw: tensor {i} has shape {tuple(p.shape)}, its gradient {tuple(g.shape)}")
-        if not _dense(p):
-            raise SFShapeError(f"adamw: tensor {i} has gaps or overlaps in memory (shape {tuple(p.shape)}, strides "
+        if g.shape != shape:
+            raise SFShapeError(f"adamw: tensor {i} has shape {tuple(shape)}, its gradient {tuple(g.shape)}")
+        plain = p.is_contiguous()
+        if not plain and not _dense(p):
+            raise SFShapeError(f"adamw: tensor {i} has gaps or overlaps in memory (shape {tuple(shape)}, strides "
                                f"{p.stride()})")
-        if not _same_layout(p, g):
-            g = torch.empty_strided(p.shape, p.stride(), dtype=g.dtype, device=g.device).copy_(g)
+        if not (g.is_contiguous() if plain else g.stride() == p.stride()):
+            with torch.no_grad():
+                g = torch.empty_strided(shape, p.stride(), dtype=g.dtype, device=device).copy_(g)
             kept.append(g)
         n = p.numel()
         sf8 = isinstance(m, SF8Moment)
         if sf8 != isinstance(v, SF8Moment):
             raise SFTypeError(f"adamw: tensor {i} has one moment in sf8 and one that is not")
         if sf8:
-            _check_sf8(m, n, p.device, f"adamw: first moment of tensor {i}")
-            _check_sf8(v, n, p.device, f"adamw: second moment of tensor {i}")
+            _check_sf8(m, n, device, "adamw: first moment of tensor", i)
+            _check_sf8(v, n, device, "adamw: second moment of tensor", i)
             words = (p.data_ptr(), g.data_ptr(), m.codes.data_ptr(), v.codes.data_ptr(), m.scale.data_ptr(),
                      v.scale.data_ptr(), n, (i * _SEED_STEP) & 0xFFFFFFFF)
         else:
             for t in (m, v):
                 if t.dtype != torch.float32:
                     raise SFTypeError(f"adamw: tensor {i} has a moment of {t.dtype}; float32 or SF8Moment")
-                if t.device != p.device or not _same_layout(p, t):
+                if t.device != device or t.shape != shape or not (t.is_contiguous() if plain else t.stride() == p.stride()):
                     raise SFShapeError(f"adamw: tensor {i} has a moment of another shape, layout or device")
             words = (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, n, 0)
         key = (p.get_device(), dt, sf8)
@@ -141,7 +139,6 @@ def _launch(buckets, lr, betas, eps, weight_decay, step, dither, constants=None)
                        dither & 0xFFFFFFFF, constants, d.stream)
 
 
-@torch.no_grad()
 def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step: int, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 0.0, dither: int = 0) -> None:
     """One AdamW step on lists of CUDA tensors, in place, on each device's
@@ -165,7 +162,6 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step: int, lr: float, beta
     _launch(buckets, lr, betas, eps, weight_decay, step, dither)
 
 
-@torch.no_grad()
 def moment_values(moments, kind: str) -> list:
     """The float32 values of moments: what the codes of each
     :class:`SF8Moment` stand for, flat in storage order, and float32 moments as
@@ -180,7 +176,7 @@ def moment_values(moments, kind: str) -> list:
         n = m.codes.numel()
         if not m.codes.is_cuda:
             raise SFShapeError(f"moment {i} must be on a CUDA device, got {m.codes.device}")
-        _check_sf8(m, n, m.codes.device, f"moment {i}")
+        _check_sf8(m, n, m.codes.device, "moment", i)
         out.append(torch.empty(n, dtype=torch.float32, device=m.codes.device))
         tables.setdefault(m.codes.get_device(), array("q")).extend(
             (out[-1].data_ptr(), m.codes.data_ptr(), 0, 0, m.scale.data_ptr(), 0, n, 0))

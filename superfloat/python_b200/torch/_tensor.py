@@ -283,8 +283,7 @@ def tensor_linear(x: torch.Tensor, weight, bias=None, *, activation: str | None 
     if packed is None and x.numel() <= _lib.SMALL_ROWS * x.shape[-1]:
         # few rows: int8 codes are half the bytes of the product's operand, and the product reads them as they are
         weight = packed = pack_weight(weight, bits, scale)
-    with torch.no_grad():
-        return _forward(x, weight, packed, bias, residual, bits, scale, act, False)
+    return _forward(x, weight, packed, bias, residual, bits, scale, act, False)
 
 
 def tensor_failures() -> int:

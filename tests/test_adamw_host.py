@@ -152,12 +152,11 @@ def test_refusals():
     sft.adamw_step([], [], [], [], **ok)              # nothing to do
 
 
-def test_dense_and_layout_rules():
-    from superfloat.python_b200.torch._optim import _dense, _same_layout
+def test_dense_rule():
+    from superfloat.python_b200.torch._optim import _dense
     t = torch.zeros(4, 6)
     assert _dense(t) and _dense(t.t()) and _dense(torch.zeros(0)) and _dense(torch.zeros(3, 1, 2).transpose(0, 1))
     assert not _dense(t[:, :5]) and not _dense(t[0].expand(3, 6)) and not _dense(t[::2])
-    assert _same_layout(t, t.clone()) and not _same_layout(t, torch.zeros(6, 4).t())
 
 
 @pytest.fixture(scope="module")
