@@ -413,7 +413,7 @@ typedef struct sfb_tensor_call {
 /* The forward pass.  A float weight is quantized first (by sfb_code_quantize's rule);
  * packed codes are expanded into `codes`, or where that is NULL, for at most
  * SFB_SMALL_ROWS rows and no z, read as they are. */
-#define SFB_SMALL_ROWS 64
+#define SFB_SMALL_ROWS 48
 SFB_API int sfb_tensor_forward(const sfb_tensor_call *call, sfb_stream stream);
 
 /* The backward pass: dz = dy act'(z), dx = (dz scale) codes, dw = dz^T x (straight

@@ -423,7 +423,7 @@ ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 I8 = 4                                     # SFB_I8: packed codes
 
 
-SMALL_ROWS = 64                            # SFB_SMALL_ROWS
+SMALL_ROWS = 48                            # SFB_SMALL_ROWS
 # the fields of sfb_tensor_call, in order: 8 bytes each
 TENSOR_CALL = ("dtype", "bits", "act", "M", "N", "K", "x", "ldx", "xpad", "ldp", "w", "ldw", "w_dtype", "per_channel",
                "codes", "ldc", "scale", "bias", "bias_dtype", "residual", "ldr", "y", "ldy", "z", "ldz", "work", "top",

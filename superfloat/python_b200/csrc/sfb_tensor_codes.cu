@@ -124,27 +124,29 @@ __global__ void __launch_bounds__(QT) code_kernel(const W *__restrict__ w, int64
 
 // A thread turns 16 codes of a row at a time; where rows do not start on 16
 // bytes it loads them one by one (the stores are aligned: the rows of `out` are).
+// Rows without gaps are one long row.  64 threads along a row, 4 rows a CTA.
 template <typename O>
 __global__ void __launch_bounds__(QT) expand_kernel(const int8_t *__restrict__ codes, int64_t N, int64_t K, int64_t ldc,
                                                     O *__restrict__ out, int64_t ldo, bool vec) {
-    const int64_t per = (K + 15) / 16, total = N * per;
-    for (int64_t i = (int64_t)blockIdx.x * QT + threadIdx.x; i < total; i += (int64_t)gridDim.x * QT) {
-        const int64_t n = i / per, k = (i - n * per) * 16;
-        const int8_t *from = codes + n * ldc + k;
-        O *to = out + n * ldo + k;
-        Vec<int8_t, 16> q;
-        if (vec && k + 16 <= K) {
-            q = *reinterpret_cast<const Vec<int8_t, 16> *>(from);
-        } else {
+    for (int64_t n = (int64_t)blockIdx.y * 4 + threadIdx.y; n < N; n += 4ll * gridDim.y) {
+#pragma unroll 4
+        for (int64_t k = ((int64_t)blockIdx.x * 64 + threadIdx.x) * 16; k < K; k += 1024ll * gridDim.x) {
+            const int8_t *from = codes + n * ldc + k;
+            O *to = out + n * ldo + k;
+            Vec<int8_t, 16> q;
+            if (vec && k + 16 <= K) {
+                q = *reinterpret_cast<const Vec<int8_t, 16> *>(from);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 16; j++) q.v[j] = k + j < K ? from[j] : (int8_t)0;
-        }
+                for (int j = 0; j < 16; j++) q.v[j] = k + j < K ? from[j] : (int8_t)0;
+            }
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            Vec<O, 8> r;
+            for (int h = 0; h < 2; h++) {
+                Vec<O, 8> r;
 #pragma unroll
-            for (int j = 0; j < 8; j++) r.v[j] = from_f<O>((float)q.v[8 * h + j]);
-            if (k + 8 * h < K) *reinterpret_cast<Vec<O, 8> *>(to + 8 * h) = r;   // a row's padding may be written
+                for (int j = 0; j < 8; j++) r.v[j] = from_f<O>((float)q.v[8 * h + j]);
+                if (k + 8 * h < K) *reinterpret_cast<Vec<O, 8> *>(to + 8 * h) = r;   // a row's padding may be written
+            }
         }
     }
 }
@@ -153,14 +155,13 @@ __global__ void __launch_bounds__(QT) expand_kernel(const int8_t *__restrict__ c
 
 __global__ void __launch_bounds__(QT) pad_kernel(const uint16_t *__restrict__ x, int64_t M, int64_t K, int64_t ldx,
                                                  uint16_t *__restrict__ out, int64_t ldo) {
-    const int64_t per = (K + 7) / 8, total = M * per;
-    for (int64_t i = (int64_t)blockIdx.x * QT + threadIdx.x; i < total; i += (int64_t)gridDim.x * QT) {
-        const int64_t m = i / per, k = (i - m * per) * 8;
-        Vec<uint16_t, 8> q;
+    for (int64_t m = (int64_t)blockIdx.y * 4 + threadIdx.y; m < M; m += 4ll * gridDim.y)
+        for (int64_t k = ((int64_t)blockIdx.x * 64 + threadIdx.x) * 8; k < K; k += 512ll * gridDim.x) {
+            Vec<uint16_t, 8> q;
 #pragma unroll
-        for (int j = 0; j < 8; j++) q.v[j] = k + j < K ? x[m * ldx + k + j] : (uint16_t)0;
-        *reinterpret_cast<Vec<uint16_t, 8> *>(out + m * ldo + k) = q;
-    }
+            for (int j = 0; j < 8; j++) q.v[j] = k + j < K ? x[m * ldx + k + j] : (uint16_t)0;
+            *reinterpret_cast<Vec<uint16_t, 8> *>(out + m * ldo + k) = q;
+        }
 }
 
 // --- the gradient of the pre-activation --------------------------------------------------------------
@@ -328,20 +329,22 @@ int tensor_quantize(const void *w, int dtype, int64_t N, int64_t K, int64_t ldw,
 
 int tensor_expand(const int8_t *codes, int64_t N, int64_t K, int64_t ldc, void *out, int64_t ldo, int dtype,
                   cudaStream_t st) {
-    const int64_t total = N * ((K + 15) / 16);
-    const unsigned grid = (unsigned)std::min<int64_t>((total + QT - 1) / QT, 16ll * sm_count());
     const bool vec = ldc % 16 == 0 && (reinterpret_cast<uintptr_t>(codes) & 15) == 0;
+    if (ldc == K && ldo == K && K % 16 == 0) K *= N, N = 1, ldc = ldo = K;
+    const int64_t room = 16ll * sm_count(), gy = std::min<int64_t>((N + 3) / 4, room),
+                  gx = std::min<int64_t>((K + 1023) / 1024, std::max<int64_t>(1, (N == 1 ? 4 : 1) * room / gy));
+    const dim3 grid((unsigned)gx, (unsigned)gy), block(64, N == 1 ? 1 : 4);
     if (dtype == SFB_BF16)
-        expand_kernel<<<grid, QT, 0, st>>>(codes, N, K, ldc, static_cast<__nv_bfloat16 *>(out), ldo, vec);
+        expand_kernel<<<grid, block, 0, st>>>(codes, N, K, ldc, static_cast<__nv_bfloat16 *>(out), ldo, vec);
     else
-        expand_kernel<<<grid, QT, 0, st>>>(codes, N, K, ldc, static_cast<__half *>(out), ldo, vec);
+        expand_kernel<<<grid, block, 0, st>>>(codes, N, K, ldc, static_cast<__half *>(out), ldo, vec);
     return check_launch("sf tensor linear (packed codes)");
 }
 
 int tensor_pad(const void *x, int64_t M, int64_t K, int64_t ldx, void *out, int64_t ldo, cudaStream_t st) {
-    const int64_t total = M * ((K + 7) / 8);
-    const unsigned grid = (unsigned)std::min<int64_t>((total + QT - 1) / QT, 16ll * sm_count());
-    pad_kernel<<<grid, QT, 0, st>>>(static_cast<const uint16_t *>(x), M, K, ldx, static_cast<uint16_t *>(out), ldo);
+    const int64_t room = 16ll * sm_count(), gy = std::min<int64_t>((M + 3) / 4, room);
+    const dim3 grid((unsigned)std::min<int64_t>((K + 511) / 512, std::max<int64_t>(1, room / gy)), (unsigned)gy);
+    pad_kernel<<<grid, dim3(64, 4), 0, st>>>(static_cast<const uint16_t *>(x), M, K, ldx, static_cast<uint16_t *>(out), ldo);
     return check_launch("sf tensor linear (rows of x)");
 }
 

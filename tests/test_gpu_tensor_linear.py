@@ -29,7 +29,7 @@ from superfloat.python_b200._errors import SFShapeError, SFTypeError, SFUnsuppor
 pytestmark = pytest.mark.gpu
 TYPES = [torch.bfloat16, torch.float16]
 ACTS = [None, "relu", "gelu", "gelu_tanh", "silu"]
-SIZES = [(1, 1, 1), (1, 16, 16), (2, 3, 5), (7, 40, 24), (16, 130, 64), (17, 64, 129), (64, 257, 72), (128, 256, 64),
+SIZES = [(1, 1, 1), (1, 16, 16), (2, 3, 5), (7, 40, 24), (16, 130, 64), (17, 64, 129), (33, 96, 256), (48, 257, 72), (49, 40, 128), (128, 256, 64),
          (129, 259, 65), (200, 515, 1000), (515, 300, 96), (1000, 33, 2049)]
 
 

@@ -48,7 +48,7 @@ def call(fn, **kw):
     dict(codes=0), dict(codes=3 * A + 2), dict(ldc=60), dict(ldc=68), dict(scale=0), dict(w_dtype=7), dict(w=0),
     dict(x=0), dict(y=0), dict(ldx=63), dict(ldw=63), dict(ldy=63), dict(ldz=63), dict(bias=A, bias_dtype=9),
     dict(residual=A, ldr=63), dict(per_channel=0, work=0), dict(x=A + 2), dict(ldx=65), dict(x=A + 2, xpad=A, ldp=63),
-    dict(x=A + 2, xpad=A + 2, ldp=64), dict(w_dtype=4, codes=0, M=65), dict(w_dtype=4, codes=0, M=8)])
+    dict(x=A + 2, xpad=A + 2, ldp=64), dict(w_dtype=4, codes=0, M=49), dict(w_dtype=4, codes=0, M=8)])
 def test_forward_refusals(lib, bad):
     assert call(lib.sfb_tensor_forward, **bad) == _lib.SFB_EINVAL and lib.sfb_last_error()
 
