@@ -26,8 +26,8 @@
 // A CTA takes one chunk of one tensor, found by bisection over the chunk counts.
 // Float32 moments: bound by memory, 28 bytes an element with float32 p and g, 6430
 // GB/s for 46.5 M elements (202 us).  sf8 moments: 16.06 bytes an element with float32
-// p and g, 10.06 with 16-bit ones, against about 88 instructions of arithmetic: 136
-// us for 46.5 M float32 elements (5500 GB/s), 328 us for 117 M of bf16 (3590 GB/s,
+// p and g, 10.06 with 16-bit ones, against about 85 instructions of arithmetic: 133
+// us for 46.5 M float32 elements (5600 GB/s), 318 us for 117 M of bf16 (3700 GB/s,
 // bound by instruction issue).
 #include <math.h>
 
@@ -59,7 +59,7 @@ struct Entry {
     float *ms, *vs;
     int64_t n;
     uint32_t seed;                            // of the dither, less the call's
-    uint32_t vec;                             // p and g are aligned for vectors of four
+    uint32_t vec;                             // all are aligned for vectors of four (sf8: eight) elements
 };
 
 template <int CAP>
@@ -236,66 +236,60 @@ __device__ __forceinline__ uint32_t bytes_of(const float (&c)[4]) {
     return __byte_perm(a, b, 0x5410);
 }
 
-// A block of 256 elements by one warp: lane l has elements 4 l .. 4 l + 3 of each half.
-// What it loads.  (Loading the next block under this one's arithmetic was slower: 22
-// registers more leave 3 CTAs an SM and spill, 157 and 411 us against 151 and 342
-// for 46.5 M float32 and 117 M bf16 elements.)
+// A block of 256 elements by one warp: lane l has elements 8 l .. 8 l + 7, one access
+// an array.  (With four elements an access, 16 accesses a lane and block for 9, 117 M
+// elements of bf16 took 328 us, now 318.  Loading the next block under this one's arithmetic
+// was slower, too: its registers cost warps.)
 template <typename T>
 struct Loaded {
-    Vec<T, 4> p[2], g[2];
-    uint32_t cm[2], cv[2];
+    Vec<T, 8> p, g;
+    uint2 cm, cv;
     float sm, sv;
 };
 
 template <typename T>
 __device__ __forceinline__ void load_block(const Entry &e, int64_t blk, int lane, Loaded<T> &q) {
-    const int64_t base = blk * AB;
-    const T *p = static_cast<const T *>(e.p), *g = static_cast<const T *>(e.g);
-    const uint8_t *mc = static_cast<const uint8_t *>(e.m), *vc = static_cast<const uint8_t *>(e.v);
+    const int64_t i = blk * AB + lane * 8;
+    const T *p = static_cast<const T *>(e.p) + i, *g = static_cast<const T *>(e.g) + i;
+    const uint8_t *mc = static_cast<const uint8_t *>(e.m) + i, *vc = static_cast<const uint8_t *>(e.v) + i;
     q.sm = e.ms[blk];
     q.sv = e.vs[blk];
-    if (base + AB <= e.n && e.vec) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int64_t i = base + h * 128 + lane * 4;
-            q.g[h] = *reinterpret_cast<const Vec<T, 4> *>(g + i);
-            q.cm[h] = *reinterpret_cast<const uint32_t *>(mc + i);
-            q.cv[h] = *reinterpret_cast<const uint32_t *>(vc + i);
-            q.p[h] = *reinterpret_cast<const Vec<T, 4> *>(p + i);
-        }
+    if (blk * AB + AB <= e.n && e.vec) {
+        q.g = *reinterpret_cast<const Vec<T, 8> *>(g);
+        q.cm = *reinterpret_cast<const uint2 *>(mc);
+        q.cv = *reinterpret_cast<const uint2 *>(vc);
+        q.p = *reinterpret_cast<const Vec<T, 8> *>(p);
         return;
     }
+    uint32_t a[2] = {0, 0}, b[2] = {0, 0};
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const int64_t i = base + h * 128 + lane * 4;
-        q.cm[h] = q.cv[h] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const bool in = i + j < e.n;
-            q.g[h].v[j] = in ? g[i + j] : from_f<T>(0.0f);
-            q.p[h].v[j] = in ? p[i + j] : from_f<T>(0.0f);
-            if (in) {
-                q.cm[h] |= (uint32_t)mc[i + j] << (8 * j);
-                q.cv[h] |= (uint32_t)vc[i + j] << (8 * j);
-            }
+    for (int j = 0; j < 8; j++) {
+        const bool in = i + j < e.n;
+        q.g.v[j] = in ? g[j] : from_f<T>(0.0f);
+        q.p.v[j] = in ? p[j] : from_f<T>(0.0f);
+        if (in) {
+            a[j / 4] |= (uint32_t)mc[j] << (8 * (j % 4));
+            b[j / 4] |= (uint32_t)vc[j] << (8 * (j % 4));
         }
     }
+    q.cm = make_uint2(a[0], a[1]);
+    q.cv = make_uint2(b[0], b[1]);
 }
 
 template <typename T>
 __device__ __forceinline__ void block_sf8(const Entry &e, int64_t blk, const Coefs &c, int lane, const Loaded<T> &q) {
-    const int64_t base = blk * AB;
-    T *p = static_cast<T *>(e.p);
-    uint8_t *mc = static_cast<uint8_t *>(e.m), *vc = static_cast<uint8_t *>(e.v);
-    const bool whole = base + AB <= e.n;
-    const uint32_t *cm = q.cm, *cv = q.cv;
+    const int64_t i = blk * AB + lane * 8;
+    T *p = static_cast<T *>(e.p) + i;
+    uint8_t *mc = static_cast<uint8_t *>(e.m) + i, *vc = static_cast<uint8_t *>(e.v) + i;
+    const bool vec = blk * AB + AB <= e.n && e.vec;
+    const uint32_t cm[2] = {q.cm.x, q.cm.y}, cv[2] = {q.cv.x, q.cv.y};
     const float sm = q.sm, sv = q.sv;
     float P[8], G[8];
     float2 M[4], V[4], S[4];                        // pairs of elements
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        P[j] = to_f(q.p[j / 4].v[j % 4]);
-        G[j] = to_f(q.g[j / 4].v[j % 4]);
+        P[j] = to_f(q.p.v[j]);
+        G[j] = to_f(q.g.v[j]);
     }
     const float um = __fmul_rn(sm, UNIT2), uv = __fmul_rn(sv, UNIT4);
     float tm = 0.0f, tv = 0.0f;
@@ -318,9 +312,16 @@ __device__ __forceinline__ void block_sf8(const Entry &e, int64_t blk, const Coe
         P[2 * j] = r.x;
         P[2 * j + 1] = r.y;
     }
+    if (vec) {
+        Vec<T, 8> r;
 #pragma unroll
-    for (int h = 0; h < 2; h++)
-        store4(p, base + h * 128 + lane * 4, e.n, e.vec, *reinterpret_cast<float(*)[4]>(P + 4 * h));
+        for (int j = 0; j < 8; j++) r.v[j] = from_f<T>(P[j]);
+        *reinterpret_cast<Vec<T, 8> *>(p) = r;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (i + j < e.n) p[j] = from_f<T>(P[j]);
+    }
     // magnitudes order as their bits, NaN above all
     const float sm1 = scale_of(__reduce_max_sync(0xffffffffu, __float_as_uint(tm) & 0x7FFFFFFFu));
     const float sv1 = scale_of(__reduce_max_sync(0xffffffffu, __float_as_uint(tv) & 0x7FFFFFFFu));
@@ -330,14 +331,15 @@ __device__ __forceinline__ void block_sf8(const Entry &e, int64_t blk, const Coe
         e.ms[blk] = sm1;
         e.vs[blk] = sv1;
     }
-    const uint32_t seed = e.seed + c.dither, i0 = (uint32_t)base + lane * 4;
+    const uint32_t seed = e.seed + c.dither, i0 = (uint32_t)i;
+    uint32_t xs[2], ys[2];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         float a[4], b[4];
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             const int j = 2 * h + k;
-            const uint32_t r0 = mixed(i0 + h * 128 + 2 * k, seed), r1 = mixed(i0 + h * 128 + 2 * k + 1, seed);
+            const uint32_t r0 = mixed(i0 + 2 * j, seed), r1 = mixed(i0 + 2 * j + 1, seed);
             // a 16-bit number u under 2^23 as a float, then (2^23 + u) 2^-16 - 2^7 = u 2^-16 exactly
             const float2 lo = fma2(make_float2(__uint_as_float(__byte_perm(r0, 0x4B000000u, 0x7610)),
                                                __uint_as_float(__byte_perm(r1, 0x4B000000u, 0x7610))),
@@ -354,19 +356,19 @@ __device__ __forceinline__ void block_sf8(const Entry &e, int64_t blk, const Coe
             b[2 * k] = y.x;
             b[2 * k + 1] = y.y;
         }
-        const int64_t i = base + h * 128 + lane * 4;
-        const uint32_t x = bytes_of(a), y = bytes_of(b);
-        if (whole) {
-            *reinterpret_cast<uint32_t *>(mc + i) = x;
-            *reinterpret_cast<uint32_t *>(vc + i) = y;
-        } else {
+        xs[h] = bytes_of(a);
+        ys[h] = bytes_of(b);
+    }
+    if (vec) {
+        *reinterpret_cast<uint2 *>(mc) = make_uint2(xs[0], xs[1]);
+        *reinterpret_cast<uint2 *>(vc) = make_uint2(ys[0], ys[1]);
+    } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (i + j < e.n) {
-                    mc[i + j] = (uint8_t)(x >> (8 * j));
-                    vc[i + j] = (uint8_t)(y >> (8 * j));
-                }
-        }
+        for (int j = 0; j < 8; j++)
+            if (i + j < e.n) {
+                mc[j] = (uint8_t)(xs[j / 4] >> (8 * (j % 4)));
+                vc[j] = (uint8_t)(ys[j / 4] >> (8 * (j % 4)));
+            }
     }
 }
 
@@ -560,8 +562,9 @@ int run_adamw(const int64_t *rows, int count, const Coefs &c, const Coefs *dev, 
         for (int i = 0; i < t.count; i++) {
             Entry &e = t.e[i];
             const uintptr_t a = reinterpret_cast<uintptr_t>(e.p) | reinterpret_cast<uintptr_t>(e.g);
-            const uintptr_t b = SF8 ? 0 : reinterpret_cast<uintptr_t>(e.m) | reinterpret_cast<uintptr_t>(e.v);
-            e.vec = (a & (4 * sizeof(T) - 1)) == 0 && (b & 15) == 0;
+            const uintptr_t b = reinterpret_cast<uintptr_t>(e.m) | reinterpret_cast<uintptr_t>(e.v);
+            // float32 moments: four elements an access; sf8: eight
+            e.vec = (a & ((SF8 ? 8 : 4) * sizeof(T) - 1)) == 0 && (b & (SF8 ? 7 : 15)) == 0;
         }
         adamw_kernel<T, SF8, CAP><<<grid, AT, 0, st>>>(t, c, dev);
         return check_launch("sfb_adamw");
