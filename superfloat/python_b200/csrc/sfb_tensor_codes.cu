@@ -178,11 +178,14 @@ constexpr int BC = 256;                  // columns: 32 threads of 8
 
 template <bool VEC, typename T>
 __device__ __forceinline__ Vec<T, 8> load8t(const T *from, int64_t left) {
-    if constexpr (VEC) return *reinterpret_cast<const Vec<T, 8> *>(from);
-    Vec<T, 8> q;
+    if constexpr (VEC) {
+        return *reinterpret_cast<const Vec<T, 8> *>(from);
+    } else {
+        Vec<T, 8> q;
 #pragma unroll
-    for (int j = 0; j < 8; j++) q.v[j] = j < left ? from[j] : from_f<T>(0.0f);
-    return q;
+        for (int j = 0; j < 8; j++) q.v[j] = j < left ? from[j] : from_f<T>(0.0f);
+        return q;
+    }
 }
 
 // VEC: N is a multiple of 8 and the rows of dy and z start on 16 bytes

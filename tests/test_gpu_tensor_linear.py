@@ -479,6 +479,56 @@ def test_a_captured_training_step(gpu):
     assert all(torch.equal(a, c) for a, c in zip(out, step(x)))
 
 
+def test_what_the_backward_pass_kept(gpu):
+    """x changed in place before the backward pass is an error; the weight may change (its codes are kept); a second
+    derivative is refused."""
+    x = randn(20, 64, dtype=torch.bfloat16)
+    w = randn(24, 64, seed=1, std=0.1).requires_grad_()
+    y = sft.tensor_linear(x, w)
+    want, = torch.autograd.grad(y, w, torch.ones_like(y), retain_graph=True)
+    with torch.no_grad():
+        w.mul_(2)
+    again, = torch.autograd.grad(y, w, torch.ones_like(y), retain_graph=True)
+    assert torch.equal(want, again)
+    x.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, w, torch.ones_like(y))
+    xr = randn(20, 64, dtype=torch.bfloat16).requires_grad_()
+    y = sft.tensor_linear(xr, w, activation="gelu")
+    g, = torch.autograd.grad(y.float().square().sum(), xr, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|twice|differentiate"):
+        g.float().sum().backward()
+
+
+def test_calls_on_two_streams_at_once(gpu):
+    """Training passes of two layers interleaved on two streams: each the bits it has alone."""
+    def layer(seed):
+        x = randn(900, 512, seed=seed, dtype=torch.bfloat16).requires_grad_()
+        w = randn(700, 512, seed=seed + 1, std=0.05).requires_grad_()
+        dy = randn(900, 700, seed=seed + 2, dtype=torch.bfloat16)
+        return x, w, dy
+
+    def run(x, w, dy):
+        y = sft.tensor_linear(x, w, activation="silu")
+        return (y.detach(), *torch.autograd.grad(y, [x, w], dy))
+
+    sets = [layer(0), layer(10)]
+    want = [run(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(*sets[i]))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        for r in g:
+            assert all(torch.equal(a, b) for a, b in zip(w, r))
+
+
 def test_runs_repeat(gpu):
     x = randn(700, 512, dtype=torch.bfloat16).requires_grad_()
     w = randn(600, 512, seed=1, std=0.05).requires_grad_()

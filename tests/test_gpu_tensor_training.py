@@ -172,6 +172,9 @@ def test_packing(gpu):
     assert half.up.scale.dtype == torch.float32 and half.up.codes.dtype == torch.int8
     with torch.no_grad():
         assert half(ids).dtype == torch.float16
+    moved = copy.deepcopy(packed).cpu().cuda()
+    with torch.no_grad():
+        assert torch.equal(moved(ids), want)
     x = torch.randn(5, 64, device="cuda").bfloat16()
     r = torch.randn(5, 160, device="cuda").bfloat16()
     fused = packed.up(x, activation="silu", residual=r)
