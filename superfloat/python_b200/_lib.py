@@ -393,6 +393,15 @@ class on_device:
             _torch.cuda.set_device(self.before)
 
 
+def call_on(index: int, fn, call) -> None:
+    """``fn(call's address, stream)`` on device ``index``'s current stream."""
+    torch = _torch or _bind_torch()
+    if index in _ready_devices and torch.cuda.current_device() == index:
+        return fn(call.buffer_info()[0], _raw_stream(index))
+    with on_device(index) as d:
+        return fn(call.buffer_info()[0], d.stream)
+
+
 def ensure_current(index: int) -> None:
     """sfb_device_init once per device, the current device left as it was."""
     if index in _ready_devices:
@@ -435,21 +444,21 @@ def code_quantize(w, dtype, N, K, ldw, bits, per_channel, codes, ldc, scale, wor
           "sf weight codes")
 
 
-def tensor_forward(call, stream) -> None:
-    """``call``: an array("q") of TENSOR_CALL's fields."""
-    rc = load().sfb_tensor_forward(call.buffer_info()[0], stream)
+def tensor_forward(index, call) -> None:
+    """``call``: an array("q") of TENSOR_CALL's fields, on device ``index``."""
+    rc = call_on(index, (_lib or load()).sfb_tensor_forward, call)
     if rc:
         check(rc, "sf tensor linear")
 
 
-def tensor_sums(M, N) -> int:
-    return int(load().sfb_tensor_sums(M, N))
-
-
-def tensor_backward(call, stream) -> None:
-    rc = load().sfb_tensor_backward(call.buffer_info()[0], stream)
+def tensor_backward(index, call) -> None:
+    rc = call_on(index, (_lib or load()).sfb_tensor_backward, call)
     if rc:
         check(rc, "sf tensor linear (backward)")
+
+
+def tensor_sums(M, N) -> int:
+    return int(load().sfb_tensor_sums(M, N))
 
 
 def tensor_failures() -> int:

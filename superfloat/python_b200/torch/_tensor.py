@@ -87,20 +87,6 @@ def _two_d(t: torch.Tensor, width: int):
     return _rows(t if t.dim() == 2 else t.reshape(-1, width), width)
 
 
-class _Room:
-    """Places in one buffer, each on 256 bytes."""
-
-    __slots__ = ("size",)
-
-    def __init__(self):
-        self.size = 0
-
-    def take(self, nbytes: int) -> int:
-        at = self.size
-        self.size = at + (nbytes + 255 & -256)
-        return at
-
-
 @torch.no_grad()
 def pack_weight(weight: torch.Tensor, dtype="sf8", scale: str = "per_channel") -> SFPackedWeight:
     """A float weight (N, K) as sf codes, once, for the calls that share it.
@@ -126,129 +112,138 @@ def pack_weight(weight: torch.Tensor, dtype="sf8", scale: str = "per_channel") -
     return SFPackedWeight(codes, scale, bits)
 
 
-def _check_operands(x, weight, bias, activation, residual):
+def _check_operands(x, weight, N, K, index, bias, activation, residual):
+    """The checks of a call whose weight is N x K on CUDA device ``index`` (-1: on the host)."""
     if activation not in _lib.ACTIVATIONS:
         raise ValueError(f"activation must be one of {tuple(_lib.ACTIVATIONS)}, got {activation!r}")
-    if x.dtype not in _TYPES:
-        raise SFTypeError(f"the input is {x.dtype}: the tensor cores take bfloat16 or float16 (accumulate=\"chain\" "
+    dt = x.dtype
+    if dt not in _TYPES:
+        raise SFTypeError(f"the input is {dt}: the tensor cores take bfloat16 or float16 (accumulate=\"chain\" "
                           f"and \"wide\" take float32)")
-    N, K = weight.shape
-    if x.dim() < 1 or x.shape[-1] != K:
-        raise SFShapeError(f"the input has shape {tuple(x.shape)}, the weight expects {K} features")
+    shape = x.shape
+    if not shape or shape[-1] != K:
+        raise SFShapeError(f"the input has shape {tuple(shape)}, the weight expects {K} features")
     if N < 1 or K < 1:
-        raise SFShapeError(f"a weight has at least one row and one column, got {tuple(weight.shape)}")
-    device = weight.codes.device if isinstance(weight, SFPackedWeight) else weight.device
-    if x.device != device or not x.is_cuda:
-        raise SFShapeError(f"the input is on {x.device}, the weight on {device}; both must be on one CUDA device")
+        raise SFShapeError(f"a weight has at least one row and one column, got {(N, K)}")
+    if index < 0 or x.get_device() != index:
+        raise SFShapeError(f"the input is on {x.device}, the weight on {weight.scale.device if index < 0 else index}; "
+                           f"both must be on one CUDA device")
     if bias is not None:
         if bias.shape != (N,):
             raise SFShapeError(f"the bias has shape {tuple(bias.shape)}, expected ({N},)")
         if bias.dtype not in _FLOATS:
             raise SFTypeError(f"the bias is {bias.dtype}; float32, bfloat16 and float16 are supported")
-        if bias.device != device:
-            raise SFShapeError(f"the bias is on {bias.device}, the weight on {device}")
+        if bias.get_device() != index:
+            raise SFShapeError(f"the bias is on {bias.device}, the weight on cuda:{index}")
     if residual is not None:
-        if residual.shape != (*x.shape[:-1], N):
-            raise SFShapeError(f"the residual has shape {tuple(residual.shape)}, expected {(*x.shape[:-1], N)}")
-        if residual.dtype != x.dtype:
-            raise SFTypeError(f"the residual is {residual.dtype}, the input {x.dtype}")
-        if residual.device != device:
-            raise SFShapeError(f"the residual is on {residual.device}, the weight on {device}")
+        if residual.shape != (*shape[:-1], N):
+            raise SFShapeError(f"the residual has shape {tuple(residual.shape)}, expected {(*shape[:-1], N)}")
+        if residual.dtype != dt:
+            raise SFTypeError(f"the residual is {residual.dtype}, the input {dt}")
+        if residual.get_device() != index:
+            raise SFShapeError(f"the residual is on {residual.device}, the weight on cuda:{index}")
 
 
-def _forward(x, weight, packed, bias, residual, bits, wscale, act, train):
+def _forward(x, weight, N, K, packed, bias, residual, bits, wscale, act, train):
     """The result and, with ``train``, what the backward pass reads: (x, its
     row stride), the pre-activation, the buffer of codes and scales and their
     places in it.  One library call, all scratch in one buffer."""
-    (N, K), kind = weight.shape, _TYPES[x.dtype]
-    out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    kind = _TYPES[x.dtype]
+    out = x.new_empty((*x.shape[:-1], N))
     x, ldx = _two_d(x, K)
-    M = x.shape[0]
+    M, x_ptr = x.shape[0], x.data_ptr()
     ldk = K + 7 & -8
     if M <= 1:
         ldx = max(ldx, ldk) if ldx % 8 == 0 else ldk
     small = packed is not None and M <= _lib.SMALL_ROWS and not train
-    room = _Room()
-    codes = 0 if small else room.take(2 * N * ldk)
+    # places in one buffer, each on 256 bytes: codes, scales, the rows' maxima, x with its rows on 16 bytes
+    codes = size = scale_at = work = xpad = 0
+    if not small:
+        size = 2 * N * ldk + 255 & -256
     if packed is None:
         w, ldw = _rows(weight, K)
-        w_ptr, w_kind = w.data_ptr(), _FLOATS[w.dtype]
-        scale_at, work = room.take(4 * N), room.take(4 * N) if wscale == "per_tensor" else None
+        w_kind = _FLOATS[w.dtype]
+        scale_at = size
+        size += 4 * N + 255 & -256
+        if wscale == "per_tensor":
+            work = size
+            size += 4 * N + 255 & -256
     else:
         w, ldw = _rows(packed.codes, K)
-        w_ptr, w_kind, scale = w.data_ptr(), _lib.I8, packed.scale.contiguous()
-    xpad = room.take(2 * M * ldk) if x.data_ptr() % 16 or ldx % 8 else None
-    buf = torch.empty(room.size, dtype=torch.uint8, device=x.device) if room.size else None
-    base = buf.data_ptr() if buf is not None else 0
-    scale_ptr = base + scale_at if packed is None else scale.data_ptr()
-    z = torch.empty(M, N, dtype=torch.float16, device=x.device) if train and act else None
+        w_kind, scale = _lib.I8, packed.scale
+        if not scale.is_contiguous():
+            scale = scale.contiguous()
+    pad = bool(x_ptr % 16 or ldx % 8)
+    if pad:
+        xpad = size
+        size += 2 * M * ldk
+    buf, base = None, 0
+    if size:
+        buf = torch.empty(size, dtype=torch.uint8, device=x.device)
+        base = buf.data_ptr()
+    z = torch.empty((M, N), dtype=torch.float16, device=x.device) if train and act else None
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
     r_ptr, ldr = 0, 0
     if residual is not None:
         residual, ldr = _two_d(residual, N)
         r_ptr = residual.data_ptr()
-    with _lib.on_device(x.get_device()) as d:
-        _lib.tensor_forward(array("q", (
-            kind, bits, act, M, N, K, x.data_ptr(), ldx, 0 if xpad is None else base + xpad, ldk, w_ptr, ldw, w_kind,
-            wscale == "per_channel", 0 if small else base + codes, ldk, scale_ptr,
-            0 if bias is None else bias.data_ptr(), 0 if bias is None else _FLOATS[bias.dtype], r_ptr, ldr,
-            out.data_ptr(), N, 0 if z is None else z.data_ptr(), N, 0 if packed or work is None else base + work,
-            0, 0, 0, 0, 0, 0, 0, 0)), d.stream)
+    _lib.tensor_forward(x.get_device(), array("q", (
+        kind, bits, act, M, N, K, x_ptr, ldx, base + xpad, ldk, w.data_ptr(), ldw, w_kind, wscale == "per_channel",
+        0 if small else base, ldk, base + scale_at if packed is None else scale.data_ptr(),
+        0 if bias is None else bias.data_ptr(), 0 if bias is None else _FLOATS[bias.dtype], r_ptr, ldr,
+        out.data_ptr(), N, 0 if z is None else z.data_ptr(), N, base + work, 0, 0, 0, 0, 0, 0, 0, 0)))
     if not train:
         return out
-    if xpad is not None:
-        x, ldx, x_at = buf, ldk, xpad
-    else:
-        x_at = 0
-    return out, x, z, buf, (scale if packed is not None else buf), (M, N, K, ldx, x_at, codes,
-                                                                    0 if packed is not None else scale_at)
+    if pad:
+        x, ldx = buf, ldk
+    return out, x, z, buf, (None if packed is None else scale), (M, N, K, ldx, xpad if pad else 0, scale_at)
 
 
 class _TensorLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, packed, bias, residual, bits, wscale, act):
-        y, xs, z, buf, scales, ctx.layout = _forward(x, packed or weight, packed, bias, residual, bits, wscale, act, True)
-        ctx.save_for_backward(xs, z, buf, scales)
-        ctx.x_shape, ctx.kind, ctx.dtype, ctx.bits, ctx.act = x.shape, _TYPES[x.dtype], x.dtype, bits, act
-        ctx.per_channel = packed is not None or wscale == "per_channel"
-        ctx.w_dtype = None if packed is not None else weight.dtype
-        ctx.b_dtype = None if bias is None else bias.dtype
+        N, K = (packed or weight).shape
+        y, xs, z, buf, scale, layout = _forward(x, weight, N, K, packed, bias, residual, bits, wscale, act, True)
+        ctx.save_for_backward(xs, z, buf, scale)
+        ctx.call = (*layout, x.shape, x.dtype, bits, act, packed is not None or wscale == "per_channel",
+                    None if weight is None else weight.dtype, None if bias is None else bias.dtype)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         want_x, want_w, _, want_b, want_r = ctx.needs_input_grad[:5]
+        gr = g if want_r else None
         if not (want_x or want_w or want_b):
-            return None, None, None, None, g if want_r else None, None, None, None
-        xs, z, buf, scales = ctx.saved_tensors
-        M, N, K, ldx, x_at, codes, scale_at = ctx.layout
-        dev, dt = buf.device, ctx.dtype
-        dx = torch.empty(ctx.x_shape, dtype=dt, device=dev) if want_x else None
-        dw = torch.empty(N, K, dtype=ctx.w_dtype, device=dev) if want_w else None
-        db = torch.empty(N, dtype=ctx.b_dtype, device=dev) if want_b else None
+            return None, None, None, None, gr, None, None, None
+        xs, z, buf, scale = ctx.saved_tensors
+        M, N, K, ldx, x_at, scale_at, shape, dt, bits, act, per_channel, w_dtype, b_dtype = ctx.call
+        dev = buf.device
+        dx = g.new_empty(shape) if want_x else None
+        dw = torch.empty((N, K), dtype=w_dtype, device=dev) if want_w else None
+        db = torch.empty((N,), dtype=b_dtype, device=dev) if want_b else None
         if M == 0:
             for t in (dw, db):
                 if t is not None:
                     t.zero_()
-            return dx, dw, None, db, g if want_r else None, None, None, None
-        g2, ldg = _two_d(g, N)
-        room, ldn, ldk = _Room(), N + 7 & -8, K + 7 & -8
-        sums = room.take(_lib.tensor_sums(M, N)) if want_b else 0
-        top = room.take(4)
-        dz = room.take(2 * M * ldn) if want_w or not ctx.per_channel else 0
-        dzs = room.take(2 * M * ldn) if want_x and ctx.per_channel else 0
-        work = torch.empty(room.size, dtype=torch.uint8, device=dev)
+            return dx, dw, None, db, gr, None, None, None
+        g, ldg = _two_d(g, N)
+        ldn, ldk = N + 7 & -8, K + 7 & -8
+        # places in one buffer: the largest scale, dz, dz s, the bias's partial sums
+        one = 2 * M * ldn + 255 & -256
+        dz = 256
+        dzs = dz + (one if want_w or not per_channel else 0)
+        sums = dzs + (one if want_x and per_channel else 0)
+        work = torch.empty(sums + (_lib.tensor_sums(M, N) if want_b else 0), dtype=torch.uint8, device=dev)
         at, base = work.data_ptr(), buf.data_ptr()
-        with _lib.on_device(work.get_device()) as d:
-            _lib.tensor_backward(array("q", (
-                ctx.kind, ctx.bits, ctx.act, M, N, K, xs.data_ptr() + x_at, ldx, 0, 0, 0, 0,
-                _FLOATS[ctx.w_dtype] if want_w else 0, ctx.per_channel, base + codes, ldk, scales.data_ptr() + scale_at,
-                0, 0, 0, 0, g2.data_ptr(), ldg, 0 if z is None else z.data_ptr(), N, at + sums, at + top, at + dz,
-                at + dzs, ldn, 0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(),
-                0 if db is None else db.data_ptr(), _FLOATS[ctx.b_dtype] if want_b else 0)), d.stream)
-        return dx, dw, None, db, g if want_r else None, None, None, None
+        _lib.tensor_backward(buf.get_device(), array("q", (
+            _TYPES[dt], bits, act, M, N, K, xs.data_ptr() + x_at, ldx, 0, 0, 0, 0, _FLOATS[w_dtype] if want_w else 0,
+            per_channel, base, ldk, base + scale_at if scale is None else scale.data_ptr(), 0, 0, 0, 0, g.data_ptr(),
+            ldg, 0 if z is None else z.data_ptr(), N, at + sums, at, at + dz, at + dzs, ldn,
+            0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(),
+            _FLOATS[b_dtype] if want_b else 0)))
+        return dx, dw, None, db, gr, None, None, None
 
 
 def tensor_linear(x: torch.Tensor, weight, bias=None, *, activation: str | None = None, residual=None, dtype="sf8",
@@ -265,25 +260,26 @@ def tensor_linear(x: torch.Tensor, weight, bias=None, *, activation: str | None 
     device; the work is queued on its current stream.  Differentiable once, in
     x, a float weight, bias and residual; the backward pass keeps x, the codes
     and the pre-activation (in fp16)."""
-    packed = weight if isinstance(weight, SFPackedWeight) else None
-    if packed is None:
+    if isinstance(weight, SFPackedWeight):
+        packed, weight = weight, None
+        (N, K), bits, index = packed.codes.shape, packed.bits, packed.codes.get_device()
+    else:
         from .._array import resolve_dtype
-        bits = resolve_dtype(dtype).bits
+        packed, bits = None, resolve_dtype(dtype).bits
         _check_width(bits)
         _core.check_args(bits, scale)
         _check_weight(weight)
-    else:
-        bits = packed.bits
-    _check_operands(x, weight, bias, activation, residual)
+        (N, K), index = weight.shape, weight.get_device()
+    _check_operands(x, packed, N, K, index, bias, activation, residual)
     act = _lib.ACTIVATIONS[activation]
     if torch.is_grad_enabled() and (x.requires_grad or (packed is None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
-        return _TensorLinear.apply(x, None if packed is not None else weight, packed, bias, residual, bits, scale, act)
-    if packed is None and x.numel() <= _lib.SMALL_ROWS * x.shape[-1]:
+        return _TensorLinear.apply(x, weight, packed, bias, residual, bits, scale, act)
+    if packed is None and x.numel() <= _lib.SMALL_ROWS * K:
         # few rows: int8 codes are half the bytes of the product's operand, and the product reads them as they are
-        weight = packed = pack_weight(weight, bits, scale)
-    return _forward(x, weight, packed, bias, residual, bits, scale, act, False)
+        packed = pack_weight(weight, bits, scale)
+    return _forward(x, weight, N, K, packed, bias, residual, bits, scale, act, False)
 
 
 def tensor_failures() -> int:
