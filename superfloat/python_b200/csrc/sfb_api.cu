@@ -3,6 +3,7 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <atomic>
 #include <mutex>
 
 #include "sfb_common.cuh"
@@ -26,9 +27,12 @@ int check_launch(const char *what) {
 }
 
 int sm_count() {
+    static std::atomic<int> known[64] = {};       // a device's number of SMs does not change
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+    if (dev >= 0 && dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+    if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
     return n;
 }
 

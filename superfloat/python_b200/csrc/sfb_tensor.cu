@@ -70,7 +70,7 @@ extern "C" int sfb_tensor_forward(const sfb_tensor_call *c, sfb_stream stream) {
                           c->z, c->ldz, c->M, c->N, c->K, st);
 }
 
-extern "C" int64_t sfb_tensor_sums(int64_t M, int64_t N) { return sfb::tensor_slope_workspace(M, N); }
+extern "C" int64_t sfb_tensor_sums(int64_t M, int64_t N) { return 4 * sfb::tensor_slope_parts(M) * N; }
 
 extern "C" int sfb_tensor_backward(const sfb_tensor_call *c, sfb_stream stream) {
     using namespace sfb;
@@ -100,19 +100,21 @@ extern "C" int sfb_tensor_backward(const sfb_tensor_call *c, sfb_stream stream) 
         rc = tensor_top(c->scale, c->N, c->top, st);
         if (rc) return rc;
     }
+    float *parts = c->db ? static_cast<float *>(c->work) : nullptr;
     if (need_dz || need_dzs || c->db)
         rc = tensor_slope(t, (int)c->act, c->y, c->ldy, c->z, c->ldz, c->M, c->N, c->scale, bits, top,
-                          need_dz ? c->dz : nullptr, need_dzs ? c->dzs : nullptr, c->ldd, c->db, (int)c->db_dtype,
-                          c->work, st);
+                          need_dz ? c->dz : nullptr, need_dzs ? c->dzs : nullptr, c->ldd, parts, st);
     if (rc) return rc;
+    const Sums sums{parts, tensor_slope_parts(c->M), c->N, c->db, (int)c->db_dtype};
     const void *dz = direct ? c->y : c->dz;
     const int64_t ldd = direct ? c->ldy : c->ldd;
-    if (c->dx) {
+    if (c->dx)
         rc = tensor_grad_x(t, one ? dz : c->dzs, one ? ldd : c->ldd, c->codes, c->ldc, top, bits, c->dx, c->K, c->M,
                            c->N, c->K, st);
-        if (rc) return rc;
-    }
+    if (rc) return rc;
     if (c->dw)
-        rc = tensor_grad_w(t, dz, ldd, c->x, c->ldx, c->dw, (int)c->w_dtype, c->K, c->M, c->N, c->K, st);
+        rc = tensor_grad_w(t, dz, ldd, c->x, c->ldx, c->dw, (int)c->w_dtype, c->K, c->M, c->N, c->K, sums, st);
+    else if (parts)
+        rc = tensor_sum(sums, st);
     return rc;
 }

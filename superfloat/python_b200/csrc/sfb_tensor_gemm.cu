@@ -19,7 +19,8 @@
 // chosen so that a lane gets 8 neighbouring channels of one column.
 // A pair of SMs (a cluster of two CTAs) shares an output tile of 256 x BN: each
 // holds 128 rows of A, half of B's columns and the sums of its own rows, and the
-// first one's warp 1 issues the products of both (cta_group::2).  Products read
+// first one's warp 1 issues the products of both (cta_group::2; the other's adds up
+// the bias's gradient).  Products read
 // their operands from shared memory at the rate at which copies write them, and
 // that is what bounds a smaller tile: 256 x 256 of bf16 moves 64 KB an SM and
 // stage of 64 against 512 cycles of products, at the 128 bytes a cycle that it
@@ -232,6 +233,7 @@ struct Epilogue {
     float unit;                  // 2^-(bits-1) where a scale or alpha stands for codes, else 1
     int bias_dtype, y_dtype;
     int64_t ldr, ldz, ldy;
+    Sums sums;                   // the bias's gradient, for the warp that has nothing to issue in the second CTA
     bool vec;                    // y (of 16 bits), z and r start on 16 bytes, and so do their rows
 };
 
@@ -502,6 +504,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             }
             mma_commit(done);
         }
+    } else if (warp == 1) {
+        if (e.sums.parts)
+            for (int64_t n = (int64_t)first * 32 + lane; n < e.sums.N; n += (int64_t)step * 32)
+                store_as(e.sums.db, n, e.sums.dtype, column_sum(e.sums, n));
     } else if (warp >= 2) {
         const int half = (warp - 2) >> 2, quad = warp & 3;   // a warp reaches the TMEM lanes 32 (warp % 4) ..
         const uint32_t lanes = (uint32_t)(32 * quad) << 16, box = smem_u32(smem + STAGES * S::STAGE) + (warp - 2) * 2048;
@@ -776,13 +782,14 @@ int tensor_grad_x(int dtype, const void *dzs, int64_t ldd, const void *codes, in
 }
 
 int tensor_grad_w(int dtype, const void *dz, int64_t ldd, const void *x, int64_t ldx, void *dw, int dw_dtype,
-                  int64_t ldw, int64_t M, int64_t N, int64_t K, cudaStream_t st) {
+                  int64_t ldw, int64_t M, int64_t N, int64_t K, const Sums &sums, cudaStream_t st) {
     const Problem p{x, dz, ldx, ldd, K, N, M, dtype};
     Epilogue e{};
     e.y = dw;
     e.unit = 1.0f;
     e.y_dtype = dw_dtype;
     e.ldy = ldw;
+    e.sums = sums;
     return launch_typed<true, true, SFB_ACT_NONE>(p, e, st);
 }
 

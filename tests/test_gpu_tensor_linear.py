@@ -573,3 +573,21 @@ def test_large_offsets(gpu):
         want, tol, _, _ = forward64(x[rows], w.codes.double(), w.scale.double(), 8, None, None, res[rows])
         close(y[rows], want, tol, torch.bfloat16)
     assert math.prod(y.shape) > 2 ** 31
+
+
+@pytest.mark.parametrize("rows,channels", [(1, 40), (65, 31), (700, 130), (2100, 64)])
+def test_the_bias_gradient_is_the_same_alone_and_beside_the_products(rows, channels):
+    """Its partial sums are added up by a kernel of their own where the weight's gradient is not wanted, else beside
+    that product: the same sums in the same order."""
+    x, w, b = randn(rows, 48, seed=1), randn(channels, 48, seed=2), randn(channels, seed=3)
+    dy, grads = randn(rows, channels, seed=4).bfloat16(), []
+    for want_x, want_w in ((False, False), (True, False), (False, True), (True, True)):
+        xs, ws, bs = (t.bfloat16().requires_grad_(want) for t, want in ((x, want_x), (w, want_w), (b, True)))
+        sft.tensor_linear(xs, ws, bs, activation="relu").backward(dy)
+        grads.append(bs.grad)
+    assert all(torch.equal(g, grads[0]) for g in grads[1:])
+    open_ = sft.tensor_linear(x.bfloat16(), w.bfloat16(), b.bfloat16(), activation="relu") > 0
+    exact = (dy.double() * open_).sum(0)
+    # float32 sums of `rows` terms, then one rounding to bf16
+    bound = dy.double().abs().sum(0) * rows * 2.0 ** -24 + exact.abs() * 2.0 ** -8
+    assert ((grads[0].double() - exact).abs() <= bound).all()
