@@ -455,32 +455,56 @@ __global__ void advance_kernel(long long *step, Coefs *out, double lr, double b1
     *out = c;
 }
 
-// the values that sf8 codes stand for
+// the values of four sf8 codes
+__device__ __forceinline__ void four_values(const char4 &x, float s, int power, float (&r)[4]) {
+    const float u = __fmul_rn(s, power == 2 ? UNIT2 : UNIT4);
+    const int q[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float y = (float)(q[j] * q[j]), l = power == 2 ? y : __fmul_rn(y, y);
+        r[j] = __fmul_rn(q[j] < 0 ? -l : l, u);
+    }
+}
+
+// the values that sf8 codes stand for: a whole chunk's loads are asked for before the
+// first store, which the compiler cannot do by itself as the two could overlap
+// (117 M codes in 91.5 us, 6410 GB/s; 106.6 us in its order)
 template <int CAP>
 __global__ void __launch_bounds__(AT) values_kernel(const __grid_constant__ Table<CAP> t, int power) {
+    constexpr int SIZE = CHUNK<false>, STEPS = SIZE / (4 * AT);
     const int k = tensor_of(t, blockIdx.x);
     const Entry &e = t.e[k];
-    const int64_t first = (int64_t)(blockIdx.x - t.start[k]) * CHUNK<false>, last = min(e.n, first + CHUNK<false>);
+    const int64_t first = (int64_t)(blockIdx.x - t.start[k]) * SIZE, last = min(e.n, first + SIZE);
     const int8_t *code = static_cast<const int8_t *>(e.g);
     float *out = static_cast<float *>(e.p);
-#pragma unroll 4
-    for (int64_t i = first + 4 * threadIdx.x; i < last; i += 4 * AT) {
-        const float s = e.ms[i / AB], u = __fmul_rn(s, power == 2 ? UNIT2 : UNIT4);
-        float r[4];
-        signed char q[4] = {0, 0, 0, 0};
-        if (i + 4 <= last) {
-            const char4 x = *reinterpret_cast<const char4 *>(code + i);
-            q[0] = x.x, q[1] = x.y, q[2] = x.z, q[3] = x.w;
-        } else {
-            for (int j = 0; j < 4; j++)
-                if (i + j < last) q[j] = code[i + j];
+    if (first + SIZE <= e.n) {
+        char4 x[STEPS];
+        float s[STEPS];
+#pragma unroll
+        for (int i = 0; i < STEPS; i++) {
+            const int64_t at = first + 4 * (threadIdx.x + AT * i);
+            x[i] = __ldcs(reinterpret_cast<const char4 *>(code + at));
+            s[i] = __ldg(e.ms + at / AB);
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int x = q[j];
-            const float y = (float)(x * x), l = power == 2 ? y : __fmul_rn(y, y);
-            r[j] = __fmul_rn(x < 0 ? -l : l, u);
+        for (int i = 0; i < STEPS; i++) {
+            float r[4];
+            four_values(x[i], s[i], power, r);
+            store4(out, first + 4 * (threadIdx.x + AT * i), last, true, r);
         }
+        return;
+    }
+    for (int64_t i = first + 4 * threadIdx.x; i < last; i += 4 * AT) {
+        char4 x = make_char4(0, 0, 0, 0);
+        if (i + 4 <= last) {
+            x = *reinterpret_cast<const char4 *>(code + i);
+        } else {
+            x.x = code[i];
+            if (i + 1 < last) x.y = code[i + 1];
+            if (i + 2 < last) x.z = code[i + 2];
+        }
+        float r[4];
+        four_values(x, e.ms[i / AB], power, r);
         store4(out, i, last, true, r);
     }
 }
