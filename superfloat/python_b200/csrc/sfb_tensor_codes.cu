@@ -173,10 +173,13 @@ __global__ void __launch_bounds__(QT) pad_kernel(const uint16_t *__restrict__ x,
 // dz = dy act'(z); written as dz (the operand of the weight's gradient) and
 // as dz[n] s[n] / top (the operand of x's gradient: the channel's scale cannot
 // wait for the product, which sums over channels; top keeps fp16 within its range),
-// each rounded once from float32.  db = sum over rows, in a fixed order: every
+// each rounded once from float32 (both operands of a product have one type; a bf16
+// gradient is then off by 2.4e-3 in the 2-norm, 1.7e-3 of it the result's own rounding).
+// db = sum over rows, in a fixed order: every
 // CTA sums its 64 rows, and an idle warp of the weight's product (or, without
 // it, a kernel) the CTAs' sums.
-// Memory bound: dy and z read, dz and / or dz s written.
+// Memory bound: dy and z read, dz and / or dz s written (8192 x 4096 of fp16, one scale:
+// 201 MB in 38 us, 5.3 TB/s).
 
 constexpr int BR = 64;                   // rows of a CTA
 constexpr int BC = 256;                  // columns: 32 threads of 8
