@@ -21,10 +21,11 @@
 // holds 128 rows of A, half of B's columns and the sums of its own rows, and the
 // first one's warp 1 issues the products of both (cta_group::2; the other's adds up
 // the bias's gradient).  4096 x 4096 x 8192 of bf16: 181 us, the tensor pipe busy for
-// 91 % of them (1520 TFLOP/s).  Products read their operands from shared memory at the rate at which copies write them, and
-// that is what bounds a smaller tile: 256 x 256 of bf16 moves 64 KB an SM and
-// stage of 64 against 512 cycles of products, at the 128 bytes a cycle that it
-// has; 128 x 128 on one SM needs 64 KB for 256 cycles (577 were measured).
+// 91 % of them (1520 TFLOP/s).  Products read their operands from shared memory at the
+// rate at which copies write them, and that is what bounds a smaller tile: 256 x 256 of
+// bf16 moves 64 KB an SM and stage of 64 against 512 cycles of products, at the 128
+// bytes a cycle that it has; 128 x 128 on one SM needs 64 KB for 256 cycles (577 were
+// measured).
 // Warp 0 issues the TMA loads (128-byte swizzle), warps 2..9 are the epilogue, two
 // to each group of 32 rows, each half of the columns, 32 at a time, the next ones'
 // TMEM load and residual in flight.  Two accumulators (2 BN TMEM columns) let a

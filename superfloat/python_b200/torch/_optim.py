@@ -139,6 +139,12 @@ def _launch(buckets, lr, betas, eps, weight_decay, step, dither, constants=None)
                        dither & 0xFFFFFFFF, constants, d.stream)
 
 
+def _changed(params):
+    """Counts the step in the parameters' versions: what autograd saved of them,
+    and the codes that a chain or wide layer keeps for its weight, are of before."""
+    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
+
+
 def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step: int, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 0.0, dither: int = 0) -> None:
     """One AdamW step on lists of CUDA tensors, in place, on each device's
@@ -160,6 +166,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step: int, lr: float, beta
     _check_rates(lr, betas, eps, weight_decay)
     buckets, _kept = _buckets(params, grads, exp_avg, exp_avg_sq)
     _launch(buckets, lr, betas, eps, weight_decay, step, dither)
+    _changed(params)
 
 
 def moment_values(moments, kind: str) -> list:
@@ -194,7 +201,10 @@ class AdamW(torch.optim.Optimizer):
     ``dither_seed`` sets the rounding of sf8 moments apart from another run's.
     ``capturable=True`` keeps the step count on the device, so that ``step()``
     can be captured into a CUDA graph and replayed; the other settings are
-    then those of the capture.  Every parameter needs its gradient then.
+    then those of the capture.  Every parameter needs its gradient then.  A
+    replay changes the parameters without their versions telling: clear the codes
+    that chain layers keep (``sft.weight_cache.clear()``) before one runs outside
+    the graph.
 
     >>> opt = sft.AdamW(model.parameters(), lr=1e-4, state="sf8")
     >>> loss.backward(); opt.step(); opt.zero_grad()
@@ -282,10 +292,12 @@ class AdamW(torch.optim.Optimizer):
             by_step.setdefault(st["step"] + 1, []).append((p, st))
         for step, items in by_step.items():
             moments = [self._moments(st) for _, st in items]
-            buckets, _kept = _buckets([p for p, _ in items], [p.grad for p, _ in items], [m for m, _ in moments],
+            params = [p for p, _ in items]
+            buckets, _kept = _buckets(params, [p.grad for p in params], [m for m, _ in moments],
                                       [v for _, v in moments])
             _launch(buckets, group["lr"], group["betas"], group["eps"], group["weight_decay"], step,
                     group["dither_seed"] + step)
+            _changed(params)
             for _, st in items:
                 st["step"] = step
 
@@ -306,6 +318,7 @@ class AdamW(torch.optim.Optimizer):
                                group["dither_seed"] & 0xFFFFFFFF, d.stream)
         _launch(buckets, group["lr"], group["betas"], group["eps"], group["weight_decay"], 1, 0,
                 constants.data_ptr())
+        _changed(with_grad)
 
     def moments(self, p) -> tuple:
         """The float32 values of a parameter's two moments, in its shape."""

@@ -359,3 +359,36 @@ def test_capture_refusals(gpu):
     next(net.parameters()).grad = None
     with pytest.raises(SFUnsupportedError, match="needs its gradient"):
         late.step()
+
+
+@pytest.mark.parametrize("state", ["float32", "sf8"])
+def test_a_step_is_seen_by_the_layers_that_keep_codes_and_by_autograd(state):
+    """A chain layer keeps its weight's codes until the weight changes; autograd refuses a parameter that changed
+    between its use and the backward pass."""
+    torch.manual_seed(0)
+    net = sft.convert(torch.nn.Sequential(torch.nn.Linear(128, 64)).cuda(), dtype="sf16")
+    x = torch.randn(4, 128, generator=gen(), device="cuda") * 0.1
+    with torch.no_grad():
+        before = net(x)
+    opt = sft.AdamW(net.parameters(), lr=0.05, state=state)
+    net(x).sum().backward()
+    opt.step()
+    fresh = sft.convert(torch.nn.Sequential(torch.nn.Linear(128, 64)).cuda(), dtype="sf16")
+    fresh.load_state_dict(net.state_dict())
+    with torch.no_grad():
+        after, want = net(x), fresh(x)
+    assert torch.equal(after, want) and not torch.equal(after, before)
+    w = net[0].weight
+    y = (w * w).sum()
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_a_step_on_inference_tensors():
+    with torch.inference_mode():
+        p, g = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
+        m, v = torch.zeros(300, device="cuda"), torch.zeros(300, device="cuda")
+        sft.adamw_step([p], [g], [m], [v], step=1, lr=0.5)
+    # a first step moves by lr times g / |g|
+    assert float((p - 0.5).abs().max()) < 1e-6
