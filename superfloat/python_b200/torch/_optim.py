@@ -86,7 +86,7 @@ def _check_rates(lr, betas, eps, weight_decay):
 def _buckets(params, grads, exp_avg, exp_avg_sq):
     """{(device index, element type, sf8): [table words]}, one entry for each
     tensor, after the checks; and the gradients that had to be laid out."""
-    buckets, kept = {}, []
+    buckets, kept, seen = {}, [], set()
     for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avg, exp_avg_sq)):
         dt, shape, device = _ELEMENT.get(p.dtype), p.shape, p.device
         if dt is None:
@@ -109,13 +109,17 @@ def _buckets(params, grads, exp_avg, exp_avg_sq):
                 g = torch.empty_strided(shape, p.stride(), dtype=g.dtype, device=device).copy_(g)
             kept.append(g)
         n = p.numel()
+        at = p.data_ptr()
+        if n and at in seen:                           # (overlaps within a launch are the library's to find)
+            raise SFShapeError(f"adamw: tensor {i} is given twice")
+        seen.add(at)
         sf8 = isinstance(m, SF8Moment)
         if sf8 != isinstance(v, SF8Moment):
             raise SFTypeError(f"adamw: tensor {i} has one moment in sf8 and one that is not")
         if sf8:
             _check_sf8(m, n, device, "adamw: first moment of tensor", i)
             _check_sf8(v, n, device, "adamw: second moment of tensor", i)
-            words = (p.data_ptr(), g.data_ptr(), m.codes.data_ptr(), v.codes.data_ptr(), m.scale.data_ptr(),
+            words = (at, g.data_ptr(), m.codes.data_ptr(), v.codes.data_ptr(), m.scale.data_ptr(),
                      v.scale.data_ptr(), n, (i * _SEED_STEP) & 0xFFFFFFFF)
         else:
             for t in (m, v):
@@ -123,7 +127,7 @@ def _buckets(params, grads, exp_avg, exp_avg_sq):
                     raise SFTypeError(f"adamw: tensor {i} has a moment of {t.dtype}; float32 or SF8Moment")
                 if t.device != device or t.shape != shape or not (t.is_contiguous() if plain else t.stride() == p.stride()):
                     raise SFShapeError(f"adamw: tensor {i} has a moment of another shape, layout or device")
-            words = (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, n, 0)
+            words = (at, g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, n, 0)
         key = (p.get_device(), dt, sf8)
         if key not in buckets:
             buckets[key] = array("q")
@@ -156,8 +160,9 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step: int, lr: float, beta
     :class:`SF8Moment`; both of a parameter's moments are of one kind.  ``step``
     counts from 1.  ``dither`` seeds the rounding of sf8 moments: another number
     each step (the step will do).  The arithmetic is float32; a 16-bit parameter
-    is rounded to nearest once.  A tensor that is given twice, or overlaps
-    another that the step writes, is refused."""
+    is rounded to nearest once.  A parameter that is given twice is refused, and so
+    is a tensor that overlaps another which the same launch (one for each device,
+    type and kind of moments) writes."""
     if not len(params) == len(grads) == len(exp_avg) == len(exp_avg_sq):
         raise SFShapeError(f"adamw: {len(params)} parameters, {len(grads)} gradients, {len(exp_avg)} and "
                            f"{len(exp_avg_sq)} moments")

@@ -392,3 +392,13 @@ def test_a_step_on_inference_tensors():
         sft.adamw_step([p], [g], [m], [v], step=1, lr=0.5)
     # a first step moves by lr times g / |g|
     assert float((p - 0.5).abs().max()) < 1e-6
+
+
+def test_a_parameter_twice_with_moments_of_two_kinds_is_refused_before_anything_runs():
+    p, g, m, v = make([5000], torch.float32)
+    before, z = p[0].clone(), [sft.SF8Moment.zeros(5000, "cuda") for _ in range(2)]
+    with pytest.raises(SFShapeError, match="given twice"):
+        sft.adamw_step(p * 2, g * 2, [m[0], z[0]], [v[0], z[1]], step=1, lr=1.0)
+    assert torch.equal(p[0], before)
+    empty = torch.empty(0, device="cuda")                    # no elements, no place in memory
+    sft.adamw_step([empty, empty], [empty, empty], [empty, empty], [empty, empty], step=1, lr=1.0)
