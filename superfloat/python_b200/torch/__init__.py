@@ -27,6 +27,7 @@ from ._modules import (ConversionReport, SFConfig, SFConv2d, SFHFConv1D, SFLinea
 from ._optim import AdamW, SF8Moment, adamw_step, moment_values
 from ._status import SFLayerStatus, capture_status, last_status, reset_status
 from ._tensor import SFPackedWeight, pack_weight, tensor_failures, tensor_linear
+from ._wide import wide_weight_cache  # noqa: F401
 
 
 def _bits(dtype) -> int:

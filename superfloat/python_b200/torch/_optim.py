@@ -208,8 +208,8 @@ class AdamW(torch.optim.Optimizer):
     can be captured into a CUDA graph and replayed; the other settings are
     then those of the capture.  Every parameter needs its gradient then.  A
     replay changes the parameters without their versions telling: clear the codes
-    that chain layers keep (``sft.weight_cache.clear()``) before one runs outside
-    the graph.
+    that chain and wide layers keep (``sft.weight_cache.clear()``,
+    ``sft.wide_weight_cache.clear()``) before one runs outside the graph.
 
     >>> opt = sft.AdamW(model.parameters(), lr=1e-4, state="sf8")
     >>> loss.backward(); opt.step(); opt.zero_grad()

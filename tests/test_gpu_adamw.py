@@ -402,3 +402,29 @@ def test_a_parameter_twice_with_moments_of_two_kinds_is_refused_before_anything_
     assert torch.equal(p[0], before)
     empty = torch.empty(0, device="cuda")                    # no elements, no place in memory
     sft.adamw_step([empty, empty], [empty, empty], [empty, empty], [empty, empty], step=1, lr=1.0)
+
+
+@pytest.mark.parametrize("mode", ["chain", "wide"])
+def test_replayed_steps_and_the_codes_that_layers_keep(mode):
+    """A replay does not count in the parameters' versions: the layers' codes are cleared by hand."""
+    torch.manual_seed(0)
+    make_net = lambda: sft.convert(torch.nn.Sequential(torch.nn.Linear(128, 64)).cuda(), dtype="sf16",  # noqa: E731
+                                   accumulate=mode, attention=False)
+    net, x = make_net(), torch.randn(4, 128, generator=gen(), device="cuda") * 0.1
+    opt = sft.AdamW(net.parameters(), lr=0.05, capturable=True)
+    for p in net.parameters():
+        p.grad = torch.ones_like(p)
+    opt.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    with torch.no_grad():
+        before = net(x)
+        graph.replay()
+        sft.weight_cache.clear()
+        sft.wide_weight_cache.clear()
+        after = net(x)
+        fresh = make_net()
+        fresh.load_state_dict(net.state_dict())
+        assert torch.equal(after, fresh(x)) and not torch.equal(after, before)
