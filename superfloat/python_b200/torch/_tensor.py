@@ -179,9 +179,9 @@ def _forward(x, weight, N, K, packed, bias, residual, bits, wscale, act, train):
         size += 2 * M * ldk
     buf, base = None, 0
     if size:
-        buf = torch.empty(size, dtype=torch.uint8, device=x.device)
+        buf = x.new_empty(size, dtype=torch.uint8)
         base = buf.data_ptr()
-    z = torch.empty((M, N), dtype=torch.float16, device=x.device) if train and act else None
+    z = x.new_empty((M, N), dtype=torch.float16) if train and act else None
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
     r_ptr, ldr = 0, 0
@@ -200,6 +200,43 @@ def _forward(x, weight, N, K, packed, bias, residual, bits, wscale, act, train):
     return out, x, z, buf, (None if packed is None else scale), (M, N, K, ldx, xpad if pad else 0, scale_at)
 
 
+def _gradients(ctx, g):
+    want_x, want_w, _, want_b, want_r = ctx.needs_input_grad[:5]
+    gr = g if want_r else None
+    if not (want_x or want_w or want_b):
+        return None, None, None, None, gr, None, None, None
+    xs, z, buf, scale = ctx.saved_tensors
+    M, N, K, ldx, x_at, scale_at, shape, dt, bits, act, per_channel, w_dtype, b_dtype = ctx.call
+    dx = g.new_empty(shape) if want_x else None
+    dw = g.new_empty((N, K), dtype=w_dtype) if want_w else None
+    db = g.new_empty((N,), dtype=b_dtype) if want_b else None
+    if M == 0:
+        for t in (dw, db):
+            if t is not None:
+                t.zero_()
+        return dx, dw, None, db, gr, None, None, None
+    g, ldg = _two_d(g, N)
+    ldn, ldk = N + 7 & -8, K + 7 & -8
+    # places in one buffer: the largest scale, dz, dz s, the bias's partial sums
+    one = 2 * M * ldn + 255 & -256
+    dz = 256
+    dzs = dz + (one if want_w or not per_channel else 0)
+    sums = dzs + (one if want_x and per_channel else 0)
+    work = buf.new_empty(sums + (_lib.tensor_sums(M, N) if want_b else 0))
+    at, base = work.data_ptr(), buf.data_ptr()
+    _lib.tensor_backward(buf.get_device(), array("q", (
+        _TYPES[dt], bits, act, M, N, K, xs.data_ptr() + x_at, ldx, 0, 0, 0, 0, _FLOATS[w_dtype] if want_w else 0,
+        per_channel, base, ldk, base + scale_at if scale is None else scale.data_ptr(), 0, 0, 0, 0, g.data_ptr(),
+        ldg, 0 if z is None else z.data_ptr(), N, at + sums, at, at + dz, at + dzs, ldn,
+        0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(),
+        _FLOATS[b_dtype] if want_b else 0)))
+    return dx, dw, None, db, gr, None, None, None
+
+
+# with create_graph=True: gradients that refuse to be differentiated again
+_gradients_once = torch.autograd.function.once_differentiable(_gradients)
+
+
 class _TensorLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, packed, bias, residual, bits, wscale, act):
@@ -211,39 +248,9 @@ class _TensorLinear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        want_x, want_w, _, want_b, want_r = ctx.needs_input_grad[:5]
-        gr = g if want_r else None
-        if not (want_x or want_w or want_b):
-            return None, None, None, None, gr, None, None, None
-        xs, z, buf, scale = ctx.saved_tensors
-        M, N, K, ldx, x_at, scale_at, shape, dt, bits, act, per_channel, w_dtype, b_dtype = ctx.call
-        dev = buf.device
-        dx = g.new_empty(shape) if want_x else None
-        dw = torch.empty((N, K), dtype=w_dtype, device=dev) if want_w else None
-        db = torch.empty((N,), dtype=b_dtype, device=dev) if want_b else None
-        if M == 0:
-            for t in (dw, db):
-                if t is not None:
-                    t.zero_()
-            return dx, dw, None, db, gr, None, None, None
-        g, ldg = _two_d(g, N)
-        ldn, ldk = N + 7 & -8, K + 7 & -8
-        # places in one buffer: the largest scale, dz, dz s, the bias's partial sums
-        one = 2 * M * ldn + 255 & -256
-        dz = 256
-        dzs = dz + (one if want_w or not per_channel else 0)
-        sums = dzs + (one if want_x and per_channel else 0)
-        work = torch.empty(sums + (_lib.tensor_sums(M, N) if want_b else 0), dtype=torch.uint8, device=dev)
-        at, base = work.data_ptr(), buf.data_ptr()
-        _lib.tensor_backward(buf.get_device(), array("q", (
-            _TYPES[dt], bits, act, M, N, K, xs.data_ptr() + x_at, ldx, 0, 0, 0, 0, _FLOATS[w_dtype] if want_w else 0,
-            per_channel, base, ldk, base + scale_at if scale is None else scale.data_ptr(), 0, 0, 0, 0, g.data_ptr(),
-            ldg, 0 if z is None else z.data_ptr(), N, at + sums, at, at + dz, at + dzs, ldn,
-            0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(),
-            _FLOATS[b_dtype] if want_b else 0)))
-        return dx, dw, None, db, gr, None, None, None
+        # (the wrapper alone takes 5 us of a call)
+        return (_gradients_once if torch.is_grad_enabled() else _gradients)(ctx, g)
 
 
 def tensor_linear(x: torch.Tensor, weight, bias=None, *, activation: str | None = None, residual=None, dtype="sf8",
