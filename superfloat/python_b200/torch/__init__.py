@@ -72,4 +72,5 @@ def matmul(a, b, dtype="sf16", headroom="bound", name="matmul", *, accumulate="c
 __all__ = ["quantize", "linear", "matmul", "SFLinear", "SFConv2d", "SFHFConv1D", "SFConfig", "convert",
            "find_lm_heads", "is_hf_conv1d", "conversion_report", "ConversionReport", "last_status",
            "reset_status", "capture_status", "SFLayerStatus", "compile_report", "compile_reports", "GraphReport",
-           "SFPackedLinear", "pack", "SFPackedWeight", "pack_weight", "tensor_linear", "tensor_failures", "AdamW", "SF8Moment", "adamw_step", "moment_values"]
+           "SFPackedLinear", "pack", "SFPackedWeight", "pack_weight", "tensor_linear", "tensor_failures",
+           "AdamW", "SF8Moment", "adamw_step", "moment_values"]
