@@ -32,14 +32,21 @@ __device__ __forceinline__ float column_sum(const Sums &s, int64_t n) {
     return v[0];
 }
 
+// a matrix of 16-bit elements, and where it is copied with its rows on 16-byte boundaries
+struct Rows {
+    const void *x;                            // null: no copy
+    int64_t M, K, ldx;
+    void *out;
+    int64_t ldo;
+};
+
 // codes and scales of a float weight; work: 4 N bytes, for one scale only
 int tensor_quantize(const void *w, int dtype, int64_t N, int64_t K, int64_t ldw, int bits, bool per_channel, void *codes,
                     int64_t ldc, int codes_dtype, float *scale, void *work, cudaStream_t st);
-// packed codes as the products' operand
+// packed codes as the products' operand, and in the same launch a copy of `rows`, if any
 int tensor_expand(const int8_t *codes, int64_t N, int64_t K, int64_t ldc, void *out, int64_t ldo, int dtype,
-                  cudaStream_t st);
-// a matrix of 16-bit elements with its rows on 16-byte boundaries
-int tensor_pad(const void *x, int64_t M, int64_t K, int64_t ldx, void *out, int64_t ldo, cudaStream_t st);
+                  const Rows &rows, cudaStream_t st);
+int tensor_pad(const Rows &rows, cudaStream_t st);
 int tensor_top(const float *scale, int64_t N, float *top, cudaStream_t st);
 int tensor_small(int dtype, const void *x, int64_t ldx, const int8_t *codes, int64_t ldc, const float *scale, int bits,
                  const void *bias, int bias_dtype, int act, const void *residual, int64_t ldr, void *y, int64_t ldy,
