@@ -54,15 +54,14 @@ extern "C" int sfb_tensor_forward(const sfb_tensor_call *c, sfb_stream stream) {
     float *scale = const_cast<float *>(c->scale);
     const int t = (int)c->dtype, bits = (int)c->bits, bd = (int)c->bias_dtype, act = (int)c->act;
     const Rows rows{pad ? c->x : nullptr, c->M, c->K, c->ldx, c->xpad, c->ldp};
-    const bool expand = packed && !small && c->M > 0;
     if (!packed)
         rc = tensor_quantize(c->w, (int)c->w_dtype, c->N, c->K, c->ldw, bits, c->per_channel != 0, c->codes, c->ldc, t,
-                             scale, c->work, st);
-    else if (expand)
+                             scale, c->work, rows, st);
+    else if (!small && c->M > 0)
         rc = tensor_expand(static_cast<const int8_t *>(c->w), c->N, c->K, c->ldw, c->codes, c->ldc, t, rows, st);
+    else if (pad)
+        rc = tensor_pad(rows, st);
     if (rc || c->M == 0) return rc;
-    if (pad && !expand) rc = tensor_pad(rows, st);
-    if (rc) return rc;
     const void *x = pad ? c->xpad : c->x;
     const int64_t ldx = pad ? c->ldp : c->ldx;
     if (small)

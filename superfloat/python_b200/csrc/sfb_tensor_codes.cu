@@ -12,6 +12,24 @@ namespace {
 
 constexpr int QT = 256;
 
+// --- rows on 16-byte boundaries ----------------------------------------------------------------------
+
+// 64 threads along a row, 8 elements each, 4 rows a block of 256; block (bx, by) of gx by gy
+__device__ __forceinline__ void pad_rows(const Rows &r, int tx, int ty, int bx, int gx, int by, int gy) {
+    const uint16_t *x = static_cast<const uint16_t *>(r.x);
+    for (int64_t m = (int64_t)by * 4 + ty; m < r.M; m += 4ll * gy)
+        for (int64_t k = ((int64_t)bx * 64 + tx) * 8; k < r.K; k += 512ll * gx) {
+            Vec<uint16_t, 8> q;
+#pragma unroll
+            for (int j = 0; j < 8; j++) q.v[j] = k + j < r.K ? x[m * r.ldx + k + j] : (uint16_t)0;
+            *reinterpret_cast<Vec<uint16_t, 8> *>(static_cast<uint16_t *>(r.out) + m * r.ldo + k) = q;
+        }
+}
+
+__global__ void __launch_bounds__(QT) pad_kernel(Rows r) {
+    pad_rows(r, threadIdx.x, threadIdx.y, blockIdx.x, gridDim.x, blockIdx.y, gridDim.y);
+}
+
 // --- codes of a float weight -------------------------------------------------------------------------
 //
 // s = amax / m (m = M / 2^(N-1), 1 where amax is 0) in float64, kept as float32;
@@ -84,7 +102,12 @@ __global__ void __launch_bounds__(QT) amax_kernel(const W *__restrict__ w, int64
 template <typename W, typename O>
 __global__ void __launch_bounds__(QT) code_kernel(const W *__restrict__ w, int64_t N, int64_t K, int64_t ldw, bool vec,
                                                   int bits, const uint32_t *__restrict__ amax, O *codes, int64_t ldc,
-                                                  bool whole, float *scale) {
+                                                  bool whole, float *scale, Rows rows) {
+    if (blockIdx.y == 1) {                     // x's copy, in the launch that the call makes anyway
+        pad_rows(rows, threadIdx.x & 63, threadIdx.x >> 6, 0, 1, blockIdx.x, gridDim.x);
+        return;
+    }
+    if ((int64_t)blockIdx.x * (QT / 32) >= N) return;
     __shared__ uint32_t s_top[QT / 32];
     const int lane = threadIdx.x & 31;
     const int64_t n = (int64_t)blockIdx.x * (QT / 32) + threadIdx.x / 32;
@@ -124,21 +147,6 @@ __global__ void __launch_bounds__(QT) code_kernel(const W *__restrict__ w, int64
     }
 }
 
-// --- rows on 16-byte boundaries ----------------------------------------------------------------------
-
-// 64 threads along a row, 8 elements each, a row for each threadIdx.y
-__device__ __forceinline__ void pad_rows(const Rows &r) {
-    for (int64_t m = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; m < r.M; m += (int64_t)blockDim.y * gridDim.y)
-        for (int64_t k = ((int64_t)blockIdx.x * 64 + threadIdx.x) * 8; k < r.K; k += 512ll * gridDim.x) {
-            Vec<uint16_t, 8> q;
-#pragma unroll
-            for (int j = 0; j < 8; j++) q.v[j] = k + j < r.K ? static_cast<const uint16_t *>(r.x)[m * r.ldx + k + j] : (uint16_t)0;
-            *reinterpret_cast<Vec<uint16_t, 8> *>(static_cast<uint16_t *>(r.out) + m * r.ldo + k) = q;
-        }
-}
-
-__global__ void __launch_bounds__(QT) pad_kernel(Rows r) { pad_rows(r); }
-
 // --- packed codes in the activations' type -----------------------------------------------------------
 
 // A thread turns 16 codes of a row at a time; where rows do not start on 16
@@ -150,7 +158,7 @@ template <typename O>
 __global__ void __launch_bounds__(QT) expand_kernel(const int8_t *__restrict__ codes, int64_t N, int64_t K, int64_t ldc,
                                                     O *__restrict__ out, int64_t ldo, bool vec, Rows rows) {
     if (blockIdx.z == 1) {
-        pad_rows(rows);
+        pad_rows(rows, threadIdx.x, threadIdx.y, blockIdx.x, gridDim.x, blockIdx.y, gridDim.y);
         return;
     }
     for (int64_t n = (int64_t)blockIdx.y * 4 + threadIdx.y; n < N; n += 4ll * gridDim.y) {
@@ -298,38 +306,41 @@ __global__ void __launch_bounds__(1024) top_kernel(const float *__restrict__ sca
 
 template <typename W>
 int quantize_from(const W *w, int64_t N, int64_t K, int64_t ldw, int bits, bool per_channel, void *codes, int64_t ldc,
-                  int out, float *scale, uint32_t *amax, cudaStream_t st) {
+                  int out, float *scale, uint32_t *amax, const Rows &rows, cudaStream_t st) {
     const bool vec = (reinterpret_cast<uintptr_t>(w) & 15) == 0 && ldw * sizeof(W) % 16 == 0;
     const unsigned grid = (unsigned)((N + QT / 32 - 1) / (QT / 32));
     if (!per_channel) amax_kernel<W><<<grid, QT, 0, st>>>(w, N, K, ldw, vec, amax);
     const uint32_t *top = per_channel ? nullptr : amax;
+    const dim3 both(std::max<unsigned>(grid, rows.x ? (unsigned)std::min<int64_t>((rows.M + 3) / 4, 16ll * sm_count()) : 0),
+                    rows.x ? 2 : 1);
     // a row of 16-bit codes is padded to a multiple of 8; one of int8 only where the caller's stride says so
     if (out == SFB_I8)
-        code_kernel<W, int8_t><<<grid, QT, 0, st>>>(w, N, K, ldw, vec, bits, top, static_cast<int8_t *>(codes), ldc,
+        code_kernel<W, int8_t><<<both, QT, 0, st>>>(w, N, K, ldw, vec, bits, top, static_cast<int8_t *>(codes), ldc,
                                                     K % 8 == 0 && ldc % 8 == 0 && (reinterpret_cast<uintptr_t>(codes) & 7) == 0,
-                                                    scale);
+                                                    scale, rows);
     else if (out == SFB_BF16)
-        code_kernel<W, __nv_bfloat16><<<grid, QT, 0, st>>>(w, N, K, ldw, vec, bits, top,
-                                                           static_cast<__nv_bfloat16 *>(codes), ldc, true, scale);
+        code_kernel<W, __nv_bfloat16><<<both, QT, 0, st>>>(w, N, K, ldw, vec, bits, top,
+                                                           static_cast<__nv_bfloat16 *>(codes), ldc, true, scale, rows);
     else
-        code_kernel<W, __half><<<grid, QT, 0, st>>>(w, N, K, ldw, vec, bits, top, static_cast<__half *>(codes), ldc,
-                                                    true, scale);
+        code_kernel<W, __half><<<both, QT, 0, st>>>(w, N, K, ldw, vec, bits, top, static_cast<__half *>(codes), ldc,
+                                                    true, scale, rows);
     return check_launch("sf weight codes");
 }
 
 }  // namespace
 
 int tensor_quantize(const void *w, int dtype, int64_t N, int64_t K, int64_t ldw, int bits, bool per_channel, void *codes,
-                    int64_t ldc, int codes_dtype, float *scale, void *work, cudaStream_t st) {
+                    int64_t ldc, int codes_dtype, float *scale, void *work, const Rows &rows,
+                    cudaStream_t st) {
     uint32_t *amax = static_cast<uint32_t *>(work);
     if (dtype == SFB_F32)
         return quantize_from(static_cast<const float *>(w), N, K, ldw, bits, per_channel, codes, ldc, codes_dtype,
-                             scale, amax, st);
+                             scale, amax, rows, st);
     if (dtype == SFB_BF16)
         return quantize_from(static_cast<const __nv_bfloat16 *>(w), N, K, ldw, bits, per_channel, codes, ldc,
-                             codes_dtype, scale, amax, st);
+                             codes_dtype, scale, amax, rows, st);
     return quantize_from(static_cast<const __half *>(w), N, K, ldw, bits, per_channel, codes, ldc, codes_dtype, scale,
-                         amax, st);
+                         amax, rows, st);
 }
 
 namespace {
@@ -415,6 +426,6 @@ extern "C" int sfb_code_quantize(const void *w, int dtype, int64_t N, int64_t K,
     if (N >= (1ll << 31)) return set_error(SFB_ERANGE, "sfb_code_quantize: %lld rows", (long long)N);
     if (N == 0 || K == 0) return SFB_OK;
     if (!w || !codes || !scale || (!per_channel && !work)) return set_error(SFB_EINVAL, "sfb_code_quantize: null pointer");
-    return tensor_quantize(w, dtype, N, K, ldw, bits, per_channel != 0, codes, ldc, SFB_I8, scale, work,
+    return tensor_quantize(w, dtype, N, K, ldw, bits, per_channel != 0, codes, ldc, SFB_I8, scale, work, Rows{},
                            static_cast<cudaStream_t>(stream));
 }

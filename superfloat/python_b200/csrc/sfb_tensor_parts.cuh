@@ -40,9 +40,11 @@ struct Rows {
     int64_t ldo;
 };
 
-// codes and scales of a float weight; work: 4 N bytes, for one scale only
+// codes and scales of a float weight (work: 4 N bytes, for one scale only), and in the same launch a copy of
+// `rows`, if any
 int tensor_quantize(const void *w, int dtype, int64_t N, int64_t K, int64_t ldw, int bits, bool per_channel, void *codes,
-                    int64_t ldc, int codes_dtype, float *scale, void *work, cudaStream_t st);
+                    int64_t ldc, int codes_dtype, float *scale, void *work, const Rows &rows,
+                    cudaStream_t st);
 // packed codes as the products' operand, and in the same launch a copy of `rows`, if any
 int tensor_expand(const int8_t *codes, int64_t N, int64_t K, int64_t ldc, void *out, int64_t ldo, int dtype,
                   const Rows &rows, cudaStream_t st);
