@@ -458,6 +458,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             }
             if (__any_sync(0xffffffffu, *failed)) break;
         }
+        // The last stages' commits still have to arrive here, the second CTA's from the first one's products: neither
+        // CTA may end before its own have come.  They do under the last tile's epilogue.
+        for (int it = issued > STAGES ? issued - STAGES : 0; it < issued; it++)
+            if (__any_sync(0xffffffffu, *failed) || !all_wait(empty(it % STAGES), (it / STAGES) & 1, spin)) {
+                *failed = 1;
+                break;
+            }
     } else if (warp == 1 && rank == 0) {
         constexpr uint32_t id = instruction<T, A_MN, B_MN, BN>();
         bool ok = !(stall && !all_wait(never, 0, spin));
@@ -505,6 +512,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             }
             mma_commit(done);
         }
+        __syncwarp();
+        if (ok && !all_wait(done, 0, spin)) *failed = 1;
     } else if (warp == 1) {
         if (e.sums.parts)
             for (int64_t n = (int64_t)first * 32 + lane; n < e.sums.N; n += (int64_t)step * 32)
