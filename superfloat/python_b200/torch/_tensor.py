@@ -87,6 +87,17 @@ def _two_d(t: torch.Tensor, width: int):
     return _rows(t if t.dim() == 2 else t.reshape(-1, width), width)
 
 
+def _rows_on16(t: torch.Tensor, width: int):
+    """(t, row stride): t (2-D, 16 bits) with its rows on 16 bytes, copied where they are not."""
+    t, ld = _rows(t, width)
+    if t.shape[0] <= 1:
+        ld = width + 7 & -8
+    if t.data_ptr() % 16 or ld % 8:
+        ld = width + 7 & -8
+        t = t.new_empty(t.shape[0], ld)[:, :width].copy_(t)
+    return t, ld
+
+
 @torch.no_grad()
 def pack_weight(weight: torch.Tensor, dtype="sf8", scale: str = "per_channel") -> SFPackedWeight:
     """A float weight (N, K) as sf codes, once, for the calls that share it.
@@ -145,9 +156,9 @@ def _check_operands(x, weight, N, K, index, bias, activation, residual):
 
 
 def _forward(x, weight, N, K, packed, bias, residual, bits, wscale, act, train):
-    """The result and, with ``train``, what the backward pass reads: (x, its
-    row stride), the pre-activation, the buffer of codes and scales and their
-    places in it.  One library call, all scratch in one buffer."""
+    """The result and, with ``train``, what the backward pass reads: x (None where
+    the buffer holds a copy of it), the pre-activation, the buffer of codes and
+    scales, and the places in it.  One library call, all scratch in one buffer."""
     kind = _TYPES[x.dtype]
     out = x.new_empty((*x.shape[:-1], N))
     x, ldx = _two_d(x, K)
@@ -195,9 +206,35 @@ def _forward(x, weight, N, K, packed, bias, residual, bits, wscale, act, train):
         out.data_ptr(), N, 0 if z is None else z.data_ptr(), N, base + work, 0, 0, 0, 0, 0, 0, 0, 0)))
     if not train:
         return out
-    if pad:
-        x, ldx = buf, ldk
-    return out, x, z, buf, (None if packed is None else scale), (M, N, K, ldx, xpad if pad else 0, scale_at)
+    return out, (None if pad else x), z, buf, (None if packed is None else scale), (M, N, K, xpad, scale_at)
+
+
+def _form(t):
+    """What the backward pass relies on in a tensor that was kept; saved-tensor hooks
+    may lay it out again but not change these."""
+    return None if t is None else (t.dtype, t.shape, t.device)
+
+
+def _kept(ctx):
+    """What the forward pass kept: (x or None, its row stride, the pre-activation, the
+    buffer, the scales).  The layouts are those of the tensors that come back, which
+    saved-tensor hooks (activation offloading) may have copied: a slice of a wider
+    buffer comes back compact."""
+    saved = ctx.saved_tensors
+    for t, form in zip(saved, ctx.forms):
+        if _form(t) != form:
+            error = SFTypeError if t is not None and form is not None and t.dtype != form[0] else SFShapeError
+            raise error(f"tensor_linear: the backward pass kept {form}, a saved-tensor hook gave back {_form(t)}")
+    xs, z, buf, scale = saved
+    ldx = 0
+    if xs is not None:
+        xs, ldx = _rows_on16(xs, ctx.call[2])
+    if z is not None:
+        z = z.contiguous()
+    buf = buf.contiguous()
+    if buf.data_ptr() % 16:
+        buf = buf.clone()
+    return xs, ldx, z, buf, None if scale is None else scale.contiguous()
 
 
 def _gradients(ctx, g):
@@ -205,8 +242,7 @@ def _gradients(ctx, g):
     gr = g if want_r else None
     if not (want_x or want_w or want_b):
         return None, None, None, None, gr, None, None, None
-    xs, z, buf, scale = ctx.saved_tensors
-    M, N, K, ldx, x_at, scale_at, shape, dt, bits, act, per_channel, w_dtype, b_dtype = ctx.call
+    M, N, K, x_at, scale_at, shape, dt, bits, act, per_channel, w_dtype, b_dtype = ctx.call
     dx = g.new_empty(shape) if want_x else None
     dw = g.new_empty((N, K), dtype=w_dtype) if want_w else None
     db = g.new_empty((N,), dtype=b_dtype) if want_b else None
@@ -215,6 +251,7 @@ def _gradients(ctx, g):
             if t is not None:
                 t.zero_()
         return dx, dw, None, db, gr, None, None, None
+    xs, ldx, z, buf, scale = _kept(ctx)
     g, ldg = _two_d(g, N)
     ldn, ldk = N + 7 & -8, K + 7 & -8
     # places in one buffer: the largest scale, dz, dz s, the bias's partial sums
@@ -224,8 +261,12 @@ def _gradients(ctx, g):
     sums = dzs + (one if want_x and per_channel else 0)
     work = buf.new_empty(sums + (_lib.tensor_sums(M, N) if want_b else 0))
     at, base = work.data_ptr(), buf.data_ptr()
+    if xs is None:
+        x_ptr, ldx = base + x_at, ldk
+    else:
+        x_ptr = xs.data_ptr()
     _lib.tensor_backward(buf.get_device(), array("q", (
-        _TYPES[dt], bits, act, M, N, K, xs.data_ptr() + x_at, ldx, 0, 0, 0, 0, _FLOATS[w_dtype] if want_w else 0,
+        _TYPES[dt], bits, act, M, N, K, x_ptr, ldx, 0, 0, 0, 0, _FLOATS[w_dtype] if want_w else 0,
         per_channel, base, ldk, base + scale_at if scale is None else scale.data_ptr(), 0, 0, 0, 0, g.data_ptr(),
         ldg, 0 if z is None else z.data_ptr(), N, at + sums, at, at + dz, at + dzs, ldn,
         0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(),
@@ -243,6 +284,7 @@ class _TensorLinear(torch.autograd.Function):
         N, K = (packed or weight).shape
         y, xs, z, buf, scale, layout = _forward(x, weight, N, K, packed, bias, residual, bits, wscale, act, True)
         ctx.save_for_backward(xs, z, buf, scale)
+        ctx.forms = (_form(xs), _form(z), _form(buf), _form(scale))
         ctx.call = (*layout, x.shape, x.dtype, bits, act, packed is not None or wscale == "per_channel",
                     None if weight is None else weight.dtype, None if bias is None else bias.dtype)
         return y
