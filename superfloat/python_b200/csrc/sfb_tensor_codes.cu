@@ -200,6 +200,14 @@ __global__ void __launch_bounds__(QT) expand_kernel(const int8_t *__restrict__ c
 constexpr int BR = 64;                   // rows of a CTA
 constexpr int BC = 256;                  // columns: 32 threads of 8
 
+// A CTA's place: its columns first, in one grid dimension, as a convolution's rows
+// (images x their pixels) pass the 65535 x 64 that the others reach.
+__device__ __forceinline__ void place_of(int64_t N, int64_t &row, int64_t &column) {
+    const unsigned across = (unsigned)((N + BC - 1) / BC);
+    row = blockIdx.x / across;
+    column = blockIdx.x % across;
+}
+
 template <bool VEC, typename T>
 __device__ __forceinline__ Vec<T, 8> load8t(const T *from, int64_t left) {
     if constexpr (VEC) {
@@ -220,13 +228,15 @@ slope_kernel(const T *__restrict__ dy, int64_t ldy, const __half *__restrict__ z
              T *__restrict__ dzs, int64_t ldd, float *__restrict__ sums) {
     __shared__ float s_sum[8][BC];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int64_t n0 = (int64_t)blockIdx.x * BC + tx * 8, left = N - n0;
-    const int64_t r1 = min(M, (int64_t)(blockIdx.y + 1) * BR);
+    int64_t by, bx;
+    place_of(N, by, bx);
+    const int64_t n0 = bx * BC + tx * 8, left = N - n0;
+    const int64_t r1 = min(M, (by + 1) * BR);
     float acc[8] = {}, f[8];
     if (dzs) {
-        const float by = top ? __fdiv_rn(1.0f, *top) : unit;
+        const float share = top ? __fdiv_rn(1.0f, *top) : unit;
 #pragma unroll
-        for (int j = 0; j < 8; j++) f[j] = j < left ? scale[n0 + j] * by : 0.0f;
+        for (int j = 0; j < 8; j++) f[j] = j < left ? scale[n0 + j] * share : 0.0f;
     }
     auto row = [&](int64_t r, const Vec<T, 8> &g, const Vec<__half, 8> &h) {
         float d[8];
@@ -252,7 +262,7 @@ slope_kernel(const T *__restrict__ dy, int64_t ldy, const __half *__restrict__ z
         }
     };
     if (left > 0) {
-        int64_t r = (int64_t)blockIdx.y * BR + ty;
+        int64_t r = by * BR + ty;
 #pragma unroll 1
         for (; r + 8 < r1; r += 16) {                     // two rows' loads in flight
             const Vec<T, 8> g0 = load8t<VEC>(dy + r * ldy + n0, left), g1 = load8t<VEC>(dy + (r + 8) * ldy + n0, left);
@@ -275,12 +285,12 @@ slope_kernel(const T *__restrict__ dy, int64_t ldy, const __half *__restrict__ z
 #pragma unroll
         for (int j = 0; j < 8; j++) s_sum[ty][tx * 8 + j] = acc[j];
         __syncthreads();
-        const int64_t n = (int64_t)blockIdx.x * BC + threadIdx.x;
+        const int64_t n = bx * BC + threadIdx.x;
         if (n < N) {
             float v = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; i++) v += s_sum[i][threadIdx.x];
-            sums[(int64_t)blockIdx.y * N + n] = v;
+            sums[by * N + n] = v;
         }
     }
 }
@@ -387,10 +397,11 @@ int64_t tensor_slope_parts(int64_t M) { return (M + BR - 1) / BR; }
 int tensor_slope(int dtype, int act, const void *dy, int64_t ldy, const void *z, int64_t ldz, int64_t M, int64_t N,
                  const float *scale, int bits, const float *top, void *dz, void *dzs, int64_t ldd, float *sums,
                  cudaStream_t st) {
-    const int64_t parts = tensor_slope_parts(M);
-    if (parts > 65535) return set_error(SFB_ERANGE, "sf tensor linear: %lld rows", (long long)M);
+    const int64_t blocks = tensor_slope_parts(M) * ((N + BC - 1) / BC);
+    if (blocks >= 1ll << 31)
+        return set_error(SFB_ERANGE, "sf tensor linear: a gradient of %lld x %lld", (long long)M, (long long)N);
     const float unit = 1.0f / (float)(1 << (bits - 1));
-    const dim3 grid((unsigned)((N + BC - 1) / BC), (unsigned)parts);
+    const unsigned grid = (unsigned)blocks;
     const bool vec = N % 8 == 0 && ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(dy) & 15) == 0 &&
                      (act == SFB_ACT_NONE || (ldz % 8 == 0 && (reinterpret_cast<uintptr_t>(z) & 15) == 0));
     return with_activation(act, [&](auto a) {
