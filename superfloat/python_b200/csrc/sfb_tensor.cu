@@ -93,12 +93,12 @@ extern "C" int sfb_tensor_backward(const sfb_tensor_call *c, sfb_stream stream) 
         return set_error(SFB_EINVAL, "%s: no room for the pre-activation's gradient", what);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int t = (int)c->dtype, bits = (int)c->bits;
-    // fp16: dz s would leave its range where the scales are small; s / max s is within it
+    // fp16: dz s would leave its range where the scales are small; s over the largest one with a code is within it
     const float *top = one ? c->scale : nullptr;
     if (need_dzs && t == SFB_F16) {
         if (!c->top) return set_error(SFB_EINVAL, "%s: null pointer", what);
         top = c->top;
-        rc = tensor_top(c->scale, c->N, c->top, st);
+        rc = tensor_top(c->scale, c->N, c->codes, c->ldc, c->K, c->top, st);
         if (rc) return rc;
     }
     float *parts = c->db ? static_cast<float *>(c->work) : nullptr;

@@ -236,7 +236,10 @@ slope_kernel(const T *__restrict__ dy, int64_t ldy, const __half *__restrict__ z
     if (dzs) {
         const float share = top ? __fdiv_rn(1.0f, *top) : unit;
 #pragma unroll
-        for (int j = 0; j < 8; j++) f[j] = j < left ? scale[n0 + j] * share : 0.0f;
+        for (int j = 0; j < 8; j++) {
+            f[j] = j < left ? scale[n0 + j] * share : 0.0f;
+            if (fabsf(f[j]) > 1.001f && top) f[j] = 1.0f;        // a channel without a code, larger than `top`
+        }
     }
     auto row = [&](int64_t r, const Vec<T, 8> &g, const Vec<__half, 8> &h) {
         float d[8];
@@ -300,11 +303,39 @@ __global__ void __launch_bounds__(32) sum_kernel(Sums s) {
     if (n < s.N) store_as(s.db, n, s.dtype, column_sum(s, n));
 }
 
-// the largest of the scales
-__global__ void __launch_bounds__(1024) top_kernel(const float *__restrict__ scale, int64_t N, float *top) {
+// The largest of the scales whose channel has a code other than 0: a row of zeros has
+// the scale 1 by rule, and beside weights of 1e-3 would leave dz s / 1 below fp16's
+// normal range.  Only rows of that scale are looked at; others without a code (a
+// caller's own scales) stay within the range by what they give.  At least 2^-126, so
+// that its reciprocal is finite.
+__global__ void __launch_bounds__(1024) top_kernel(const float *__restrict__ scale, int64_t N,
+                                                   const uint16_t *__restrict__ codes, int64_t ldc, int64_t K, float *top) {
     __shared__ uint32_t s_top[32];
-    uint32_t t = 0;                                    // scales are above 0, and NaN above all
-    for (int64_t n = threadIdx.x; n < N; n += 1024) t = max(t, __float_as_uint(scale[n]) & 0x7FFFFFFFu);
+    uint32_t t = 0x00800000u;                          // magnitudes order as their bits, NaN above all
+    for (int64_t n = threadIdx.x; n < N; n += 1024) {
+        const uint32_t s = __float_as_uint(scale[n]) & 0x7FFFFFFFu;
+        if (s == 0x3F800000u) {
+            bool any = false;
+            for (int64_t k0 = 0; k0 < K && !any; k0 += 64) {
+                uint4 q[8];                            // all asked for before the first is waited for
+#pragma unroll
+                for (int u = 0; u < 8; u++)
+                    q[u] = k0 + 8 * u < K ? __ldg(reinterpret_cast<const uint4 *>(codes + n * ldc + k0 + 8 * u))
+                                          : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int u = 0; u < 8; u++) {
+                    const uint32_t w[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {      // (what is past K is a row's padding)
+                        const int64_t k = k0 + 8 * u + 2 * i;
+                        any |= ((w[i] & 0x7FFFu) && k < K) || ((w[i] & 0x7FFF0000u) && k + 1 < K);
+                    }
+                }
+            }
+            if (!any) continue;
+        }
+        t = max(t, s);
+    }
     t = __reduce_max_sync(0xffffffffu, t);
     if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = t;
     __syncthreads();
@@ -387,8 +418,8 @@ int tensor_pad(const Rows &rows, cudaStream_t st) {
     return check_launch("sf tensor linear (rows of x)");
 }
 
-int tensor_top(const float *scale, int64_t N, float *top, cudaStream_t st) {
-    top_kernel<<<1, 1024, 0, st>>>(scale, N, top);
+int tensor_top(const float *scale, int64_t N, const void *codes, int64_t ldc, int64_t K, float *top, cudaStream_t st) {
+    top_kernel<<<1, 1024, 0, st>>>(scale, N, static_cast<const uint16_t *>(codes), ldc, K, top);
     return check_launch("sf tensor linear (largest scale)");
 }
 

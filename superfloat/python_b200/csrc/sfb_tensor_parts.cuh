@@ -49,7 +49,7 @@ int tensor_quantize(const void *w, int dtype, int64_t N, int64_t K, int64_t ldw,
 int tensor_expand(const int8_t *codes, int64_t N, int64_t K, int64_t ldc, void *out, int64_t ldo, int dtype,
                   const Rows &rows, cudaStream_t st);
 int tensor_pad(const Rows &rows, cudaStream_t st);
-int tensor_top(const float *scale, int64_t N, float *top, cudaStream_t st);
+int tensor_top(const float *scale, int64_t N, const void *codes, int64_t ldc, int64_t K, float *top, cudaStream_t st);
 int tensor_small(int dtype, const void *x, int64_t ldx, const int8_t *codes, int64_t ldc, const float *scale, int bits,
                  const void *bias, int bias_dtype, int act, const void *residual, int64_t ldr, void *y, int64_t ldy,
                  int64_t M, int64_t N, int64_t K, cudaStream_t st);
