@@ -9,7 +9,8 @@ the reference's (src/sf/torch/_ops.py:184-417):
   activations;
 * ``sf::linear_tensor(x, weight, bias, bits, wscale, name)``: the linear over
   sf4..sf8 codes on the tensor cores (``accumulate="tensor"``, no counterpart
-  in the reference): bfloat16 or float16 in and out;
+  in the reference): bfloat16 or float16 in and out; its gradient is
+  ``sf::linear_tensor_backward``;
 * ``sf::linear_wide(x, weight, bias, bits, shift, name)`` and
   ``sf::matmul_wide(a, b, bits, shift, name)``: the same on the MX engine
   (``accumulate="wide"``) with the wide-mode shift rule; ``shift`` (an int)
@@ -302,15 +303,31 @@ def _linear_tensor_setup(ctx, inputs, output):
     ctx.bits, ctx.wscale = inputs[3], inputs[4]
 
 
+def _wanted(t: Optional[torch.Tensor], want: bool, like: torch.Tensor) -> torch.Tensor:
+    return t if want else like.new_empty(0)
+
+
+# an op of its own, so that a traced training graph has the gradient as one node too
+@torch.library.custom_op("sf::linear_tensor_backward", mutates_args=())
+def linear_tensor_backward(g: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
+                           bits: int, wscale: str, want_x: bool, want_w: bool,
+                           want_b: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The gradients of sf::linear_tensor's x, weight and bias; empty where not wanted."""
+    grads = _tensor.plain_gradients(g, x, weight, bias, bits, wscale, want_x, want_w, want_b)
+    return tuple(_wanted(t, want, x) for t, want in zip(grads, (want_x, want_w, want_b)))
+
+
+@linear_tensor_backward.register_fake
+def _(g, x, weight, bias, bits, wscale, want_x, want_w, want_b):
+    return (x.new_empty(x.shape if want_x else 0), weight.new_empty(weight.shape) if want_w else x.new_empty(0),
+            bias.new_empty(bias.shape) if want_b else x.new_empty(0))
+
+
 def _linear_tensor_backward(ctx, g):
-    """The layer again, differentiated by its own backward pass: the op keeps only its inputs."""
-    inputs = [t.detach().requires_grad_(need) for t, need in zip(ctx.saved_tensors, ctx.needs_input_grad)]
-    with torch.enable_grad():
-        y = _tensor.tensor_linear(*inputs, dtype=ctx.bits, scale=ctx.wscale)
-    wanted = [t for t in inputs if t.requires_grad]
-    grads = iter(torch.autograd.grad(y, wanted, g))
-    out = [next(grads) if t.requires_grad else None for t in inputs]
-    return (*out, *[None] * (6 - len(out)))
+    x, weight, *bias = ctx.saved_tensors
+    wants = [*ctx.needs_input_grad[:2], bool(bias) and ctx.needs_input_grad[2]]
+    grads = torch.ops.sf.linear_tensor_backward(g, x, weight, bias[0] if bias else None, ctx.bits, ctx.wscale, *wants)
+    return (*(t if want else None for t, want in zip(grads, wants)), None, None, None)
 
 
 torch.library.register_autograd("sf::linear_tensor", _linear_tensor_backward, setup_context=_linear_tensor_setup)

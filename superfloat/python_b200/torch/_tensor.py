@@ -237,12 +237,10 @@ def _kept(ctx):
     return xs, ldx, z, buf, None if scale is None else scale.contiguous()
 
 
-def _gradients(ctx, g):
-    want_x, want_w, _, want_b, want_r = ctx.needs_input_grad[:5]
-    gr = g if want_r else None
-    if not (want_x or want_w or want_b):
-        return None, None, None, None, gr, None, None, None
-    M, N, K, x_at, scale_at, shape, dt, bits, act, per_channel, w_dtype, b_dtype = ctx.call
+def _backward(g, kept, call, want_x, want_w, want_b):
+    """The gradients (dx, dw, db) that are wanted, else None.  ``kept()`` gives (x or
+    None, its row stride, the pre-activation, the buffer, the scales)."""
+    M, N, K, x_at, scale_at, shape, dt, bits, act, per_channel, w_dtype, b_dtype = call
     dx = g.new_empty(shape) if want_x else None
     dw = g.new_empty((N, K), dtype=w_dtype) if want_w else None
     db = g.new_empty((N,), dtype=b_dtype) if want_b else None
@@ -250,8 +248,8 @@ def _gradients(ctx, g):
         for t in (dw, db):
             if t is not None:
                 t.zero_()
-        return dx, dw, None, db, gr, None, None, None
-    xs, ldx, z, buf, scale = _kept(ctx)
+        return dx, dw, db
+    xs, ldx, z, buf, scale = kept()
     g, ldg = _two_d(g, N)
     ldn, ldk = N + 7 & -8, K + 7 & -8
     # places in one buffer: the largest scale, dz, dz s, the bias's partial sums
@@ -271,7 +269,30 @@ def _gradients(ctx, g):
         ldg, 0 if z is None else z.data_ptr(), N, at + sums, at, at + dz, at + dzs, ldn,
         0 if dx is None else dx.data_ptr(), 0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(),
         _FLOATS[b_dtype] if want_b else 0)))
+    return dx, dw, db
+
+
+def _gradients(ctx, g):
+    want_x, want_w, _, want_b, want_r = ctx.needs_input_grad[:5]
+    gr = g if want_r else None
+    if not (want_x or want_w or want_b):
+        return None, None, None, None, gr, None, None, None
+    dx, dw, db = _backward(g, lambda: _kept(ctx), ctx.call, want_x, want_w, want_b)
     return dx, dw, None, db, gr, None, None, None
+
+
+@torch.no_grad()
+def plain_gradients(g, x, weight, bias, bits, wscale, want_x, want_w, want_b):
+    """(dx, dw, db), None where not wanted, of the layer without activation and residual
+    from its own inputs: the weight's codes are made again (a forward pass of no rows)."""
+    N, K = weight.shape
+    _check_weight(weight)
+    _check_operands(x, None, N, K, weight.get_device(), bias, None, None)
+    *_, buf, scale, layout = _forward(x.new_empty((0, K)), weight, N, K, None, None, None, bits, wscale, 0, True)
+    rows = x if x.dim() == 2 else x.reshape(-1, K)
+    call = (rows.shape[0], *layout[1:], x.shape, x.dtype, bits, 0, wscale == "per_channel", weight.dtype,
+            None if bias is None else bias.dtype)
+    return _backward(g, lambda: (*_rows_on16(rows, K), None, buf, scale), call, want_x, want_w, want_b)
 
 
 # with create_graph=True: gradients that refuse to be differentiated again
