@@ -449,6 +449,10 @@ SFB_API int sfb_adamw(const int64_t *table, int count, int dtype, int sf8, doubl
                       double eps, double weight_decay, int64_t step, unsigned dither, const void *constants,
                       sfb_stream stream);
 
+/* What sfb_adamw refuses of a table, without a launch: for a step that takes
+ * several calls (types, kinds of moments, devices), before the first of them. */
+SFB_API int sfb_adamw_check(const int64_t *table, int count, int dtype, int sf8);
+
 /* Adds one to the step counter in device memory and writes the constants of
  * that step: what a step captured into a graph replays before its sfb_adamw. */
 SFB_API int sfb_adamw_advance(int64_t *step, void *constants, double lr, double beta1, double beta2, double eps,

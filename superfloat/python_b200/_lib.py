@@ -75,6 +75,7 @@ SIGNATURES = {
     "sfb_tensor_failures": (_i32, [_p]),
     "sfb_adamw": (_i32, [_p, _i32, _i32, _i32, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
                          ctypes.c_double, _i64, ctypes.c_uint, _p, _p]),
+    "sfb_adamw_check": (_i32, [_p, _i32, _i32, _i32]),
     "sfb_adamw_advance": (_i32, [_p, _p, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
                                  ctypes.c_double, ctypes.c_uint, _p]),
     "sfb_sf8_values": (_i32, [_p, _i32, _i32, _p]),
@@ -417,6 +418,10 @@ def ensure_current(index: int) -> None:
 def adamw(table, count, dtype, sf8, lr, betas, eps, weight_decay, step, dither, constants, stream) -> None:
     check(load().sfb_adamw(table, count, dtype, int(sf8), lr, betas[0], betas[1], eps, weight_decay, step, dither,
                            constants, stream), "sf adamw step")
+
+
+def adamw_check(table, count, dtype, sf8) -> None:
+    check(load().sfb_adamw_check(table, count, dtype, int(sf8)), "sf adamw step")
 
 
 def adamw_advance(step, constants, lr, betas, eps, weight_decay, seed, stream) -> None:

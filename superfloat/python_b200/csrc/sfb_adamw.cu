@@ -607,17 +607,10 @@ int run_typed(const int64_t *rows, int count, bool sf8, const Coefs &c, const Co
                          : run_adamw<T, false, MAX_CAP>(rows, count, c, dev, st);
 }
 
-}  // namespace
-}  // namespace sfb
-
-extern "C" int sfb_adamw(const int64_t *table, int count, int dtype, int sf8, double lr, double beta1, double beta2,
-                         double eps, double weight_decay, int64_t step, unsigned dither, const void *constants,
-                         sfb_stream stream) {
-    using namespace sfb;
+int check_table(const int64_t *table, int count, int dtype, bool sf8) {
     if (count < 0 || (count > 0 && !table)) return set_error(SFB_EINVAL, "sfb_adamw: no table");
     if (dtype != SFB_F32 && dtype != SFB_BF16 && dtype != SFB_F16)
         return set_error(SFB_EINVAL, "sfb_adamw: element type %d", dtype);
-    if (!constants && step < 1) return set_error(SFB_EINVAL, "sfb_adamw: step %lld", (long long)step);
     const int size = dtype == SFB_F32 ? 4 : 2;
     for (int i = 0; i < count; i++) {
         const int64_t *r = table + (int64_t)i * WORDS;
@@ -629,11 +622,26 @@ extern "C" int sfb_adamw(const int64_t *table, int count, int dtype, int sf8, do
             return set_error(SFB_EINVAL, "sfb_adamw: tensor %d is not aligned to its type", i);
     }
     try {
-        const int rc = check_overlap(table, count, size, sf8 != 0);
-        if (rc) return rc;
+        return check_overlap(table, count, size, sf8);
     } catch (const std::exception &) {
         return set_error(SFB_ERANGE, "sfb_adamw: no host memory for a table of %d tensors", count);
     }
+}
+
+}  // namespace
+}  // namespace sfb
+
+extern "C" int sfb_adamw_check(const int64_t *table, int count, int dtype, int sf8) {
+    return sfb::check_table(table, count, dtype, sf8 != 0);
+}
+
+extern "C" int sfb_adamw(const int64_t *table, int count, int dtype, int sf8, double lr, double beta1, double beta2,
+                         double eps, double weight_decay, int64_t step, unsigned dither, const void *constants,
+                         sfb_stream stream) {
+    using namespace sfb;
+    if (!constants && step < 1) return set_error(SFB_EINVAL, "sfb_adamw: step %lld", (long long)step);
+    const int rc = check_table(table, count, dtype, sf8 != 0);
+    if (rc) return rc;
     const Coefs c = constants ? Coefs{} : coefs_of(lr, beta1, beta2, eps, weight_decay, step, dither);
     const Coefs *dev = static_cast<const Coefs *>(constants);
     cudaStream_t st = static_cast<cudaStream_t>(stream);

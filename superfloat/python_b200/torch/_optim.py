@@ -135,6 +135,13 @@ def _buckets(params, grads, exp_avg, exp_avg_sq):
     return buckets, kept
 
 
+def _check_launches(launches) -> None:
+    """What the library refuses of each (key, table), before any of them is launched: a step
+    happens as a whole or not at all."""
+    for (_, dt, sf8), words in launches:
+        _lib.adamw_check(words.buffer_info()[0], len(words) // _lib.ADAMW_WORDS, dt, sf8)
+
+
 def _launch(buckets, lr, betas, eps, weight_decay, step, dither, constants=None):
     for (index, dt, sf8), words in buckets.items():
         with _lib.on_device(index) as d:
@@ -162,7 +169,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step: int, lr: float, beta
     each step (the step will do).  The arithmetic is float32; a 16-bit parameter
     is rounded to nearest once.  A parameter that is given twice is refused, and so
     is a tensor that overlaps another which the same launch (one for each device,
-    type and kind of moments) writes."""
+    type and kind of moments) writes.  Nothing of a refused call has run."""
     if not len(params) == len(grads) == len(exp_avg) == len(exp_avg_sq):
         raise SFShapeError(f"adamw: {len(params)} parameters, {len(grads)} gradients, {len(exp_avg)} and "
                            f"{len(exp_avg_sq)} moments")
@@ -170,6 +177,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step: int, lr: float, beta
         raise ValueError(f"step must be an int of at least 1, got {step!r}")
     _check_rates(lr, betas, eps, weight_decay)
     buckets, _kept = _buckets(params, grads, exp_avg, exp_avg_sq)
+    _check_launches(list(buckets.items())[1:])         # (the first one's own call checks it)
     _launch(buckets, lr, betas, eps, weight_decay, step, dither)
     _changed(params)
 
@@ -270,6 +278,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        todo = []                                      # everything is checked before anything runs
         for group in self.param_groups:
             _check_rates(group["lr"], group["betas"], group["eps"], group["weight_decay"])
             with_grad = [p for p in group["params"] if p.grad is not None]
@@ -284,46 +293,52 @@ class AdamW(torch.optim.Optimizer):
             if capturing and any(not self.state.get(p) for p in with_grad):
                 raise SFUnsupportedError("AdamW: take one step before the capture, so that the moments and the step "
                                          "counter exist")
-            if group["capturable"]:
-                self._device_step(group, with_grad)
+            todo += (self._device_step if group["capturable"] else self._host_steps)(group, with_grad)
+        launches = [item for _, buckets, *_ in todo for item in buckets.items()]
+        _check_launches(launches[0 if todo and todo[0][3] is None else 1:])
+        for group, buckets, params, step, _kept in todo:
+            rates = group["lr"], group["betas"], group["eps"], group["weight_decay"]
+            if step is None:
+                counter, constants = group["_counter"]
+                with _lib.on_device(counter.get_device()) as d:
+                    _lib.adamw_advance(counter.data_ptr(), constants.data_ptr(), float(rates[0]),
+                                       tuple(map(float, rates[1])), float(rates[2]), float(rates[3]),
+                                       group["dither_seed"] & 0xFFFFFFFF, d.stream)
+                _launch(buckets, *rates, 1, 0, constants.data_ptr())
             else:
-                self._host_step(group, with_grad)
+                _launch(buckets, *rates, step, group["dither_seed"] + step)
+                for p in params:
+                    self.state[p]["step"] = step
+            _changed(params)
         return loss
 
-    def _host_step(self, group, with_grad):
+    def _tables(self, params):
+        moments = [self._moments(self.state[p]) for p in params]
+        return _buckets(params, [p.grad for p in params], [m for m, _ in moments], [v for _, v in moments])
+
+    def _host_steps(self, group, with_grad):
+        """[(group, tables, parameters, their step, gradients laid out)], one for each step count in the group."""
         by_step = {}
         for p in with_grad:
-            st = self._begin(p, group)
-            by_step.setdefault(st["step"] + 1, []).append((p, st))
-        for step, items in by_step.items():
-            moments = [self._moments(st) for _, st in items]
-            params = [p for p, _ in items]
-            buckets, _kept = _buckets(params, [p.grad for p in params], [m for m, _ in moments],
-                                      [v for _, v in moments])
-            _launch(buckets, group["lr"], group["betas"], group["eps"], group["weight_decay"], step,
-                    group["dither_seed"] + step)
-            _changed(params)
-            for _, st in items:
-                st["step"] = step
+            by_step.setdefault(self._begin(p, group)["step"] + 1, []).append(p)
+        steps = []
+        for step, params in by_step.items():
+            buckets, kept = self._tables(params)
+            steps.append((group, buckets, params, step, kept))
+        return steps
 
     def _device_step(self, group, with_grad):
+        """The same for a group whose step count is on the device (the step is None)."""
         if len(with_grad) != len(group["params"]):
             raise SFUnsupportedError("AdamW: with capturable=True every parameter of the group needs its gradient "
                                      "(one step count serves the group)")
         if len({p.device for p in with_grad}) != 1:
             raise SFUnsupportedError("AdamW: with capturable=True a group's parameters are on one device")
-        states = [self._begin(p, group) for p in with_grad]
-        counter, constants = self._counter(group)
-        moments = [self._moments(st) for st in states]
-        buckets, _kept = _buckets(with_grad, [p.grad for p in with_grad], [m for m, _ in moments],
-                                  [v for _, v in moments])
-        with _lib.on_device(counter.get_device()) as d:
-            _lib.adamw_advance(counter.data_ptr(), constants.data_ptr(), float(group["lr"]),
-                               tuple(map(float, group["betas"])), float(group["eps"]), float(group["weight_decay"]),
-                               group["dither_seed"] & 0xFFFFFFFF, d.stream)
-        _launch(buckets, group["lr"], group["betas"], group["eps"], group["weight_decay"], 1, 0,
-                constants.data_ptr())
-        _changed(with_grad)
+        for p in with_grad:
+            self._begin(p, group)
+        self._counter(group)
+        buckets, kept = self._tables(with_grad)
+        return [(group, buckets, with_grad, None, kept)]
 
     def moments(self, p) -> tuple:
         """The float32 values of a parameter's two moments, in its shape."""
