@@ -371,18 +371,35 @@ class AdamW(torch.optim.Optimizer):
             g.pop("_counter", None)
         return d
 
+    @torch.no_grad()
     def load_state_dict(self, state_dict):
-        """As torch's, but the moments keep their own types (torch would cast them to the parameter's)."""
+        """As torch's, but the moments keep their own types (torch would cast them to the
+        parameter's), and values go into the buffers that the optimizer has where they
+        fit: a captured step names those, and goes on from what was loaded.  sf8 moments
+        are in storage order: the parameters' strides are those of the saved run."""
         groups = state_dict["param_groups"]
+        old, counters = dict(self.state), [g.get("_counter") for g in self.param_groups]
         super().load_state_dict({**state_dict, "state": {}})
-        own = [p for g in self.param_groups for p in g["params"]]
-        saved = [i for g in groups for i in g["params"]]
+        saved = iter([i for g in groups for i in g["params"]])
         self.state.clear()
-        for p, i in zip(own, saved):
-            st = state_dict["state"].get(i)
-            if not st:
-                continue
-            self.state[p] = {k: t.to(device=p.device, copy=True) if isinstance(t, torch.Tensor) else t
-                             for k, t in st.items()}
-        for g in self.param_groups:
-            g["_counter"] = None
+        for g, counter in zip(self.param_groups, counters):
+            for p in g["params"]:
+                st, mine = state_dict["state"].get(next(saved)), old.get(p)
+                if not st and mine and counter is not None:
+                    st = {k: torch.zeros_like(t) if isinstance(t, torch.Tensor) else 0 for k, t in mine.items()}
+                if st:
+                    self.state[p] = {k: self._loaded(p, t, (mine or {}).get(k)) if isinstance(t, torch.Tensor) else t
+                                     for k, t in st.items()}
+            if counter is not None:
+                counter[0].fill_(max((self.state[p]["step"] for p in g["params"] if self.state.get(p)), default=0))
+            g["_counter"] = counter
+
+    @staticmethod
+    def _loaded(p, t, mine):
+        """The values of a saved tensor in the parameter's own (``mine``) or, where they do not fit, a new one."""
+        if mine is None or mine.is_inference() or (mine.shape, mine.dtype, mine.device) != (t.shape, t.dtype, p.device):
+            if t.shape == p.shape and t.dtype == torch.float32:
+                mine = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+            else:
+                mine = torch.empty_like(t, device=p.device)
+        return mine.copy_(t)
