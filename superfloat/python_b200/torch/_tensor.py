@@ -18,6 +18,7 @@ from array import array
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from .._errors import SFShapeError, SFTypeError, SFUnsupportedError
@@ -316,6 +317,13 @@ class _TensorLinear(torch.autograd.Function):
         return (_gradients_once if torch.is_grad_enabled() else _gradients)(ctx, g)
 
 
+def _refuse_tangents(*tensors) -> None:
+    """Within a dual level: a tangent would be dropped, as the layer has no rule for it."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise SFUnsupportedError("tensor_linear has no forward-mode derivative; its gradients are reverse mode")
+
+
 def tensor_linear(x: torch.Tensor, weight, bias=None, *, activation: str | None = None, residual=None, dtype="sf8",
                   scale: str = "per_channel") -> torch.Tensor:
     """``act(x Wq^T + bias) + residual`` over sf4..sf8 codes on the tensor cores.
@@ -330,6 +338,8 @@ def tensor_linear(x: torch.Tensor, weight, bias=None, *, activation: str | None 
     device; the work is queued on its current stream.  Differentiable once, in
     x, a float weight, bias and residual; the backward pass keeps x, the codes
     and the pre-activation (in fp16)."""
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x, weight.scale if isinstance(weight, SFPackedWeight) else weight, bias, residual)
     if isinstance(weight, SFPackedWeight):
         packed, weight = weight, None
         (N, K), bits, index = packed.codes.shape, packed.bits, packed.codes.get_device()
