@@ -157,7 +157,7 @@ def _changed(params):
 
 
 def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step: int, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
-               weight_decay: float = 0.0, dither: int = 0) -> None:
+               weight_decay: float = 0.0, dither: int | None = None) -> None:
     """One AdamW step on lists of CUDA tensors, in place, on each device's
     current stream.
 
@@ -165,8 +165,9 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step: int, lr: float, beta
     in memory (a gradient of another layout is copied).  ``exp_avg`` and
     ``exp_avg_sq``: float32 tensors of the parameter's layout, or
     :class:`SF8Moment`; both of a parameter's moments are of one kind.  ``step``
-    counts from 1.  ``dither`` seeds the rounding of sf8 moments: another number
-    each step (the step will do).  The arithmetic is float32; a 16-bit parameter
+    counts from 1.  ``dither`` seeds the rounding of sf8 moments and is another number
+    each step, the step itself if it is not given: rounded the same way each time, a
+    moment that changes by less than a code's step would never move.  The arithmetic is float32; a 16-bit parameter
     is rounded to nearest once.  A parameter that is given twice is refused, and so
     is a tensor that overlaps another which the same launch (one for each device,
     type and kind of moments) writes.  Nothing of a refused call has run."""
@@ -178,7 +179,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step: int, lr: float, beta
     _check_rates(lr, betas, eps, weight_decay)
     buckets, _kept = _buckets(params, grads, exp_avg, exp_avg_sq)
     _check_launches(list(buckets.items())[1:])         # (the first one's own call checks it)
-    _launch(buckets, lr, betas, eps, weight_decay, step, dither)
+    _launch(buckets, lr, betas, eps, weight_decay, step, step if dither is None else dither)
     _changed(params)
 
 
