@@ -437,8 +437,9 @@ SFB_API int sfb_tensor_failures(int64_t *count);
  * straight-through training uses torch's optimizers.  `table` is HOST memory,
  * eight words a tensor: the device addresses of the parameter, its gradient, the
  * first and the second moment, the scales of the first and of the second moment
- * (sf8 only), the number of elements, and a seed that sets this tensor's dither
- * apart from the others'.  Parameters and gradients are dtype (SFB_F32, SFB_BF16
+ * (sf8 only), the number of elements, and a seed of this tensor's dither: element
+ * e draws a hash of e 0x9E3779B1 + seed + dither, so two tensors draw apart where
+ * that differs.  Parameters and gradients are dtype (SFB_F32, SFB_BF16
  * or SFB_F16); the moments float32, or with sf8 != 0 int8 codes and one float32
  * scale for every 256 elements.  `dither` seeds the rounding of sf8 codes: give
  * another number each step.  `constants` NULL: the constants come from lr .. step.

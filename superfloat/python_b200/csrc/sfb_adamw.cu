@@ -111,7 +111,9 @@ __device__ __forceinline__ void moments(float &m, float &v, float g, const Coefs
     v = __fadd_rn(__fmul_rn(v, c.b2), __fmul_rn(__fmul_rn(g, c.a2), g));
 }
 
-// 32 mixed bits of a counter (two rounds of multiply and xor-shift)
+// 32 mixed bits of a counter: two rounds of multiply and xor-shift, with the shifts and
+// multipliers of Chris Wellons' published search for integer hashes of least bias.  A
+// seed is a place in the counter's sequence: two seeds give the same draws, shifted.
 __device__ __forceinline__ uint32_t mixed(uint32_t i, uint32_t seed) {
     uint32_t h = i * 0x9E3779B1u + seed;
     h ^= h >> 16;

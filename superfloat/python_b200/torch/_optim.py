@@ -29,7 +29,10 @@ SF8_FROM = 4096                    # AdamW(state="sf8") keeps smaller tensors' m
 _ELEMENT = {torch.float32: _lib.ELEMENT["float32"], torch.bfloat16: _lib.ELEMENT["bfloat16"],
             torch.float16: _lib.ELEMENT["float16"]}
 _POWER = {"first": 2, "second": 4}
-_SEED_STEP = 0x9E3779B9            # between the dithers of neighbouring tensors
+# Between the dithers of neighbouring tensors.  All draw from one sequence (csrc/sfb_adamw.cu, `mixed`), each from its
+# own place: element e of tensor i + 1 draws what element e + 1 of tensor i draws eight steps later.  Each draw is
+# uniform, so each moment's rounding is unbiased; draws of different tensors are not independent over steps.
+_SEED_STEP = 0x9E3779B9
 
 
 @dataclass
@@ -212,7 +215,9 @@ class AdamW(torch.optim.Optimizer):
 
     ``state``: "float32", or "sf8" for moments of one byte an element (tensors
     below 4096 elements, biases and norms mostly, keep float32 moments).
-    ``dither_seed`` sets the rounding of sf8 moments apart from another run's.
+    ``dither_seed`` moves the rounding of sf8 moments on by so many steps: two runs
+    draw apart from each other where their seeds differ by more than their steps.
+    The parameters of each group draw as those of the first.
     ``capturable=True`` keeps the step count on the device, so that ``step()``
     can be captured into a CUDA graph and replayed; the other settings are
     then those of the capture.  Every parameter needs its gradient then.  A
