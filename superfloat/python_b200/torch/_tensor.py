@@ -210,10 +210,10 @@ def _forward(x, weight, N, K, packed, bias, residual, bits, wscale, act, train):
     return out, (None if pad else x), z, buf, (None if packed is None else scale), (M, N, K, xpad, scale_at)
 
 
-def _form(t):
-    """What the backward pass relies on in a tensor that was kept; saved-tensor hooks
-    may lay it out again but not change these."""
-    return None if t is None else (t.dtype, t.shape, t.device)
+def _refuse_kept(t, dtype, shape, device):
+    error = SFShapeError if t.dtype is dtype else SFTypeError
+    raise error(f"tensor_linear: the backward pass kept a tensor of {dtype}, {tuple(shape)} on {device}; a saved-tensor "
+                f"hook gave back {t.dtype}, {tuple(t.shape)} on {t.device}")
 
 
 def _kept(ctx):
@@ -221,21 +221,29 @@ def _kept(ctx):
     buffer, the scales).  The layouts are those of the tensors that come back, which
     saved-tensor hooks (activation offloading) may have copied: a slice of a wider
     buffer comes back compact."""
-    saved = ctx.saved_tensors
-    for t, form in zip(saved, ctx.forms):
-        if _form(t) != form:
-            error = SFTypeError if t is not None and form is not None and t.dtype != form[0] else SFShapeError
-            raise error(f"tensor_linear: the backward pass kept {form}, a saved-tensor hook gave back {_form(t)}")
-    xs, z, buf, scale = saved
-    ldx = 0
-    if xs is not None:
-        xs, ldx = _rows_on16(xs, ctx.call[2])
-    if z is not None:
-        z = z.contiguous()
-    buf = buf.contiguous()
-    if buf.data_ptr() % 16:
+    xs, z, buf, scale = ctx.saved_tensors
+    (M, N, K), dt, ldx = ctx.call[:3], ctx.call[6], 0
+    size, device = ctx.buffer
+    if buf.dtype is not torch.uint8 or buf.numel() != size or buf.device != device:
+        _refuse_kept(buf, torch.uint8, (size,), device)
+    if buf.data_ptr() % 16 or not buf.is_contiguous():
         buf = buf.clone()
-    return xs, ldx, z, buf, None if scale is None else scale.contiguous()
+    if xs is not None:
+        if xs.dtype is not dt or xs.shape != (M, K) or xs.device != device:
+            _refuse_kept(xs, dt, (M, K), device)
+        ldx, inner = xs.stride()
+        if inner != 1 or ldx % 8 or ldx < K or M == 1 or xs.data_ptr() % 16:
+            xs, ldx = _rows_on16(xs, K)
+    if z is not None:
+        if z.dtype is not torch.float16 or z.shape != (M, N) or z.device != device:
+            _refuse_kept(z, torch.float16, (M, N), device)
+        if not z.is_contiguous():
+            z = z.contiguous()
+    if scale is not None:
+        if scale.dtype is not torch.float32 or scale.shape != (N,) or scale.device != device:
+            _refuse_kept(scale, torch.float32, (N,), device)
+        scale = scale.contiguous()
+    return xs, ldx, z, buf, scale
 
 
 def _backward(g, kept, call, want_x, want_w, want_b):
@@ -306,7 +314,7 @@ class _TensorLinear(torch.autograd.Function):
         N, K = (packed or weight).shape
         y, xs, z, buf, scale, layout = _forward(x, weight, N, K, packed, bias, residual, bits, wscale, act, True)
         ctx.save_for_backward(xs, z, buf, scale)
-        ctx.forms = (_form(xs), _form(z), _form(buf), _form(scale))
+        ctx.buffer = buf.numel(), buf.device
         ctx.call = (*layout, x.shape, x.dtype, bits, act, packed is not None or wscale == "per_channel",
                     None if weight is None else weight.dtype, None if bias is None else bias.dtype)
         return y
