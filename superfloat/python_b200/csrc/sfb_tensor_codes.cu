@@ -305,44 +305,63 @@ __global__ void __launch_bounds__(32) sum_kernel(Sums s) {
 
 // The largest of the scales whose channel has a code other than 0: a row of zeros has
 // the scale 1 by rule, and beside weights of 1e-3 would leave dz s / 1 below fp16's
-// normal range.  Only rows of that scale are looked at; others without a code (a
-// caller's own scales) stay within the range by what they give.  At least 2^-126, so
-// that its reciprocal is finite.
+// normal range.  Only rows of that scale are looked at, and only where no larger one
+// makes it idle; others without a code (a caller's own scales) stay within the range by
+// what they give.  At least 2^-126, so that its reciprocal is finite.
+// One CTA: 2.4 us for 4096 scales, and the whole of it reads the rows in question, 16
+// bytes a thread (a thread to a row took 82 us for one row of 4096).
 __global__ void __launch_bounds__(1024) top_kernel(const float *__restrict__ scale, int64_t N,
                                                    const uint16_t *__restrict__ codes, int64_t ldc, int64_t K, float *top) {
+    constexpr uint32_t ONE = 0x3F800000u;
     __shared__ uint32_t s_top[32];
+    __shared__ int s_rows[1024], s_count;
     uint32_t t = 0x00800000u;                          // magnitudes order as their bits, NaN above all
+    int ones = 0;
     for (int64_t n = threadIdx.x; n < N; n += 1024) {
         const uint32_t s = __float_as_uint(scale[n]) & 0x7FFFFFFFu;
-        if (s == 0x3F800000u) {
-            bool any = false;
-            for (int64_t k0 = 0; k0 < K && !any; k0 += 64) {
-                uint4 q[8];                            // all asked for before the first is waited for
-#pragma unroll
-                for (int u = 0; u < 8; u++)
-                    q[u] = k0 + 8 * u < K ? __ldg(reinterpret_cast<const uint4 *>(codes + n * ldc + k0 + 8 * u))
-                                          : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int u = 0; u < 8; u++) {
-                    const uint32_t w[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {      // (what is past K is a row's padding)
-                        const int64_t k = k0 + 8 * u + 2 * i;
-                        any |= ((w[i] & 0x7FFFu) && k < K) || ((w[i] & 0x7FFF0000u) && k + 1 < K);
-                    }
-                }
-            }
-            if (!any) continue;
-        }
-        t = max(t, s);
+        if (s == ONE) ones = 1;
+        else t = max(t, s);
     }
     t = __reduce_max_sync(0xffffffffu, t);
     if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = t;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        t = __reduce_max_sync(0xffffffffu, s_top[threadIdx.x]);
-        if (threadIdx.x == 0) *top = __uint_as_float(t);
+    ones = __syncthreads_or(ones);
+    t = __reduce_max_sync(0xffffffffu, s_top[threadIdx.x & 31]);
+    if (ones && t < ONE) {                             // the same for all threads
+        const int64_t per = (K + 7) / 8;               // pieces of 16 bytes a row
+        int live = 0;
+        for (int64_t n0 = 0; n0 < N && !live; n0 += 1024) {
+            __syncthreads();
+            if (threadIdx.x == 0) s_count = 0;
+            __syncthreads();
+            const int64_t n = n0 + threadIdx.x;
+            if (n < N && (__float_as_uint(scale[n]) & 0x7FFFFFFFu) == ONE) s_rows[atomicAdd(&s_count, 1)] = threadIdx.x;
+            __syncthreads();
+            const int64_t pieces = s_count * per;
+            for (int64_t i = threadIdx.x; i - threadIdx.x < pieces && !live; i += 4 * 1024) {
+                uint4 q[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const int64_t at = i + 1024 * u;
+                    q[u] = at < pieces ? __ldg(reinterpret_cast<const uint4 *>(codes + (n0 + s_rows[at / per]) * ldc) + at % per)
+                                       : make_uint4(0, 0, 0, 0);
+                }
+                int any = 0;
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const uint32_t w[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
+                    const int64_t k = (i + 1024 * u) % per * 8;
+#pragma unroll
+                    for (int j = 0; j < 4; j++)        // (what is past K is a row's padding)
+                        any |= ((w[j] & 0x7FFFu) && k + 2 * j < K) || ((w[j] & 0x7FFF0000u) && k + 2 * j + 1 < K);
+                }
+                live = __syncthreads_or(any);
+            }
+        }
+        if (live) t = ONE;
+    } else if (ones) {
+        t = max(t, ONE);
     }
+    if (threadIdx.x == 0) *top = __uint_as_float(t);
 }
 
 template <typename W>
