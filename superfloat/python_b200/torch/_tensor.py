@@ -294,9 +294,14 @@ def _gradients(ctx, g):
 def plain_gradients(g, x, weight, bias, bits, wscale, want_x, want_w, want_b):
     """(dx, dw, db), None where not wanted, of the layer without activation and residual
     from its own inputs: the weight's codes are made again (a forward pass of no rows)."""
-    N, K = weight.shape
     _check_weight(weight)
+    N, K = weight.shape
     _check_operands(x, None, N, K, weight.get_device(), bias, None, None)
+    if g.shape != (*x.shape[:-1], N) or g.dtype != x.dtype or g.device != x.device:
+        raise SFShapeError(f"the result's gradient is {g.dtype}, {tuple(g.shape)} on {g.device}; expected {x.dtype}, "
+                           f"{(*x.shape[:-1], N)} on {x.device}")
+    if want_b and bias is None:
+        raise SFShapeError("there is no bias to have a gradient")
     *_, buf, scale, layout = _forward(x.new_empty((0, K)), weight, N, K, None, None, None, bits, wscale, 0, True)
     rows = x if x.dim() == 2 else x.reshape(-1, K)
     call = (rows.shape[0], *layout[1:], x.shape, x.dtype, bits, 0, wscale == "per_channel", weight.dtype,

@@ -5,6 +5,7 @@ import torch
 import torch.nn as nn
 
 import superfloat.python_b200.torch as sft
+from superfloat.python_b200._errors import SFShapeError
 from test_gpu_tensor_linear import randn
 from test_gpu_tensor_training import batch, loss_of, model
 
@@ -52,3 +53,18 @@ def test_no_rows_and_a_second_derivative(gpu):
     g, = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="autograd formula|differentiate"):
         g.float().sum().backward()
+
+
+def test_the_gradient_op_refuses_what_does_not_fit(gpu):
+    """Called by hand: a gradient of another size, type or device than the result's is refused before a launch."""
+    x, w, g = randn(20, 16, dtype=torch.bfloat16), randn(24, 16), randn(20, 24, seed=1, dtype=torch.bfloat16)
+    op = torch.ops.sf.linear_tensor_backward
+    for bad in (g[:19], g[:, :23], g.float(), g.cpu(), g[None]):
+        with pytest.raises(SFShapeError, match="gradient"):
+            op(bad, x, w, None, 8, "per_tensor", True, True, False)
+    with pytest.raises(SFShapeError, match="no bias"):
+        op(g, x, w, None, 8, "per_tensor", True, True, True)
+    with pytest.raises(SFShapeError, match="features"):
+        op(g, x[:, :8], w, None, 8, "per_tensor", True, True, False)
+    gx, gw, gb = op(g, x, w, None, 8, "per_tensor", True, False, False)
+    assert gx.shape == x.shape and gw.numel() == 0 and gb.numel() == 0
