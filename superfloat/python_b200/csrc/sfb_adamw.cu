@@ -17,7 +17,8 @@
 // would never move.  A second moment above zero keeps a code of at least one, or
 // the quotient would divide by eps alone.  A block whose largest moment is below
 // 1e-30 is held as zero.  A moment that is not finite makes the block's scale
-// infinite or NaN, and every moment of the block then reads as NaN.
+// infinite or NaN; every moment of the block then reads as that or as NaN, and as NaN
+// after the next step.
 // The codes depend on the last bits of m and v, so each float32 operation on the
 // way to a code is one IEEE rounding (the __f*_rn forms are not contracted to fma).
 //

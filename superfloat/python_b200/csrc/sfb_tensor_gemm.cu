@@ -745,6 +745,10 @@ int launch(const Problem &p, Epilogue e, cudaStream_t st) {
 // so the wider tile wins unless it leaves pairs without one.  Measured, 256 and 128
 // columns: 4096 x 4096 x 8192 forward 199 and 246 us, 8192 x 4096 x 4096 w grad 254 and
 // 262; 4096 x 768 x 2304 w grad 25.1 and 16.0, 128 x 4096 x 4096 x grad 24.0 and 14.7.
+// With 768 deep, where a tile's epilogue is as long as its products, the rule still
+// holds for the forward product (z kept, gelu_tanh; 4096 and 8192 rows of 2304
+// channels: 23.6 and 25.3, 39.1 and 43.7) and x's gradient of 4096 x 768 (19.7 and
+// 19.8), but takes the slower side for that of 8192 x 768 (30.5 and 27.1).
 int columns(int64_t R, int64_t C) {
     const int64_t rt = (R + 2 * BM - 1) / (2 * BM), n = sm_count() / 2;
     const int64_t wide = (rt * ((C + 255) / 256) + n - 1) / n, narrow = (rt * ((C + 127) / 128) + n - 1) / n;

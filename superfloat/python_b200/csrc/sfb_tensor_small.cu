@@ -14,10 +14,10 @@
 // only the lane that asked for them reads: nothing to synchronise, and 32 KB a CTA
 // in flight without a register.  (Two segments ahead in registers: 10.8 us for one
 // row of 4096 x 4096; eight ahead: 14, a CTA of 155 registers a thread to an SM.)
-// 48 rows is where the products of 256 channels by 128 rows on tcgen05, with the codes
-// expanded first, overtake it: for 48 rows 8192 x 4096 takes 27 us here and 38 there,
-// 4096 x 4096 15 and 26, a head of 50257 x 768 46 and 41; for 64 rows 41 and 38, 22
-// and 26, 72 and 41.
+// 48 rows is one number for where the products of 256 channels by 128 rows on tcgen05,
+// with the codes expanded first, overtake it, which depends on the shape: for 48 rows
+// 8192 x 4096 takes 27 us here and 38 there, 4096 x 4096 15 and 26, a head of 50257 x
+// 768 46 and 41; for 64 rows 41 and 38, 22 and 26, 72 and 41.
 // (32 channels a warp, to halve the loads of x, was slower: it spills.)
 // A CTA of 8 warps covers 8 / ks groups of 16 channels; ks warps share a group,
 // each every ks-th segment of 64, and their sums are added in a fixed order.

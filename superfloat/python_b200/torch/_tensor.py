@@ -348,9 +348,10 @@ def tensor_linear(x: torch.Tensor, weight, bias=None, *, activation: str | None 
     are then the weight's own).  ``bias`` (N,): float32 or 16 bits.
     ``activation``: None, "relu", "gelu" (erf), "gelu_tanh" or "silu".
     Sums are float32; the result is rounded once.  Everything is on one CUDA
-    device; the work is queued on its current stream.  Differentiable once, in
-    x, a float weight, bias and residual; the backward pass keeps x, the codes
-    and the pre-activation (in fp16)."""
+    device; the work is queued on its current stream.  Differentiable once, by
+    reverse mode, in x, a float weight, bias and residual; the backward pass keeps
+    x, the codes and the pre-activation (in fp16), and rounds the pre-activation's
+    gradient to x's type, as it is an operand of the weight's and x's gradients."""
     if forward_ad._current_level >= 0:
         _refuse_tangents(x, weight.scale if isinstance(weight, SFPackedWeight) else weight, bias, residual)
     if isinstance(weight, SFPackedWeight):
