@@ -278,6 +278,15 @@ class AdamW(torch.optim.Optimizer):
             group["_counter"] = c
         return c
 
+    def _count_on_host(self, group):
+        """The device's step count into the parameters' states, where the group was capturable."""
+        if group.get("_counter") is not None:
+            done = int(group["_counter"][0])
+            for p in group["params"]:
+                if self.state.get(p):
+                    self.state[p]["step"] = done
+            group["_counter"] = None
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -299,6 +308,8 @@ class AdamW(torch.optim.Optimizer):
             if capturing and any(not self.state.get(p) for p in with_grad):
                 raise SFUnsupportedError("AdamW: take one step before the capture, so that the moments and the step "
                                          "counter exist")
+            if not group["capturable"]:
+                self._count_on_host(group)
             todo += (self._device_step if group["capturable"] else self._host_steps)(group, with_grad)
         launches = [item for _, buckets, *_ in todo for item in buckets.items()]
         _check_launches(launches[0 if todo and todo[0][3] is None else 1:])
@@ -398,7 +409,7 @@ class AdamW(torch.optim.Optimizer):
                                      for k, t in st.items()}
             if counter is not None:
                 counter[0].fill_(max((self.state[p]["step"] for p in g["params"] if self.state.get(p)), default=0))
-            g["_counter"] = counter
+            g["_counter"] = counter if g["capturable"] else None
 
     @staticmethod
     def _loaded(p, t, mine):

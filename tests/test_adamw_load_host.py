@@ -96,3 +96,14 @@ def test_a_state_of_before_the_first_step():
     plain = begun(params())
     plain.load_state_dict(fresh)
     assert all(not plain.state.get(p) for p in plain.param_groups[0]["params"])
+
+
+def test_a_state_of_another_setting():
+    """Saved without capturable: the steps are counted on the host from there on."""
+    saved = begun(params()).state_dict()
+    opt = begun(params(), capturable=True)
+    opt.param_groups[0]["_counter"][0].fill_(9)
+    opt.load_state_dict(saved)
+    assert not opt.param_groups[0]["capturable"] and all(opt.steps_done(p) == 3 for p in opt.param_groups[0]["params"])
+    opt.state[opt.param_groups[0]["params"][0]]["step"] = 4
+    assert opt.state_dict()["state"][0]["step"] == 4
