@@ -464,6 +464,71 @@ SFB_API int sfb_adamw_advance(int64_t *step, void *constants, double lr, double 
  * 4 the scales, 6 the number of elements. */
 SFB_API int sfb_sf8_values(const int64_t *table, int count, int power, sfb_stream stream);
 
+/* Layer norm over the last dimension, y = (x - mean) r w + b with r = 1 / sqrt(var + eps),
+ * statistics in float32.  No counterpart in the reference.  Rows of D elements, at most
+ * 65536, row strides in elements; x, y and their gradients are of `dtype` (SFB_F32, BF16
+ * or F16), w and b of a type of their own.  Every field has 8 bytes. */
+typedef struct sfb_norm_call {
+    int64_t dtype, M, D;
+    const void *x;
+    int64_t ldx;
+    const void *w;                          /* D of w_dtype, or NULL: 1 */
+    int64_t w_dtype;
+    const void *b;                          /* D of b_dtype, or NULL: 0 */
+    int64_t b_dtype;
+    double eps;
+    void *y;                                /* the result; in the backward pass its gradient, which is read */
+    int64_t ldy;
+    float *stats;                           /* M pairs (mean, r): written by the forward pass (nullable), read by the backward */
+    void *dx;                               /* backward: the gradients that are wanted */
+    int64_t lddx;
+    void *dw, *db;                          /* of w_dtype and b_dtype */
+    void *work;                             /* backward, dw or db: sfb_norm_work bytes on a 16-byte boundary */
+} sfb_norm_call;
+
+SFB_API int sfb_norm_forward(const sfb_norm_call *call, sfb_stream stream);
+SFB_API int64_t sfb_norm_work(int64_t M, int64_t D);
+SFB_API int sfb_norm_backward(const sfb_norm_call *call, sfb_stream stream);
+
+/* Distillation from a teacher's top logits.  No counterpart in the reference.  A row's loss is
+ * T^2 sum_i p_i (log p_i - log q_i): p the softmax of its K teacher's entries / T, q that of
+ * its V logits / T.  An entry is absent where its index is not in 0 .. V - 1 or its logit is
+ * -inf; a row without entries, or of weight 0, gives 0 and is not read.  Row r of the logits is
+ * at (r / inner) so + (r % inner) si, in elements; of their gradient at (r / inner) go + (r % inner) gi.
+ * Every field has 8 bytes. */
+#define SFB_REDUCE_NONE 0
+#define SFB_REDUCE_SUM 1
+#define SFB_REDUCE_MEAN 2                   /* over the weights of the rows with an entry; 0 where they add up to 0 */
+#define SFB_WEIGHT_NONE (-2)
+#define SFB_WEIGHT_BYTES (-1)               /* truth values */
+typedef struct sfb_distill_call {
+    int64_t dtype, M, V;
+    const void *logits;
+    int64_t inner, so, si, K;               /* K: at most 1024 */
+    const void *teacher;                    /* M x K of t_dtype, rows ldt apart */
+    int64_t t_dtype, ldt;
+    const void *index;                      /* M x K of int64, or int32 where i_long is 0 */
+    int64_t i_long, ldi;
+    const void *weight;                     /* M of w_dtype */
+    int64_t w_dtype, reduction;
+    double temperature;
+    float *loss;                            /* sum and mean: one */
+    float *rows;                            /* M: the rows' losses */
+    float *parts;                           /* mean: sfb_distill_parts(M) */
+    float *stats;                           /* 3 M: written by the forward pass (nullable), read by the backward */
+    void *grad;                             /* of dtype; forward: written too, for an upstream gradient of one (nullable) */
+    int64_t go, gi;
+    const float *upstream;                  /* backward: one, or (SFB_REDUCE_NONE) M */
+    int64_t skip;                           /* backward: grad is the forward pass's, nothing to do where upstream is one */
+} sfb_distill_call;
+
+SFB_API int64_t sfb_distill_parts(int64_t M);
+SFB_API int sfb_distill_forward(const sfb_distill_call *call, sfb_stream stream);
+SFB_API int sfb_distill_backward(const sfb_distill_call *call, sfb_stream stream);
+
+/* A number for the graph capture that the stream is in, 0 if it is in none, -1 on an error. */
+SFB_API int64_t sfb_capture_id(sfb_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct as _struct
 import threading
 
 from ._errors import SFDeviceError, SFLaunchError, SFShapeError
@@ -79,6 +80,13 @@ SIGNATURES = {
     "sfb_adamw_advance": (_i32, [_p, _p, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
                                  ctypes.c_double, ctypes.c_uint, _p]),
     "sfb_sf8_values": (_i32, [_p, _i32, _i32, _p]),
+    "sfb_norm_forward": (_i32, [_p, _p]),
+    "sfb_norm_work": (_i64, [_i64, _i64]),
+    "sfb_norm_backward": (_i32, [_p, _p]),
+    "sfb_distill_parts": (_i64, [_i64]),
+    "sfb_distill_forward": (_i32, [_p, _p]),
+    "sfb_distill_backward": (_i32, [_p, _p]),
+    "sfb_capture_id": (_i64, [_p]),
 }
 
 _lib = None
@@ -470,3 +478,61 @@ def tensor_failures() -> int:
     n = ctypes.c_int64()
     check(load().sfb_tensor_failures(ctypes.addressof(n)), "sf tensor linear")
     return n.value
+
+
+# --- layer norm and the distillation loss --------------------------------------------------------------------------
+
+# the fields of sfb_norm_call and sfb_distill_call, in order: 8 bytes each, a double as its bits (`bits_of`)
+NORM_CALL = ("dtype", "M", "D", "x", "ldx", "w", "w_dtype", "b", "b_dtype", "eps", "y", "ldy", "stats", "dx", "lddx", "dw",
+             "db", "work")
+DISTILL_CALL = ("dtype", "M", "V", "logits", "inner", "so", "si", "K", "teacher", "t_dtype", "ldt", "index", "i_long", "ldi",
+                "weight", "w_dtype", "reduction", "temperature", "loss", "rows", "parts", "stats", "grad", "go", "gi",
+                "upstream", "skip")
+NORM_MOST = 65536                          # features of a layer norm
+DISTILL_MOST = 1024                        # entries of a row
+REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+WEIGHT_NONE, WEIGHT_BYTES = -2, -1
+
+
+def bits_of(value: float) -> int:
+    """A double as the 8-byte integer of the same bits."""
+    return _struct.unpack("q", _struct.pack("d", value))[0]
+
+
+def norm_forward(index, call) -> None:
+    rc = call_on(index, (_lib or load()).sfb_norm_forward, call)
+    if rc:
+        check(rc, "sf layer norm")
+
+
+def norm_backward(index, call) -> None:
+    rc = call_on(index, (_lib or load()).sfb_norm_backward, call)
+    if rc:
+        check(rc, "sf layer norm (backward)")
+
+
+def norm_work(M, D) -> int:
+    return int((_lib or load()).sfb_norm_work(M, D))
+
+
+def distill_forward(index, call) -> None:
+    rc = call_on(index, (_lib or load()).sfb_distill_forward, call)
+    if rc:
+        check(rc, "sf distillation")
+
+
+def distill_backward(index, call) -> None:
+    rc = call_on(index, (_lib or load()).sfb_distill_backward, call)
+    if rc:
+        check(rc, "sf distillation (backward)")
+
+
+def distill_parts(M) -> int:
+    return int((_lib or load()).sfb_distill_parts(M))
+
+
+def capture_id(index) -> int:
+    """A number for the graph capture that device ``index``'s current stream is in; 0: in none."""
+    if _torch is None:
+        _bind_torch()
+    return int((_lib or load()).sfb_capture_id(_raw_stream(index)))

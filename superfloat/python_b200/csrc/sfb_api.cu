@@ -83,3 +83,13 @@ extern "C" int sfb_device_init(int device) {
                          device, major, minor);
     return SFB_OK;
 }
+
+extern "C" int64_t sfb_capture_id(sfb_stream stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return -1;
+    }
+    return status == cudaStreamCaptureStatusNone ? 0 : (int64_t)id + 1;
+}

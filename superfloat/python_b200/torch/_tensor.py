@@ -330,11 +330,11 @@ class _TensorLinear(torch.autograd.Function):
         return (_gradients_once if torch.is_grad_enabled() else _gradients)(ctx, g)
 
 
-def _refuse_tangents(*tensors) -> None:
-    """Within a dual level: a tangent would be dropped, as the layer has no rule for it."""
+def _refuse_tangents(*tensors, what="tensor_linear") -> None:
+    """Within a dual level: a tangent would be dropped, as the operator has no rule for it."""
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-            raise SFUnsupportedError("tensor_linear has no forward-mode derivative; its gradients are reverse mode")
+            raise SFUnsupportedError(f"{what} has no forward-mode derivative; its gradients are reverse mode")
 
 
 def tensor_linear(x: torch.Tensor, weight, bias=None, *, activation: str | None = None, residual=None, dtype="sf8",
