@@ -486,7 +486,7 @@ def tensor_failures() -> int:
 NORM_CALL = ("dtype", "M", "D", "x", "ldx", "w", "w_dtype", "b", "b_dtype", "eps", "y", "ldy", "stats", "dx", "lddx", "dw",
              "db", "work")
 DISTILL_CALL = ("dtype", "M", "V", "logits", "inner", "so", "si", "K", "teacher", "t_dtype", "ldt", "index", "i_long", "ldi",
-                "weight", "w_dtype", "reduction", "temperature", "loss", "rows", "parts", "stats", "grad", "go", "gi",
+                "weight", "w_dtype", "reduction", "temperature", "loss", "rows", "parts", "weights", "stats", "block", "grad", "go", "gi",
                 "upstream", "skip")
 NORM_MOST = 65536                          # features of a layer norm
 DISTILL_MOST = 1024                        # entries of a row

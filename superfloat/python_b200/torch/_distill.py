@@ -115,51 +115,57 @@ def _strides_of(grad, logits):
     return inner * V, V
 
 
+def _kept_at(kept, words, keep):
+    """The places of the rows' statistics and of the entries."""
+    at = kept.data_ptr()
+    return (at + 16 * words[1] * (words[7] + 3 & -4)) if keep else 0, at
+
+
 def _forward(logits, teacher, index, weight, temperature, reduction, keep, with_grad):
     words, held = _call(logits, teacher, index, weight, temperature, reduction)
     M, logits, dev = words[1], held[0], logits.device
     mean, none = reduction == "mean", reduction == "none"
     parts = _lib.distill_parts(M) if mean else 0
     out = torch.empty(logits.shape[:-1] if none else (), dtype=torch.float32, device=dev)
-    # one buffer: the rows' losses, the partial sums of weights
-    room = torch.empty((0 if none else M) + parts, dtype=torch.float32, device=dev)
-    stats = torch.empty(3 * M, dtype=torch.float32, device=dev) if keep else None
+    # places in one buffer: the rows' weights, their losses, the partial sums of the weights; the entries and, for the
+    # backward pass, three numbers a row in another
+    room = torch.empty(M + (0 if none else M) + parts, dtype=torch.float32, device=dev)
+    kept = torch.empty(M * (4 * (words[7] + 3 & -4) + (3 if keep else 0)), dtype=torch.float32, device=dev)
     grad, go, gi = None, 0, 0
     if with_grad:
         grad = _like(logits)
         go, gi = _strides_of(grad, logits)
     at = room.data_ptr()
     _lib.distill_forward(logits.get_device(), array("q", (
-        *words, 0 if none else out.data_ptr(), out.data_ptr() if none else at, at + (0 if none else 4 * M),
-        0 if stats is None else stats.data_ptr(), 0 if grad is None else grad.data_ptr(), go, gi, 0, 0)))
-    return out, held, stats, grad
+        *words, 0 if none else out.data_ptr(), out.data_ptr() if none else at + 4 * M, at + (4 if none else 8) * M, at,
+        *_kept_at(kept, words, keep), 0 if grad is None else grad.data_ptr(), go, gi, 0, 0)))
+    return out, words, held[0], kept, grad
 
 
 def _gradients(ctx, g):
-    logits, teacher, index, weight, stats = ctx.saved_tensors
-    for t, kept in zip((logits, teacher, index, weight, stats), ctx.kept):
-        if t is None:
-            continue
-        kind, size, device = kept
+    logits, kept = ctx.saved_tensors
+    for t, (kind, size, device) in zip((logits, kept), ctx.kept):
         if t.dtype is not kind or t.shape != size or t.device != device:
             raise (SFShapeError if t.dtype is kind else SFTypeError)(
                 f"distill_loss: the backward pass kept a tensor of {kind}, {tuple(size)} on {device}; a saved-tensor hook "
                 f"gave back {t.dtype}, {tuple(t.shape)} on {t.device}")
-    temperature, reduction, captured = ctx.call
+    words, strides, captured = ctx.call
     grad, ctx.grad = ctx.grad, None
     # The forward pass's gradient is the one of this call where nothing can have come between: another backward pass has
-    # its own, and so has one that a graph replays without the forward pass.
-    if grad is not None and _lib.capture_id(logits.get_device()) != captured:
-        grad = None
-    words, held = _call(logits, teacher, index, weight, temperature, reduction)
-    if grad is not None and held[0].stride() != ctx.strides:       # a hook gave the logits back in another layout
+    # its own, and so has one that a graph replays without the forward pass, or one whose logits a hook laid out anew.
+    if grad is not None and (_lib.capture_id(logits.get_device()) != captured or logits.stride() != strides):
         grad = None
     skip = grad is not None
+    logits, inner, so, si = _two_strides(logits)
     if not skip:
-        grad = _like(held[0])
-    g, stats = g.contiguous(), stats.contiguous()
-    _lib.distill_backward(held[0].get_device(), array("q", (
-        *words, 0, 0, 0, stats.data_ptr(), grad.data_ptr(), *_strides_of(grad, held[0]), g.data_ptr(), int(skip))))
+        grad = _like(logits)
+    g, kept = g.contiguous(), kept.contiguous()
+    if kept.data_ptr() % 16:
+        kept = kept.clone()
+    _lib.distill_backward(logits.get_device(), array("q", (
+        *words[:3], logits.data_ptr(), inner, so, si, words[7], 0, words[9], words[10], 0, words[12], words[13], 0,
+        _lib.WEIGHT_NONE, *words[16:], 0, 0, 0, 0, *_kept_at(kept, words, True), grad.data_ptr(), *_strides_of(grad, logits),
+        g.data_ptr(), int(skip))))
     return grad, None, None, None, None, None
 
 
@@ -173,11 +179,11 @@ class _DistillLoss(torch.autograd.Function):
         # The gradient with the loss: the row is at hand, and a backward pass that gets a gradient of one has nothing to
         # do.  float16's waits for the scale that its loss gets, below which it would round to zero.
         with_grad = reduction != "none" and logits.dtype is not torch.float16
-        loss, held, stats, grad = _forward(logits, teacher, index, weight, temperature, reduction, True, with_grad)
-        ctx.save_for_backward(*held, stats)
-        ctx.kept = [None if t is None else (t.dtype, t.shape, t.device) for t in (*held, stats)]
-        ctx.grad, ctx.strides = grad, held[0].stride()
-        ctx.call = temperature, reduction, _lib.capture_id(logits.get_device()) if with_grad else 0
+        loss, words, rows, kept, grad = _forward(logits, teacher, index, weight, temperature, reduction, True, with_grad)
+        ctx.save_for_backward(rows, kept)
+        ctx.kept = [(t.dtype, t.shape, t.device) for t in (rows, kept)]
+        ctx.grad = grad
+        ctx.call = words, rows.stride(), _lib.capture_id(logits.get_device()) if with_grad else 0
         return loss
 
     @staticmethod

@@ -36,7 +36,7 @@ def lib():
 A = 1 << 20                                    # addresses that no launch ever sees
 NORM = dict(dtype=2, M=10, D=64, x=A, ldx=64, y=2 * A, ldy=64, eps=_lib.bits_of(1e-5), stats=3 * A, dx=4 * A, lddx=64, work=5 * A)
 DISTILL = dict(dtype=2, M=10, V=64, logits=A, inner=10, si=64, K=4, teacher=2 * A, ldt=4, index=3 * A, i_long=1, ldi=4,
-               w_dtype=-2, reduction=2, temperature=_lib.bits_of(1.0), loss=4 * A, rows=5 * A, parts=6 * A, stats=7 * A,
+               w_dtype=-2, reduction=2, temperature=_lib.bits_of(1.0), loss=4 * A, rows=5 * A, parts=6 * A, stats=7 * A, block=10 * A, weights=11 * A,
                grad=8 * A, gi=64, upstream=9 * A)
 
 
@@ -61,9 +61,9 @@ def test_norm_backward_refusals(lib, bad):
 
 
 @pytest.mark.parametrize("bad", [
-    dict(dtype=4), dict(t_dtype=4), dict(w_dtype=4), dict(w_dtype=0), dict(M=-1), dict(V=0), dict(K=-1), dict(inner=0), dict(ldt=3), dict(ldi=3),
+    dict(dtype=4), dict(t_dtype=4), dict(w_dtype=4), dict(M=-1), dict(V=0), dict(K=-1), dict(inner=0), dict(ldt=3), dict(ldi=3),
     dict(temperature=0), dict(temperature=_lib.bits_of(math.nan)), dict(temperature=_lib.bits_of(1e7)), dict(reduction=3),
-    dict(reduction=-1), dict(logits=0), dict(teacher=0), dict(index=0), dict(logits=A + 1), dict(grad=8 * A + 1)])
+    dict(reduction=-1), dict(logits=0), dict(so=-1), dict(gi=-8), dict(logits=A + 1), dict(grad=8 * A + 1)])
 def test_distill_refusals(lib, bad):
     for fn in (lib.sfb_distill_forward, lib.sfb_distill_backward):
         assert call(fn, _lib.DISTILL_CALL, DISTILL, bad) == _lib.SFB_EINVAL and lib.sfb_last_error()
@@ -71,9 +71,9 @@ def test_distill_refusals(lib, bad):
 
 def test_more_refusals(lib):
     forward, backward, fields = lib.sfb_distill_forward, lib.sfb_distill_backward, _lib.DISTILL_CALL
-    for bad in (dict(loss=0), dict(rows=0), dict(parts=0)):
+    for bad in (dict(loss=0), dict(rows=0), dict(parts=0), dict(weights=0), dict(block=0), dict(teacher=0), dict(index=0), dict(w_dtype=0)):
         assert call(forward, fields, DISTILL, bad) == _lib.SFB_EINVAL
-    for bad in (dict(grad=0), dict(stats=0), dict(upstream=0)):
+    for bad in (dict(grad=0), dict(stats=0), dict(block=0), dict(block=A + 4), dict(upstream=0)):
         assert call(backward, fields, DISTILL, bad) == _lib.SFB_EINVAL
     for bad in (dict(K=1025, ldt=1025, ldi=1025), dict(V=1 << 31)):
         assert call(forward, fields, DISTILL, bad) == call(backward, fields, DISTILL, bad) == _lib.SFB_ERANGE
@@ -83,7 +83,7 @@ def test_more_refusals(lib):
     # nothing to do
     assert call(lib.sfb_norm_forward, _lib.NORM_CALL, NORM, dict(M=0, x=0, y=0)) == _lib.SFB_OK
     assert call(backward, fields, DISTILL, dict(M=0)) == _lib.SFB_OK
-    assert lib.sfb_distill_parts(0) == 0 and lib.sfb_distill_parts(257) == 2
+    assert lib.sfb_distill_parts(0) == 0 and lib.sfb_distill_parts(9) == 2
     assert lib.sfb_norm_work(0, 0) == 0 and lib.sfb_norm_work(5, 65537) == 0
 
 
