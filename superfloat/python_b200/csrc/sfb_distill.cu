@@ -10,12 +10,16 @@
 // Bound by memory, and nearly by the rate of exponentials (two an element, 16 a cycle and SM):
 // the row is read once, into shared memory, and its gradient written once, from there.  Maximum,
 // sum and gradient are three passes over shared memory, of which a thread reads what it has
-// copied itself (cp.async), so that nothing waits for the whole row; the next row's copy is in
-// flight meanwhile.  A row is split over a cluster of up to 8 CTAs, so that two CTAs with two rows
-// each fit an SM, and so that few rows still occupy the GPU; they exchange (maximum, sum) through one
-// another's memory, with one barrier a row.  What depends on the teacher's entries alone is made by
-// a launch before; a warp of its own makes the row's loss and the elements of the gradient
-// that have an entry.
+// copied itself (cp.async), so that nothing waits for the whole row, and asks for the next row's
+// vectors once it has used its own of this one.  A row is split over a cluster of up to 8 CTAs, so that
+// four fit an SM, one's sums running under another's copies and a third one's stores, and so that
+// few rows still occupy the GPU.  What depends on the teacher's entries alone is made by a launch
+// before; a warp of its own makes the row's loss and the elements of the gradient that have an
+// entry.
+// 4096 x 50257 of bf16, a fifth of the rows masked: 162 us, 5.1 TB/s; 2047 x 32001 of float32: 94 us, 5.6 TB/s.
+// Measured on the way: two CTAs an SM with 100 KB of a row each 176, five with 34 KB 197; two buffers
+// a CTA, the next row's copy under this one's sums, 188 (two CTAs) and 196 (one, of a whole row);
+// the gradient one row behind the sums 243.
 // Rows start anywhere: a position in shared memory has the alignment of its address.  What
 // shared memory does not hold is read from memory three times.
 // Statistics and sums are float32.  2^x is taken of x log2(e) / T - b, with one b, the
@@ -30,7 +34,7 @@
 namespace sfb {
 namespace {
 
-constexpr int THREADS = 480, WARPS = THREADS / 32;   // that have the row
+constexpr int THREADS = 224, WARPS = THREADS / 32;   // that have the row
 constexpr int ALL = THREADS + 32;                    // and the warp that has the entries
 constexpr int MAX_K = 1024;
 constexpr int PART = 8;                              // rows of a CTA that takes entries, a warp each
@@ -387,13 +391,13 @@ __device__ __forceinline__ void copy_row(const Part<T> &q, T *row, bool live) {
 // --- a row's kernel ------------------------------------------------------------------------------------------
 
 template <typename T, bool GRAD>
-__global__ void __launch_bounds__(ALL, 2) row_kernel(const __grid_constant__ Distill p) {
+__global__ void __launch_bounds__(ALL, 4) row_kernel(const __grid_constant__ Distill p) {
     constexpr int E = Wide<T>::E;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Shared s;
     const int k4 = (int)((p.K + 3) & ~3);
     float *entries = reinterpret_cast<float *>(smem);                 // two rows' p, mass, near, where
-    T *rows = reinterpret_cast<T *>(entries + 8 * k4);                // two rows
+    T *row = reinterpret_cast<T *>(entries + 8 * k4);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t n = cluster_size(), rank = cluster_rank();
     const int64_t step = gridDim.x / n;
@@ -424,9 +428,8 @@ __global__ void __launch_bounds__(ALL, 2) row_kernel(const __grid_constant__ Dis
     if (warp < WARPS) {
         float weight = p.weights[r0], next = r0 + step < p.M ? p.weights[r0 + step] : 0.0f;
         Part<T> ahead = part_of<T>(p, r0, rank);
-        copy_row(ahead, rows, weight != 0.0f);
+        copy_row(ahead, row, weight != 0.0f);
         for (int64_t r = r0; r < p.M; r += step) {
-            T *row = rows + turn * p.held;
             const bool live = weight != 0.0f;
             const Part<T> q = ahead;
             if (tid == 0)
@@ -434,10 +437,8 @@ __global__ void __launch_bounds__(ALL, 2) row_kernel(const __grid_constant__ Dis
                                  (uint32_t)__cvta_generic_to_shared(&s.bar[turn])),
                              "r"(expected)
                              : "memory");
-            if (r + step < p.M) ahead = part_of<T>(p, r + step, rank);
-            copy_row(ahead, rows + (turn ^ 1) * p.held, next != 0.0f);
             const float after = r + 2 * step < p.M ? p.weights[r + 2 * step] : 0.0f;
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
             float2 soft = make_float2(ninf(), 0.0f);
             if (live) {
                 // the vectors around the row's ends: what is not the row's becomes -inf
@@ -485,29 +486,38 @@ __global__ void __launch_bounds__(ALL, 2) row_kernel(const __grid_constant__ Dis
                 T *to = static_cast<T *>(p.grad) + place(p, r, p.go, p.gi);
                 if (p.same) {
                     T *to0 = to - q.lead + q.first;
-                    auto put = [&](int i, uint4 w, auto is_far) {
-                        float v[E];
-                        open16<T>(w, v);
-#pragma unroll
-                        for (int j = 0; j < E; j++) v[j] = live ? power<decltype(is_far)::value>(v[j], soft.x, base, p.unit) * scale : 0.0f;
-                        if (whole(q, i)) {
-                            *reinterpret_cast<uint4 *>(to0 + (int64_t)i * E) = close16<T>(v);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < E; j++)
-                                if (i * E + j >= q.begin && i * E + j < q.end) to0[(int64_t)i * E + j] = from_f<T>(v[j]);
-                        }
-                    };
-                    auto rest = [&](auto is_far) {
-                        for (int i = q.inside + tid; i < q.vectors; i += THREADS) put(i, live ? vector_at(q, i) : make_uint4(0, 0, 0, 0), is_far);
-                    };
-                    if (far(soft.x, p.unit)) {
-                        for (int i = tid; i < q.inside; i += THREADS) put(i, *reinterpret_cast<const uint4 *>(row + i * E), std::true_type());
-                        rest(std::true_type());
+                    uint4 *out = reinterpret_cast<uint4 *>(to0);
+                    // the vectors of the row alone, from `from` on `count` of them
+                    const int from = q.begin > 0, count = max(q.end / E - from, 0);
+                    if (!live) {
+                        for (int i = tid; i < count; i += THREADS) out[from + i] = make_uint4(0, 0, 0, 0);
                     } else {
+                        auto slope = [&](uint4 w, auto is_far) {
+                            float v[E];
+                            open16<T>(w, v);
+#pragma unroll
+                            for (int j = 0; j < E; j++) v[j] = power<decltype(is_far)::value>(v[j], soft.x, base, p.unit) * scale;
+                            return close16<T>(v);
+                        };
+                        auto all = [&](auto is_far) {
+                            // (a thread's vectors are those that it has copied)
 #pragma unroll 2
-                        for (int i = tid; i < q.inside; i += THREADS) put(i, *reinterpret_cast<const uint4 *>(row + i * E), std::false_type());
-                        rest(std::false_type());
+                            for (int i = tid; i < q.inside; i += THREADS)
+                                if ((unsigned)(i - from) < (unsigned)count) out[i] = slope(*reinterpret_cast<const uint4 *>(row + i * E), is_far);
+                            for (int i = q.inside + tid; i < q.vectors; i += THREADS)
+                                if ((unsigned)(i - from) < (unsigned)count) out[i] = slope(vector_at(q, i), is_far);
+                        };
+                        if (far(soft.x, p.unit)) all(std::true_type());
+                        else all(std::false_type());
+                    }
+                    // the elements around them, fewer than a vector's at either end
+                    if (warp == 0) {
+                        const int head = from ? min(E, q.end) : 0, tail = max(q.end / E * E, head);
+                        for (int u = lane; u < q.end - tail + head; u += 32) {
+                            const int at = u < head ? u : tail + u - head;
+                            if (at >= q.begin)
+                                to0[at] = from_f<T>(live ? power_of(to_f(q.at[at]), soft.x, base, p.unit) * scale : 0.0f);
+                        }
                     }
                 } else {
                     T *to0 = to - q.lead + q.first;
@@ -519,14 +529,18 @@ __global__ void __launch_bounds__(ALL, 2) row_kernel(const __grid_constant__ Dis
                     // here a thread reads what others have copied, and will copy over
                     asm volatile("bar.sync 2, %0;" ::"n"(THREADS) : "memory");
                 }
-                asm volatile("bar.arrive 1, %0;" ::"n"(ALL) : "memory");
             }
+            // the next row's copies, to where this thread has read what it needs
+            if (r + step < p.M) {
+                ahead = part_of<T>(p, r + step, rank);
+                copy_row(ahead, row, next != 0.0f);
+            }
+            if constexpr (GRAD) asm volatile("bar.arrive 1, %0;" ::"n"(ALL) : "memory");
             weight = next;
             next = after;
             parity ^= turn;
             turn ^= 1;
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
         // the next row's entries are copied while this one's are used
         auto copy = [&](int64_t r, int i) {
@@ -656,7 +670,7 @@ __global__ void __launch_bounds__(GT, 3) gradient_kernel(const __grid_constant__
 
 // --- launches ------------------------------------------------------------------------------------------------
 
-constexpr int64_t ROOM = 104 * 1024;     // dynamic shared memory of a CTA of which two fit an SM
+constexpr int64_t ROOM = 53 * 1024;      // dynamic shared memory of a CTA of which four fit an SM
 
 // the kernel's shared memory, once a device and context
 template <typename K>
@@ -693,17 +707,17 @@ int launch_rows(Distill p, cudaStream_t st) {
     const int rc = allow(row_kernel<T, GRAD>, ready, ROOM);
     if (rc) return rc;
     constexpr int64_t E = 16 / sizeof(T);
-    const int64_t entries = 32 * ((p.K + 3) & ~3ll), room = (ROOM - entries) / 2 / 16 * E, span = p.V + E - 1;
+    const int64_t entries = 32 * ((p.K + 3) & ~3ll), room = (ROOM - entries) / 16 * E, span = p.V + E - 1;
     auto chunk_of = [&](int64_t c) { return ((span + c - 1) / c + E - 1) / E * E; };
     int64_t c = 1;
-    // A cluster as large as lets shared memory hold two of its rows; larger ones where rows are few, a chunk being 4096
+    // A cluster as large as lets shared memory hold its part; larger ones where rows are few, a chunk being 4096
     // elements at least.
     while (c < 8 && (chunk_of(c) > room || (p.M * c < 2 * sm_count() && chunk_of(2 * c) >= 4096))) c *= 2;
     p.chunk = (int)chunk_of(c);
     p.held = (int)std::min<int64_t>(p.chunk, room);
     cudaLaunchConfig_t cfg{};
     cfg.blockDim = dim3(ALL);
-    cfg.dynamicSmemBytes = (size_t)(entries + 2 * p.held * (int64_t)sizeof(T));
+    cfg.dynamicSmemBytes = (size_t)(entries + p.held * (int64_t)sizeof(T));
     cfg.gridDim = dim3((unsigned)c);
     cfg.stream = st;
     cudaLaunchAttribute a{};
