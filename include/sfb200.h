@@ -528,6 +528,41 @@ SFB_API int64_t sfb_distill_parts(int64_t M);
 SFB_API int sfb_distill_forward(const sfb_distill_call *call, sfb_stream stream);
 SFB_API int sfb_distill_backward(const sfb_distill_call *call, sfb_stream stream);
 
+/* The gated feed-forward product over sf4..sf8 codes: h = act(x Wg^T + bg) (x Wu^T + bu), both weights N x K, as
+ * sfb_tensor_call's.  No counterpart in the reference.  Np stands for N rounded up to a multiple of 16: codes and scales
+ * are those of the gate, rows up to Np of zeros, then of the other weight. */
+typedef struct sfb_gated_call {
+    int64_t dtype, bits, act, M, N, K;      /* x is M x K */
+    const void *x;
+    int64_t ldx;
+    void *xpad;                             /* M x ldp of dtype, where x's rows do not start on 16 bytes */
+    int64_t ldp;
+    const void *gate, *up;                  /* float weights of w_dtype, or packed codes (SFB_I8) */
+    int64_t ldg, ldu, w_dtype, per_channel;
+    const float *gate_scale, *up_scale;     /* packed: N each */
+    void *codes;                            /* 2 Np x ldc of dtype: written by the forward pass, read by the backward */
+    int64_t ldc;
+    float *scale;                           /* 2 Np: likewise */
+    const void *gate_bias, *up_bias;        /* N each, of their types, or NULL */
+    int64_t gate_bias_dtype, up_bias_dtype;
+    void *y;                                /* M x N: h; in the backward pass its gradient, which is read */
+    int64_t ldy;
+    float *z;                               /* M x 2 Np: both products, kept for the backward pass (nullable) */
+    int64_t ldz;
+    void *work;                             /* forward, one scale: 8 N bytes; backward with a bias's gradient: sfb_gated_sums bytes */
+    float *top;                             /* backward, fp16: one float */
+    void *dz, *dzs;                         /* backward: M x ldd of dtype, ldd at least 2 Np */
+    int64_t ldd;
+    void *dx, *dgate, *dup;                 /* the gradients that are wanted: M x K, N x K each of w_dtype (one product where dup
+                                               follows Np rows after dgate: that has 2 Np rows then) */
+    void *dgate_bias, *dup_bias;
+} sfb_gated_call;
+
+/* The forward pass; `codes` NULL: for packed weights, at most SFB_SMALL_ROWS rows and no z, read as they are. */
+SFB_API int sfb_gated_forward(const sfb_gated_call *call, sfb_stream stream);
+SFB_API int64_t sfb_gated_sums(int64_t M, int64_t N);
+SFB_API int sfb_gated_backward(const sfb_gated_call *call, sfb_stream stream);
+
 /* A number for the graph capture that the stream is in, 0 if it is in none, -1 on an error. */
 SFB_API int64_t sfb_capture_id(sfb_stream stream);
 

@@ -80,6 +80,9 @@ SIGNATURES = {
     "sfb_adamw_advance": (_i32, [_p, _p, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double,
                                  ctypes.c_double, ctypes.c_uint, _p]),
     "sfb_sf8_values": (_i32, [_p, _i32, _i32, _p]),
+    "sfb_gated_forward": (_i32, [_p, _p]),
+    "sfb_gated_sums": (_i64, [_i64, _i64]),
+    "sfb_gated_backward": (_i32, [_p, _p]),
     "sfb_norm_forward": (_i32, [_p, _p]),
     "sfb_norm_work": (_i64, [_i64, _i64]),
     "sfb_norm_backward": (_i32, [_p, _p]),
@@ -472,6 +475,30 @@ def tensor_backward(index, call) -> None:
 
 def tensor_sums(M, N) -> int:
     return int(load().sfb_tensor_sums(M, N))
+
+
+# the fields of sfb_gated_call, in order
+GATED_CALL = ("dtype", "bits", "act", "M", "N", "K", "x", "ldx", "xpad", "ldp", "gate", "up", "ldg", "ldu", "w_dtype",
+              "per_channel", "gate_scale", "up_scale", "codes", "ldc", "scale", "gate_bias", "up_bias", "gate_bias_dtype",
+              "up_bias_dtype", "y", "ldy", "z", "ldz", "work", "top", "dz", "dzs", "ldd", "dx", "dgate", "dup", "dgate_bias",
+              "dup_bias")
+
+
+def gated_forward(index, call) -> None:
+    """``call``: an array("q") of GATED_CALL's fields, on device ``index``."""
+    rc = call_on(index, (_lib or load()).sfb_gated_forward, call)
+    if rc:
+        check(rc, "sf gated product")
+
+
+def gated_backward(index, call) -> None:
+    rc = call_on(index, (_lib or load()).sfb_gated_backward, call)
+    if rc:
+        check(rc, "sf gated product (backward)")
+
+
+def gated_sums(M, N) -> int:
+    return int((_lib or load()).sfb_gated_sums(M, N))
 
 
 def tensor_failures() -> int:

@@ -91,28 +91,49 @@ __device__ __forceinline__ uint32_t row_top(const W *row, int64_t K, bool vec, i
     return __reduce_max_sync(0xffffffffu, top);
 }
 
+// One weight, or the two of a gated product, N rows each; the second one's codes and scales are `next` rows on.
+template <typename W> struct Weights {
+    const W *w[2];
+    int64_t ldw[2], next;
+    bool vec[2];
+    int count;
+};
+
 template <typename W>
-__global__ void __launch_bounds__(QT) amax_kernel(const W *__restrict__ w, int64_t N, int64_t K, int64_t ldw, bool vec,
-                                                  uint32_t *amax) {
+__global__ void __launch_bounds__(QT) amax_kernel(const __grid_constant__ Weights<W> ws, int64_t N, int64_t K, uint32_t *amax) {
     const int64_t n = (int64_t)blockIdx.x * (QT / 32) + threadIdx.x / 32;
     if (n >= N) return;
-    const uint32_t top = row_top(w + n * ldw, K, vec, threadIdx.x & 31);
-    if ((threadIdx.x & 31) == 0) amax[n] = top;
+    const int y = blockIdx.y;
+    const uint32_t top = row_top(ws.w[y] + n * ws.ldw[y], K, ws.vec[y], threadIdx.x & 31);
+    if ((threadIdx.x & 31) == 0) amax[y * N + n] = top;
 }
 
-// amax: of the rows, for one scale; null for a scale a row
+// amax: of the rows, for one scale a matrix; null for a scale a row
 template <typename W, typename O>
-__global__ void __launch_bounds__(QT) code_kernel(const W *__restrict__ w, int64_t N, int64_t K, int64_t ldw, bool vec,
+__global__ void __launch_bounds__(QT) code_kernel(const __grid_constant__ Weights<W> ws, int64_t N, int64_t K,
                                                   int bits, const uint32_t *__restrict__ amax, O *codes, int64_t ldc,
                                                   bool whole, float *scale, Rows rows) {
-    if (blockIdx.y == 1) {                     // x's copy, in the launch that the call makes anyway
+    const int y = blockIdx.y;
+    if (y == ws.count) {                       // x's copy, in the launch that the call makes anyway
         pad_rows(rows, threadIdx.x & 63, threadIdx.x >> 6, 0, 1, blockIdx.x, gridDim.x);
         return;
     }
-    if ((int64_t)blockIdx.x * (QT / 32) >= N) return;
+    if (y == 1) {
+        codes += ws.next * ldc;
+        scale += ws.next;
+        if (amax) amax += N;
+    }
+    const W *w = ws.w[y];
+    const int64_t ldw = ws.ldw[y];
+    const bool vec = ws.vec[y];
+    if ((int64_t)blockIdx.x * (QT / 32) >= max(N, ws.next)) return;
     __shared__ uint32_t s_top[QT / 32];
     const int lane = threadIdx.x & 31;
     const int64_t n = (int64_t)blockIdx.x * (QT / 32) + threadIdx.x / 32;
+    if (n >= N && n < ws.next) {               // between the two weights: zeros, that products may sum over
+        if (lane == 0) scale[n] = 1.0f;
+        for (int64_t k = lane; k < K; k += 32) codes[n * ldc + k] = O();
+    }
     uint32_t top = 0;
     if (amax) {
         for (int64_t i = threadIdx.x; i < N; i += QT) top = max(top, amax[i]);
@@ -303,7 +324,7 @@ slope_kernel(const T *__restrict__ dy, int64_t ldy, const __half *__restrict__ z
 
 __global__ void __launch_bounds__(32) sum_kernel(Sums s) {
     const int64_t n = (int64_t)blockIdx.x * 32 + threadIdx.x;
-    if (n < s.N) store_as(s.db, n, s.dtype, column_sum(s, n));
+    if (n < s.N) store_sum(s, n, column_sum(s, n));
 }
 
 // The largest of the scales whose channel has a code other than 0: a row of zeros has
@@ -368,42 +389,50 @@ __global__ void __launch_bounds__(1024) top_kernel(const float *__restrict__ sca
 }
 
 template <typename W>
-int quantize_from(const W *w, int64_t N, int64_t K, int64_t ldw, int bits, bool per_channel, void *codes, int64_t ldc,
-                  int out, float *scale, uint32_t *amax, const Rows &rows, cudaStream_t st) {
-    const bool vec = (reinterpret_cast<uintptr_t>(w) & 15) == 0 && ldw * sizeof(W) % 16 == 0;
-    const unsigned grid = (unsigned)((N + QT / 32 - 1) / (QT / 32));
-    if (!per_channel) amax_kernel<W><<<grid, QT, 0, st>>>(w, N, K, ldw, vec, amax);
+int quantize_from(const W *w, int64_t ldw, const W *w2, int64_t ldw2, int64_t N, int64_t Np, int64_t K, int bits,
+                  bool per_channel, void *codes, int64_t ldc, int out, float *scale, uint32_t *amax, const Rows &rows,
+                  cudaStream_t st) {
+    auto on16 = [](const W *p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * sizeof(W) % 16 == 0; };
+    Weights<W> ws{{w, w2}, {ldw, ldw2}, Np, {on16(w, ldw), on16(w2, ldw2)}, w2 ? 2 : 1};
+    const unsigned grid = (unsigned)((std::max(N, Np) + QT / 32 - 1) / (QT / 32));
+    if (!per_channel) amax_kernel<W><<<dim3(grid, ws.count), QT, 0, st>>>(ws, N, K, amax);
     const uint32_t *top = per_channel ? nullptr : amax;
     const dim3 both(std::max<unsigned>(grid, rows.x ? (unsigned)std::min<int64_t>((rows.M + 3) / 4, 16ll * sm_count()) : 0),
-                    rows.x ? 2 : 1);
+                    ws.count + (rows.x ? 1 : 0));
     // a row of 16-bit codes is padded to a multiple of 8; one of int8 only where the caller's stride says so
     if (out == SFB_I8)
-        code_kernel<W, int8_t><<<both, QT, 0, st>>>(w, N, K, ldw, vec, bits, top, static_cast<int8_t *>(codes), ldc,
+        code_kernel<W, int8_t><<<both, QT, 0, st>>>(ws, N, K, bits, top, static_cast<int8_t *>(codes), ldc,
                                                     K % 8 == 0 && ldc % 8 == 0 && (reinterpret_cast<uintptr_t>(codes) & 7) == 0,
                                                     scale, rows);
     else if (out == SFB_BF16)
-        code_kernel<W, __nv_bfloat16><<<both, QT, 0, st>>>(w, N, K, ldw, vec, bits, top,
+        code_kernel<W, __nv_bfloat16><<<both, QT, 0, st>>>(ws, N, K, bits, top,
                                                            static_cast<__nv_bfloat16 *>(codes), ldc, true, scale, rows);
     else
-        code_kernel<W, __half><<<both, QT, 0, st>>>(w, N, K, ldw, vec, bits, top, static_cast<__half *>(codes), ldc,
+        code_kernel<W, __half><<<both, QT, 0, st>>>(ws, N, K, bits, top, static_cast<__half *>(codes), ldc,
                                                     true, scale, rows);
     return check_launch("sf weight codes");
 }
 
 }  // namespace
 
+int tensor_quantize2(const void *w, int64_t ldw, const void *w2, int64_t ldw2, int dtype, int64_t N, int64_t Np, int64_t K,
+                     int bits, bool per_channel, void *codes, int64_t ldc, int codes_dtype, float *scale, void *work,
+                     const Rows &rows, cudaStream_t st) {
+    uint32_t *amax = static_cast<uint32_t *>(work);
+    auto from = [&](auto type) {
+        using W = decltype(type);
+        return quantize_from(static_cast<const W *>(w), ldw, static_cast<const W *>(w2), ldw2, N, Np, K, bits, per_channel,
+                             codes, ldc, codes_dtype, scale, amax, rows, st);
+    };
+    if (dtype == SFB_F32) return from(float());
+    if (dtype == SFB_BF16) return from(__nv_bfloat16());
+    return from(__half());
+}
+
 int tensor_quantize(const void *w, int dtype, int64_t N, int64_t K, int64_t ldw, int bits, bool per_channel, void *codes,
                     int64_t ldc, int codes_dtype, float *scale, void *work, const Rows &rows,
                     cudaStream_t st) {
-    uint32_t *amax = static_cast<uint32_t *>(work);
-    if (dtype == SFB_F32)
-        return quantize_from(static_cast<const float *>(w), N, K, ldw, bits, per_channel, codes, ldc, codes_dtype,
-                             scale, amax, rows, st);
-    if (dtype == SFB_BF16)
-        return quantize_from(static_cast<const __nv_bfloat16 *>(w), N, K, ldw, bits, per_channel, codes, ldc,
-                             codes_dtype, scale, amax, rows, st);
-    return quantize_from(static_cast<const __half *>(w), N, K, ldw, bits, per_channel, codes, ldc, codes_dtype, scale,
-                         amax, rows, st);
+    return tensor_quantize2(w, ldw, nullptr, 0, dtype, N, 0, K, bits, per_channel, codes, ldc, codes_dtype, scale, work, rows, st);
 }
 
 namespace {

@@ -148,6 +148,15 @@ __device__ __forceinline__ void tma_load_operand(uint32_t dst, const CUtensorMap
         : "memory");
 }
 
+// 128 rows of two operands, 16 of the one and 16 of the other in turn: coordinates k and the first group of 16
+__device__ __forceinline__ void tma_load_gated(uint32_t dst, const CUtensorMap *map, int c0, int group, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
+        "{%2, %3, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(c0), "r"(0), "r"(group), "r"(bar)
+        : "memory");
+}
+
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
@@ -234,6 +243,11 @@ struct Epilogue {
     float unit;                  // 2^-(bits-1) where a scale or alpha stands for codes, else 1
     int bias_dtype, y_dtype;
     int64_t ldr, ldz, ldy;
+    // of a gated product: the up half's scales, bias and columns of z (float32), Np after the gate's
+    const void *bias2;
+    int bias2_dtype;
+    int64_t half;
+    float *zf;
     Sums sums;                   // the bias's gradient, for the warp that has nothing to issue in the second CTA
     bool vec;                    // y (of 16 bits), z and r start on 16 bytes, and so do their rows
 };
@@ -351,6 +365,43 @@ __device__ __forceinline__ void box_out(uint32_t box, const uint32_t (&w)[16], u
     }
 }
 
+// A gated box: 16 channels by 32 columns.  A lane has the channel lane mod 16 in the 16 columns 16 (lane / 16) ..; turned
+// around, lane l has the channels 8 (l mod 2) .. + 7 of column 8 (2 h + l / 2 mod 2) + l / 4, for h of 0 and 1.
+__device__ __forceinline__ uint32_t gated_at(int row, int piece) {
+    return row * 64 + (((piece ^ (row >> 1) ^ (row >> 3 << 1)) & 3) << 4);
+}
+
+__device__ __forceinline__ void gated_out(uint32_t box, const uint32_t (&w)[8], uint16_t *to, int64_t ld, int cols, int chans,
+                                          bool vec, int lane) {
+    const int row = lane & 15, side = lane >> 4;
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + gated_at(row, 2 * side + i)), "r"(w[4 * i]),
+                         "r"(w[4 * i + 1]), "r"(w[4 * i + 2]), "r"(w[4 * i + 3])
+                         : "memory");
+        __syncwarp();
+        const int i = lane >> 3, q = lane & 7, part = 8 * (lane & 1);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t from = box + gated_at(8 * (q >> 1 & 1) + 2 * i + (q & 1), 2 * h + (q >> 2));
+            uint4 o;
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(o.x), "=r"(o.y), "=r"(o.z), "=r"(o.w)
+                         : "r"(from)
+                         : "memory");
+            const int c = 8 * (2 * h + (lane >> 1 & 1)) + (lane >> 2);
+            if (c < cols) store8(to + c * ld + part, o, chans - part);
+        }
+        __syncwarp();
+    } else if (row < chans) {
+        to += row;
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+            if (16 * side + j < cols) to[(16 * side + j) * ld] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+    }
+}
+
 struct Tiles {
     int rt, ct, total;               // of rows, of columns
 };
@@ -371,7 +422,9 @@ struct Shape {
     static constexpr int SMEM = STAGES * STAGE + SMEM_BOXES + 512 + 1024;
 };
 
-template <typename T, bool A_MN, bool B_MN, int BN, int ACT>
+// GATED: operand A is two of N rows, 16 channels of the one and 16 of the other in turn, so that a warp's 32 TMEM lanes hold
+// both products of 16 channels and two exchanges of a register join them
+template <typename T, bool A_MN, bool B_MN, int BN, int ACT, bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, int nkb, int64_t R,
             int64_t C, Tiles tiles, const __grid_constant__ Epilogue e, unsigned spin, int stall) {
@@ -442,6 +495,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                         if constexpr (A_MN) {
 #pragma unroll
                             for (int i = 0; i < BM / 64; i++) tma_load_operand(ah + i * 8192, &tmA, r0 + i * 64, k, bar);
+                        } else if constexpr (GATED) {
+                            tma_load_gated(ah, &tmA, k, r0 / 32, bar);
                         } else {
                             tma_load_operand(ah, &tmA, k, r0, bar);
                         }
@@ -517,7 +572,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     } else if (warp == 1) {
         if (e.sums.parts)
             for (int64_t n = (int64_t)first * 32 + lane; n < e.sums.N; n += (int64_t)step * 32)
-                store_as(e.sums.db, n, e.sums.dtype, column_sum(e.sums, n));
+                store_sum(e.sums, n, column_sum(e.sums, n));
     } else if (warp >= 2) {
         const int half = (warp - 2) >> 2, quad = warp & 3;   // a warp reaches the TMEM lanes 32 (warp % 4) ..
         const uint32_t lanes = (uint32_t)(32 * quad) << 16, box = smem_u32(smem + STAGES * S::STAGE) + (warp - 2) * 2048;
@@ -529,12 +584,16 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             int tr, tc;
             tile_of(tiles, t, tr, tc);
             const int acc = i & 1;
-            const int64_t r0 = (int64_t)(tr * 2 + rank) * BM + quad * 32, c0 = (int64_t)tc * BN + half * (BN / 2);
-            const int chans = (int)min((int64_t)32, R - r0), cols = (int)min((int64_t)(BN / 2), C - c0);
+            const int64_t rows = (int64_t)(tr * 2 + rank) * BM + quad * 32, c0 = (int64_t)tc * BN + half * (BN / 2);
+            // the warp's first channel, how many it has (GATED: R counts channels, two rows of the tile each)
+            const int64_t r0 = GATED ? rows / 2 : rows;
+            const int chans = (int)min((int64_t)(GATED ? 16 : 32), R - r0), cols = (int)min((int64_t)(BN / 2), C - c0);
             const int count = chans > 0 && cols > 0 ? (cols + 31) / 32 : 0;
-            const bool mine = lane < chans;
-            const float scale = mine && e.scale ? e.scale[r0 + lane] * alpha : alpha;
-            const float bias = mine && e.bias ? load_as(e.bias, r0 + lane, e.bias_dtype) : 0.0f;
+            const int chan = GATED ? lane & 15 : lane;
+            const bool mine = chan < chans, up = GATED && lane >= 16;
+            const float scale = mine && e.scale ? e.scale[r0 + chan + (up ? e.half : 0)] * alpha : alpha;
+            const void *const offset = up ? e.bias2 : e.bias;
+            const float bias = mine && offset ? load_as(offset, r0 + chan, up ? e.bias2_dtype : e.bias_dtype) : 0.0f;
             // the residual of box b: as box_turn has it or, unaligned, the lane's channel in 32 columns
             uint32_t rnext[16];
             auto fetch = [&](int b) {
@@ -588,6 +647,26 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 }
 #pragma unroll
                 for (int j = 0; j < 32; j++) v[j] = fmaf(v[j], scale, bias);
+                if constexpr (GATED) {
+                    if (e.zf && mine) {
+                        float *to = e.zf + c * e.ldz + r0 + chan + (up ? e.half : 0);
+#pragma unroll
+                        for (int j = 0; j < 32; j++, to += e.ldz)
+                            if (j < left) *to = v[j];
+                    }
+                    // a lane of the gate's joins the first 16 columns, one of the other's the last
+                    float h[16];
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const float got = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[16 + j], 16);
+                        h[j] = activate<ACT>(up ? got : v[j]) * (up ? v[16 + j] : got);
+                    }
+                    uint32_t q[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) q[j] = pack2<T>(h[2 * j], h[2 * j + 1]);
+                    gated_out(box, q, static_cast<uint16_t *>(e.y) + c * e.ldy + r0, e.ldy, left, chans, e.vec, lane);
+                    continue;
+                }
                 if (z) {
 #pragma unroll
                     for (int j = 0; j < 16; j++) w[j] = kept2<ACT>(v[2 * j], v[2 * j + 1]);
@@ -705,10 +784,27 @@ bool rows_on16(const void *p, int64_t ld) {
     return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0);
 }
 
-template <typename T, bool A_MN, bool B_MN, int BN, int ACT>
+// The two operands of a gated product, N rows each (Np apart, a multiple of 16), as one of four dimensions: a box has 64 of
+// the contraction, 16 rows, both operands, 4 groups of 16 rows.  The rows' order in shared memory is that of the box.
+int gated_map(CUtensorMap *map, const void *base, int dtype, int64_t Np, int64_t cols, int64_t ld) {
+    EncodeTiled enc = encoder();
+    if (!enc) return set_error(SFB_ECUDA, "sf gated product: cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t dims[4] = {(cuuint64_t)cols, 16, 2, (cuuint64_t)(Np / 16)};
+    const cuuint64_t strides[3] = {(cuuint64_t)ld * 2, (cuuint64_t)(Np * ld) * 2, (cuuint64_t)ld * 32};
+    const cuuint32_t box[4] = {64, 16, 2, 4};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = enc(map, dtype == SFB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                           4, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(SFB_ECUDA, "sf gated product: tensor map encoding failed (%d)", (int)r);
+    return SFB_OK;
+}
+
+template <typename T, bool A_MN, bool B_MN, int BN, int ACT, bool GATED>
 int launch(const Problem &p, Epilogue e, cudaStream_t st) {
     using S = Shape<BN>;
-    auto *kernel = gemm_kernel<T, A_MN, B_MN, BN, ACT>;
+    auto *kernel = gemm_kernel<T, A_MN, B_MN, BN, ACT, GATED>;
     static std::mutex lock;
     static unsigned long long ready[64] = {};          // the CUDA context whose attribute is set, per device
     int dev = 0;
@@ -725,13 +821,16 @@ int launch(const Problem &p, Epilogue e, cudaStream_t st) {
     }
     e.vec = (e.y_dtype == SFB_F32 || rows_on16(e.y, e.ldy)) && rows_on16(e.z, e.ldz) && rows_on16(e.residual, e.ldr);
     CUtensorMap tmA, tmB;
-    int rc = A_MN ? operand_map(&tmA, p.A, p.dtype, p.K, p.R, p.lda, 64) : operand_map(&tmA, p.A, p.dtype, p.R, p.K, p.lda, BM);
+    int rc = GATED  ? gated_map(&tmA, p.A, p.dtype, e.half, p.K, p.lda)
+             : A_MN ? operand_map(&tmA, p.A, p.dtype, p.K, p.R, p.lda, 64)
+                    : operand_map(&tmA, p.A, p.dtype, p.R, p.K, p.lda, BM);
     if (!rc)
         rc = B_MN ? operand_map(&tmB, p.B, p.dtype, p.K, p.C, p.ldb, 64)
                   : operand_map(&tmB, p.B, p.dtype, p.C, p.K, p.ldb, S::BNL);
     if (rc) return rc;
     Tiles t;
-    t.rt = (int)((p.R + 2 * BM - 1) / (2 * BM));
+    const int64_t lines = GATED ? 2 * e.half : p.R;                    // rows of operand A
+    t.rt = (int)((lines + 2 * BM - 1) / (2 * BM));
     t.ct = (int)((p.C + BN - 1) / BN);
     t.total = t.rt * t.ct;
     kernel<<<2 * std::min(t.total, sm_count() / 2), THREADS, S::SMEM, st>>>(
@@ -755,13 +854,13 @@ int columns(int64_t R, int64_t C) {
     return 512 * wide <= 390 * narrow ? 256 : 128;
 }
 
-template <bool A_MN, bool B_MN, int ACT>
+template <bool A_MN, bool B_MN, int ACT, bool GATED = false>
 int launch_typed(const Problem &p, const Epilogue &e, cudaStream_t st) {
-    const bool wide = columns(p.R, p.C) == 256;
+    const bool wide = columns(GATED ? 2 * e.half : p.R, p.C) == 256;
     if (p.dtype == SFB_BF16)
-        return wide ? launch<__nv_bfloat16, A_MN, B_MN, 256, ACT>(p, e, st)
-                    : launch<__nv_bfloat16, A_MN, B_MN, 128, ACT>(p, e, st);
-    return wide ? launch<__half, A_MN, B_MN, 256, ACT>(p, e, st) : launch<__half, A_MN, B_MN, 128, ACT>(p, e, st);
+        return wide ? launch<__nv_bfloat16, A_MN, B_MN, 256, ACT, GATED>(p, e, st)
+                    : launch<__nv_bfloat16, A_MN, B_MN, 128, ACT, GATED>(p, e, st);
+    return wide ? launch<__half, A_MN, B_MN, 256, ACT, GATED>(p, e, st) : launch<__half, A_MN, B_MN, 128, ACT, GATED>(p, e, st);
 }
 
 }  // namespace
@@ -783,6 +882,26 @@ int tensor_product(int dtype, const void *x, int64_t ldx, const void *codes, int
     e.ldz = ldz;
     e.ldy = ldy;
     return with_activation(act, [&](auto a) { return launch_typed<false, false, decltype(a)::value>(p, e, st); });
+}
+
+int tensor_gated_product(int dtype, const void *x, int64_t ldx, const void *codes, int64_t ldw, const float *scale, int bits,
+                         const void *bias, int bias_dtype, const void *bias2, int bias2_dtype, int act, void *y, int64_t ldy,
+                         float *z, int64_t ldz, int64_t M, int64_t N, int64_t Np, int64_t K, cudaStream_t st) {
+    const Problem p{codes, x, ldw, ldx, N, M, K, dtype};
+    Epilogue e{};
+    e.scale = scale;
+    e.bias = bias;
+    e.bias2 = bias2;
+    e.half = Np;
+    e.zf = z;
+    e.y = y;
+    e.unit = 1.0f / (float)(1 << (bits - 1));
+    e.bias_dtype = bias_dtype;
+    e.bias2_dtype = bias2_dtype;
+    e.y_dtype = dtype;
+    e.ldz = ldz;
+    e.ldy = ldy;
+    return with_activation(act, [&](auto a) { return launch_typed<false, false, decltype(a)::value, true>(p, e, st); });
 }
 
 int tensor_grad_x(int dtype, const void *dzs, int64_t ldd, const void *codes, int64_t ldw, const float *top, int bits,

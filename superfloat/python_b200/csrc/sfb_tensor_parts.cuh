@@ -16,7 +16,17 @@ struct Sums {
     int64_t count, N;
     void *db;
     int dtype;
+    // of a gated product: columns from `half` on are the second bias's, each of the two having `width`; else half is 0
+    void *db2;
+    int dtype2;
+    int64_t half, width;
 };
+
+__device__ __forceinline__ void store_sum(const Sums &s, int64_t n, float v) {
+    if (s.half == 0) store_as(s.db, n, s.dtype, v);
+    else if (n < s.width && s.db) store_as(s.db, n, s.dtype, v);
+    else if (n >= s.half && n - s.half < s.width && s.db2) store_as(s.db2, n - s.half, s.dtype2, v);
+}
 
 __device__ __forceinline__ float column_sum(const Sums &s, int64_t n) {
     float v[32] = {};
@@ -45,6 +55,11 @@ struct Rows {
 int tensor_quantize(const void *w, int dtype, int64_t N, int64_t K, int64_t ldw, int bits, bool per_channel, void *codes,
                     int64_t ldc, int codes_dtype, float *scale, void *work, const Rows &rows,
                     cudaStream_t st);
+// the same of two weights of N rows, the second one's codes and scales Np rows on; rows between are zeros of scale 1
+// (work: 8 N bytes)
+int tensor_quantize2(const void *w, int64_t ldw, const void *w2, int64_t ldw2, int dtype, int64_t N, int64_t Np, int64_t K,
+                     int bits, bool per_channel, void *codes, int64_t ldc, int codes_dtype, float *scale, void *work,
+                     const Rows &rows, cudaStream_t st);
 // packed codes as the products' operand, and in the same launch a copy of `rows`, if any
 int tensor_expand(const int8_t *codes, int64_t N, int64_t K, int64_t ldc, void *out, int64_t ldo, int dtype,
                   const Rows &rows, cudaStream_t st);
@@ -56,6 +71,14 @@ int tensor_small(int dtype, const void *x, int64_t ldx, const int8_t *codes, int
 int tensor_product(int dtype, const void *x, int64_t ldx, const void *codes, int64_t ldw, const float *scale, int bits,
                    const void *bias, int bias_dtype, int act, const void *residual, int64_t ldr, void *y, int64_t ldy,
                    void *z, int64_t ldz, int64_t M, int64_t N, int64_t K, cudaStream_t st);
+// act(gate) up of the two products, codes (2 Np rows) as tensor_quantize2 leaves them; z (nullable): both products, 2 Np float32 a row
+int tensor_gated_product(int dtype, const void *x, int64_t ldx, const void *codes, int64_t ldw, const float *scale, int bits,
+                         const void *bias, int bias_dtype, const void *bias2, int bias2_dtype, int act, void *y, int64_t ldy,
+                         float *z, int64_t ldz, int64_t M, int64_t N, int64_t Np, int64_t K, cudaStream_t st);
+int tensor_gated_small(int dtype, const void *x, int64_t ldx, const int8_t *gate, int64_t ldg, const float *gate_scale,
+                       const int8_t *up, int64_t ldu, const float *up_scale, int bits, const void *bias, int bias_dtype,
+                       const void *bias2, int bias2_dtype, int act, void *y, int64_t ldy, int64_t M, int64_t N, int64_t K,
+                       cudaStream_t st);
 int64_t tensor_slope_parts(int64_t M);          // rows of partial sums
 int tensor_slope(int dtype, int act, const void *dy, int64_t ldy, const void *z, int64_t ldz, int64_t M, int64_t N,
                  const float *scale, int bits, const float *top, void *dz, void *dzs, int64_t ldd, float *sums,

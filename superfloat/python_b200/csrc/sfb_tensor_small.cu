@@ -134,6 +134,11 @@ struct Small {
     const int8_t *codes;
     const float *scale;
     const void *bias, *residual;
+    const int8_t *codes2;                      // of a gated product: the up half's
+    const float *scale2;
+    const void *bias2;
+    int64_t ldc2;
+    int bias2_dtype;
     void *y;
     int64_t ldx, ldc, ldr, ldy, N, K;
     float unit;
@@ -146,7 +151,8 @@ constexpr int DEEP = 4;
 // in the loop (the questions are half of its instructions); ON16, rows on 16 bytes; ANY.
 enum { WHOLE, ON16, ANY };
 
-template <typename T, int MT, int LIE, int ACT>
+// GATED: the 16 rows of a group are 8 channels of the gate and the same 8 of the other weight
+template <typename T, int MT, int LIE, int ACT, bool GATED>
 __global__ void __launch_bounds__(32 * WARPS, MT <= 2 ? 4 : MT == 4 ? 3 : 2) small_kernel(Small p) {
     __shared__ union {
         uint4 codes[DEEP][2][32 * WARPS];
@@ -154,9 +160,10 @@ __global__ void __launch_bounds__(32 * WARPS, MT <= 2 ? 4 : MT == 4 ? 3 : 2) sma
     } s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int groups = WARPS / p.ks, group = warp / p.ks, part = warp % p.ks;
-    const int64_t n0 = ((int64_t)blockIdx.x * groups + group) * 16;
+    constexpr int CHANS = GATED ? 8 : 16;      // channels of a group
+    const int64_t n0 = ((int64_t)blockIdx.x * groups + group) * CHANS;
     // channels past the last read the last one's codes, rows past the last the last one: their sums are not stored
-    const int8_t *row0 = p.codes + min(n0 + g, p.N - 1) * p.ldc, *row1 = p.codes + min(n0 + g + 8, p.N - 1) * p.ldc;
+    const int8_t *row0 = p.codes + min(n0 + g, p.N - 1) * p.ldc, *row1 = GATED ? p.codes2 + min(n0 + g, p.N - 1) * p.ldc2 : p.codes + min(n0 + g + 8, p.N - 1) * p.ldc;
     const T *x[MT];
 #pragma unroll
     for (int i = 0; i < MT; i++) x[i] = static_cast<const T *>(p.x) + (int64_t)min(i * 8 + g, p.M - 1) * p.ldx;
@@ -221,42 +228,57 @@ __global__ void __launch_bounds__(32 * WARPS, MT <= 2 ? 4 : MT == 4 ? 3 : 2) sma
         s.sum[warp][g + 8][i * 8 + 2 * t + 1] = d[i][3];
     }
     __syncthreads();
-    for (int o = threadIdx.x; o < groups * 16 * p.M; o += 32 * WARPS) {
-        const int c = o % (groups * 16), m = o / (groups * 16);
-        const int64_t n = (int64_t)blockIdx.x * groups * 16 + c;
+    for (int o = threadIdx.x; o < groups * CHANS * p.M; o += 32 * WARPS) {
+        const int c = o % (groups * CHANS), m = o / (groups * CHANS);
+        const int64_t n = (int64_t)blockIdx.x * groups * CHANS + c;
         if (n >= p.N) continue;
         float v = 0.0f;
-        for (int i = 0; i < p.ks; i++) v += s.sum[(c / 16) * p.ks + i][c % 16][m];
+        for (int i = 0; i < p.ks; i++) v += s.sum[(c / CHANS) * p.ks + i][c % CHANS][m];
         v = fmaf(v, p.scale[n] * p.unit, p.bias ? load_as(p.bias, n, p.bias_dtype) : 0.0f);
         v = activate<ACT>(v);
+        if constexpr (GATED) {
+            float u = 0.0f;
+            for (int i = 0; i < p.ks; i++) u += s.sum[(c / CHANS) * p.ks + i][c % CHANS + 8][m];
+            v *= fmaf(u, p.scale2[n] * p.unit, p.bias2 ? load_as(p.bias2, n, p.bias2_dtype) : 0.0f);
+        }
         if (p.residual) v += to_f(static_cast<const T *>(p.residual)[m * p.ldr + n]);
         static_cast<T *>(p.y)[m * p.ldy + n] = from_f<T>(v);
     }
 }
 
-template <typename T, int MT, int LIE>
+template <typename T, int MT, int LIE, bool GATED>
 int launch(const Small &p, int act, cudaStream_t st) {
-    const int64_t groups = (p.N + 15) / 16;
+    const int64_t groups = GATED ? (p.N + 7) / 8 : (p.N + 15) / 16;
     const int per = WARPS / p.ks;
     const unsigned grid = (unsigned)((groups + per - 1) / per);
     return with_activation(act, [&](auto a) {
-        small_kernel<T, MT, LIE, decltype(a)::value><<<grid, 32 * WARPS, 0, st>>>(p);
+        small_kernel<T, MT, LIE, decltype(a)::value, GATED><<<grid, 32 * WARPS, 0, st>>>(p);
         return check_launch("sf tensor linear (few rows)");
     });
 }
 
-template <typename T, int MT>
+bool on16(const int8_t *p, int64_t ld) { return p == nullptr || (ld % 16 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0); }
+
+template <typename T, int MT, bool GATED>
 int by_lie(const Small &p, int act, cudaStream_t st) {
-    if (p.ldc % 16 || (reinterpret_cast<uintptr_t>(p.codes) & 15)) return launch<T, MT, ANY>(p, act, st);
-    return p.K % SEG ? launch<T, MT, ON16>(p, act, st) : launch<T, MT, WHOLE>(p, act, st);
+    if (!on16(p.codes, p.ldc) || !on16(p.codes2, p.ldc2)) return launch<T, MT, ANY, GATED>(p, act, st);
+    return p.K % SEG ? launch<T, MT, ON16, GATED>(p, act, st) : launch<T, MT, WHOLE, GATED>(p, act, st);
 }
 
-template <typename T>
+template <typename T, bool GATED>
 int by_rows(const Small &p, int act, cudaStream_t st) {
-    if (p.M <= 8) return by_lie<T, 1>(p, act, st);
-    if (p.M <= 16) return by_lie<T, 2>(p, act, st);
-    if (p.M <= 32) return by_lie<T, 4>(p, act, st);
-    return by_lie<T, 6>(p, act, st);
+    if (p.M <= 8) return by_lie<T, 1, GATED>(p, act, st);
+    if (p.M <= 16) return by_lie<T, 2, GATED>(p, act, st);
+    if (p.M <= 32) return by_lie<T, 4, GATED>(p, act, st);
+    return by_lie<T, 6, GATED>(p, act, st);
+}
+
+// warps that share a group of channels: as many as fill the SMs, each with two segments at least
+int share(int64_t groups, int64_t K) {
+    const int64_t segs = (K + SEG - 1) / SEG;
+    int ks = 8;
+    while (ks > 1 && (segs < 2 * ks || groups * ks > 32ll * sm_count())) ks /= 2;
+    return ks;
 }
 
 }  // namespace
@@ -264,12 +286,51 @@ int by_rows(const Small &p, int act, cudaStream_t st) {
 int tensor_small(int dtype, const void *x, int64_t ldx, const int8_t *codes, int64_t ldc, const float *scale, int bits,
                  const void *bias, int bias_dtype, int act, const void *residual, int64_t ldr, void *y, int64_t ldy,
                  int64_t M, int64_t N, int64_t K, cudaStream_t st) {
-    Small p{x, codes, scale, bias, residual, y, ldx, ldc, ldr, ldy, N, K, 1.0f / (float)(1 << (bits - 1)), (int)M, 8,
-            bias_dtype};
-    // warps that share a group of channels: as many as fill the SMs, each with two segments at least
-    const int64_t groups = (N + 15) / 16, segs = (K + SEG - 1) / SEG;
-    while (p.ks > 1 && (segs < 2 * p.ks || groups * p.ks > 32ll * sm_count())) p.ks /= 2;
-    return dtype == SFB_BF16 ? by_rows<__nv_bfloat16>(p, act, st) : by_rows<__half>(p, act, st);
+    Small p{};
+    p.x = x;
+    p.codes = codes;
+    p.scale = scale;
+    p.bias = bias;
+    p.residual = residual;
+    p.y = y;
+    p.ldx = ldx;
+    p.ldc = ldc;
+    p.ldr = ldr;
+    p.ldy = ldy;
+    p.N = N;
+    p.K = K;
+    p.unit = 1.0f / (float)(1 << (bits - 1));
+    p.M = (int)M;
+    p.bias_dtype = bias_dtype;
+    p.ks = share((N + 15) / 16, K);
+    return dtype == SFB_BF16 ? by_rows<__nv_bfloat16, false>(p, act, st) : by_rows<__half, false>(p, act, st);
+}
+
+int tensor_gated_small(int dtype, const void *x, int64_t ldx, const int8_t *gate, int64_t ldg, const float *gate_scale,
+                       const int8_t *up, int64_t ldu, const float *up_scale, int bits, const void *bias, int bias_dtype,
+                       const void *bias2, int bias2_dtype, int act, void *y, int64_t ldy, int64_t M, int64_t N, int64_t K,
+                       cudaStream_t st) {
+    Small p{};
+    p.x = x;
+    p.codes = gate;
+    p.codes2 = up;
+    p.scale = gate_scale;
+    p.scale2 = up_scale;
+    p.bias = bias;
+    p.bias2 = bias2;
+    p.y = y;
+    p.ldx = ldx;
+    p.ldc = ldg;
+    p.ldc2 = ldu;
+    p.ldy = ldy;
+    p.N = N;
+    p.K = K;
+    p.unit = 1.0f / (float)(1 << (bits - 1));
+    p.M = (int)M;
+    p.bias_dtype = bias_dtype;
+    p.bias2_dtype = bias2_dtype;
+    p.ks = share((N + 7) / 8, K);
+    return dtype == SFB_BF16 ? by_rows<__nv_bfloat16, true>(p, act, st) : by_rows<__half, true>(p, act, st);
 }
 
 }  // namespace sfb

@@ -25,6 +25,7 @@ from ._core import weight_cache  # noqa: F401
 from ._distill import distill_loss
 from ._modules import (ConversionReport, SFConfig, SFConv2d, SFHFConv1D, SFLinear, SFPackedLinear, conversion_report,
                        convert, find_lm_heads, is_hf_conv1d, pack)
+from ._gated import tensor_gated
 from ._norm import layer_norm
 from ._optim import AdamW, SF8Moment, adamw_step, moment_values
 from ._status import SFLayerStatus, capture_status, last_status, reset_status
@@ -75,4 +76,5 @@ __all__ = ["quantize", "linear", "matmul", "SFLinear", "SFConv2d", "SFHFConv1D",
            "find_lm_heads", "is_hf_conv1d", "conversion_report", "ConversionReport", "last_status",
            "reset_status", "capture_status", "SFLayerStatus", "compile_report", "compile_reports", "GraphReport",
            "SFPackedLinear", "pack", "SFPackedWeight", "pack_weight", "tensor_linear", "tensor_failures",
-           "AdamW", "SF8Moment", "adamw_step", "moment_values", "layer_norm", "distill_loss"]
+           "AdamW", "SF8Moment", "adamw_step", "moment_values", "tensor_gated", "layer_norm",
+           "distill_loss"]

@@ -15,7 +15,7 @@ from superfloat.python_b200._errors import SFShapeError
 from superfloat.python_b200.torch._distill import _like, _strides_of, _two_strides
 
 
-@pytest.mark.parametrize("name,fields", [("norm", _lib.NORM_CALL), ("distill", _lib.DISTILL_CALL)])
+@pytest.mark.parametrize("name,fields", [("norm", _lib.NORM_CALL), ("distill", _lib.DISTILL_CALL), ("gated", _lib.GATED_CALL)])
 def test_the_call_structs_are_the_headers(name, fields):
     """Python fills the structs as arrays of 8-byte words: the header's fields in the header's order, none shorter."""
     text = open(os.path.join(REPO, "include", "sfb200.h")).read()
