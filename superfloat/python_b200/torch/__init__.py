@@ -23,8 +23,8 @@ from . import _ops  # noqa: F401  (registers the sf:: custom ops)
 from ._backend import GraphReport, compile_report, compile_reports, superfloat  # noqa: F401
 from ._core import weight_cache  # noqa: F401
 from ._distill import distill_loss
-from ._modules import (ConversionReport, SFConfig, SFConv2d, SFHFConv1D, SFLinear, SFPackedLinear, conversion_report,
-                       convert, find_lm_heads, is_hf_conv1d, pack)
+from ._modules import (ConversionReport, SFConfig, SFConv2d, SFGatedFeedForward, SFHFConv1D, SFLayerNorm, SFLinear,
+                       SFPackedGatedFeedForward, SFPackedLinear, conversion_report, convert, find_lm_heads, is_hf_conv1d, pack)
 from ._gated import tensor_gated
 from ._norm import layer_norm
 from ._optim import AdamW, SF8Moment, adamw_step, moment_values
@@ -75,6 +75,6 @@ def matmul(a, b, dtype="sf16", headroom="bound", name="matmul", *, accumulate="c
 __all__ = ["quantize", "linear", "matmul", "SFLinear", "SFConv2d", "SFHFConv1D", "SFConfig", "convert",
            "find_lm_heads", "is_hf_conv1d", "conversion_report", "ConversionReport", "last_status",
            "reset_status", "capture_status", "SFLayerStatus", "compile_report", "compile_reports", "GraphReport",
-           "SFPackedLinear", "pack", "SFPackedWeight", "pack_weight", "tensor_linear", "tensor_failures",
-           "AdamW", "SF8Moment", "adamw_step", "moment_values", "tensor_gated", "layer_norm",
-           "distill_loss"]
+           "SFPackedLinear", "SFGatedFeedForward", "SFPackedGatedFeedForward", "SFLayerNorm", "pack", "SFPackedWeight",
+           "pack_weight", "tensor_linear", "tensor_failures", "AdamW", "SF8Moment", "adamw_step", "moment_values",
+           "tensor_gated", "layer_norm", "distill_loss"]

@@ -50,8 +50,9 @@ def _check(logits, teacher, index, temperature, weight, reduction):
                               f"supported")
         if weight.requires_grad:
             raise SFTypeError("distill_loss: the rows' weights have no gradient; pass them detached")
+    at = logits.get_device()
     for t, name in ((teacher, "teacher's logits"), (index, "teacher's indexes"), (weight, "rows' weights")):
-        if t is not None and t.device != logits.device:
+        if t is not None and t.get_device() != at:
             raise SFShapeError(f"distill_loss: the {name} are on {t.device}, the logits on {logits.device}")
     if teacher.requires_grad and torch.is_grad_enabled():
         raise SFTypeError("distill_loss: the teacher's logits have no gradient; pass them detached")
@@ -61,6 +62,8 @@ def _two_strides(t):
     """(t, rows of the inner dimension, outer stride, inner stride): t's rows as at most two nested runs of rows whose
     elements are contiguous, copied where they are not."""
     V = t.shape[-1]
+    if t.is_contiguous():
+        return t, max(1, t.numel() // V), 0, V
     if t.stride(-1) == 1 or V == 1:
         runs = []                                     # (size, stride), the innermost first; runs that follow on join
         for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
@@ -79,9 +82,10 @@ def _two_strides(t):
 def _like(t):
     """An empty tensor for t's gradient: laid out as t where that wastes at most a quarter, so that the rows of both lie
     alike on 16 bytes, else compact."""
-    size, at = t.element_size(), t.storage_offset()
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return torch.empty_like(t)
     span = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    lead = t.data_ptr() % 16 // size
+    lead = t.data_ptr() % 16 // t.element_size()
     # every stride covers what lies inside it: no two elements share a place
     inside, apart = 1, True
     for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
@@ -109,10 +113,8 @@ def _call(logits, teacher, index, weight, temperature, reduction):
 
 def _strides_of(grad, logits):
     """The gradient's strides by the logits' two runs of rows."""
-    if grad.stride() == logits.stride():
-        return _two_strides(logits)[2:]
-    inner, V = _two_strides(logits)[1], logits.shape[-1]
-    return inner * V, V
+    _, inner, so, si = _two_strides(logits)
+    return (so, si) if grad.stride() == logits.stride() else (inner * logits.shape[-1], logits.shape[-1])
 
 
 def _kept_at(kept, words, keep):

@@ -17,7 +17,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import _core, _tensor
+from . import _core, _gated, _norm, _tensor
 from ._ops import call_linear
 
 
@@ -179,6 +179,93 @@ class SFConv2d(nn.Module):
                 f"padding={self.padding}, {self.sf.describe()}, name={self.sf_name!r}")
 
 
+class SFLayerNorm(nn.Module):
+    """``nn.LayerNorm`` over the last dimension on the B200's own kernel (:func:`layer_norm`); its parameters are the
+    source's."""
+
+    def __init__(self, norm: nn.LayerNorm):
+        super().__init__()
+        if len(norm.normalized_shape) != 1:
+            raise ValueError(f"normalized_shape={tuple(norm.normalized_shape)} (only the last dimension is converted)")
+        self.normalized_shape, self.eps = tuple(norm.normalized_shape), norm.eps
+        self.weight, self.bias = norm.weight, norm.bias
+        self.train(norm.training)
+
+    def forward(self, x):
+        if x.shape[-1:] != self.normalized_shape:
+            from .._errors import SFShapeError
+            raise SFShapeError(f"the input has shape {tuple(x.shape)}, the norm is over {self.normalized_shape[0]} features")
+        return _norm.layer_norm(x, self.weight, self.bias, self.eps)
+
+    def extra_repr(self):
+        return f"{self.normalized_shape}, eps={self.eps}, weight={self.weight is not None}, bias={self.bias is not None}"
+
+
+# activation modules by class name (torch's and Hugging Face's; transformers is never imported)
+_GATES = {"SiLU": "silu", "SiLUActivation": "silu", "ReLU": "relu", "GELUActivation": "gelu", "PytorchGELUTanh": "gelu_tanh",
+          "GELUTanh": "gelu_tanh"}
+
+
+def _gate_activation(act):
+    if isinstance(act, nn.GELU):
+        return "gelu_tanh" if act.approximate == "tanh" else "gelu"
+    return _GATES.get(type(act).__name__)
+
+
+def gated_block(m: nn.Module):
+    """(activation, "") of a gated feed-forward block that :class:`SFGatedFeedForward` can stand for, (None, "") of another
+    module, (None, why) of a block that it cannot.  A block is recognised by its children (``gate_proj``, ``up_proj``,
+    ``down_proj``, ``act_fn``) and by what it computes on two rows."""
+    parts = [m._modules.get(n) for n in ("gate_proj", "up_proj", "down_proj")]
+    if not all(isinstance(p, nn.Linear) for p in parts):
+        return None, ""
+    gate, up, down = parts
+    if any(_custom_forward(p, nn.Linear) for p in parts):
+        return None, "a projection has a forward of its own"
+    act = _gate_activation(getattr(m, "act_fn", None))
+    if act is None:
+        return None, f"activation {type(getattr(m, 'act_fn', None)).__name__}"
+    if set(m._modules) - {"gate_proj", "up_proj", "down_proj", "act_fn"}:
+        return None, "it has other children"
+    if gate.weight.shape != up.weight.shape or gate.weight.dtype != up.weight.dtype:
+        return None, "its first two projections differ in shape or type"
+    if gate.weight.is_meta:
+        return None, "its weights are on the meta device"
+    with torch.no_grad():
+        x = torch.linspace(-2, 2, 2 * gate.in_features, device=gate.weight.device).view(2, -1).to(gate.weight.dtype)
+        try:
+            same = torch.equal(m(x), down(m.act_fn(gate(x)) * up(x)))
+        except Exception as e:  # noqa: BLE001  (a model's own forward may raise)
+            return None, f"its forward did not run on two rows ({type(e).__name__})"
+    return (act, "") if same else (None, "it computes something else than down(act(gate(x)) * up(x))")
+
+
+class SFGatedFeedForward(nn.Module):
+    """A gated feed-forward block ``down(act(gate(x)) * up(x))`` with SF arithmetic on the tensor cores: the first two
+    projections and their product are one operator (:func:`tensor_gated`), the last is an SF linear layer.  The
+    children and their parameters are the source's."""
+
+    def __init__(self, block: nn.Module, name: str, cfg: SFConfig, down: SFConfig | None = None):
+        super().__init__()
+        if cfg.accumulate != "tensor":
+            raise ValueError("a gated block is one operator with accumulate=\"tensor\" only")
+        self.activation, why = gated_block(block)
+        if self.activation is None:
+            raise ValueError(why or "not a gated feed-forward block")
+        self.sf, self.sf_name = cfg, name
+        self.gate_proj, self.up_proj, self.act_fn = block.gate_proj, block.up_proj, block.act_fn
+        self.down_proj = SFLinear.from_float(block.down_proj, f"{name}.down_proj" if name else "down_proj", down or cfg)
+        self.train(block.training)
+
+    def forward(self, x):
+        gate, up = self.gate_proj, self.up_proj
+        return self.down_proj(_gated.tensor_gated(x, gate.weight, up.weight, gate.bias, up.bias, activation=self.activation,
+                                                  dtype=self.sf.bits, scale=self.sf.scale))
+
+    def extra_repr(self):
+        return f"activation={self.activation}, {self.sf.describe()}, name={self.sf_name!r}"
+
+
 @dataclass
 class ConversionReport:
     converted: list = field(default_factory=list)     # (name, kind)
@@ -276,7 +363,8 @@ class _Converter:
     replaces it, the report.  A module reached twice (a shared submodule) is
     replaced once and the alias recorded."""
 
-    def __init__(self, cfg, cfg16, per_layer, keep_ids, keep_names):
+    def __init__(self, cfg, cfg16, per_layer, keep_ids, keep_names, fuse=False):
+        self.fuse = fuse                        # gated blocks and layer norms as one operator each
         self.cfg, self.cfg16 = cfg, cfg16
         self.per_layer = per_layer              # path -> SFConfig (widths=)
         self.keep_ids, self.keep_names = keep_ids, keep_names
@@ -301,7 +389,11 @@ class _Converter:
     def _make(self, module, path):
         """(SF replacement or None, whether the module is a leaf of the walk)."""
         kind = type(module).__name__
-        if isinstance(module, (SFLinear, SFConv2d, SFHFConv1D)):
+        if self.fuse:
+            made = self._fused(module, path, kind)
+            if made is not None:
+                return made, True
+        if isinstance(module, (SFLinear, SFConv2d, SFHFConv1D, SFGatedFeedForward)):
             self.report.converted.append((path, kind + " (already SF)"))
             return None, True
         if isinstance(module, nn.Linear):
@@ -330,6 +422,29 @@ class _Converter:
             self._skip(path, kind, "no SF version here; runs in float")
             return None, True
         return None, False                      # a container: walk into it
+
+    def _fused(self, module, path, kind):
+        """A layer norm's or gated block's replacement, or None: the module is looked at as any other then."""
+        if isinstance(module, nn.LayerNorm):
+            if _custom_forward(module, nn.LayerNorm):
+                self._skip(path, kind, f"a subclass of nn.LayerNorm with its own forward ({kind}); runs as it was")
+            elif len(module.normalized_shape) != 1:
+                self._skip(path, kind, f"normalized_shape={tuple(module.normalized_shape)}; runs as it was")
+            else:
+                self.report.converted.append((path, "LayerNorm"))
+                return SFLayerNorm(module)
+            return None
+        act, why = gated_block(module)
+        at = [f"{path}.{n}" if path else n for n in ("gate_proj", "up_proj", "down_proj")]
+        if act and len({self.per_layer.get(p, self.cfg).bits for p in at[:2]}) > 1:
+            act, why = None, "its first two projections are given two widths"
+        if act is None:
+            if why:
+                self._skip(path, kind, f"not one operator: {why}; its layers are converted one by one")
+            return None
+        cfg, _, down = (self.config_for(module._modules[n], p) for n, p in zip(("gate_proj", "up_proj", "down_proj"), at))
+        self.report.converted.append((path, "gated feed-forward"))
+        return SFGatedFeedForward(module, path, cfg, down)
 
     def replace(self, module, path):
         seen = self.replaced.get(id(module))
@@ -396,17 +511,39 @@ class SFPackedLinear(nn.Module):
                 f"dtype=sf{self.bits}, name={self.sf_name!r}")
 
 
+class SFPackedGatedFeedForward(nn.Module):
+    """A :class:`SFGatedFeedForward` laid out once for serving: three packed projections, of which the first two and their
+    product are one operator."""
+
+    def __init__(self, gate: SFPackedLinear, up: SFPackedLinear, down: nn.Module, activation: str, name: str = ""):
+        super().__init__()
+        self.gate_proj, self.up_proj, self.down_proj = gate, up, down
+        self.activation, self.sf_name = activation, name
+
+    def forward(self, x):
+        gate, up = (_tensor.SFPackedWeight(p.codes, p.scale, p.bits) for p in (self.gate_proj, self.up_proj))
+        return self.down_proj(_gated.tensor_gated(x, gate, up, self.gate_proj.bias, self.up_proj.bias,
+                                                  activation=self.activation))
+
+    def extra_repr(self):
+        return f"activation={self.activation}, name={self.sf_name!r}"
+
+
 def pack(model: nn.Module, inplace: bool = False) -> nn.Module:
     """Replace the SF linear layers of accumulate="tensor" (SFLinear, SFHFConv1D)
-    by :class:`SFPackedLinear`: their weights' codes are made once, and a weight
-    takes one byte an element.  Other layers stay as they are; a layer that the
-    model reaches twice is packed once."""
+    by :class:`SFPackedLinear`, and their gated blocks by :class:`SFPackedGatedFeedForward`:
+    the weights' codes are made once, and a weight takes one byte an element.  Other
+    layers stay as they are; a layer that the model reaches twice is packed once."""
     if not inplace:
         model = copy.deepcopy(model)
     done = {}
 
     def packed(m):
-        if id(m) not in done:
+        if id(m) not in done and isinstance(m, SFGatedFeedForward):
+            gate, up = (SFPackedLinear(_tensor.pack_weight(p.weight, m.sf.bits, m.sf.scale), p.bias, f"{m.sf_name}.{n}")
+                        for p, n in ((m.gate_proj, "gate_proj"), (m.up_proj, "up_proj")))
+            done[id(m)] = (m, SFPackedGatedFeedForward(gate, up, packed(m.down_proj), m.activation, m.sf_name).train(m.training))
+        elif id(m) not in done:
             w = m.weight.t() if isinstance(m, SFHFConv1D) else m.weight
             p = _tensor.pack_weight(w, m.sf.bits, m.sf.scale)
             # (the layer itself is kept, so that its id stays its own)
@@ -414,7 +551,7 @@ def pack(model: nn.Module, inplace: bool = False) -> nn.Module:
         return done[id(m)][1]
 
     def wanted(m):
-        return isinstance(m, (SFLinear, SFHFConv1D)) and m.sf.accumulate == "tensor"
+        return isinstance(m, (SFLinear, SFHFConv1D, SFGatedFeedForward)) and m.sf.accumulate == "tensor"
 
     if wanted(model):
         return packed(model)
@@ -442,13 +579,18 @@ def _keep_plan(model, keep_sf16, bits):
 def convert(model: nn.Module, dtype="sf16", scale: str = "per_tensor", headroom: str = "bound",
             inplace: bool = False, *, accumulate: str = "chain", shift=None, calibration: str = "heuristic",
             keep_sf16="auto", attention="auto", nonlinear: str = "float",
-            widths: dict | None = None) -> nn.Module:
+            widths: dict | None = None, fuse: bool = False) -> nn.Module:
     """Swap ``nn.Linear``, ``nn.Conv2d`` and Hugging Face ``Conv1D`` for SF
     layers (src/sf/torch/_modules.py:295-537).  ``keep_sf16`` ("auto": the LM
     head; False; or module names) keeps layers at sf16 when ``dtype`` is
     narrower; ``widths`` ({name: dtype}) gives layers their own width.
     ``accumulate="tensor"`` runs the layers on the tensor cores, for a model in
-    bfloat16 or float16; it ends at sf8, so "auto" keeps nothing there."""
+    bfloat16 or float16; it ends at sf8, so "auto" keeps nothing there.  ``fuse`` (with
+    accumulate="tensor") also swaps gated feed-forward blocks, down(act(gate(x)) *
+    up(x)) over children of these names, and ``nn.LayerNorm`` for modules that are one
+    operator each (:class:`SFGatedFeedForward`, :class:`SFLayerNorm`)."""
+    if fuse and accumulate != "tensor":
+        raise ValueError("fuse=True is for accumulate=\"tensor\"")
     if calibration not in ("heuristic",):
         raise ValueError(f"calibration must be 'heuristic', got {calibration!r}")
     if attention not in ("auto", False, None):
@@ -474,7 +616,7 @@ def convert(model: nn.Module, dtype="sf16", scale: str = "per_tensor", headroom:
         _unknown_names(model, widths, "widths")
         per_layer = {n: SFConfig(_bits_of(d), scale, headroom, accumulate, shift) for n, d in widths.items()}
     cfg16 = cfg if accumulate == "tensor" else SFConfig(16, scale, headroom, accumulate, shift)
-    return _Converter(cfg, cfg16, per_layer, keep_ids, keep_names).run(model)
+    return _Converter(cfg, cfg16, per_layer, keep_ids, keep_names, fuse).run(model)
 
 
 def conversion_report(model: nn.Module) -> ConversionReport:

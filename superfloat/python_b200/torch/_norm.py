@@ -23,16 +23,17 @@ def _check(x, weight, bias, eps):
         raise SFTypeError(f"layer_norm: the input is {x.dtype}; float32, bfloat16 and float16 are supported")
     if not x.is_cuda:
         raise SFShapeError(f"layer_norm: the input must be on a CUDA device, got {x.device}")
-    if not x.dim() or not 1 <= x.shape[-1] <= _lib.NORM_MOST:
-        raise SFShapeError(f"layer_norm: the last dimension has 1 to {_lib.NORM_MOST} features, got {tuple(x.shape)}")
+    shape, at = x.shape, x.get_device()
+    if not shape or not 1 <= shape[-1] <= _lib.NORM_MOST:
+        raise SFShapeError(f"layer_norm: the last dimension has 1 to {_lib.NORM_MOST} features, got {tuple(shape)}")
     for t, name in ((weight, "weight"), (bias, "bias")):
         if t is None:
             continue
-        if t.shape != x.shape[-1:]:
+        if t.shape != shape[-1:]:
             raise SFShapeError(f"layer_norm: the {name} has shape {tuple(t.shape)}, expected ({x.shape[-1]},)")
         if t.dtype not in _FLOATS:
             raise SFTypeError(f"layer_norm: the {name} is {t.dtype}; float32, bfloat16 and float16 are supported")
-        if t.device != x.device:
+        if t.get_device() != at:
             raise SFShapeError(f"layer_norm: the {name} is on {t.device}, the input on {x.device}")
     if not eps >= 0:
         raise ValueError(f"layer_norm: eps must not be negative, got {eps}")
