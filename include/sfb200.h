@@ -528,6 +528,10 @@ SFB_API int64_t sfb_distill_parts(int64_t M);
 SFB_API int sfb_distill_forward(const sfb_distill_call *call, sfb_stream stream);
 SFB_API int sfb_distill_backward(const sfb_distill_call *call, sfb_stream stream);
 
+/* How many CTAs have given up a bounded wait on the current device since the library was loaded (the rows they had are
+ * NaN); waits for the device. */
+SFB_API int sfb_distill_failures(int64_t *count);
+
 /* The gated feed-forward product over sf4..sf8 codes: h = act(x Wg^T + bg) (x Wu^T + bu), both weights N x K, as
  * sfb_tensor_call's.  No counterpart in the reference.  Np stands for N rounded up to a multiple of 16: codes and scales
  * are those of the gate, rows up to Np of zeros, then of the other weight. */

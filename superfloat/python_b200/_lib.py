@@ -89,6 +89,7 @@ SIGNATURES = {
     "sfb_distill_parts": (_i64, [_i64]),
     "sfb_distill_forward": (_i32, [_p, _p]),
     "sfb_distill_backward": (_i32, [_p, _p]),
+    "sfb_distill_failures": (_i32, [_p]),
     "sfb_capture_id": (_i64, [_p]),
 }
 
@@ -502,9 +503,10 @@ def gated_sums(M, N) -> int:
 
 
 def tensor_failures() -> int:
-    n = ctypes.c_int64()
+    n, m = ctypes.c_int64(), ctypes.c_int64()
     check(load().sfb_tensor_failures(ctypes.addressof(n)), "sf tensor linear")
-    return n.value
+    check(load().sfb_distill_failures(ctypes.addressof(m)), "sf distillation")
+    return n.value + m.value
 
 
 # --- layer norm and the distillation loss --------------------------------------------------------------------------

@@ -32,6 +32,10 @@
 #include "sfb_tensor.cuh"
 
 namespace sfb {
+
+unsigned wait_polls();                        // the calling thread's sfb_wide_wait_limit
+int wait_stall();
+
 namespace {
 
 constexpr int THREADS = 224, WARPS = THREADS / 32;   // that have the row
@@ -59,6 +63,8 @@ struct Distill {
     int same;                            // the gradient's rows lie on 16 bytes as the logits' do
     int skip;                            // nothing to do where the upstream gradient is one
     float temperature, unit;             // unit = log2(e) / T
+    unsigned spin;                       // polls of a wait
+    int stall;                           // the tests': the first row's parts never come
 };
 
 __device__ __forceinline__ uint32_t cluster_size() {
@@ -258,6 +264,8 @@ struct Shared {
 
 constexpr unsigned kSpinLimit = 1u << 26;             // polls of one wait, some seconds
 
+__device__ unsigned long long g_failures;             // CTAs that gave up a wait
+
 // A row's exchange.  Every warp sends its part to every CTA of the cluster, each part counted by the receiver's barrier:
 // a cluster's own barrier also waits until the row before has reached memory.  Places and barriers alternate between two:
 // a part of the row after next is sent once the next row's are complete, that is, after all have read this row's.
@@ -274,9 +282,9 @@ __device__ __forceinline__ void send_part(Shared &s, int turn, uint32_t n, uint3
 }
 
 // false once a wait has run out: the row is then NaN, and no later one is waited for
-__device__ __forceinline__ bool wait_parts(Shared &s, int turn, int parity) {
+__device__ __forceinline__ bool wait_parts(Shared &s, int turn, int parity, unsigned spin) {
     const uint32_t bar = (uint32_t)__cvta_generic_to_shared(&s.bar[turn]);
-    for (unsigned i = 0; i < kSpinLimit; i++) {
+    for (unsigned i = 0; i < spin; i++) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred q;\n\t"
@@ -432,10 +440,10 @@ __global__ void __launch_bounds__(ALL, 4) row_kernel(const __grid_constant__ Dis
         for (int64_t r = r0; r < p.M; r += step) {
             const bool live = weight != 0.0f;
             const Part<T> q = ahead;
-            if (tid == 0)
+            if (tid == 0 && fine)                     // (a phase that has not ended takes no second arrival)
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
                                  (uint32_t)__cvta_generic_to_shared(&s.bar[turn])),
-                             "r"(expected)
+                             "r"(expected + (p.stall ? 8 : 0))
                              : "memory");
             const float after = r + 2 * step < p.M ? p.weights[r + 2 * step] : 0.0f;
             asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -478,7 +486,7 @@ __global__ void __launch_bounds__(ALL, 4) row_kernel(const __grid_constant__ Dis
                 soft = soft_warp(make_float2(m, sum[0] + sum[1]), p.unit);
             }
             send_part(s, turn, n, rank, soft);
-            fine = fine && wait_parts(s, turn, parity);
+            fine = fine && wait_parts(s, turn, parity, p.spin);
             if constexpr (GRAD) {
                 soft = soft_all(s.soft[turn], (int)n * (WARPS + 1), p.unit);
                 const float base = base_of(soft.x, p.unit);
@@ -563,7 +571,7 @@ __global__ void __launch_bounds__(ALL, 4) row_kernel(const __grid_constant__ Dis
             __syncwarp();
             const bool live = weight != 0.0f;         // (if not, its entries were not made)
             send_part(s, turn, n, rank, make_float2(ninf(), 0.0f));      // what it read of the row before is free
-            fine = fine && wait_parts(s, turn, parity);
+            fine = fine && wait_parts(s, turn, parity, p.spin);
             float2 soft = soft_all(s.soft[turn], (int)n * (WARPS + 1), p.unit);
             if (!fine) soft.y = __int_as_float(0x7FC00000);
             const float base = base_of(soft.x, p.unit), inv = __fdiv_rn(1.0f, soft.y);
@@ -605,7 +613,10 @@ __global__ void __launch_bounds__(ALL, 4) row_kernel(const __grid_constant__ Dis
         asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     // (a CTA ends only once all parts sent to it have come, unless a wait ran out)
-    if (!__syncthreads_and(fine) && n > 1) cluster_barrier();
+    if (!__syncthreads_and(fine)) {
+        if (tid == 0) atomicAdd(&g_failures, 1ull);
+        if (n > 1) cluster_barrier();
+    }
 }
 
 // --- the gradient alone --------------------------------------------------------------------------------------
@@ -815,6 +826,8 @@ Distill distill_of(const sfb_distill_call *c) {
     p.w_dtype = (int)c->w_dtype;
     p.temperature = (float)c->temperature;
     p.unit = (float)(1.4426950408889634 / c->temperature);
+    p.spin = wait_polls() ? wait_polls() : kSpinLimit;
+    p.stall = wait_stall();
     if (c->M > 0) {
         const int64_t outer = (c->M - 1) / c->inner, in = std::min(c->M, c->inner) - 1;
         p.last = outer * c->so + in * c->si + c->V;
@@ -829,6 +842,15 @@ Distill distill_of(const sfb_distill_call *c) {
 
 }  // namespace
 }  // namespace sfb
+
+extern "C" int sfb_distill_failures(int64_t *count) {
+    using namespace sfb;
+    unsigned long long n = 0;
+    if (!count) return set_error(SFB_EINVAL, "sfb_distill_failures: null pointer");
+    if (cudaMemcpyFromSymbol(&n, g_failures, sizeof n) != cudaSuccess) return check_launch("sfb_distill_failures");
+    *count = (int64_t)n;
+    return SFB_OK;
+}
 
 extern "C" int64_t sfb_distill_parts(int64_t M) { return M > 0 ? (M + sfb::PART - 1) / sfb::PART : 0; }
 

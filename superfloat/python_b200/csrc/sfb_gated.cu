@@ -222,7 +222,7 @@ extern "C" int sfb_gated_forward(const sfb_gated_call *c, sfb_stream stream) {
                            {c->gate_scale, c->up_scale},
                            {c->ldg, c->ldu},
                            {vec(c->gate, c->ldg), vec(c->up, c->ldu)}};
-            const int64_t room = 8ll * sm_count(), gy = std::min<int64_t>((Np + 3) / 4, room);
+            const int64_t room = 8ll * sm_count(), gy = std::min<int64_t>((Np + 3) / 4, 65535);
             const dim3 grid((unsigned)std::min<int64_t>((c->K + 1023) / 1024, std::max<int64_t>(1, room / gy)), (unsigned)gy, 2);
             if (t == SFB_BF16)
                 gated_expand_kernel<<<grid, dim3(64, 4), 0, st>>>(p, c->N, Np, c->K, static_cast<__nv_bfloat16 *>(c->codes), c->ldc, c->scale);

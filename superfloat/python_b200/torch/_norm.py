@@ -49,7 +49,7 @@ def _address(t):
 
 def _forward(x, weight, bias, eps, keep):
     D = x.shape[-1]
-    y = x.new_empty(x.shape)
+    y = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
     x, ldx = _two_d(x, D)
     M, index = x.shape[0], x.get_device()
     stats = x.new_empty((M, 2), dtype=torch.float32) if keep else None

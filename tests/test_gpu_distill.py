@@ -333,6 +333,23 @@ def test_kept_tensors_on_the_host(gpu):
         check(x, t, i, g=torch.tensor(3.0, device="cuda"))
 
 
+def test_a_wait_that_runs_out_is_reported(gpu):
+    """Parts of a row that never come: the rows are NaN, it is counted, and the next call is as if nothing had been."""
+    from superfloat.python_b200 import _lib
+    x, (t, i) = randn(5, 9000), entries(5, 9000, 3, absent=False)
+    want = sft.distill_loss(x, t, i, reduction="none")
+    before = sft.tensor_failures()
+    _lib.load().sfb_wide_wait_limit(2000, 1)
+    try:
+        z = x.detach().requires_grad_()
+        loss = sft.distill_loss(z, t, i)
+        g, = torch.autograd.grad(loss, z)
+    finally:
+        _lib.load().sfb_wide_wait_limit(0, 0)
+    assert bool(loss.isnan()) and bool(g.isnan().all()) and sft.tensor_failures() > before
+    assert torch.equal(sft.distill_loss(x, t, i, reduction="none"), want)
+
+
 def test_refusals(gpu):
     x, t, i = randn(4, 30), randn(4, 3), torch.zeros(4, 3, dtype=torch.int64, device="cuda")
     for bad in (dict(reduction="max"), dict(temperature=0.0), dict(temperature=float("nan")), dict(temperature=-1.0)):
