@@ -14,18 +14,6 @@ constexpr int QT = 256;
 
 // --- rows on 16-byte boundaries ----------------------------------------------------------------------
 
-// 64 threads along a row, 8 elements each, 4 rows a block of 256; block (bx, by) of gx by gy
-__device__ __forceinline__ void pad_rows(const Rows &r, int tx, int ty, int bx, int gx, int by, int gy) {
-    const uint16_t *x = static_cast<const uint16_t *>(r.x);
-    for (int64_t m = (int64_t)by * 4 + ty; m < r.M; m += 4ll * gy)
-        for (int64_t k = ((int64_t)bx * 64 + tx) * 8; k < r.K; k += 512ll * gx) {
-            Vec<uint16_t, 8> q;
-#pragma unroll
-            for (int j = 0; j < 8; j++) q.v[j] = k + j < r.K ? x[m * r.ldx + k + j] : (uint16_t)0;
-            *reinterpret_cast<Vec<uint16_t, 8> *>(static_cast<uint16_t *>(r.out) + m * r.ldo + k) = q;
-        }
-}
-
 __global__ void __launch_bounds__(QT) pad_kernel(Rows r) {
     pad_rows(r, threadIdx.x, threadIdx.y, blockIdx.x, gridDim.x, blockIdx.y, gridDim.y);
 }

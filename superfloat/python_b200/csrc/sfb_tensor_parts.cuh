@@ -42,6 +42,56 @@ __device__ __forceinline__ float column_sum(const Sums &s, int64_t n) {
     return v[0];
 }
 
+// four codes as two pairs of the activations' type
+template <typename T> __device__ __forceinline__ void widen(uint32_t w, uint32_t &lo, uint32_t &hi);
+
+// 0x43cc as bf16 is 128 + (c mod 128), or twice that form's 128 where bit 7 is set: the
+// difference of the two is c in two's complement, exactly
+template <>
+__device__ __forceinline__ void widen<__nv_bfloat16>(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    const uint32_t a = __byte_perm(w, 0x43434343u, 0x4140), b = __byte_perm(w, 0x43434343u, 0x4342);
+    const uint32_t a0 = a & 0xFF7FFF7Fu, a1 = a & 0xFF80FF80u, b0 = b & 0xFF7FFF7Fu, b1 = b & 0xFF80FF80u;
+    __nv_bfloat162 x = __hsub2(reinterpret_cast<const __nv_bfloat162 &>(a0), reinterpret_cast<const __nv_bfloat162 &>(a1));
+    __nv_bfloat162 y = __hsub2(reinterpret_cast<const __nv_bfloat162 &>(b0), reinterpret_cast<const __nv_bfloat162 &>(b1));
+    lo = reinterpret_cast<uint32_t &>(x);
+    hi = reinterpret_cast<uint32_t &>(y);
+}
+
+// 0x64uu as fp16 is 1024 + u; with u = c + 128 less 1152 it is c
+template <>
+__device__ __forceinline__ void widen<__half>(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    w ^= 0x80808080u;
+    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 c = __half2half2(__ushort_as_half((unsigned short)0x6480));
+    __half2 x = __hsub2(reinterpret_cast<const __half2 &>(a), c), y = __hsub2(reinterpret_cast<const __half2 &>(b), c);
+    lo = reinterpret_cast<uint32_t &>(x);
+    hi = reinterpret_cast<uint32_t &>(y);
+}
+
+// 16 codes of a row from k on, those at or past K as 0, where rows do not start on 16 bytes: from the whole words around
+// them, each holding at least one of the row's codes, shifted into place
+__device__ __forceinline__ uint4 shift_codes(const int8_t *row, int64_t k, int64_t K) {
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (k >= K) return make_uint4(0, 0, 0, 0);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(row + k), end = reinterpret_cast<uintptr_t>(row + K);
+    const uint32_t *from = reinterpret_cast<const uint32_t *>(at & ~(uintptr_t)3);
+    const uint32_t shift = 8 * (uint32_t)(at & 3);
+    uint32_t a = __ldg(from);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t b = reinterpret_cast<uintptr_t>(from + i + 1) < end ? __ldg(from + i + 1) : 0u;
+        w[i] = __funnelshift_r(a, b, shift);
+        a = b;
+    }
+    const int left = (int)min((int64_t)16, K - k);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int keep = left - 4 * i;
+        w[i] &= keep >= 4 ? 0xFFFFFFFFu : keep <= 0 ? 0u : (1u << (8 * keep)) - 1u;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // a matrix of 16-bit elements, and where it is copied with its rows on 16-byte boundaries
 struct Rows {
     const void *x;                            // null: no copy
@@ -49,6 +99,18 @@ struct Rows {
     void *out;
     int64_t ldo;
 };
+
+// 64 threads along a row, 8 elements each, 4 rows a block of 256; block (bx, by) of gx by gy
+__device__ __forceinline__ void pad_rows(const Rows &r, int tx, int ty, int bx, int gx, int by, int gy) {
+    const uint16_t *x = static_cast<const uint16_t *>(r.x);
+    for (int64_t m = (int64_t)by * 4 + ty; m < r.M; m += 4ll * gy)
+        for (int64_t k = ((int64_t)bx * 64 + tx) * 8; k < r.K; k += 512ll * gx) {
+            Vec<uint16_t, 8> q;
+#pragma unroll
+            for (int j = 0; j < 8; j++) q.v[j] = k + j < r.K ? x[m * r.ldx + k + j] : (uint16_t)0;
+            *reinterpret_cast<Vec<uint16_t, 8> *>(static_cast<uint16_t *>(r.out) + m * r.ldo + k) = q;
+        }
+}
 
 // codes and scales of a float weight (work: 4 N bytes, for one scale only), and in the same launch a copy of
 // `rows`, if any

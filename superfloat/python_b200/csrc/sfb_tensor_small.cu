@@ -30,32 +30,6 @@ namespace {
 
 constexpr int WARPS = 8, SEG = 64;
 
-// four codes as two pairs of the activations' type
-template <typename T> __device__ __forceinline__ void widen(uint32_t w, uint32_t &lo, uint32_t &hi);
-
-// 0x43cc as bf16 is 128 + (c mod 128), or twice that form's 128 where bit 7 is set: the
-// difference of the two is c in two's complement, exactly
-template <>
-__device__ __forceinline__ void widen<__nv_bfloat16>(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    const uint32_t a = __byte_perm(w, 0x43434343u, 0x4140), b = __byte_perm(w, 0x43434343u, 0x4342);
-    const uint32_t a0 = a & 0xFF7FFF7Fu, a1 = a & 0xFF80FF80u, b0 = b & 0xFF7FFF7Fu, b1 = b & 0xFF80FF80u;
-    __nv_bfloat162 x = __hsub2(reinterpret_cast<const __nv_bfloat162 &>(a0), reinterpret_cast<const __nv_bfloat162 &>(a1));
-    __nv_bfloat162 y = __hsub2(reinterpret_cast<const __nv_bfloat162 &>(b0), reinterpret_cast<const __nv_bfloat162 &>(b1));
-    lo = reinterpret_cast<uint32_t &>(x);
-    hi = reinterpret_cast<uint32_t &>(y);
-}
-
-// 0x64uu as fp16 is 1024 + u; with u = c + 128 less 1152 it is c
-template <>
-__device__ __forceinline__ void widen<__half>(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    w ^= 0x80808080u;
-    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
-    const __half2 c = __half2half2(__ushort_as_half((unsigned short)0x6480));
-    __half2 x = __hsub2(reinterpret_cast<const __half2 &>(a), c), y = __hsub2(reinterpret_cast<const __half2 &>(b), c);
-    lo = reinterpret_cast<uint32_t &>(x);
-    hi = reinterpret_cast<uint32_t &>(y);
-}
-
 template <typename T>
 __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                       uint32_t b1) {
@@ -69,7 +43,7 @@ __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, u
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 codes of a row from k on, those at or past K as 0: into `to` ...
+// 16 codes of a row from k on, those at or past K as 0: into `to` (where rows do not start on 16 bytes, shift_codes)
 template <bool WHOLE>
 __device__ __forceinline__ void fetch_codes(uint4 *to, const int8_t *row, int64_t k, int64_t K) {
     if constexpr (WHOLE) {
@@ -82,30 +56,6 @@ __device__ __forceinline__ void fetch_codes(uint4 *to, const int8_t *row, int64_
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)),
                  "l"(bytes ? row + k : row), "r"(bytes)
                  : "memory");
-}
-
-// ... or, where rows do not start on 16 bytes, from the whole words around them, each holding at least one of the
-// row's codes, shifted into place
-__device__ __forceinline__ uint4 shift_codes(const int8_t *row, int64_t k, int64_t K) {
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (k >= K) return make_uint4(0, 0, 0, 0);
-    const uintptr_t at = reinterpret_cast<uintptr_t>(row + k), end = reinterpret_cast<uintptr_t>(row + K);
-    const uint32_t *from = reinterpret_cast<const uint32_t *>(at & ~(uintptr_t)3);
-    const uint32_t shift = 8 * (uint32_t)(at & 3);
-    uint32_t a = __ldg(from);
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t b = reinterpret_cast<uintptr_t>(from + i + 1) < end ? __ldg(from + i + 1) : 0u;
-        w[i] = __funnelshift_r(a, b, shift);
-        a = b;
-    }
-    const int left = (int)min((int64_t)16, K - k);
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int keep = left - 4 * i;
-        w[i] &= keep >= 4 ? 0xFFFFFFFFu : keep <= 0 ? 0u : (1u << (8 * keep)) - 1u;
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // 16 elements of a row of x from k on, those at or past K as 0; rows start on 16 bytes
