@@ -515,7 +515,7 @@ typedef struct sfb_distill_call {
     float *loss;                            /* sum and mean: one */
     float *rows;                            /* M: the rows' losses */
     float *parts;                           /* mean: sfb_distill_parts(M) */
-    float *weights;                         /* M: scratch of the forward pass */
+    float *weights;                         /* M + 1: scratch of the forward pass */
     float *stats;                           /* 3 M: written by the forward pass (nullable), read by the backward */
     float *block;                           /* 4 M k4 on a 16-byte boundary, k4 the multiple of 4 from K on: likewise */
     void *grad;                             /* of dtype; forward: written too, for an upstream gradient of one (nullable) */

@@ -117,6 +117,10 @@ def _strides_of(grad, logits):
     return (so, si) if grad.stride() == logits.stride() else (inner * logits.shape[-1], logits.shape[-1])
 
 
+def _kept_size(words, keep):
+    return words[1] * (4 * (words[7] + 3 & -4) + (3 if keep else 0))
+
+
 def _kept_at(kept, words, keep):
     """The places of the rows' statistics and of the entries."""
     at = kept.data_ptr()
@@ -129,17 +133,17 @@ def _forward(logits, teacher, index, weight, temperature, reduction, keep, with_
     mean, none = reduction == "mean", reduction == "none"
     parts = _lib.distill_parts(M) if mean else 0
     out = torch.empty(logits.shape[:-1] if none else (), dtype=torch.float32, device=dev)
-    # places in one buffer: the rows' weights, their losses, the partial sums of the weights; the entries and, for the
-    # backward pass, three numbers a row in another
-    room = torch.empty(M + (0 if none else M) + parts, dtype=torch.float32, device=dev)
-    kept = torch.empty(M * (4 * (words[7] + 3 & -4) + (3 if keep else 0)), dtype=torch.float32, device=dev)
+    # places in one buffer: the entries and, for the backward pass, three numbers a row; then, for this call alone, the
+    # rows' losses, the partial sums of the weights, the rows' weights and a counter
+    kept = torch.empty(_kept_size(words, keep) + (1 if none else 2) * M + parts + 1, dtype=torch.float32, device=dev)
     grad, go, gi = None, 0, 0
     if with_grad:
         grad = _like(logits)
         go, gi = _strides_of(grad, logits)
-    at = room.data_ptr()
+    at = kept.data_ptr() + 4 * _kept_size(words, keep)
+    rows = 0 if none else 4 * M
     _lib.distill_forward(logits.get_device(), array("q", (
-        *words, 0 if none else out.data_ptr(), out.data_ptr() if none else at + 4 * M, at + (4 if none else 8) * M, at,
+        *words, 0 if none else out.data_ptr(), out.data_ptr() if none else at, at + rows, at + rows + 4 * parts,
         *_kept_at(kept, words, keep), 0 if grad is None else grad.data_ptr(), go, gi, 0, 0)))
     return out, words, held[0], kept, grad
 
