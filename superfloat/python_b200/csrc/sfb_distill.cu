@@ -16,7 +16,7 @@
 // few rows still occupy the GPU.  What depends on the teacher's entries alone is made by a launch
 // before; a warp of its own makes the row's loss and the elements of the gradient that have an
 // entry.
-// 4096 x 50257 of bf16, a fifth of the rows masked: 162 us, 5.1 TB/s; 2047 x 32001 of float32: 94 us, 5.6 TB/s.
+// 4096 x 50257 of bf16, a fifth of the rows masked: 162 us, 5.1 TB/s; 2047 x 32001 of float32: 94-98 us, 5.5 TB/s.
 // Measured on the way: two CTAs an SM with 100 KB of a row each 176, five with 34 KB 197; two buffers
 // a CTA, the next row's copy under this one's sums, 188 (two CTAs) and 196 (one, of a whole row);
 // the gradient one row behind the sums 243.

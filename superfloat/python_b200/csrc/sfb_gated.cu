@@ -7,6 +7,8 @@
 // Both products of the forward pass are one (sfb_tensor_gemm.cu), over the codes of both weights, of which operand A has
 // 16 rows of the one and 16 of the other in turn: x is read once, and act(g) u is made where both are in registers.
 // (g and u as two layers: another write and read of M x N each, and the product as a third launch.)
+// 4096 x 4096 by 2 x 8192 of bf16: 328 us, 1676 TFLOP/s, the tensor pipe 93 % busy; one row from packed codes of these
+// sizes 20 us (two calls of the linear layer 22), 16 rows 26 (30).
 // The backward pass is two products over both weights' channels together, [dg s | du s] times the codes and [dg | du]^T x.
 #include <algorithm>
 
@@ -65,7 +67,7 @@ __global__ void __launch_bounds__(256) gated_expand_kernel(const __grid_constant
 // channel's scale (that of x's), each rounded once; g and u come in float32, as dg = dh u act'(g) has u's whole rounding:
 // in fp16 a u of 11 bits would add to dz's and the result's rounding a third of the same size.
 // Sums over the rows, for the biases, as the linear layer's: 64 rows a CTA, in a fixed order.
-// Memory bound: 2 + 8 bytes a channel and row read, 4 or 8 written.
+// Memory bound: 2 + 8 bytes a channel and row read, 4 or 8 written.  8192 x 5632 of fp16, 830 MB: 146 us, 5.7 TB/s.
 
 constexpr int BR = 64, BC = 256;
 
