@@ -490,6 +490,10 @@ SFB_API int sfb_norm_forward(const sfb_norm_call *call, sfb_stream stream);
 SFB_API int64_t sfb_norm_work(int64_t M, int64_t D);
 SFB_API int sfb_norm_backward(const sfb_norm_call *call, sfb_stream stream);
 
+/* How many CTAs (of rows of more than 8192 elements) have given up a bounded wait on the current device since the library
+ * was loaded (the rows they had are NaN); waits for the device. */
+SFB_API int sfb_norm_failures(int64_t *count);
+
 /* Distillation from a teacher's top logits.  No counterpart in the reference.  A row's loss is
  * T^2 sum_i p_i (log p_i - log q_i): p the softmax of its K teacher's entries / T, q that of
  * its V logits / T.  An entry is absent where its index is not in 0 .. V - 1 or its logit is

@@ -86,6 +86,7 @@ SIGNATURES = {
     "sfb_norm_forward": (_i32, [_p, _p]),
     "sfb_norm_work": (_i64, [_i64, _i64]),
     "sfb_norm_backward": (_i32, [_p, _p]),
+    "sfb_norm_failures": (_i32, [_p]),
     "sfb_distill_parts": (_i64, [_i64]),
     "sfb_distill_forward": (_i32, [_p, _p]),
     "sfb_distill_backward": (_i32, [_p, _p]),
@@ -503,10 +504,12 @@ def gated_sums(M, N) -> int:
 
 
 def tensor_failures() -> int:
-    n, m = ctypes.c_int64(), ctypes.c_int64()
-    check(load().sfb_tensor_failures(ctypes.addressof(n)), "sf tensor linear")
-    check(load().sfb_distill_failures(ctypes.addressof(m)), "sf distillation")
-    return n.value + m.value
+    n, total, lib = ctypes.c_int64(), 0, load()
+    for count, what in ((lib.sfb_tensor_failures, "sf tensor linear"), (lib.sfb_norm_failures, "sf layer norm"),
+                        (lib.sfb_distill_failures, "sf distillation")):
+        check(count(ctypes.addressof(n)), what)
+        total += n.value
+    return total
 
 
 # --- layer norm and the distillation loss --------------------------------------------------------------------------

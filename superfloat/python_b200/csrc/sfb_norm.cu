@@ -19,6 +19,10 @@
 #include "sfb_tensor.cuh"
 
 namespace sfb {
+
+unsigned wait_polls();                        // the calling thread's sfb_wide_wait_limit
+int wait_stall();
+
 namespace {
 
 constexpr int E = 8;                     // neighbouring elements of a thread
@@ -34,7 +38,13 @@ struct Norm {
     int64_t M, D, ldx, ldy, lddy, lddx;
     int w_dtype, b_dtype;
     float eps, share;                    // share = 1 / D
+    unsigned spin;                       // polls of a wait
+    int stall;                           // the tests': the first exchange never ends
 };
+
+constexpr unsigned kSpinLimit = 1u << 26;             // polls of one wait, some seconds
+
+__device__ unsigned long long g_failures;             // CTAs that gave up a wait
 
 // Where a thread's elements lie: E neighbouring ones (VEC: rows, weight and bias start on 16 bytes), or one in every
 // `step`, so that unaligned accesses of a warp are to neighbouring elements.
@@ -139,41 +149,86 @@ __device__ __forceinline__ void cluster_barrier() {
 // enough: what a use overwrites was read before the barrier of the use between.  Those of warps that a CTA does not have
 // are zeros: the others are read four at a time (one at a time, in a loop, they were a third of the forward pass's
 // instructions, which bound it).
+// (a kernel for clusters of its own: with both in one, rows that a CTA holds took 34.8 us of 8192 x 4096 forward, not 32.8)
+enum Of { WARPS, CTAS, CLUSTERS };
+
 struct __align__(16) Team {
     float one[2][TEAM / 32];
     float2 two[2][TEAM / 32];
     float2 ctas[2][8];
+    unsigned long long bar[2];
+    int gave_up;
 };
 
+template <Of TO>
 __device__ __forceinline__ void clear(Team &s) {
     if (threadIdx.x < TEAM / 32) {
         s.one[0][threadIdx.x] = s.one[1][threadIdx.x] = 0.0f;
         s.two[0][threadIdx.x] = s.two[1][threadIdx.x] = make_float2(0.0f, 0.0f);
     }
-    __syncthreads();
+    if (TO == CLUSTERS && threadIdx.x == 0) {
+        s.gave_up = 0;
+        for (int i = 0; i < 2; i++)
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(&s.bar[i])) : "memory");
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if constexpr (TO == CLUSTERS) cluster_barrier();  // the others' barriers are set
+    else __syncthreads();
 }
 
-// of the cluster's CTAs
-__device__ __forceinline__ float2 cluster_sum(float2 v, float2 (&places)[8], uint32_t n) {
-    if (threadIdx.x < n) {
-        const uint32_t mine = (uint32_t)__cvta_generic_to_shared(&places[cluster_rank()]);
-        uint32_t there;
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(mine), "r"((uint32_t)threadIdx.x));
-        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(v.x), "f"(v.y) : "memory");
-    }
+// once all rows are done: a CTA ends only when all parts sent to it have come, unless a wait ran out
+__device__ __forceinline__ void leave(Team &s) {
+    __syncthreads();
+    if (!s.gave_up) return;
+    if (threadIdx.x == 0) atomicAdd(&g_failures, 1ull);
     cluster_barrier();
-    v = places[0];
-    for (uint32_t i = 1; i < n; i++) v.x += places[i].x, v.y += places[i].y;
+}
+
+// Of the cluster's CTAs, each of which sends its part to all, counted by the receiver's barrier: a cluster's own barrier
+// also waits until the row before has reached memory (bf16 forward and backward, 8192 x 8200: 425 us and 330, 4096 x
+// 16384: 270 and 212).  Places and barriers alternate between two: a part of the use after next is sent once the next
+// one's are complete, that is, after all have read this one's.  A wait that runs out makes the row NaN and ends the CTA's part in the exchange: the others'
+// waits run out in turn, and nothing is on its way to a CTA that ends.
+__device__ __forceinline__ float2 cluster_sum(float2 v, Team &s, int turn, uint32_t n, const Norm &p) {
+    const int at = turn & 1, parity = turn >> 1 & 1;
+    const uint32_t bar = (uint32_t)__cvta_generic_to_shared(&s.bar[at]);
+    const bool fine = *reinterpret_cast<volatile int *>(&s.gave_up) == 0;
+    if (threadIdx.x == 0 && fine)
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(n * 8 + (p.stall ? 8 : 0))
+                     : "memory");
+    if (threadIdx.x < n && fine) {
+        uint32_t place, there;
+        const uint32_t mine = (uint32_t)__cvta_generic_to_shared(&s.ctas[at][cluster_rank()]);
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(place) : "r"(mine), "r"((uint32_t)threadIdx.x));
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(bar), "r"((uint32_t)threadIdx.x));
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(place),
+                     "f"(v.x), "f"(v.y), "r"(there)
+                     : "memory");
+    }
+    uint32_t ok = 0;
+    for (unsigned i = 0; fine && !ok && i < p.spin; i++)
+        asm volatile(
+            "{\n\t.reg .pred q;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 q, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, q;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+    if (!ok) {
+        *reinterpret_cast<volatile int *>(&s.gave_up) = 1;
+        return make_float2(__int_as_float(0x7FC00000), __int_as_float(0x7FC00000));
+    }
+    v = s.ctas[at][0];
+    for (uint32_t i = 1; i < n; i++) v.x += s.ctas[at][i].x, v.y += s.ctas[at][i].y;
     return v;
 }
 
-template <bool WARP>
-__device__ __forceinline__ float team_sum(float v, Team &s, int &turn) {
+template <Of TO>
+__device__ __forceinline__ float team_sum(float v, Team &s, int &turn, const Norm &n) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if constexpr (!WARP) {
-        const int p = turn;
-        turn ^= 1;
+    if constexpr (TO != WARPS) {
+        const int p = turn & 1;
         if ((threadIdx.x & 31) == 0) s.one[p][threadIdx.x >> 5] = v;
         __syncthreads();
         v = 0.0f;
@@ -183,22 +238,21 @@ __device__ __forceinline__ float team_sum(float v, Team &s, int &turn) {
             const float4 q = reinterpret_cast<const float4 *>(s.one[p])[i];
             v += (q.x + q.y) + (q.z + q.w);
         }
-        const uint32_t n = cluster_size();
-        if (n > 1) v = cluster_sum(make_float2(v, 0.0f), s.ctas[p], n).x;
+        if constexpr (TO == CLUSTERS) v = cluster_sum(make_float2(v, 0.0f), s, turn, cluster_size(), n).x;
+        turn++;
     }
     return v;
 }
 
-template <bool WARP>
-__device__ __forceinline__ float2 team_sum(float2 v, Team &s, int &turn) {
+template <Of TO>
+__device__ __forceinline__ float2 team_sum(float2 v, Team &s, int &turn, const Norm &n) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
         v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
     }
-    if constexpr (!WARP) {
-        const int p = turn;
-        turn ^= 1;
+    if constexpr (TO != WARPS) {
+        const int p = turn & 1;
         if ((threadIdx.x & 31) == 0) s.two[p][threadIdx.x >> 5] = v;
         __syncthreads();
         v = make_float2(0.0f, 0.0f);
@@ -209,8 +263,8 @@ __device__ __forceinline__ float2 team_sum(float2 v, Team &s, int &turn) {
             v.x += (a.x + a.z) + (b.x + b.z);
             v.y += (a.y + a.w) + (b.y + b.w);
         }
-        const uint32_t n = cluster_size();
-        if (n > 1) v = cluster_sum(v, s.ctas[p], n);
+        if constexpr (TO == CLUSTERS) v = cluster_sum(v, s, turn, cluster_size(), n);
+        turn++;
     }
     return v;
 }
@@ -221,10 +275,10 @@ struct Place {
     int t, step;
 };
 
-template <bool WARP, int C>
+template <Of TO, int C>
 __device__ __forceinline__ Place team_place(const Norm &p) {
     Place q;
-    if constexpr (WARP) {
+    if constexpr (TO == WARPS) {
         q.row = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
         q.rows = (int64_t)gridDim.x * (blockDim.x / 32);
         q.base = 0;
@@ -232,12 +286,12 @@ __device__ __forceinline__ Place team_place(const Norm &p) {
         q.t = threadIdx.x & 31;
         q.step = 32;
     } else {
-        const uint32_t n = cluster_size();
+        const uint32_t n = TO == CLUSTERS ? cluster_size() : 1;
         q.row = blockIdx.x / n;
         q.rows = gridDim.x / n;
         q.t = threadIdx.x;
         q.step = blockDim.x;
-        q.base = (int64_t)cluster_rank() * q.step * C * E;
+        q.base = (int64_t)(TO == CLUSTERS ? cluster_rank() : 0) * q.step * C * E;
         q.end = min(p.D, q.base + (int64_t)q.step * C * E);
     }
     return q;
@@ -275,15 +329,14 @@ __device__ __forceinline__ void copied(Vec<T, E> (&q)[C], const uint4 *slot) {
 
 template <typename T> struct Ahead { static constexpr int FORWARD = sizeof(T) == 2 ? 4 : 3, BACKWARD = sizeof(T) == 2 ? 3 : 2; };
 
-template <typename T, bool VEC, bool WARP, int C>
-__global__ void __launch_bounds__(WARP ? 128 : TEAM) forward_kernel(const __grid_constant__ Norm p) {
+template <typename T, bool VEC, Of TO, int C>
+__global__ void __launch_bounds__(TO == WARPS ? 128 : TEAM) forward_kernel(const __grid_constant__ Norm p) {
     constexpr int S = Ahead<T>::FORWARD;
     extern __shared__ __align__(16) uint4 ring[];
     __shared__ Team s;
     int turn = 0;
-    const Place q = team_place<WARP, C>(p);
-    if (!WARP) clear(s);
-    if (!WARP && cluster_size() > 1) cluster_barrier();  // the others' memory is there
+    const Place q = team_place<TO, C>(p);
+    if constexpr (TO != WARPS) clear<TO>(s);
     const int lines = Slot<T, C>::LINES * blockDim.x;
     const uint32_t at = (uint32_t)__cvta_generic_to_shared(ring);
     const T *x = static_cast<const T *>(p.x);
@@ -327,7 +380,7 @@ __global__ void __launch_bounds__(WARP ? 128 : TEAM) forward_kernel(const __grid
 #pragma unroll
                 for (int i = 0; i < C; i++) fetch<T, VEC>(raw[i], x + (r + q.rows) * p.ldx, q.base, i, q.t, q.step, q.end);
         }
-        const float mean = team_sum<WARP>(sum, s, turn) * p.share;
+        const float mean = team_sum<TO>(sum, s, turn, p) * p.share;
         sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < C; i++) {
@@ -338,7 +391,7 @@ __global__ void __launch_bounds__(WARP ? 128 : TEAM) forward_kernel(const __grid
                 sum = fmaf(v[i][j], v[i][j], sum);
             }
         }
-        const float rs = rsqrtf(fmaf(team_sum<WARP>(sum, s, turn), p.share, p.eps));
+        const float rs = rsqrtf(fmaf(team_sum<TO>(sum, s, turn, p), p.share, p.eps));
         if (p.stats && q.t == 0 && q.base == 0) *reinterpret_cast<float2 *>(p.stats + 2 * r) = make_float2(mean, rs);
         T *out = static_cast<T *>(p.y) + r * p.ldy;
 #pragma unroll
@@ -349,20 +402,18 @@ __global__ void __launch_bounds__(WARP ? 128 : TEAM) forward_kernel(const __grid
             put<T, VEC>(out, y, q.base, i, q.t, q.step, q.end);
         }
     }
-    // (a CTA of a cluster ends only once the others have written into its memory: their writes precede a barrier that
-    // it has passed)
+    if constexpr (TO == CLUSTERS) leave(s);
 }
 
-template <typename T, bool VEC, bool WARP, int C>
-__global__ void __launch_bounds__(WARP ? 128 : TEAM, 1) backward_kernel(const __grid_constant__ Norm p) {
+template <typename T, bool VEC, Of TO, int C>
+__global__ void __launch_bounds__(TO == WARPS ? 128 : TEAM, 1) backward_kernel(const __grid_constant__ Norm p) {
     constexpr int S = Ahead<T>::BACKWARD;
     extern __shared__ __align__(16) uint4 ring[];
     __shared__ Team s;
-    __shared__ float joined[WARP ? 2 * 32 * C * E : 1];
+    __shared__ float joined[TO == WARPS ? 2 * 32 * C * E : 1];
     int turn = 0;
-    const Place q = team_place<WARP, C>(p);
-    if (!WARP) clear(s);
-    if (!WARP && cluster_size() > 1) cluster_barrier();
+    const Place q = team_place<TO, C>(p);
+    if constexpr (TO != WARPS) clear<TO>(s);
     const int lines = Slot<T, C>::LINES * blockDim.x;
     const uint32_t at = (uint32_t)__cvta_generic_to_shared(ring);
     const T *x = static_cast<const T *>(p.x), *dy = static_cast<const T *>(p.dy);
@@ -421,7 +472,7 @@ __global__ void __launch_bounds__(WARP ? 128 : TEAM, 1) backward_kernel(const __
             if constexpr (!VEC) load(r + q.rows);
             stats = __ldg(reinterpret_cast<const float2 *>(p.stats) + r + q.rows);
         }
-        sum = team_sum<WARP>(sum, s, turn);
+        sum = team_sum<TO>(sum, s, turn, p);
         const float a = sum.x * p.share, c = sum.y * p.share;
         if (p.dx) {
             T *out = static_cast<T *>(p.dx) + r * p.lddx;
@@ -434,8 +485,9 @@ __global__ void __launch_bounds__(WARP ? 128 : TEAM, 1) backward_kernel(const __
             }
         }
     }
+    if constexpr (TO == CLUSTERS) leave(s);
     if (!p.parts) return;
-    if constexpr (WARP) {
+    if constexpr (TO == WARPS) {
         // the CTA's warps, one after another
         for (int n = 0; n < (int)blockDim.x / 32; n++) {
             if ((int)threadIdx.x / 32 == n)
@@ -453,7 +505,7 @@ __global__ void __launch_bounds__(WARP ? 128 : TEAM, 1) backward_kernel(const __
         }
         if (threadIdx.x / 32 != blockDim.x / 32 - 1) return;
     }
-    float *out = p.parts + (int64_t)(WARP ? blockIdx.x : q.row) * 2 * p.D;
+    float *out = p.parts + (int64_t)(TO == WARPS ? blockIdx.x : q.row) * 2 * p.D;
     // (partial sums start on 16 bytes where D is a multiple of 4: VEC has multiples of 8)
 #pragma unroll
     for (int i = 0; i < C; i++) {
@@ -522,16 +574,33 @@ int64_t backward_teams(int64_t M, const Teams &t) {
 
 constexpr int RING = 160 * 1024;         // dynamic shared memory of a CTA at most
 
-// A kernel's CUDA context whose attributes are set, per device, and how many CTAs of a size fit an SM
+// A kernel's CUDA context whose attributes are set, per device, and how many CTAs of a size (clusters of 2, 4 or 8 of them)
+// the device holds at once: more clusters than that are a second wave, as long as the first (2048 x 65536 of bf16 forward
+// 405 us and 248, backward included 828 and 504)
 struct Known {
     std::mutex lock;
     unsigned long long ctx[64];
-    int per[64][TEAM / 32 + 1];
+    int at_once[64][4][TEAM / 32 + 1];
 };
 
-// CTAs an SM, 0 on an error
+cudaLaunchConfig_t config(const Teams &t, int64_t grid, int64_t ring, cudaStream_t st, cudaLaunchAttribute &a) {
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3((unsigned)(grid * t.ctas));
+    c.blockDim = dim3(t.threads);
+    c.dynamicSmemBytes = (size_t)ring;
+    c.stream = st;
+    a = cudaLaunchAttribute{};
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x = t.ctas;
+    a.val.clusterDim.y = a.val.clusterDim.z = 1;
+    c.attrs = &a;
+    c.numAttrs = t.ctas > 1 ? 1 : 0;
+    return c;
+}
+
+// CTAs or clusters at once, 0 on an error
 template <typename K>
-int ready(K *kernel, Known &known, int threads, int64_t ring, const char *what) {
+int ready(K *kernel, Known &known, const Teams &t, int64_t ring, const char *what) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return set_error(0, "%s: no current CUDA device", what);
     std::lock_guard<std::mutex> g(known.lock);
@@ -539,76 +608,79 @@ int ready(K *kernel, Known &known, int threads, int64_t ring, const char *what) 
     if (ctx == 0 || known.ctx[dev] != ctx) {
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RING) != cudaSuccess)
             return check_launch(what), 0;
-        for (int &n : known.per[dev]) n = 0;
+        for (auto &sizes : known.at_once[dev])
+            for (int &n : sizes) n = 0;
         known.ctx[dev] = context_id();
     }
-    int &per = known.per[dev][threads / 32];
-    if (per == 0 && cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, (size_t)ring) != cudaSuccess)
-        return check_launch(what), 0;
-    return std::max(per, 1);
+    int &n = known.at_once[dev][t.ctas == 8 ? 3 : t.ctas / 2][t.threads / 32];
+    if (n == 0) {
+        int found = 0;
+        cudaLaunchAttribute a;
+        const cudaLaunchConfig_t c = config(t, sm_count(), ring, nullptr, a);
+        if (t.ctas > 1 ? cudaOccupancyMaxActiveClusters(&found, kernel, &c) != cudaSuccess
+                       : cudaOccupancyMaxActiveBlocksPerMultiprocessor(&found, kernel, t.threads, (size_t)ring) != cudaSuccess)
+            return check_launch(what), 0;
+        n = std::max(found, 1) * (t.ctas > 1 ? 1 : sm_count());
+    }
+    return n;
 }
 
 template <typename K>
 int launch(K *kernel, const Norm &p, const Teams &t, int64_t grid, int64_t ring, cudaStream_t st, const char *what) {
-    cudaLaunchConfig_t c{};
-    c.gridDim = dim3((unsigned)(grid * t.ctas));
-    c.blockDim = dim3(t.threads);
-    c.dynamicSmemBytes = (size_t)ring;
-    c.stream = st;
-    cudaLaunchAttribute a{};
-    a.id = cudaLaunchAttributeClusterDimension;
-    a.val.clusterDim.x = t.ctas;
-    a.val.clusterDim.y = a.val.clusterDim.z = 1;
-    c.attrs = &a;
-    c.numAttrs = t.ctas > 1 ? 1 : 0;
+    cudaLaunchAttribute a;
+    const cudaLaunchConfig_t c = config(t, grid, ring, st, a);
     cudaLaunchKernelEx(&c, kernel, p);
     return check_launch(what);
 }
 
-template <typename T, bool VEC, bool WARP, int C>
+template <typename T, bool VEC, Of TO, int C>
 int forward(const Norm &p, const Teams &t, cudaStream_t st) {
     const int64_t ring = VEC ? Ahead<T>::FORWARD * Slot<T, C>::LINES * 16ll * t.threads : 0;
     static Known known;
     const char *what = "sf layer norm";
-    const int per = ready(forward_kernel<T, VEC, WARP, C>, known, t.threads, ring, what);
-    if (per == 0) return SFB_ECUDA;
-    const int64_t rows = WARP ? (p.M + 3) / 4 : p.M;
-    const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)per * sm_count() / t.ctas));
-    return launch(forward_kernel<T, VEC, WARP, C>, p, t, grid, ring, st, what);
+    const int at_once = ready(forward_kernel<T, VEC, TO, C>, known, t, ring, what);
+    if (at_once == 0) return SFB_ECUDA;
+    const int64_t rows = TO == WARPS ? (p.M + 3) / 4 : p.M;
+    return launch(forward_kernel<T, VEC, TO, C>, p, t, std::min<int64_t>(rows, at_once), ring, st, what);
 }
 
-template <typename T, bool VEC, bool WARP, int C>
-int backward(const Norm &p, const Teams &t, cudaStream_t st) {
+template <typename T, bool VEC, Of TO, int C>
+int backward(const Norm &p, const Teams &t, cudaStream_t st, int64_t &teams) {
     const int64_t ring = VEC ? 2 * Ahead<T>::BACKWARD * Slot<T, C>::LINES * 16ll * t.threads : 0;
     static Known known;
     const char *what = "sf layer norm (backward)";
-    if (ready(backward_kernel<T, VEC, WARP, C>, known, t.threads, ring, what) == 0) return SFB_ECUDA;
-    return launch(backward_kernel<T, VEC, WARP, C>, p, t, backward_teams(p.M, t), ring, st, what);
+    const int at_once = ready(backward_kernel<T, VEC, TO, C>, known, t, ring, what);
+    if (at_once == 0) return SFB_ECUDA;
+    teams = backward_teams(p.M, t);
+    if (TO == CLUSTERS) teams = std::min<int64_t>(teams, at_once);
+    return launch(backward_kernel<T, VEC, TO, C>, p, t, teams, ring, st, what);
 }
 
-// the kernel for a type, alignment and length
+// the kernel for a type, alignment and length; backwards also how many rows of partial sums there are
 template <typename T, bool VEC>
-int run(const Norm &p, const Teams &t, bool back, cudaStream_t st) {
-    auto go = [&](auto warp, auto chunks) {
-        constexpr bool WARP = decltype(warp)::value;
-        constexpr int C = decltype(chunks)::value;
-        return back ? backward<T, VEC, WARP, C>(p, t, st) : forward<T, VEC, WARP, C>(p, t, st);
-    };
+int run(const Norm &p, const Teams &t, int64_t *teams, cudaStream_t st) {
     using std::integral_constant;
-    if (!t.warp) return go(std::false_type(), integral_constant<int, 2>());
+    auto go = [&](auto to, auto chunks) {
+        constexpr Of TO = decltype(to)::value;
+        constexpr int C = decltype(chunks)::value;
+        return teams ? backward<T, VEC, TO, C>(p, t, st, *teams) : forward<T, VEC, TO, C>(p, t, st);
+    };
+    const integral_constant<Of, WARPS> warps;
+    if (t.ctas > 1) return go(integral_constant<Of, CLUSTERS>(), integral_constant<int, 2>());
+    if (!t.warp) return go(integral_constant<Of, CTAS>(), integral_constant<int, 2>());
     switch (t.chunks) {
-        case 1: return go(std::true_type(), integral_constant<int, 1>());
-        case 2: return go(std::true_type(), integral_constant<int, 2>());
-        case 3: return go(std::true_type(), integral_constant<int, 3>());
+        case 1: return go(warps, integral_constant<int, 1>());
+        case 2: return go(warps, integral_constant<int, 2>());
+        case 3: return go(warps, integral_constant<int, 3>());
     }
-    return go(std::true_type(), integral_constant<int, 4>());
+    return go(warps, integral_constant<int, 4>());
 }
 
-int run(const Norm &p, int64_t dtype, bool vec, bool back, cudaStream_t st) {
+int run(const Norm &p, int64_t dtype, bool vec, int64_t *teams, cudaStream_t st) {
     const Teams t = teams_of(p.D);
-    if (dtype == SFB_F32) return vec ? run<float, true>(p, t, back, st) : run<float, false>(p, t, back, st);
-    if (dtype == SFB_BF16) return vec ? run<__nv_bfloat16, true>(p, t, back, st) : run<__nv_bfloat16, false>(p, t, back, st);
-    return vec ? run<__half, true>(p, t, back, st) : run<__half, false>(p, t, back, st);
+    if (dtype == SFB_F32) return vec ? run<float, true>(p, t, teams, st) : run<float, false>(p, t, teams, st);
+    if (dtype == SFB_BF16) return vec ? run<__nv_bfloat16, true>(p, t, teams, st) : run<__nv_bfloat16, false>(p, t, teams, st);
+    return vec ? run<__half, true>(p, t, teams, st) : run<__half, false>(p, t, teams, st);
 }
 
 bool is_float(int64_t t) { return t == SFB_F32 || t == SFB_BF16 || t == SFB_F16; }
@@ -642,6 +714,8 @@ Norm norm_of(const sfb_norm_call *c) {
     p.b_dtype = (int)c->b_dtype;
     p.eps = (float)c->eps;
     p.share = (float)(1.0 / (double)c->D);
+    p.spin = wait_polls() ? wait_polls() : kSpinLimit;
+    p.stall = wait_stall();
     return p;
 }
 
@@ -660,7 +734,16 @@ extern "C" int sfb_norm_forward(const sfb_norm_call *c, sfb_stream stream) {
     p.ldy = c->ldy;
     const int size = c->dtype == SFB_F32 ? 4 : 2;
     const bool vec = c->D % 8 == 0 && rows16(c->x, c->ldx, size) && rows16(c->y, c->ldy, size) && rows16(c->w, 0, 0) && rows16(c->b, 0, 0);
-    return run(p, c->dtype, vec, false, static_cast<cudaStream_t>(stream));
+    return run(p, c->dtype, vec, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int sfb_norm_failures(int64_t *count) {
+    using namespace sfb;
+    unsigned long long n = 0;
+    if (!count) return set_error(SFB_EINVAL, "sfb_norm_failures: null pointer");
+    if (cudaMemcpyFromSymbol(&n, g_failures, sizeof n) != cudaSuccess) return check_launch("sfb_norm_failures");
+    *count = (int64_t)n;
+    return SFB_OK;
 }
 
 extern "C" int64_t sfb_norm_work(int64_t M, int64_t D) {
@@ -692,11 +775,12 @@ extern "C" int sfb_norm_backward(const sfb_norm_call *c, sfb_stream stream) {
     const bool vec = c->D % 8 == 0 && rows16(c->x, c->ldx, size) && rows16(c->y, c->ldy, size) &&
                      rows16(c->dx, c->lddx, size) && rows16(c->w, 0, 0);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    rc = run(p, c->dtype, vec, true, st);
+    int64_t teams = 0;
+    rc = run(p, c->dtype, vec, &teams, st);
     if (rc || !p.parts) return rc;
     auto join = [&](auto *kernel, int64_t columns) {
         kernel<<<(unsigned)((2 * c->D + columns - 1) / columns), 512, 0, st>>>(
-            p.parts, backward_teams(c->M, teams_of(c->D)), c->D, c->dw, (int)c->w_dtype, c->db, (int)c->b_dtype);
+            p.parts, teams, c->D, c->dw, (int)c->w_dtype, c->db, (int)c->b_dtype);
     };
     if (2 * c->D < 32ll * sm_count()) join(join_kernel<8>, 8);
     else join(join_kernel<32>, 32);

@@ -377,8 +377,8 @@ def tensor_linear(x: torch.Tensor, weight, bias=None, *, activation: str | None 
 
 
 def tensor_failures() -> int:
-    """How many CTAs of the tensor-core products and of the distillation loss have
-    given up a bounded wait on the current device since the library was loaded; the
+    """How many CTAs of the tensor-core products, of long layer norms and of the
+    distillation loss have given up a bounded wait on the current device since the library was loaded; the
     outputs of such a CTA are NaN.  Waits for the device."""
     _lib.ensure_current(torch.cuda.current_device())
     return _lib.tensor_failures()

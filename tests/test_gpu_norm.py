@@ -230,6 +230,46 @@ def test_kept_tensors_on_the_host(gpu):
         close(a, v, t)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,d", [(900, 8200), (700, 8201), (500, 16384), (500, 20001), (300, 65536), (150, 40001)])
+def test_long_rows_in_turn(gpu, m, d, dtype):
+    """Clusters that take rows one after another, and the same in two streams at once and in a replayed graph.
+    (A column's sum: 300 rows of 16 clusters are 19 to a cluster and 16 to be joined, of the 116 that are allowed.)"""
+    x, w, b = randn(m, d, seed=1, dtype=dtype) + 1, 1 + randn(d, seed=2, std=0.3), randn(d, seed=3)
+    dy = randn(m, d, seed=4, dtype=dtype)
+    got = run(x, w, b, dy)
+    for g, (v, t) in zip(got, formula(x, w, b, dy)):
+        close(g, v, t)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    again = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            again.append(run(x, w, b, dy))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        y = sft.layer_norm(x, w, b)
+    graph.replay()
+    assert torch.equal(y, got[0])
+    for other in again:
+        assert all(torch.equal(g, o) for g, o in zip(got, other))
+
+
+def test_a_wait_that_runs_out_is_reported(gpu):
+    """Parts of a long row that never come: the rows are NaN, it is counted, and the next call is as if nothing had been."""
+    from superfloat.python_b200 import _lib
+    x = randn(7, 20000)
+    want, before = sft.layer_norm(x), sft.tensor_failures()
+    _lib.load().sfb_wide_wait_limit(2000, 1)
+    try:
+        y = sft.layer_norm(x)
+    finally:
+        _lib.load().sfb_wide_wait_limit(0, 0)
+    assert bool(y.isnan().all()) and sft.tensor_failures() > before
+    assert torch.equal(sft.layer_norm(x), want)
+
+
 def test_refusals(gpu):
     x, w = randn(4, 8), randn(8)
     with pytest.raises(SFTypeError):
