@@ -154,9 +154,9 @@ __device__ __forceinline__ float warp_sum(float v) {
 // what is taken from x unit before 2^x; a row (or part) of nothing but -inf has none
 __device__ __forceinline__ float base_of(float m, float unit) { return m == ninf() ? 0.0f : __fmul_rn(m, unit); }
 
-// Where x log2(e) / T would leave float32's range (a row of the type's lowest value) the difference is taken first.
-// Neighbouring numbers are so far apart there that the maximum has 1 and all others 0.
-__device__ __forceinline__ bool far(float m, float unit) { return fabsf(m) * unit > 1e37f && m != ninf(); }
+// Where the rounding of m log2(e) / T is not small (half a step is 1 from 2^24 on and 64 from 2^30 on, so that powers would
+// leave float32's range) the difference of x and m is taken first: a row at -1e30, as masks leave it, or a temperature of 1e-6.
+__device__ __forceinline__ bool far(float m, float unit) { return fabsf(m) * unit > 16777216.0f && m != ninf(); }
 
 template <bool FAR>
 __device__ __forceinline__ float power(float x, float m, float base, float unit) {
@@ -284,10 +284,13 @@ __device__ __forceinline__ bool wait_parts(Shared &s, int turn, int parity, unsi
     return false;
 }
 
-// what a part's sum is multiplied with where the whole has the maximum m, of base `base`; a part of nothing is (-inf, 0)
+// What a part's sum is multiplied with where the whole has the maximum m, of base `base`; a part of nothing is (-inf, 0).
+// Parts of which one side or both are far have powers of the maximum itself: what a base is rounded by counts there.
 __device__ __forceinline__ float factor_of(float x, float m, float base, float unit) {
-    if (m == ninf() || far(m, unit)) return x == m ? 1.0f : 0.0f;
-    return exp2_fast(__fmul_rn(x, unit) - base);      // (from the bases that the sums have, rounded as they are)
+    if (x == m || x == ninf()) return x == m ? 1.0f : 0.0f;
+    if (!far(m, unit) && !far(x, unit)) return exp2_fast(__fmul_rn(x, unit) - base);      // (from the bases that the sums have)
+    auto off = [&](float v) { return far(v, unit) ? 0.0f : fmaf(v, unit, -base_of(v, unit)); };
+    return exp2_fast(fmaf(x - m, unit, off(m) - off(x)));
 }
 
 // (maximum, sum of the powers) of a warp's parts: the same in all lanes
