@@ -517,14 +517,20 @@ __global__ void __launch_bounds__(ALL, 4) row_kernel(const __grid_constant__ Dis
                         }
                     }
                 } else {
+                    // Rows of the gradient that lie differently: elements, a warp those of the vectors that its own lanes
+                    // have copied (32 in a row), so that it waits for nobody else's copies and nobody for its reading.
                     T *to0 = to - q.lead + q.first;
-                    for (int u = q.begin + tid; u < q.end; u += THREADS) {
-                        float v = 0.0f;
-                        if (live) v = power_of(to_f(u < q.inside * E ? row[u] : q.at[u]), soft.x, base, p.unit) * scale;
-                        to0[u] = from_f<T>(v);
-                    }
-                    // here a thread reads what others have copied, and will copy over
-                    asm volatile("bar.sync 2, %0;" ::"n"(THREADS) : "memory");
+                    __syncwarp();
+                    for (int i0 = warp * 32; i0 < q.vectors; i0 += THREADS)
+#pragma unroll
+                        for (int j = 0; j < E; j++) {
+                            const int u = i0 * E + j * 32 + lane;
+                            if (u < q.begin || u >= q.end) continue;
+                            float v = 0.0f;
+                            if (live) v = power_of(to_f(u < q.inside * E ? row[u] : q.at[u]), soft.x, base, p.unit) * scale;
+                            to0[u] = from_f<T>(v);
+                        }
+                    __syncwarp();                     // the next copies go over what was read here
                 }
             }
             // the next row's copies, to where this thread has read what it needs
