@@ -244,9 +244,13 @@ __global__ void __launch_bounds__(32 * PART) entry_kernel(const __grid_constant_
 struct Shared {
     float2 soft[2][8 * (WARPS + 1)];     // (maximum, sum) of every warp of the cluster
     unsigned long long bar[2];
+    unsigned long long done;             // counts the warps that have written their part of a row's gradient
+    unsigned long long left;             // the first row at which a warp has left the exchange
     float share[ALL / 32];
     int last;
 };
+
+constexpr unsigned long long NONE = ~0ull;
 
 constexpr unsigned kSpinLimit = 1u << 26;             // polls of one wait, some seconds
 
@@ -267,11 +271,12 @@ __device__ __forceinline__ void send_part(Shared &s, int turn, uint32_t n, uint3
                  : "memory");
 }
 
-// false once a wait has run out: the row is then NaN, and no later one is waited for
-__device__ __forceinline__ bool wait_parts(Shared &s, int turn, int parity, unsigned spin) {
-    const uint32_t bar = (uint32_t)__cvta_generic_to_shared(&s.bar[turn]);
-    for (unsigned i = 0; i < spin; i++) {
-        uint32_t ok;
+// False where the wait has run out, for the whole warp.  It sends and waits no more then: parts of a later row would be
+// counted as this one's by a CTA that is still at it, and the others' waits run out in turn.
+__device__ __forceinline__ bool wait_for(const unsigned long long &on, int parity, unsigned spin) {
+    const uint32_t bar = (uint32_t)__cvta_generic_to_shared(&on);
+    uint32_t ok = 0;
+    for (unsigned i = 0; !ok && i < spin; i++)
         asm volatile(
             "{\n\t.reg .pred q;\n\t"
             "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 q, [%1], %2;\n\t"
@@ -279,9 +284,7 @@ __device__ __forceinline__ bool wait_parts(Shared &s, int turn, int parity, unsi
             : "=r"(ok)
             : "r"(bar), "r"(parity)
             : "memory");
-        if (ok) return true;
-    }
-    return false;
+    return __all_sync(0xffffffffu, ok);
 }
 
 // What a part's sum is multiplied with where the whole has the maximum m, of base `base`; a part of nothing is (-inf, 0).
@@ -385,6 +388,23 @@ __device__ __forceinline__ void copy_row(const Part<T> &q, T *row, bool live) {
     asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
+// What a CTA that gave up a wait leaves of the row `r` and of those after it: NaN, and 0 as ever where a row does not count.
+template <typename T, bool GRAD>
+__device__ __noinline__ void lost_rows(const Distill &p, int64_t r, int64_t step, uint32_t rank) {
+    for (; r < p.M; r += step) {
+        const float lost = p.weights[r] != 0.0f ? __int_as_float(0x7FC00000) : 0.0f;
+        if (rank == 0 && threadIdx.x == 0) {
+            p.rows[r] = lost;
+            if (p.stats) p.stats[3 * r] = p.stats[3 * r + 1] = p.stats[3 * r + 2] = lost;
+        }
+        if constexpr (GRAD) {
+            const Part<T> q = part_of<T>(p, r, rank);
+            T *to0 = static_cast<T *>(p.grad) + place(p, r, p.go, p.gi) - q.lead + q.first;
+            for (int u = q.begin + threadIdx.x; u < q.end; u += ALL) to0[u] = from_f<T>(lost);
+        }
+    }
+}
+
 // --- a row's kernel ------------------------------------------------------------------------------------------
 
 template <typename T, bool GRAD>
@@ -404,6 +424,8 @@ __global__ void __launch_bounds__(ALL, 4) row_kernel(const __grid_constant__ Dis
             const uint32_t bar = (uint32_t)__cvta_generic_to_shared(&s.bar[i]);
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
         }
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(&s.done)), "n"(WARPS) : "memory");
+        s.left = NONE;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (n > 1) cluster_barrier();                     // the others' barriers are set
@@ -420,7 +442,7 @@ __global__ void __launch_bounds__(ALL, 4) row_kernel(const __grid_constant__ Dis
         share = w == 0.0f ? 0.0f : __fdiv_rn(1.0f, w);
     }
     int turn = 0, parity = 0;
-    bool fine = true;
+    int64_t left = -1;                                // the row at which a wait of this warp has run out
     const int64_t r0 = blockIdx.x / n;
     if (warp < WARPS) {
         float weight = p.weights[r0], next = r0 + step < p.M ? p.weights[r0 + step] : 0.0f;
@@ -429,7 +451,7 @@ __global__ void __launch_bounds__(ALL, 4) row_kernel(const __grid_constant__ Dis
         for (int64_t r = r0; r < p.M; r += step) {
             const bool live = weight != 0.0f;
             const Part<T> q = ahead;
-            if (tid == 0 && fine)                     // (a phase that has not ended takes no second arrival)
+            if (tid == 0)
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
                                  (uint32_t)__cvta_generic_to_shared(&s.bar[turn])),
                              "r"(expected + (p.stall ? 8 : 0))
@@ -475,11 +497,14 @@ __global__ void __launch_bounds__(ALL, 4) row_kernel(const __grid_constant__ Dis
                 soft = soft_warp(make_float2(m, sum[0] + sum[1]), p.unit);
             }
             send_part(s, turn, n, rank, soft);
-            fine = fine && wait_parts(s, turn, parity, p.spin);
+            if (!wait_for(s.bar[turn], parity, p.spin)) {
+                left = r;
+                break;
+            }
             if constexpr (GRAD) {
                 soft = soft_all(s.soft[turn], (int)n * (WARPS + 1), p.unit);
                 const float base = base_of(soft.x, p.unit);
-                const float scale = fine ? __fdiv_rn(1.0f, soft.y) * (weight * share * p.temperature) : __int_as_float(0x7FC00000);
+                const float scale = __fdiv_rn(1.0f, soft.y) * (weight * share * p.temperature);
                 T *to = static_cast<T *>(p.grad) + place(p, r, p.go, p.gi);
                 if (p.same) {
                     T *to0 = to - q.lead + q.first;
@@ -538,7 +563,12 @@ __global__ void __launch_bounds__(ALL, 4) row_kernel(const __grid_constant__ Dis
                 ahead = part_of<T>(p, r + step, rank);
                 copy_row(ahead, row, next != 0.0f);
             }
-            if constexpr (GRAD) asm volatile("bar.arrive 1, %0;" ::"n"(ALL) : "memory");
+            if constexpr (GRAD) {
+                __syncwarp();
+                if (lane == 0)
+                    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"((uint32_t)__cvta_generic_to_shared(&s.done))
+                                 : "memory");
+            }
             weight = next;
             next = after;
             parity ^= turn;
@@ -566,9 +596,11 @@ __global__ void __launch_bounds__(ALL, 4) row_kernel(const __grid_constant__ Dis
             __syncwarp();
             const bool live = weight != 0.0f;         // (if not, its entries were not made)
             send_part(s, turn, n, rank, make_float2(ninf(), 0.0f));      // what it read of the row before is free
-            fine = fine && wait_parts(s, turn, parity, p.spin);
-            float2 soft = soft_all(s.soft[turn], (int)n * (WARPS + 1), p.unit);
-            if (!fine) soft.y = __int_as_float(0x7FC00000);
+            if (!wait_for(s.bar[turn], parity, p.spin)) {
+                left = r;
+                break;
+            }
+            const float2 soft = soft_all(s.soft[turn], (int)n * (WARPS + 1), p.unit);
             const float base = base_of(soft.x, p.unit), inv = __fdiv_rn(1.0f, soft.y);
             if (rank == 0) {
                 float loss = 0.0f;
@@ -591,8 +623,12 @@ __global__ void __launch_bounds__(ALL, 4) row_kernel(const __grid_constant__ Dis
                 }
             }
             if constexpr (GRAD) {
-                // the elements with an entry, after the others have written the whole row
-                asm volatile("bar.sync 1, %0;" ::"n"(ALL) : "memory");
+                // the elements with an entry, after the others have written the whole row (a warp that has left the
+                // exchange does not say so: hence a wait with a limit here too)
+                if (!wait_for(s.done, turn, p.spin)) {
+                    left = r;
+                    break;
+                }
                 T *to = static_cast<T *>(p.grad) + place(p, r, p.go, p.gi);
                 const int64_t lo = (int64_t)rank * p.chunk - part_of<T>(p, r, rank).lead, hi = lo + p.chunk;     // of this CTA
                 const float factor = weight * share * p.temperature;
@@ -608,8 +644,12 @@ __global__ void __launch_bounds__(ALL, 4) row_kernel(const __grid_constant__ Dis
         asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     // (a CTA ends only once all parts sent to it have come, unless a wait ran out)
-    if (!__syncthreads_and(fine)) {
+    if (left >= 0 && lane == 0) atomicMin(&s.left, (unsigned long long)left);
+    __syncthreads();
+    if (s.left != NONE) {
+        lost_rows<T, GRAD>(p, (int64_t)s.left, step, rank);
         if (tid == 0) atomicAdd(&g_failures, 1ull);
+        __syncthreads();
         if (n > 1) cluster_barrier();
     }
     // the last cluster to end adds the rows' losses up, in a fixed order (a launch of its own was 3 us, and 4 of the host's)
