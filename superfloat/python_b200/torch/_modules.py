@@ -11,11 +11,13 @@ reason and run as they were.
 from __future__ import annotations
 
 import copy
+import inspect
 from dataclasses import dataclass, field
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.overrides import TorchFunctionMode
 
 from . import _core, _gated, _norm, _tensor
 from ._ops import call_linear
@@ -201,43 +203,122 @@ class SFLayerNorm(nn.Module):
         return f"{self.normalized_shape}, eps={self.eps}, weight={self.weight is not None}, bias={self.bias is not None}"
 
 
-# activation modules by class name (torch's and Hugging Face's; transformers is never imported)
-_GATES = {"SiLU": "silu", "SiLUActivation": "silu", "ReLU": "relu", "GELUActivation": "gelu", "PytorchGELUTanh": "gelu_tanh",
-          "GELUTanh": "gelu_tanh"}
+class _Recorded(TorchFunctionMode):
+    """The calls of torch functions (operators, methods and attributes of tensors among them) while it is entered."""
+
+    def __init__(self):
+        super().__init__()
+        self.calls = []                         # (function, arguments, keywords, result)
+
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        out = func(*args, **(kwargs or {}))
+        self.calls.append((func, args, kwargs or {}, out))
+        return out
+
+
+_PRODUCTS = {torch.mul, torch.multiply, torch.Tensor.mul, torch.Tensor.multiply, torch.Tensor.mul_, torch.Tensor.multiply_}
+_RELUS = {F.relu, torch.relu, torch.relu_, torch.Tensor.relu, torch.Tensor.relu_}
+
+
+def _activation_called(func, args, kwargs):
+    """tensor_gated's name for the activation that a recorded call is, or None."""
+    options = {k: v for k, v in kwargs.items() if k != "inplace"}
+    if func is F.gelu:
+        name = {"none": "gelu", "tanh": "gelu_tanh"}.get(options.pop("approximate", "none"))
+    else:
+        name = "silu" if func is F.silu else "relu" if func in _RELUS else None
+    return name if len(args) == 1 and not options else None
 
 
 def _gate_activation(act):
-    if isinstance(act, nn.GELU):
-        return "gelu_tanh" if act.approximate == "tanh" else "gelu"
-    return _GATES.get(type(act).__name__)
+    """tensor_gated's name for an activation module, known by the one function that it calls; None for any other."""
+    t = torch.linspace(-2, 2, 8)
+    try:
+        with torch.no_grad(), _Recorded() as seen:
+            out = act(t)
+    except Exception:  # noqa: BLE001  (not an activation, or not one for a vector on the host)
+        return None
+    if len(seen.calls) != 1:
+        return None
+    func, args, kwargs, result = seen.calls[0]
+    return _activation_called(func, args, kwargs) if args and args[0] is t and result is out else None
+
+
+def _expression(calls, x, result, projections):
+    """What ``result`` is in terms of x by the recorded calls, as text; None where one of them is not a projection, an
+    activation or a product of two of these.  ``projections``: their names by (id of the weight, id of the bias)."""
+    made = {id(x): "x"}
+    for func, args, kwargs, out in calls:
+        known = [str(made.get(id(t))) for t in args]
+        if func is F.linear and len(args) == 3 and not kwargs:
+            made[id(out)] = f"{projections.get((id(args[1]), id(args[2])))}({known[0]})"
+        elif func in _PRODUCTS and len(args) == 2 and not kwargs:
+            made[id(out)] = " * ".join(sorted(known))
+        else:
+            act = _activation_called(func, args, kwargs)
+            if act is None:
+                return None
+            made[id(out)] = f"{act}({known[0]})"
+    return made.get(id(result))
+
+
+def _hooked(m):
+    return any(getattr(m, h, None) for h in ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks"))
 
 
 def gated_block(m: nn.Module):
     """(activation, "") of a gated feed-forward block that :class:`SFGatedFeedForward` can stand for, (None, "") of another
     module, (None, why) of a block that it cannot.  A block is recognised by its children (``gate_proj``, ``up_proj``,
-    ``down_proj``, ``act_fn``) and by what it computes on two rows."""
+    ``down_proj``, ``act_fn``) and by every call that its forward makes on tensors, in training and in evaluation, with
+    gradients and without: three projections, the activation and one product, each of what the ones before have made."""
     parts = [m._modules.get(n) for n in ("gate_proj", "up_proj", "down_proj")]
     if not all(isinstance(p, nn.Linear) for p in parts):
         return None, ""
     gate, up, down = parts
     if any(_custom_forward(p, nn.Linear) for p in parts):
         return None, "a projection has a forward of its own"
-    act = _gate_activation(getattr(m, "act_fn", None))
+    act_fn = getattr(m, "act_fn", None)
+    if any(map(_hooked, (m, gate, up, act_fn))):
+        return None, "it has hooks"
+    act = _gate_activation(act_fn)
     if act is None:
-        return None, f"activation {type(getattr(m, 'act_fn', None)).__name__}"
+        return None, f"activation {type(act_fn).__name__}"
     if set(m._modules) - {"gate_proj", "up_proj", "down_proj", "act_fn"}:
         return None, "it has other children"
+    if m._parameters or m._buffers:
+        return None, "it has parameters or buffers of its own"
     if gate.weight.shape != up.weight.shape or gate.weight.dtype != up.weight.dtype:
         return None, "its first two projections differ in shape or type"
     if gate.weight.is_meta:
         return None, "its weights are on the meta device"
-    with torch.no_grad():
+    takes = list(inspect.signature(m.forward).parameters.values())
+    if len(takes) != 1 or takes[0].kind not in (takes[0].POSITIONAL_ONLY, takes[0].POSITIONAL_OR_KEYWORD):
+        return None, "its forward does not take one argument"
+    keys = [(id(p.weight), id(p.bias)) for p in parts]
+    projections = dict(zip(keys, ("gate", "up", "down")))      # (those that share their parameters share a name)
+    g, u, d = map(projections.get, keys)
+    want = f"{d}({' * '.join(sorted((f'{act}({g}(x))', f'{u}(x)')))})"
+    modes = [(t, t.training) for t in m.modules()]
+    try:
         x = torch.linspace(-2, 2, 2 * gate.in_features, device=gate.weight.device).view(2, -1).to(gate.weight.dtype)
-        try:
-            same = torch.equal(m(x), down(m.act_fn(gate(x)) * up(x)))
-        except Exception as e:  # noqa: BLE001  (a model's own forward may raise)
-            return None, f"its forward did not run on two rows ({type(e).__name__})"
-    return (act, "") if same else (None, "it computes something else than down(act(gate(x)) * up(x))")
+        x.requires_grad_()
+        grads = (False,) if torch.is_inference_mode_enabled() or gate.weight.is_inference() else (False, True)
+        for training in (False, True):
+            for t, _ in modes:
+                t.training = training
+            for grad in grads:
+                with torch.set_grad_enabled(grad), _Recorded() as seen:
+                    out = m(x)
+                # (modes that the forward enters are no calls, but show in what these make)
+                if (len(seen.calls) != 5 or _expression(seen.calls, x, out, projections) != want
+                        or any(r.requires_grad is not grad or r.dtype is not x.dtype for *_, r in seen.calls)):
+                    return None, "it computes something else than down(act(gate(x)) * up(x))"
+    except Exception as e:  # noqa: BLE001  (a model's own forward may raise)
+        return None, f"its forward did not run on two rows ({type(e).__name__})"
+    finally:
+        for t, training in modes:
+            t.training = training
+    return act, ""
 
 
 class SFGatedFeedForward(nn.Module):
@@ -245,11 +326,15 @@ class SFGatedFeedForward(nn.Module):
     projections and their product are one operator (:func:`tensor_gated`), the last is an SF linear layer.  The
     children and their parameters are the source's."""
 
-    def __init__(self, block: nn.Module, name: str, cfg: SFConfig, down: SFConfig | None = None):
+    def __init__(self, block: nn.Module, name: str, cfg: SFConfig, down: SFConfig | None = None, *, activation=None):
+        """``activation``: what :func:`gated_block` says of the block, where it has been asked."""
         super().__init__()
         if cfg.accumulate != "tensor":
             raise ValueError("a gated block is one operator with accumulate=\"tensor\" only")
-        self.activation, why = gated_block(block)
+        why = ""
+        self.activation = activation
+        if activation is None:
+            self.activation, why = gated_block(block)
         if self.activation is None:
             raise ValueError(why or "not a gated feed-forward block")
         self.sf, self.sf_name = cfg, name
@@ -444,7 +529,7 @@ class _Converter:
             return None
         cfg, _, down = (self.config_for(module._modules[n], p) for n, p in zip(("gate_proj", "up_proj", "down_proj"), at))
         self.report.converted.append((path, "gated feed-forward"))
-        return SFGatedFeedForward(module, path, cfg, down)
+        return SFGatedFeedForward(module, path, cfg, down, activation=act)
 
     def replace(self, module, path):
         seen = self.replaced.get(id(module))
@@ -586,9 +671,9 @@ def convert(model: nn.Module, dtype="sf16", scale: str = "per_tensor", headroom:
     narrower; ``widths`` ({name: dtype}) gives layers their own width.
     ``accumulate="tensor"`` runs the layers on the tensor cores, for a model in
     bfloat16 or float16; it ends at sf8, so "auto" keeps nothing there.  ``fuse`` (with
-    accumulate="tensor") also swaps gated feed-forward blocks, down(act(gate(x)) *
-    up(x)) over children of these names, and ``nn.LayerNorm`` for modules that are one
-    operator each (:class:`SFGatedFeedForward`, :class:`SFLayerNorm`)."""
+    accumulate="tensor") also swaps gated feed-forward blocks, whose forward is down(act(gate(x)) *
+    up(x)) over children ``gate_proj``, ``up_proj`` and ``down_proj`` and nothing else, and
+    ``nn.LayerNorm`` for modules that are one operator each (:class:`SFGatedFeedForward`, :class:`SFLayerNorm`)."""
     if fuse and accumulate != "tensor":
         raise ValueError("fuse=True is for accumulate=\"tensor\"")
     if calibration not in ("heuristic",):
