@@ -181,14 +181,30 @@ class SFConv2d(nn.Module):
                 f"padding={self.padding}, {self.sf.describe()}, name={self.sf_name!r}")
 
 
+def convertible_norm(norm: nn.LayerNorm):
+    from .. import _lib
+    if len(norm.normalized_shape) != 1:
+        return False, f"normalized_shape={tuple(norm.normalized_shape)} (only the last dimension is converted)"
+    if not 1 <= norm.normalized_shape[0] <= _lib.NORM_MOST:
+        return False, f"normalized_shape={tuple(norm.normalized_shape)} (1 to {_lib.NORM_MOST} features are converted)"
+    for name in ("weight", "bias"):
+        if name not in norm._parameters:
+            return False, f"its {name} is computed"
+        p = norm._parameters[name]
+        if p is not None and p.dtype not in _tensor._FLOATS:
+            return False, f"its {name} is {p.dtype} (float32, bfloat16 and float16 are converted)"
+    return True, ""
+
+
 class SFLayerNorm(nn.Module):
     """``nn.LayerNorm`` over the last dimension on the B200's own kernel (:func:`layer_norm`); its parameters are the
     source's."""
 
     def __init__(self, norm: nn.LayerNorm):
         super().__init__()
-        if len(norm.normalized_shape) != 1:
-            raise ValueError(f"normalized_shape={tuple(norm.normalized_shape)} (only the last dimension is converted)")
+        ok, why = convertible_norm(norm)
+        if not ok:
+            raise ValueError(why)
         self.normalized_shape, self.eps = tuple(norm.normalized_shape), norm.eps
         self.weight, self.bias = norm.weight, norm.bias
         self.train(norm.training)
@@ -511,10 +527,11 @@ class _Converter:
     def _fused(self, module, path, kind):
         """A layer norm's or gated block's replacement, or None: the module is looked at as any other then."""
         if isinstance(module, nn.LayerNorm):
-            if _custom_forward(module, nn.LayerNorm):
+            ok, why = convertible_norm(module)
+            if _custom_forward(module, nn.LayerNorm) or "forward" in vars(module):
                 self._skip(path, kind, f"a subclass of nn.LayerNorm with its own forward ({kind}); runs as it was")
-            elif len(module.normalized_shape) != 1:
-                self._skip(path, kind, f"normalized_shape={tuple(module.normalized_shape)}; runs as it was")
+            elif not ok or _hooked(module):
+                self._skip(path, kind, f"{why or 'it has hooks'}; runs as it was")
             else:
                 self.report.converted.append((path, "LayerNorm"))
                 return SFLayerNorm(module)
