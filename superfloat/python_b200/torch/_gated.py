@@ -97,9 +97,10 @@ def _gradients(ctx, grad):
     dx = grad.new_empty(shape) if want_x else None
     dg = du = None
     if want_g and want_u:
-        # one product makes both: rows of the gate's, and of the other's Np on
+        # one product makes both: rows of the gate's, and of the other's Np on (each counts its own changes: a view of
+        # `both` would count the other's too, and a graph that has saved one refuse what was done to the other)
         both = grad.new_empty((2 * Np, K), dtype=w_dtype)
-        dg, du = both[:N], both[Np:Np + N]
+        dg, du = both[:N].data, both[Np:Np + N].data
     elif want_g or want_u:
         dw = grad.new_empty((N, K), dtype=w_dtype)
         dg, du = (dw, None) if want_g else (None, dw)
