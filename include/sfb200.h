@@ -467,7 +467,8 @@ SFB_API int sfb_sf8_values(const int64_t *table, int count, int power, sfb_strea
 /* Layer norm over the last dimension, y = (x - mean) r w + b with r = 1 / sqrt(var + eps),
  * statistics in float32.  No counterpart in the reference.  Rows of D elements, at most
  * 65536, row strides in elements; x, y and their gradients are of `dtype` (SFB_F32, BF16
- * or F16), w and b of a type of their own.  Every field has 8 bytes. */
+ * or F16), w and b of a type of their own.  Operands start on an element, the statistics on
+ * 8 bytes.  Every field has 8 bytes. */
 typedef struct sfb_norm_call {
     int64_t dtype, M, D;
     const void *x;
@@ -499,7 +500,7 @@ SFB_API int sfb_norm_failures(int64_t *count);
  * its V logits / T.  An entry is absent where its index is not in 0 .. V - 1 or its logit is
  * -inf; a row without entries, or of weight 0, gives 0 and is not read.  Row r of the logits is
  * at (r / inner) so + (r % inner) si, in elements; of their gradient at (r / inner) go + (r % inner) gi.
- * Every field has 8 bytes. */
+ * Operands start on an element.  Every field has 8 bytes. */
 #define SFB_REDUCE_NONE 0
 #define SFB_REDUCE_SUM 1
 #define SFB_REDUCE_MEAN 2                   /* over the weights of the rows with an entry; 0 where they add up to 0 */
@@ -538,7 +539,7 @@ SFB_API int sfb_distill_failures(int64_t *count);
 
 /* The gated feed-forward product over sf4..sf8 codes: h = act(x Wg^T + bg) (x Wu^T + bu), both weights N x K, as
  * sfb_tensor_call's.  No counterpart in the reference.  Np stands for N rounded up to a multiple of 16: codes and scales
- * are those of the gate, rows up to Np of zeros, then of the other weight. */
+ * are those of the gate, rows up to Np of zeros, then of the other weight.  Operands start on an element. */
 typedef struct sfb_gated_call {
     int64_t dtype, bits, act, M, N, K;      /* x is M x K */
     const void *x;

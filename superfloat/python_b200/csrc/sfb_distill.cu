@@ -847,10 +847,14 @@ int check(const sfb_distill_call *c, const char *what, bool forward) {
     if (c->M > 0 && (!c->logits || (c->K > 0 && !c->block) ||
                      (forward && ((c->K > 0 && (!c->teacher || !c->index)) || (c->w_dtype != SFB_WEIGHT_NONE && !c->weight)))))
         return set_error(SFB_EINVAL, "%s: null pointer", what);
-    const uintptr_t size = c->dtype == SFB_F32 ? 4 : 2;
-    if (reinterpret_cast<uintptr_t>(c->block) & 15) return set_error(SFB_EINVAL, "%s: the entries' scratch starts on 16 bytes", what);
-    if (reinterpret_cast<uintptr_t>(c->logits) % size || reinterpret_cast<uintptr_t>(c->grad) % size)
-        return set_error(SFB_EINVAL, "%s: the logits or their gradient do not start on an element", what);
+    const uintptr_t size = size_of(c->dtype);
+    if (!lies_on(c->block, 16)) return set_error(SFB_EINVAL, "%s: the entries' scratch starts on 16 bytes", what);
+    if (!lies_on(c->logits, size) || !lies_on(c->grad, size) || !lies_on(c->teacher, size_of(c->t_dtype)) ||
+        !lies_on(c->index, c->i_long ? 8 : 4) || (is_float(c->w_dtype) && !lies_on(c->weight, size_of(c->w_dtype))))
+        return set_error(SFB_EINVAL, "%s: an operand does not start on an element", what);
+    for (const void *p : {static_cast<const float *>(c->loss), static_cast<const float *>(c->rows), static_cast<const float *>(c->parts),
+                          static_cast<const float *>(c->weights), static_cast<const float *>(c->stats), c->upstream})
+        if (!lies_on(p, 4)) return set_error(SFB_EINVAL, "%s: a float32 buffer does not start on an element", what);
     return SFB_OK;
 }
 

@@ -184,6 +184,12 @@ int check(const sfb_gated_call *c, const char *what, bool codes) {
     if (c->M >= most || c->N >= most / 2 || c->K >= most || ((c->N + 63) / 64) * ((c->M + 127) / 128) >= most ||
         ((c->K + 255) / 256) * ((c->M + 127) / 128) >= most || ((c->K + 255) / 256) * ((c->N + 63) / 64) >= most)
         return set_error(SFB_ERANGE, "%s: a size of %lld x %lld x %lld", what, (long long)c->M, (long long)c->N, (long long)c->K);
+    const uintptr_t w = size_of(c->w_dtype), g = size_of(c->gate_bias_dtype), u = size_of(c->up_bias_dtype);
+    if (!lies_on(c->x, 2) || !lies_on(c->y, 2) || !lies_on(c->dx, 2) || !lies_on(c->gate, w) || !lies_on(c->up, w) ||
+        !lies_on(c->dgate, w) || !lies_on(c->dup, w) || !lies_on(c->gate_bias, g) || !lies_on(c->dgate_bias, g) ||
+        !lies_on(c->up_bias, u) || !lies_on(c->dup_bias, u) || !lies_on(c->gate_scale, 4) || !lies_on(c->up_scale, 4) ||
+        !lies_on(c->scale, 4) || !lies_on(c->z, 4) || !lies_on(c->work, 4) || !lies_on(c->top, 4))
+        return set_error(SFB_EINVAL, "%s: an operand does not start on an element", what);
     if (codes && (!c->codes || !on16(c->codes, c->ldc) || c->ldc < c->K || !c->scale))
         return set_error(SFB_EINVAL, "%s: the codes' rows must start on 16 bytes", what);
     return SFB_OK;

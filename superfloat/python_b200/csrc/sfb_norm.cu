@@ -698,6 +698,11 @@ int check(const sfb_norm_call *c, const char *what) {
         return set_error(SFB_EINVAL, "%s: a parameter's type", what);
     if (c->ldx < c->D || c->ldy < c->D) return set_error(SFB_EINVAL, "%s: a row stride is shorter than its row", what);
     if (c->M > 0 && (!c->x || !c->y)) return set_error(SFB_EINVAL, "%s: null pointer", what);
+    if (!lies_on(c->stats, 8)) return set_error(SFB_EINVAL, "%s: the statistics start on 8 bytes", what);
+    const uintptr_t size = size_of(c->dtype), w = size_of(c->w_dtype), b = size_of(c->b_dtype);
+    if (!lies_on(c->x, size) || !lies_on(c->y, size) || !lies_on(c->dx, size) || !lies_on(c->w, w) || !lies_on(c->dw, w) ||
+        !lies_on(c->b, b) || !lies_on(c->db, b))
+        return set_error(SFB_EINVAL, "%s: an operand does not start on an element", what);
     return SFB_OK;
 }
 
@@ -762,8 +767,7 @@ extern "C" int sfb_norm_backward(const sfb_norm_call *c, sfb_stream stream) {
         return set_error(SFB_EINVAL, "%s: null pointer, or a row stride that is shorter than its row", what);
     if ((c->dw && !is_float(c->w_dtype)) || (c->db && !is_float(c->b_dtype)))
         return set_error(SFB_EINVAL, "%s: a gradient's type", what);
-    if ((reinterpret_cast<uintptr_t>(c->stats) & 7) || (reinterpret_cast<uintptr_t>(c->work) & 15))
-        return set_error(SFB_EINVAL, "%s: the statistics start on 8 bytes, the scratch on 16", what);
+    if (!lies_on(c->work, 16)) return set_error(SFB_EINVAL, "%s: the scratch starts on 16 bytes", what);
     if (!c->dx && !c->dw && !c->db) return SFB_OK;
     Norm p = norm_of(c);
     p.dy = c->y;

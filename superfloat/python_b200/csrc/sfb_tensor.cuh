@@ -134,4 +134,8 @@ int with_activation(int act, F f) {
     return set_error(SFB_EINVAL, "sf tensor linear: activation %d", act);
 }
 
+// an element type's bytes, and whether an address (null included) is a multiple of a power of two
+inline uintptr_t size_of(int64_t dtype) { return dtype == SFB_F32 ? 4 : dtype == SFB_I8 ? 1 : 2; }
+inline bool lies_on(const void *p, uintptr_t size) { return (reinterpret_cast<uintptr_t>(p) & (size - 1)) == 0; }
+
 }  // namespace sfb
