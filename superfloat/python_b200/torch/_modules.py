@@ -644,7 +644,8 @@ def pack(model: nn.Module, inplace: bool = False) -> nn.Module:
         if id(m) not in done and isinstance(m, SFGatedFeedForward):
             gate, up = (SFPackedLinear(_tensor.pack_weight(p.weight, m.sf.bits, m.sf.scale), p.bias, f"{m.sf_name}.{n}")
                         for p, n in ((m.gate_proj, "gate_proj"), (m.up_proj, "up_proj")))
-            done[id(m)] = (m, SFPackedGatedFeedForward(gate, up, packed(m.down_proj), m.activation, m.sf_name).train(m.training))
+            down = packed(m.down_proj) if wanted(m.down_proj) else m.down_proj
+            done[id(m)] = (m, SFPackedGatedFeedForward(gate, up, down, m.activation, m.sf_name).train(m.training))
         elif id(m) not in done:
             w = m.weight.t() if isinstance(m, SFHFConv1D) else m.weight
             p = _tensor.pack_weight(w, m.sf.bits, m.sf.scale)
