@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(256) gated_expand_kernel(const __grid_constant
                 if constexpr (VEC) q = *reinterpret_cast<const uint4 *>(codes + n * ldc + k);
                 else q = shift_codes(codes + n * ldc, k, K);
             }
-            // (without conversions, which an SM makes at an eighth of the rate of sums: 43.5 us for 2 x 8192 x 4096, now 39)
+            // (without conversions, which an SM makes at an eighth of the rate of sums: 43.5 us for 2 x 8192 x 4096, now 41)
             const uint32_t four[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
             for (int h = 0; h < 2; h++) {

@@ -4,7 +4,8 @@
 //   dx = r (gy - mean(gy) - xh mean(gy xh)),  gy = dy w
 //   dw = sum over rows of dy xh,  db = sum over rows of dy
 //
-// Bound by memory, and nearly by instructions: a row is read once and written once.  The
+// A row is read once and written once.  Bound by the wait for a row's sums: at 16384 x 4096 of bf16 neither
+// DRAM (47 % of its rate forward, 63 % backward) nor issue (57 %, 70 %) is full.  The
 // variance is taken from the deviations, not from a sum of squares, which would cancel where
 // a row's mean is far from 0.  All sums are float32; results are rounded once.
 // A row belongs to a team: a warp (up to 1024 elements), a CTA (up to 8192) or a cluster
@@ -12,7 +13,7 @@
 // Teams take row after row, the next ones' copies in flight.  The backward pass keeps dw and db of a
 // team's own columns in registers; what the teams leave, one row of partial sums for every
 // CTA (or cluster), is added up by a second launch in a fixed order.
-// 16384 x 4096 of bf16: forward 61 us (4.4 TB/s), backward 75 us (5.4 TB/s) and 7 for the sums.
+// 16384 x 4096 of bf16: forward 55 us (4.8 TB/s), backward 71 us (5.7 TB/s) and 7 for the sums.
 #include <algorithm>
 #include <mutex>
 
