@@ -617,14 +617,16 @@ __global__ void __launch_bounds__(ALL, 4) row_kernel(const __grid_constant__ Dis
                 float loss = 0.0f;
                 if (live) {
                     // p (log p - log q) in base 2; where that leaves float32's range (a logit of the type's lowest value) the
-                    // difference of the logits itself, beside which the logarithms are nothing
+                    // difference of the logits itself, beside which the logarithms are nothing (but for a NaN, of a row
+                    // with an infinity)
                     const float off = log2f(soft.y);
                     float low = 0.0f;
                     for (int i = lane; i < (int)p.K; i += 32) {
                         const float z = far(soft.x, p.unit) ? (near[i] - soft.x) * p.unit : fmaf(near[i], p.unit, -base);
                         if (e[i] == 0.0f) continue;
-                        if (z > -1e30f) loss = fmaf(e[i], log2f(e[i]) - z + off, loss);
-                        else low = fmaf(e[i], soft.x - near[i], low);
+                        const bool in = z > -1e30f;
+                        loss = fmaf(e[i], (in ? log2f(e[i]) - z : 0.0f) + off, loss);
+                        if (!in) low = fmaf(e[i], soft.x - near[i], low);
                     }
                     loss = warp_sum(loss) * (0.69314718056f * p.temperature * p.temperature) * (weight * share);
                     if (__any_sync(0xffffffffu, low != 0.0f)) loss += warp_sum(low) * p.temperature * (weight * share);
