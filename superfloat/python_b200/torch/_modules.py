@@ -279,7 +279,8 @@ def _expression(calls, x, result, projections):
 
 
 def _hooked(m):
-    return any(getattr(m, h, None) for h in ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks"))
+    """Whether a call of the module does more than its class's forward: by hooks, or a forward set on the module itself."""
+    return "forward" in getattr(m, "__dict__", ()) or any(getattr(m, h, None) for h in ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks"))
 
 
 def gated_block(m: nn.Module):

@@ -211,3 +211,12 @@ def test_inference_mode():
         assert isinstance(convert(nn.Sequential(block))[0], sft.SFGatedFeedForward)
         assert "something else" in reason(Clamped())
     assert isinstance(convert(nn.Sequential(block), inplace=True)[0], sft.SFGatedFeedForward)
+
+
+@pytest.mark.parametrize("where", ["gate_proj", "up_proj", "act_fn", None])
+def test_a_forward_set_on_the_module(where):
+    block = Gated()
+    m = block if where is None else getattr(block, where)
+    own, seen = m.forward, []
+    m.forward = lambda x: (seen.append(1), own(x))[1]
+    assert "hooks" in reason(block)
